@@ -1,0 +1,347 @@
+"""The paged cache (tc_kv_write, tc_kv_read) and attention over it (tc_attn)
+against the same in 64 bits (tests/paged.py)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from paged import DT, HALF, TOP, Batch, attn_bound, attn_exact, scaled
+
+pytestmark = pytest.mark.gpu
+
+XTYPES, CTYPES = ["F32", "F16", "BF16"], ["F16", "BF16", "I8", "E4M3"]
+# (new rows, length): from the first token, appended, none new, an empty sequence, over page borders
+RAGGED = [(3, 3), (1, 17), (0, 9), (5, 40), (0, 0), (16, 16), (2, 33)]
+
+
+def rows_of(rng, T, heads, dim, xtype, spread=1.0):
+    return torch.from_numpy((spread * rng.standard_normal((T, heads, dim))).astype(np.float32)).to(DT[xtype])
+
+
+# ---- write and read ---------------------------------------------------------------------------------------------
+
+
+def written(b, name, x):
+    """The cache after tc_kv_write of x: (values as held, scales), numpy fp32."""
+    held = b.host[name].float().numpy().copy()
+    sc = b.host[name + "_scale"].numpy().copy() if scaled(b.ctype) else None
+    x = x.float().numpy()
+    for t, s, pos in b.rows():
+        w = b.slot(s, pos)
+        if w is None:
+            continue
+        r = x[t]
+        if sc is not None:
+            d = (np.abs(r).max(-1) / np.float32(TOP[b.ctype])).astype(np.float32)
+            d[d == 0] = 1
+            sc[w[0], :, w[1]] = d
+            r = (r / d[:, None]).astype(np.float32)
+            r = np.rint(r) if b.ctype == "I8" else torch.from_numpy(r).to(DT["E4M3"]).float().numpy()
+        else:
+            r = torch.from_numpy(r).to(DT[b.ctype]).float().numpy()
+        held[w[0], :, w[1]] = r
+    return held, sc
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("xtype", XTYPES)
+@pytest.mark.parametrize("kv_heads,dim,page", [(4, 128, 16), (1, 16, 48), (3, 80, 32), (2, 256, 64)])
+def test_kv_write(tc, dev, xtype, ctype, kv_heads, dim, page):
+    """Every slot of the batch holds its row's values and every other one what it held; ties, rows of zeros,
+    large and small rows."""
+    rng = np.random.default_rng(dim + page)
+    b = Batch(rng, RAGGED, page, kv_heads, dim, ctype, pad_rows=2)
+    k, v = (rows_of(rng, b.T, kv_heads, dim, xtype) for _ in range(2))
+    k[0] = 0
+    k[1, :, :4] = torch.tensor([127.0, 0.5, 2.5, -1.5])  # halves of steps where the scale is 1
+    k[1, :, 4:] = 3.5
+    v[2] *= 1e4
+    v[3] *= 1e-4
+    b.to(dev)
+    tc.kv_write(b.cache, b.batch, k.to(dev), v.to(dev))
+    for name, x in (("k", k), ("v", v)):
+        held, sc = written(b, name, x)
+        assert np.array_equal(b.dev[name].float().cpu().numpy(), held), name
+        if sc is not None:
+            assert np.array_equal(b.dev[name + "_scale"].cpu().numpy(), sc), name
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("xtype", XTYPES)
+@pytest.mark.parametrize("kv_heads,dim,page", [(4, 128, 16), (1, 48, 48), (3, 112, 32)])
+def test_kv_read(tc, dev, xtype, ctype, kv_heads, dim, page):
+    """Rows come back as value * scale, rounded once; rows past the last sequence are left alone."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, RAGGED, page, kv_heads, dim, ctype, pad_rows=3).to(dev)
+    out = tuple(torch.full((b.T, kv_heads, dim), 7.0, dtype=DT[xtype], device=dev) for _ in range(2))
+    tc.kv_read(b.cache, b.batch, b.T, DT[xtype], out=out)
+    for name, got in zip(("k", "v"), out):
+        want = np.full((b.T, kv_heads, dim), 7.0)
+        value = b.value(name)
+        for t, s, pos in b.rows():
+            p, i = b.slot(s, pos)
+            want[t] = value[p, :, i]
+        got = got.double().cpu().numpy()
+        # value * scale is rounded to fp32 and then to the rows' type
+        err = np.abs(got - want)
+        assert (err <= np.abs(want) * (HALF[xtype] * 1.001 + 2.0 ** -24) + 2.0 ** -25).all(), (name, err.max())
+        assert (got[-3:] == 7).all()
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+def test_kv_write_extremes(tc, dev, ctype):
+    """A row with an infinity or a NaN reads back as NaNs, its neighbours do not; a row of the smallest
+    numbers reads back within a step of it."""
+    rng = np.random.default_rng(5)
+    b = Batch(rng, [(4, 20)], 16, 2, 64, ctype).to(dev)
+    k = rows_of(rng, 4, 2, 64, "F32")
+    v = k.clone()
+    k[0, 0, 5], k[1, 1, 7], k[2, 0, 63] = float("inf"), float("nan"), float("-inf")
+    v[3] = 1e-44
+    tc.kv_write(b.cache, b.batch, k.to(dev), v.to(dev))
+    rk, rv = (x.cpu() for x in tc.kv_read(b.cache, b.batch, 4, torch.float32))
+    bad = torch.zeros(4, 2, dtype=torch.bool)
+    bad[0, 0] = bad[1, 1] = bad[2, 0] = True
+    assert torch.equal(rk.isnan().all(-1), bad) and torch.equal(rk.isnan().any(-1), bad)
+    assert (rv[3].abs() <= 2e-44).all()
+
+
+def test_kv_strided_rows(tc, dev):
+    """q, k and v as parts of one fused product's rows."""
+    rng = np.random.default_rng(6)
+    b = Batch(rng, [(5, 21), (1, 4)], 16, 2, 64, "F16").to(dev)
+    rows = rows_of(rng, 6, 8, 64, "F32").to(dev)  # 4 query heads, 2 of keys, 2 of values
+    q, k, v = rows[:, :4], rows[:, 4:6], rows[:, 6:]
+    tc.kv_write(b.cache, b.batch, k, v)
+    got = tc.attn(b.cache, b.batch, q, 0.125)
+    for name, x in (("k", k), ("v", v)):
+        assert np.array_equal(b.dev[name].float().cpu().numpy(), written(b, name, x.cpu())[0])
+    assert torch.equal(got, tc.attn(b.cache, b.batch, q.contiguous(), 0.125))
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+
+
+def check_attn(tc, dev, b, heads, xtype, scale, window=0, spread=1.0, seed=0):
+    rng = np.random.default_rng(seed)
+    q = rows_of(rng, b.T, heads, b.dim, xtype, spread)
+    out = torch.full((b.T, heads, b.dim), 7.0, dtype=DT[xtype], device=dev)
+    tc.attn(b.cache, b.batch, q.to(dev), scale, window=window, out=out)
+    got = out.double().cpu().numpy()
+    want, mass, terms = attn_exact(b, q.double().numpy(), scale, window)
+    n = max(total for _, total in b.seqs)
+    bound = attn_bound(xtype, b.ctype, b.dim, n, want, mass, terms)
+    used = int(b.start[-1])
+    err = np.abs(got - want)[:used]
+    worst = (err / bound[:used]).max() if used else 0
+    assert (got[used:] == 7).all()
+    assert not (worst > 1) and np.isfinite(got).all(), worst
+    return got, bound
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("xtype", XTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 4, 64, 16), (14, 2, 128, 32), (8, 1, 256, 48), (3, 3, 80, 16), (6, 2, 16, 64)])
+def test_attn_ragged(tc, dev, xtype, ctype, heads, kv_heads, dim, page):
+    rng = np.random.default_rng(heads + dim)
+    b = Batch(rng, RAGGED, page, kv_heads, dim, ctype, pad_rows=2).to(dev)
+    check_attn(tc, dev, b, heads, xtype, dim ** -0.5)
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("xtype", XTYPES)
+def test_attn_decode_lengths(tc, dev, xtype, ctype):
+    """One token each at lengths around every tile and page border."""
+    rng = np.random.default_rng(1)
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, 127, 128, 129, 255, 256, 257, 500, 1025]
+    b = Batch(rng, [(1, n) for n in lens], 16, 2, 64, ctype).to(dev)
+    check_attn(tc, dev, b, 6, xtype, 0.125)
+
+
+@pytest.mark.parametrize("ctype,xtype,dim", [("BF16", "BF16", 128), ("F16", "F32", 128), ("I8", "F16", 64), ("E4M3", "BF16", 256),
+                                             ("BF16", "F32", 96), ("I8", "F32", 256), ("F16", "F16", 192), ("BF16", "F16", 64)])
+@pytest.mark.parametrize("n,total", [(130, 130), (65, 400), (257, 300), (40, 1000)])
+def test_attn_prompts(tc, dev, ctype, xtype, dim, n, total):
+    rng = np.random.default_rng(n)
+    b = Batch(rng, [(n, total), (1, 70), (9, 9)], 32, 2, dim, ctype).to(dev)
+    check_attn(tc, dev, b, 6, xtype, dim ** -0.5)
+
+
+@pytest.mark.parametrize("window", [1, 7, 16, 33, 64, 100, 4096])
+@pytest.mark.parametrize("ctype,xtype", [("F16", "F32"), ("E4M3", "BF16"), ("BF16", "BF16")])
+def test_attn_window(tc, dev, window, ctype, xtype):
+    rng = np.random.default_rng(window)
+    b = Batch(rng, [(1, 300), (150, 200), (5, 64), (3, 3), (30, 95)], 16, 2, 64, ctype).to(dev)
+    check_attn(tc, dev, b, 8, xtype, 0.125, window=window)
+
+
+@pytest.mark.parametrize("xtype", XTYPES)
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("spread,scale", [(60.0, 0.125), (1e-6, 0.125), (1.0, 0.0)])
+def test_attn_sharp_and_flat(tc, dev, xtype, ctype, spread, scale):
+    """Softmaxes of one token, and flat ones."""
+    rng = np.random.default_rng(2)
+    b = Batch(rng, [(1, 200), (70, 90)], 16, 1, 64, ctype).to(dev)
+    check_attn(tc, dev, b, 4, xtype, scale, spread=spread)
+
+
+def test_attn_large_and_small_values(tc, dev):
+    """Rows of q far outside fp16's range, and factors of very different sizes."""
+    rng = np.random.default_rng(3)
+    b = Batch(rng, [(1, 100), (40, 60)], 16, 1, 64, "I8")
+    b.host["v_scale"] *= torch.from_numpy(np.exp2(rng.integers(-40, 40, b.host["v_scale"].shape)).astype(np.float32))
+    b.host["k_scale"] *= 2.0 ** -20
+    b.to(dev)
+    check_attn(tc, dev, b, 4, "F32", 0.125, spread=2.0 ** 20)
+    check_attn(tc, dev, b, 4, "BF16", 0.125, spread=2.0 ** 20)
+    b = Batch(rng, [(1, 100), (40, 60)], 16, 1, 64, "BF16")
+    for name in ("k", "v"):
+        b.host[name] *= 2.0 ** 40
+    b.to(dev)
+    check_attn(tc, dev, b, 4, "F32", 2.0 ** -43)
+
+
+def test_attn_rows_that_see_nothing(tc, dev):
+    """Rows at positions below 0 (more new rows than tokens), and sequences whose pages are all missing, give
+    zeros; a missing page among others is skipped, and so is what lies past the table."""
+    rng = np.random.default_rng(4)
+    b = Batch(rng, [(5, 2), (1, 40), (3, 50), (1, 0), (2, 100)], 16, 2, 64, "F16", width=4)
+    b.table[1, :] = -1
+    b.table[2, 1] = b.n_pages
+    b.to(dev)
+    got, _ = check_attn(tc, dev, b, 4, "F32", 0.125)
+    assert (got[:3] == 0).all() and (got[5] == 0).all() and (got[9] == 0).all()
+    k = rows_of(rng, b.T, 2, 64, "F32")
+    tc.kv_write(b.cache, b.batch, k.to(dev), k.to(dev))
+    for name in ("k", "v"):
+        assert np.array_equal(b.dev[name].float().cpu().numpy(), written(b, name, k)[0])
+    rk, _ = tc.kv_read(b.cache, b.batch, b.T, torch.float32)
+    for t, s, pos in b.rows():
+        if b.slot(s, pos) is None:
+            assert (rk[t] == 0).all()
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_attn_ignores_what_it_does_not_see(tc, dev, ctype, n):
+    """Infinities and NaN behind a sequence's end, in free pages and in tokens that a row does not see change
+    nothing."""
+    rng = np.random.default_rng(7)
+    b = Batch(rng, [(n, 90), (1, 37)], 32, 2, 64, ctype)
+    clean, bound = check_attn(tc, dev, b.to(dev), 6, "F32", 0.125, window=50)
+    used = {b.slot(s, j) for s, (_, total) in enumerate(b.seqs) for j in range(total)}
+    bad = torch.ones(b.n_pages, b.page, dtype=torch.bool)
+    for p, i in used:
+        bad[p, i] = False
+    # the last row of the first sequence is seen by itself alone
+    last = b.slot(0, 89)
+    for name in ("k", "v"):
+        h = b.host[name]
+        for p, i in [(int(p), int(i)) for p, i in bad.nonzero()] + [last]:
+            if scaled(ctype):
+                b.host[name + "_scale"][p, :, i] = float("nan") if (p + i) % 2 else float("inf")
+                if ctype == "E4M3":
+                    h.view(torch.uint8)[p, :, i] = 0x7F
+            else:
+                h[p, :, i] = float("nan") if (p + i) % 2 else float("inf")
+    b.to(dev)
+    q = rows_of(np.random.default_rng(0), b.T, 6, 64, "F32")
+    got = tc.attn(b.cache, b.batch, q.to(dev), 0.125, window=50).double().cpu().numpy()
+    rest = np.arange(n + 1) != n - 1
+    assert (np.abs(got - clean)[rest] <= 2 * bound[rest]).all()
+    assert np.isnan(got[n - 1]).any()
+
+
+def test_attn_shared_pages(tc, dev):
+    """Sequences that share their first pages."""
+    rng = np.random.default_rng(8)
+    b = Batch(rng, [(1, 70), (4, 68), (90, 150)], 16, 2, 64, "BF16")
+    b.table[1, :4] = b.table[0, :4]
+    b.table[2, :3] = b.table[0, :3]
+    check_attn(tc, dev, b.to(dev), 4, "BF16", 0.125)
+
+
+def test_attn_step_as_a_graph(tc, dev):
+    """Write, attention and read of a chunk captured once and replayed with other lengths, pages and rows:
+    every replay gives the eager calls' bits, with eager work of other sizes between the replays."""
+    rng = np.random.default_rng(9)
+    sizes = [[(1, 70), (3, 33), (60, 61)], [(1, 500), (0, 0), (63, 200)], [(2, 2), (60, 90), (2, 3)]]
+    steps = [Batch(rng, s, 16, 2, 64, "I8", spare=40 - sum(-(-t // 16) for _, t in s) + 40, width=40) for s in sizes]
+    live = Batch(rng, sizes[0], 16, 2, 64, "I8", spare=80 - 11, width=40).to(dev)
+    other = Batch(rng, [(1, 3000)], 16, 4, 128, "F16").to(dev)
+    T = 64
+    q = torch.zeros(T, 8, 64, device=dev)
+    kv = torch.zeros(2, T, 2, 64, device=dev)
+    tc.attn_reserve(8, T)
+
+    def work():
+        tc.kv_write(live.cache, live.batch, kv[0], kv[1])
+        o = tc.attn(live.cache, live.batch, q, 0.125)
+        return o, *tc.kv_read(live.cache, live.batch, T, torch.float32)
+
+    work()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = work()
+    for turn in range(2):
+        for b in steps:
+            for name, t in b.host.items():
+                live.dev[name].zero_()
+                live.dev[name][:t.shape[0]] = t.to(dev)[:live.n_pages]
+            live.batch.start.copy_(torch.from_numpy(b.start))
+            live.batch.length.copy_(torch.from_numpy(b.length))
+            live.batch.table.copy_(torch.from_numpy(b.table))
+            q.copy_(rows_of(rng, T, 8, 64, "F32"))
+            kv.copy_(rows_of(rng, 2 * T, 2, 64, "F32").reshape(2, T, 2, 64))
+            for o in outs:
+                o.fill_(3.0)
+            tc.attn(other.cache, other.batch, torch.randn(1, 8, 128, device=dev), 0.1)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            got = [o[:b.start[-1]].clone() for o in outs]
+            want = [o[:b.start[-1]] for o in work()]
+            for x, y in zip(got, want):
+                assert torch.equal(x, y), (turn, b.seqs)
+
+
+def test_attn_on_another_stream(tc, dev):
+    rng = np.random.default_rng(10)
+    b = Batch(rng, [(1, 900), (40, 300)], 16, 2, 128, "BF16").to(dev)
+    q = rows_of(rng, b.T, 14, 128, "BF16").to(dev)
+    want = tc.attn(b.cache, b.batch, q, 0.09)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = tc.attn(b.cache, b.batch, q, 0.09)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_attn_cache_beyond_4_gib(tc, dev):
+    """Pages whose bytes lie past 32-bit offsets."""
+    page, kvh, dim = 1024, 8, 256
+    n_pages = (9 << 30) // (page * kvh * dim * 2)
+    k, v = (torch.zeros(n_pages, kvh, page, dim, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    import tc_hip
+    cache = tc_hip.KVCache(k, v)
+    g = torch.Generator().manual_seed(0)
+    table = torch.tensor([[n_pages - 1, 1, n_pages - 2]], dtype=torch.int32, device=dev)
+    batch = tc_hip.KVBatch(torch.tensor([0, 2500], dtype=torch.int32, device=dev),
+                           torch.tensor([2500], dtype=torch.int32, device=dev), table)
+    rows = [torch.randn(2500, kvh, dim, generator=g).to(torch.bfloat16) for _ in range(2)]
+    tc.kv_write(cache, batch, *(r.to(dev) for r in rows))
+    back = tc.kv_read(cache, batch, 2500, torch.bfloat16)
+    for x, y in zip(rows, back):
+        assert torch.equal(x, y.cpu())
+    assert int((k != 0).any(-1).sum()) == 2500 * kvh
+    q = torch.randn(1, 8, dim, generator=g).to(torch.bfloat16)
+    one = tc_hip.KVBatch(torch.tensor([0, 1], dtype=torch.int32, device=dev), batch.length, table)
+    got = tc.attn(cache, one, q.to(dev), 0.0625).double().cpu()
+    kd, vd = (r.double() for r in rows)
+    for h in range(8):
+        p = torch.softmax(kd[:, h] @ q[0, h].double() * 0.0625, 0)
+        want, mass = p @ vd[:, h], p @ vd[:, h].abs()
+        assert ((got[0, h] - want).abs() <= mass * (2.0 ** -8 + 2e-3) + 2.0 ** -8 * want.abs()).all()

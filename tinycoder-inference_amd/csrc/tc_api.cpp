@@ -300,6 +300,17 @@ int gemm_entry_check(int type, const void *w, const float *x, const float *out, 
 
 int fail_code(int code, const char *msg) { return fail(code, "%s", msg); }
 
+void *aux_scratch(size_t need, hipStream_t st) {
+    Device *d = device();
+    if (!d) {
+        fail(TC_E_UNSUPPORTED, "no gfx950 device");
+        return nullptr;
+    }
+    if (ensure(d->aux, need, st)) return d->aux.p;
+    fail(TC_E_LAUNCH, "hipMalloc(%zu) failed", need);
+    return nullptr;
+}
+
 // Tokens per launch of the fp32-activation MFMA kernel: the bf16 pieces take 6
 // bytes per value, so long prompts go in chunks of about 96 MB of pieces
 // (2048 tokens at 8192 columns).

@@ -1,0 +1,98 @@
+// tc_attn_common.hpp -- what the paged-cache kernels share: the batch as the
+// kernels see it, element types and their conversions, and the launchers.
+#pragma once
+
+#include "tc_common.hpp"
+
+namespace tc {
+
+// Element types of rows and caches (tc_attention.h).
+enum : int { kF32 = 0, kF16 = 1, kI8 = 24, kBF16 = 30, kE4M3 = 100 };
+
+__host__ __device__ constexpr uint32_t elem_bytes(int t) { return t == kF32 ? 4 : t == kF16 || t == kBF16 ? 2 : 1; }
+__host__ __device__ constexpr bool scaled_type(int t) { return t == kI8 || t == kE4M3; }
+
+constexpr uint32_t kMaxHeadDim = 256;
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// Two bf16 of two floats, to nearest even (NaN stays NaN).
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, bf16x2{__bf16(a), __bf16(b)});
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, f16x2{_Float16(a), _Float16(b)});
+}
+
+// 8 consecutive elements of a row as floats (16-byte aligned rows).
+__device__ __forceinline__ void load8(int type, const void *p, uint64_t elem, float (&x)[8]) {
+    if (type == kF32) {
+        const f32x4 *q = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + elem);
+        const f32x4 u = q[0], v = q[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = u[i], x[4 + i] = v[i];
+    } else {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + elem);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = u[i];
+            if (type == kF16) {
+                x[2 * i] = h2f(w & 0xFFFF);
+                x[2 * i + 1] = h2f(w >> 16);
+            } else {
+                x[2 * i] = __builtin_bit_cast(float, w << 16);
+                x[2 * i + 1] = __builtin_bit_cast(float, w & 0xFFFF0000u);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store8(int type, void *p, uint64_t elem, const float (&x)[8]) {
+    if (type == kF32) {
+        f32x4 *q = reinterpret_cast<f32x4 *>(static_cast<float *>(p) + elem);
+        q[0] = f32x4{x[0], x[1], x[2], x[3]};
+        q[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+        u32x4 u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = type == kF16 ? pack_f16(x[2 * i], x[2 * i + 1]) : pack_bf16(x[2 * i], x[2 * i + 1]);
+        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + elem) = u;
+    }
+}
+
+// ---- launchers (tc_kv.hip, tc_attn.hip, tc_verify.hip) ----
+hipError_t launch_kv_write(const KvArgs &a, int ctype, int xtype, const void *k, const void *v, uint32_t k_stride,
+                           uint32_t v_stride, hipStream_t st);
+hipError_t launch_kv_read(const KvArgs &a, int ctype, int xtype, void *k, void *v, hipStream_t st);
+
+struct AttnArgs {
+    KvArgs kv;
+    const void *q;
+    void *out;
+    uint32_t heads, group;  // query heads, query heads per key/value head
+    uint32_t q_stride;
+    float scale;
+    uint32_t window;
+    int xtype;
+};
+size_t attn_scratch_bytes(uint32_t heads, uint32_t n_tokens, int num_cu);
+hipError_t launch_attn(const AttnArgs &a, int ctype, int num_cu, void *scratch, hipStream_t st);
+
+struct VerifyArgs {
+    const float *logits, *draft_probs;
+    uint32_t vocab, n_seq, n_tokens;
+    const int32_t *start, *tokens;
+    const float *temperature, *accept_u, *sample_u;
+    int32_t *n_accepted, *next_token;
+};
+size_t verify_scratch_bytes(uint32_t n_tokens, uint32_t n_seq);
+hipError_t launch_verify(const VerifyArgs &a, int num_cu, void *scratch, hipStream_t st);
+
+}  // namespace tc

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "tc_kv_index.hpp"
+
 namespace tc {
 
 // GGML type ids (reference include/IModelLoader.hpp:51-62).
@@ -55,29 +57,6 @@ __host__ inline ActLayout act_layout(int wtype, uint32_t S, uint32_t cols) {
     L.dg_off = L.bs_off + up(size_t(S) * (cols / 16) * 2);
     L.bytes = L.dg_off + up(size_t(S) * (cols / 256) * dg_bytes(wtype));
     return L;
-}
-
-// Fast unsigned division by a runtime constant (Granlund-Montgomery): q = n/d
-// for n < 2^31, using a 32x32->64 multiply-high.
-struct DivMod {
-    uint32_t d, mul, shift;
-};
-
-__host__ inline DivMod make_divmod(uint32_t d) {
-    DivMod r{d, 0, 0};
-    uint32_t s = 0;
-    while ((1u << s) < d) ++s;
-    r.shift = s;
-    // mul = ceil(2^(32+s) / d) - 2^32
-    const uint64_t one = 1;
-    r.mul = uint32_t(((one << 32) * ((one << s) - d)) / d + 1);
-    return r;
-}
-
-__device__ __forceinline__ uint32_t div_fast(uint32_t n, const DivMod &m) {
-    if (m.d == 1) return n;
-    const uint32_t t = __umulhi(n, m.mul);
-    return (t + ((n - t) >> 1)) >> (m.shift - 1);
 }
 
 // fp16 bits -> fp32 (exact, including subnormals).

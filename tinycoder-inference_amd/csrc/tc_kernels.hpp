@@ -190,5 +190,8 @@ int gemm_mfma_into(int type, const void *w, const float *x, float *out, uint32_t
 int gemm_entry_check(int type, const void *w, const float *x, const float *out, uint32_t S, uint32_t rows,
                      uint32_t cols, uint32_t blocks_per_row);
 int fail_code(int code, const char *msg);
+// The current device's intermediates buffer (Device::aux), grown to `need` bytes
+// for a call on st; null (with the error set) where that fails.
+void *aux_scratch(size_t need, hipStream_t st);
 
 }  // namespace tc

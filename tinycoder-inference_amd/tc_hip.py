@@ -18,7 +18,10 @@ BLOCK_SIZE = {Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256, I
 
 TC_OK, TC_E_UNSUPPORTED, TC_E_LAUNCH, TC_E_ARG = 0, -1, -2, -3
 
-# Every function the C header declares, with its ctypes signature.
+# Element types of rows and caches (tc_attention.h).
+F32, F16, I8, BF16, E4M3 = 0, 1, 24, 30, 100
+
+# Every function the C headers declare, with its ctypes signature.
 _P, _U32, _I = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int
 SIGNATURES = {
     "tc_available": (_I, []),
@@ -54,6 +57,11 @@ SIGNATURES = {
     "tc_gemm_noalloc_scratch_bytes": (ctypes.c_size_t, []),
     "tc_host_weights_register": (_I, [_P, ctypes.c_size_t]),
     "tc_host_weights_unregister": (_I, [_P]),
+    "tc_kv_write": (_I, [_P, _P, _I, _P, _P, _U32, _U32, _P]),
+    "tc_kv_read": (_I, [_P, _P, _I, _P, _P, _P]),
+    "tc_attn": (_I, [_P, _P, _I, _P, _U32, _P, _U32, ctypes.c_float, _U32, _P]),
+    "tc_attn_reserve": (_I, [_U32, _U32]),
+    "tc_spec_verify": (_I, [_P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _P, _P, _P, _P]),
     "tc_gguf_open": (_P, [ctypes.c_char_p]),
     "tc_gguf_open_metadata": (_P, [ctypes.c_char_p]),
     "tc_gguf_close": (None, [_P]),
@@ -83,7 +91,12 @@ def row_bytes(qtype, cols):
     return cols // BLOCK_SIZE[qtype] * TYPE_SIZE[qtype]
 
 
+_LOADED = {}
+
+
 def load_library(path=LIB_PATH):
+    if path in _LOADED:
+        return _LOADED[path]
     # torch ships its own libamdhip64.so.7; it must be the HIP runtime this
     # library binds to, or the streams and memory torch hands over belong to
     # another runtime instance. Importing torch first makes the loader reuse it.
@@ -96,7 +109,79 @@ def load_library(path=LIB_PATH):
         f = getattr(lib, name)
         f.restype = res
         f.argtypes = args
+    _LOADED[path] = lib
     return lib
+
+
+def _elem_type(dtype):
+    """The tc_attention.h element type of a torch dtype."""
+    import torch
+    t = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8,
+         torch.float8_e4m3fn: E4M3}.get(dtype)
+    if t is None:
+        raise TCError(TC_E_UNSUPPORTED, f"no element type for {dtype}")
+    return t
+
+
+class _CKVCache(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("n_pages", _U32), ("kv_heads", _U32), ("page_tokens", _U32),
+                ("head_dim", _U32), ("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P)]
+
+
+class _CKVBatch(ctypes.Structure):
+    _fields_ = [("n_seq", _U32), ("n_tokens", _U32), ("table_pages", _U32), ("start", _P), ("len", _P), ("table", _P)]
+
+
+def _need(ok, what):
+    if not ok:
+        raise TCError(TC_E_ARG, what)
+
+
+class KVCache:
+    """The buffers of one layer's paged cache (tc_kv_cache): k and v
+    [n_pages][kv_heads][page_tokens][head_dim] of float16, bfloat16, int8 or
+    float8_e4m3fn, for the 8-bit types with k_scale and v_scale fp32
+    [n_pages][kv_heads][page_tokens]."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype, "k and v differ or are not 4-dimensional")
+        scaled = k.dtype in (torch.int8, torch.float8_e4m3fn)
+        for t in (k_scale, v_scale):
+            _need((t is not None) == scaled, "scales go with the 8-bit types and with these only")
+            _need(t is None or (t.dtype == torch.float32 and t.shape == k.shape[:3]), "scales are fp32 [n_pages][kv_heads][page_tokens]")
+        held = [t for t in (k, v, k_scale, v_scale) if t is not None]
+        _need(all(t.is_contiguous() and t.device == k.device for t in held), "a cache is contiguous and on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
+        self.c = _CKVCache(_elem_type(k.dtype), self.n_pages, self.kv_heads, self.page_tokens, self.head_dim,
+                           *[None if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale)])
+
+    @classmethod
+    def empty(cls, dtype, n_pages, kv_heads, page_tokens, head_dim, device="cuda"):
+        """A cache of zeros."""
+        import torch
+        shape = (n_pages, kv_heads, page_tokens, head_dim)
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        if dtype not in (torch.int8, torch.float8_e4m3fn):
+            return cls(k, v)
+        return cls(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+class KVBatch:
+    """Which rows are whose, and where they lie (tc_kv_batch): start int32
+    [n_seq + 1], length int32 [n_seq], table int32 [n_seq][table_pages]. Other
+    lengths and pages may be written into the tensors between calls."""
+
+    def __init__(self, start, length, table):
+        import torch
+        n = length.numel()
+        _need(all(t.dtype == torch.int32 and t.is_contiguous() and t.device == start.device for t in (start, length, table)),
+              "start, length and table are contiguous int32 on one device")
+        _need(start.numel() == n + 1 and table.dim() == 2 and table.shape[0] == n,
+              "start has n_seq + 1 entries, table n_seq rows")
+        self.start, self.length, self.table = start, length, table
+        self.c = _CKVBatch(n, 0, table.shape[1], start.data_ptr(), length.data_ptr(), table.data_ptr())
 
 
 def _ptr(t):
@@ -279,6 +364,84 @@ class Library:
         wts = torch.empty((S, top_k), dtype=torch.float32, device=logits.device)
         self._check(self.lib.tc_moe_select(_ptr(logits), S, E, top_k, _ptr(ids), _ptr(wts), self._stream()))
         return ids, wts
+
+
+    # -- paged cache, attention, drafted tokens ---------------------------------------
+    def _kv_call(self, cache, batch, rows):
+        """The batch's C struct for `rows` [n_tokens][heads][head_dim], checked."""
+        import torch
+        _need(rows[0].dim() == 3 and all(t.shape == rows[0].shape and t.dtype == rows[0].dtype for t in rows),
+              "rows are [n_tokens][heads][head_dim], of one type")
+        T, H, D = rows[0].shape
+        for t in rows:
+            _need(t.shape[2] == cache.head_dim, f"head_dim {t.shape[2]} is not the cache's {cache.head_dim}")
+            _need(T == 0 or (t.stride(2) == 1 and (H == 1 or t.stride(1) == D)), "a row's heads are not contiguous")
+        dev = torch.cuda.current_device()
+        _need(all(t.device.type == "cuda" and t.device.index == dev for t in (*rows, cache.k, batch.start)),
+              "tensors are not on the current device")
+        batch.c.n_tokens = T
+        return batch.c
+
+    @staticmethod
+    def _row_stride(t):
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+    def kv_write(self, cache, batch, k, v):
+        """Keys and values [n_tokens][kv_heads][head_dim] (rows may be strided)
+        into their slots of the cache."""
+        _need(k.dim() == 3 and k.shape[1] == cache.kv_heads, "k is not [n_tokens][kv_heads][head_dim]")
+        b = self._kv_call(cache, batch, (k, v))
+        self._check(self.lib.tc_kv_write(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(k.dtype), _ptr(k), _ptr(v),
+                                         self._row_stride(k), self._row_stride(v), self._stream()))
+
+    def kv_read(self, cache, batch, n_tokens, dtype, out=None):
+        """The batch's n_tokens rows out of the cache: (k, v)."""
+        import torch
+        if out is None:
+            shape = (n_tokens, cache.kv_heads, cache.head_dim)
+            out = tuple(torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        k, v = out
+        _need(k.is_contiguous() and v.is_contiguous() and k.dtype == dtype and k.shape[0] == n_tokens and
+              k.shape[1] == cache.kv_heads, "outputs are contiguous [n_tokens][kv_heads][head_dim] of dtype")
+        b = self._kv_call(cache, batch, (k, v))
+        self._check(self.lib.tc_kv_read(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(dtype), _ptr(k), _ptr(v),
+                                        self._stream()))
+        return k, v
+
+    def attn(self, cache, batch, q, scale, window=0, out=None):
+        """Causal attention of q [n_tokens][heads][head_dim] (rows may be strided)
+        over the cache."""
+        import torch
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _need(out.is_contiguous(), "out is not contiguous")
+        b = self._kv_call(cache, batch, (q, out))
+        self._check(self.lib.tc_attn(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(q.dtype), _ptr(q),
+                                     self._row_stride(q), _ptr(out), q.shape[1], scale, window, self._stream()))
+        return out
+
+    def attn_reserve(self, heads, n_tokens):
+        self._check(self.lib.tc_attn_reserve(heads, n_tokens))
+
+    def spec_verify(self, logits, tokens, start, temperature, accept_u, sample_u, draft_probs=None):
+        """How many of each sequence's drafted tokens hold against the target's
+        logits [n_tokens][vocab], and the token after them: (n_accepted, next_token)."""
+        import torch
+        T, V = logits.shape
+        S = temperature.numel()
+        floats = [t for t in (logits, temperature, accept_u, sample_u, draft_probs) if t is not None]
+        _need(all(t.dtype == torch.float32 for t in floats) and tokens.dtype == start.dtype == torch.int32,
+              "tokens and start are int32, the others fp32")
+        dev = torch.cuda.current_device()
+        _need(all(t.is_contiguous() and t.device.type == "cuda" and t.device.index == dev for t in (*floats, tokens, start)),
+              "tensors are contiguous and on the current device")
+        _need(start.numel() == S + 1 and tokens.numel() == accept_u.numel() == T and sample_u.numel() == S and
+              (draft_probs is None or draft_probs.shape == logits.shape), "sizes do not agree")
+        n, tok = (torch.empty(S, dtype=torch.int32, device=logits.device) for _ in range(2))
+        self._check(self.lib.tc_spec_verify(_ptr(logits), _ptr(draft_probs), V, S, T, _ptr(start), _ptr(tokens),
+                                            _ptr(temperature), _ptr(accept_u), _ptr(sample_u), _ptr(n), _ptr(tok),
+                                            self._stream()))
+        return n, tok
 
 
 class TensorRecord:
