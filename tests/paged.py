@@ -73,13 +73,14 @@ class Batch:
 
 
 def attn_exact(b, q, scale, window=0):
-    """-> (out, bound): attention of q (fp64 [T][heads][dim]) and, for each output, sum_j p_j |v_j| and the
-    largest score error that one rounding of relative size 1 to every term of it would make."""
+    """-> (out, mass, terms, absv): attention of q (fp64 [T][heads][dim]) and, for each output, sum_j p_j |v_j|,
+    the largest score error that one rounding of relative size 1 to every term of it would make, and
+    sum_j |v_j|."""
     T, H, D = q.shape
     G = H // b.kv_heads
     k, v = b.value("k"), b.value("v")
     out, mass = np.zeros((T, H, D)), np.zeros((T, H, D))
-    terms = np.zeros((T, H, 1))
+    terms, absv = np.zeros((T, H, 1)), np.zeros((T, H, D))
     for t, s, pos in b.rows():
         lo = max(0, pos - window + 1) if window else 0
         where = [w for w in (b.slot(s, j) for j in range(lo, pos + 1)) if w is not None]
@@ -92,11 +93,12 @@ def attn_exact(b, q, scale, window=0):
             p = np.exp(z - z.max())
             p /= p.sum()
             out[t, h], mass[t, h] = p @ V, p @ np.abs(V)
+            absv[t, h] = np.abs(V).sum(0)
             terms[t, h] = (np.abs(K) @ np.abs(q[t, h])).max() * scale
-    return out, mass, terms
+    return out, mass, terms, absv
 
 
-def attn_bound(xtype, ctype, D, n, out, mass, terms):
+def attn_bound(xtype, ctype, D, n, out, mass, terms, absv):
     """How far tc_attn may be from the 64-bit result: a score is off by (D + 8) fp32 roundings of its terms
     (products, sums, scale, factor, exponential) and q's own pieces; a weight p by that much twice (its own
     and the sum's score), and by its rounding to the matrix cores' type; the n-term sums by fp32 roundings;
@@ -110,4 +112,8 @@ def attn_bound(xtype, ctype, D, n, out, mass, terms):
     # below fp16's smallest normal number, 2^-14, its step is 2^-24 whatever the value: half of it is not
     # HALF of the value
     least = 2.0 ** -25 if xtype == "F16" else 1e-30
+    # weights enter fp16 operands as 2^11 p or more, where the row's largest p is 1: half a step of fp16's
+    # subnormals, 2^-25, is 2^-36 of that p, for every token, however small its weight
+    if ctype != "BF16":
+        least = least + absv * 2.0 ** -36
     return mass * (2.1 * score + piece + (n + 16) * 2.0 ** -24) + HALF[xtype] * np.abs(out) + least

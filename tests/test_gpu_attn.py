@@ -129,9 +129,9 @@ def check_attn(tc, dev, b, heads, xtype, scale, window=0, spread=1.0, seed=0):
     out = torch.full((b.T, heads, b.dim), 7.0, dtype=DT[xtype], device=dev)
     tc.attn(b.cache, b.batch, q.to(dev), scale, window=window, out=out)
     got = out.double().cpu().numpy()
-    want, mass, terms = attn_exact(b, q.double().numpy(), scale, window)
+    want, mass, terms, absv = attn_exact(b, q.double().numpy(), scale, window)
     n = max(total for _, total in b.seqs)
-    bound = attn_bound(xtype, b.ctype, b.dim, n, want, mass, terms)
+    bound = attn_bound(xtype, b.ctype, b.dim, n, want, mass, terms, absv)
     used = int(b.start[-1])
     err = np.abs(got - want)[:used]
     worst = (err / bound[:used]).max() if used else 0

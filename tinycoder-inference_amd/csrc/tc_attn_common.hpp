@@ -84,6 +84,47 @@ struct AttnArgs {
 };
 size_t attn_scratch_bytes(uint32_t heads, uint32_t n_tokens, int num_cu);
 hipError_t launch_attn(const AttnArgs &a, int ctype, int num_cu, void *scratch, hipStream_t st);
+// ... for one cache type (tc_attn_inst.hip).
+template <int CT>
+hipError_t launch_attn_cache(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
+template <>
+hipError_t launch_attn_cache<kF16>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
+template <>
+hipError_t launch_attn_cache<kBF16>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
+template <>
+hipError_t launch_attn_cache<kI8>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
+template <>
+hipError_t launch_attn_cache<kE4M3>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
+
+// A block of rows whose tiles lie in several workgroups' parts.
+struct SplitJob {
+    uint32_t seq, r0, kvh;
+    uint32_t count;  // workgroups, from this one on (0: none)
+    uint32_t slot;   // where the first one's sums are; the others': 2 * workgroup
+};
+
+// Sums that workgroups leave for k_attn_join, two blocks of 32 rows each.
+struct SplitScratch {
+    SplitJob *jobs;  // [workgroups]
+    float *ml;       // [2 * workgroups][32][2] reference and sum of weights
+    float *o;        // [2 * workgroups][32][DP] sums
+};
+template <int DP>
+SplitScratch split_scratch(void *scratch, uint32_t grid) {
+    char *p = static_cast<char *>(scratch);
+    SplitScratch s;
+    s.jobs = reinterpret_cast<SplitJob *>(p);
+    p += (grid * sizeof(SplitJob) + 255) & ~size_t(255);
+    s.ml = reinterpret_cast<float *>(p);
+    p += size_t(grid) * 2 * 32 * 2 * 4;
+    s.o = reinterpret_cast<float *>(p);
+    return s;
+}
+// For up to two workgroups per CU of any head size.
+inline size_t attn_split_bytes(int num_cu) {
+    const size_t grid = 2 * size_t(num_cu);
+    return ((grid * sizeof(SplitJob) + 255) & ~size_t(255)) + grid * 2 * 32 * (2 + kMaxHeadDim) * 4;
+}
 
 struct VerifyArgs {
     const float *logits, *draft_probs;

@@ -1,0 +1,49 @@
+// tc_attn_inst.hip -- the attention kernels for one cache type (TC_ATTN_CACHE, one
+// object each), and the choice of the number of pieces and the padded head size.
+#include "tc_attn_split.hpp"
+
+#ifndef TC_ATTN_CACHE
+#define TC_ATTN_CACHE 30
+#endif
+
+namespace tc {
+namespace {
+
+template <int CT, int NP, int DP>
+hipError_t split(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
+    using Sh = SplitShape<CT, NP, DP>;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn_split<CT, NP, DP>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS);
+    if (attr != hipSuccess) return attr;
+    const uint32_t grid = Sh::OCC * num_cu;
+    const SplitScratch sc = split_scratch<DP>(scratch, grid);
+    k_attn_split<CT, NP, DP><<<grid, 64 * Sh::NW, Sh::LDS, st>>>(a, sc);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_attn_join<DP><<<dim3(grid, 8), 256, 0, st>>>(a, sc);
+    return hipGetLastError();
+}
+
+template <int CT, int NP>
+hipError_t by_dim(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
+    if (a.kv.dim <= 64) return split<CT, NP, 64>(a, num_cu, scratch, st);
+    if (a.kv.dim <= 128) return split<CT, NP, 128>(a, num_cu, scratch, st);
+    return split<CT, NP, 256>(a, num_cu, scratch, st);
+}
+
+}  // namespace
+
+// Pieces of q and of the weights: what a row's type has bits for.
+template <>
+hipError_t launch_attn_cache<TC_ATTN_CACHE>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
+    constexpr int CT = TC_ATTN_CACHE;
+    if constexpr (CT == kBF16) {
+        if (a.xtype == kF32) return by_dim<CT, 3>(a, num_cu, scratch, st);
+        if (a.xtype == kF16) return by_dim<CT, 2>(a, num_cu, scratch, st);
+    } else {
+        if (a.xtype == kF32) return by_dim<CT, 2>(a, num_cu, scratch, st);
+    }
+    return by_dim<CT, 1>(a, num_cu, scratch, st);
+}
+
+}  // namespace tc
