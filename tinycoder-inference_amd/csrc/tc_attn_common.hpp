@@ -103,27 +103,30 @@ struct SplitJob {
     uint32_t slot;   // where the first one's sums are; the others': 2 * workgroup
 };
 
-// Sums that workgroups leave for k_attn_join, two blocks of 32 rows each.
+// Sums that workgroups leave for k_attn_join: two blocks of rows each.
 struct SplitScratch {
-    SplitJob *jobs;  // [workgroups]
-    float *ml;       // [2 * workgroups][32][2] reference and sum of weights
-    float *o;        // [2 * workgroups][32][DP] sums
+    SplitJob *jobs;  // [parts]
+    float *ml;       // [2 * parts][rows][2] reference and sum of weights
+    float *o;        // [2 * parts][rows][DP] sums
 };
-template <int DP>
-SplitScratch split_scratch(void *scratch, uint32_t grid) {
+inline SplitScratch split_scratch(void *scratch, uint32_t parts, uint32_t rows) {
     char *p = static_cast<char *>(scratch);
     SplitScratch s;
     s.jobs = reinterpret_cast<SplitJob *>(p);
-    p += (grid * sizeof(SplitJob) + 255) & ~size_t(255);
+    p += (parts * sizeof(SplitJob) + 255) & ~size_t(255);
     s.ml = reinterpret_cast<float *>(p);
-    p += size_t(grid) * 2 * 32 * 2 * 4;
+    p += size_t(parts) * 2 * rows * 2 * 4;
     s.o = reinterpret_cast<float *>(p);
     return s;
 }
-// For up to two workgroups per CU of any head size.
-inline size_t attn_split_bytes(int num_cu) {
-    const size_t grid = 2 * size_t(num_cu);
-    return ((grid * sizeof(SplitJob) + 255) & ~size_t(255)) + grid * 2 * 32 * (2 + kMaxHeadDim) * 4;
+// Sequences of at most this many rows (new tokens * query heads per key/value
+// head) go to the kernel for few rows.
+constexpr uint32_t kSplitRows = 64;
+// ... for any call: two workgroups per CU with 32 rows, one with 256 of up to 128
+// dims or 128 of up to 256.
+inline size_t attn_part_bytes(int num_cu) {
+    const size_t cu = num_cu, jobs = (2 * cu * sizeof(SplitJob) + 255) & ~size_t(255);
+    return jobs + cu * 2 * 256 * 2 * 4 + cu * 2 * 256 * 128 * 4;
 }
 
 struct VerifyArgs {

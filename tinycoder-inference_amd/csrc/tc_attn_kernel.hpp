@@ -173,6 +173,66 @@ __device__ __forceinline__ void value4(const unsigned char *p, float (&x)[4]) {
     }
 }
 
+// v of the lane 32 away.
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// Operand of o^T += V^T P^T for dims 32 d + 0 .. 31 and tokens 16 k + 0 .. 15 of a
+// 16-bit tile in LDS.
+template <int LT, int RB>
+__device__ __forceinline__ u32x4 value_frag(const unsigned char *vt, uint32_t d, uint32_t k, uint32_t lane) {
+    const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1, half = lane >> 5;
+    u32x4 v;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint32_t r = 16 * k + 8 * half + 4 * u + l16 / 4, e = 32 * d + 16 * g16 + 4 * (l16 % 4);
+        const unsigned char *p = vt + r * RB + (((e / 8) ^ value_swizzle<RB, 2>(r)) << 4) + (e & 4) * 2;
+        const u32x2 w =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
+        v[2 * u] = w[0], v[2 * u + 1] = w[1];
+    }
+    return v;
+}
+
+// Whether a tile in LDS holds a value that is not finite.
+template <int CT, int TILE>
+__device__ __forceinline__ bool tile_not_finite(const unsigned char *vt, uint32_t lane) {
+    uint32_t bad = 0;
+    for (uint32_t i = lane; i < TILE / 16; i += 64) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(vt + 16 * i);
+        bad |= not_finite<CT>(w[0]) | not_finite<CT>(w[1]) | not_finite<CT>(w[2]) | not_finite<CT>(w[3]);
+    }
+    return __ballot(bad != 0) != 0;
+}
+
+// o += weights * values token by token, of those that the lane's row sees alone: for
+// tiles with infinities or NaN that some row must not see, which a product with a
+// weight of 0 would bring in.
+template <int CT, int RB, int DB>
+__device__ __forceinline__ void add_values_one_by_one(const unsigned char *vt, const v16f &s, uint32_t seen, uint32_t lane,
+                                                      v16f (&o)[DB]) {
+    constexpr uint32_t ES = scaled_type(CT) ? 1 : 2;
+    const uint32_t col = lane & 31, half = lane >> 5;
+    for (uint32_t i = 0; i < 16; ++i)
+        for (uint32_t h = 0; h < 2; ++h) {
+            float p = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) p = i == uint32_t(j) ? s[j] : p;
+            const bool sees = (__shfl(seen, int(col + 32 * h)) >> i) & 1;
+            p = __shfl(p, int(col + 32 * h));
+            const uint32_t r = token_of_reg(i, h);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t byte = (32 * d + 8 * k + 4 * half) * ES;
+                    float x[4];
+                    value4<CT>(vt + r * RB + (((byte / 16) ^ value_swizzle<RB, ES>(r)) << 4) + byte % 16, x);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[d][4 * k + j] = sees ? fmaf(p, x[j], o[d][4 * k + j]) : o[d][4 * k + j];
+                }
+        }
+}
+
 // Output dims e .. e + 3 (or e alone) of a row of a sequence's block.
 __device__ __forceinline__ uint64_t out_at(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row) {
     const uint32_t tok = row / a.group;
@@ -196,8 +256,178 @@ __device__ __forceinline__ void store1(const AttnArgs &a, uint32_t begin, uint32
         static_cast<uint16_t *>(a.out)[at] = uint16_t(a.xtype == kF16 ? pack_f16(x, x) : pack_bf16(x, x));
 }
 
-// v of the lane 32 away.
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// ---- the line of tiles ------------------------------------------------------
+// Every block of ROWS rows of every sequence that the launch serves, with the
+// tiles of TOKENS tokens that its rows may see, once per key/value head: head
+// after head, in each sequence after sequence, block after block, tile after tile.
+// Workgroups take equal parts of the line, so that the load is even whatever the
+// lengths are, and blocks next to each other, which read the same keys, run on one
+// XCD at about the same time.
+
+// Which sequences a launch serves: those of `least` to `most` rows (new tokens *
+// group) per key/value head.
+struct RowRange {
+    uint32_t least, most;
+};
+
+// A block of rows of a sequence: its positions, and its tiles.
+struct RowBlock {
+    uint32_t begin, rows;  // first token row; rows of the sequence (tokens * group)
+    int32_t pos0;          // position of the sequence's first token
+    int32_t first, last;   // positions of the block's first and last row
+    int32_t lo, hi;        // tokens that a row of it may see
+    uint32_t tiles;        // at least 1, so that rows which see nothing are written too
+};
+__device__ __forceinline__ uint32_t seq_row_count(const AttnArgs &a, RowRange rg, uint32_t s, uint32_t *begin) {
+    uint32_t end;
+    seq_rows(a.kv.start, a.kv.n_tokens, s, begin, &end);
+    const uint32_t rows = (end - *begin) * a.group;
+    return rows >= rg.least && rows <= rg.most ? rows : 0;
+}
+template <int ROWS, int TOKENS>
+__device__ __forceinline__ RowBlock row_block(const AttnArgs &a, uint32_t s, uint32_t r0) {
+    RowBlock b;
+    uint32_t end;
+    seq_rows(a.kv.start, a.kv.n_tokens, s, &b.begin, &end);
+    const uint32_t n = end - b.begin;
+    b.rows = n * a.group;
+    // (kept where sums with a few 2^24 do not overflow)
+    const int32_t len = min(a.kv.len[s], int32_t(kMaxPos) - 64);
+    b.pos0 = max(len, 0) - int32_t(n);
+    b.first = b.pos0 + int32_t(r0 / a.group);
+    b.last = b.pos0 + int32_t((min(r0 + ROWS, max(b.rows, 1u)) - 1) / a.group);
+    const uint64_t cap = uint64_t(a.kv.table_pages) * a.kv.page;
+    b.hi = max(0, int32_t(min(int64_t(b.last) + 1, int64_t(min(cap, uint64_t(kMaxPos - 64))))));
+    b.lo = 0;
+    if (a.window != 0 && int64_t(b.first) + 1 > int64_t(a.window))
+        b.lo = min(b.hi, int32_t(int64_t(b.first) + 1 - a.window)) & ~31;
+    b.tiles = max(1u, uint32_t(b.hi - b.lo + TOKENS - 1) / TOKENS);
+    return b;
+}
+
+// A place on the line.
+struct Place {
+    uint32_t seq, r0, kvh, off;  // off: tiles of the block that lie before it
+};
+
+struct LineMisc {
+    uint32_t blocks[512];  // blocks of the sequences up to a thread's last
+    uint64_t waves[8];
+    Place at;
+};
+
+// Inclusive sum over the workgroup's threads, and the sum of all.
+template <class T, int THREADS>
+__device__ __forceinline__ T block_scan(T v, LineMisc &lm, uint32_t tid, T *all) {
+    const uint32_t lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T u = __shfl_up(v, o);
+        if (lane >= uint32_t(o)) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) lm.waves[wave] = v;
+    __syncthreads();
+    T sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < THREADS / 64; ++w) {
+        if (w < wave) v += T(lm.waves[w]);
+        sum += T(lm.waves[w]);
+    }
+    *all = sum;
+    return v;
+}
+
+// This workgroup's part: where it starts and its number of tiles (0: none); *part:
+// that of every workgroup but the last ones, at least min_part.
+template <int ROWS, int TOKENS, int THREADS>
+__device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, uint32_t index, uint32_t parts, uint32_t min_part,
+                                           LineMisc &lm, uint32_t tid, uint64_t *part, uint64_t *left) {
+    const uint32_t per = (a.kv.n_seq + THREADS - 1) / THREADS;
+    const uint32_t s0 = min(tid * per, a.kv.n_seq), s1 = min(s0 + per, a.kv.n_seq);
+    uint32_t mine = 0, begin;
+    for (uint32_t s = s0; s < s1; ++s) mine += (seq_row_count(a, rg, s, &begin) + ROWS - 1) / ROWS;
+    uint32_t n_blocks;
+    lm.blocks[tid] = block_scan<uint32_t, THREADS>(mine, lm, tid, &n_blocks);
+    __syncthreads();
+    // the tiles of this thread's blocks
+    const uint32_t q = (n_blocks + THREADS - 1) / THREADS;
+    const uint32_t f0 = min(tid * q, n_blocks), f1 = min(f0 + q, n_blocks);
+    uint32_t s = 0, r0 = 0;
+    if (f0 < f1) {
+        uint32_t x = 0, y = THREADS - 1;  // the first thread whose sequences reach past block f0
+        while (x < y) {
+            const uint32_t mid = (x + y) / 2;
+            if (lm.blocks[mid] > f0)
+                y = mid;
+            else
+                x = mid + 1;
+        }
+        uint32_t skip = f0 - (x != 0 ? lm.blocks[x - 1] : 0);
+        for (s = x * per;; ++s) {
+            const uint32_t nb = (seq_row_count(a, rg, s, &begin) + ROWS - 1) / ROWS;
+            if (skip < nb) break;
+            skip -= nb;
+        }
+        r0 = skip * ROWS;
+    }
+    auto step = [&](uint32_t &s, uint32_t &r0) {  // to the next block, where there is one
+        r0 += ROWS;
+        if (r0 >= seq_row_count(a, rg, s, &begin)) {
+            r0 = 0;
+            do ++s;
+            while (s < a.kv.n_seq && seq_row_count(a, rg, s, &begin) == 0);
+        }
+    };
+    uint64_t tiles = 0;
+    {
+        uint32_t u = s, v = r0;
+        for (uint32_t f = f0; f < f1; ++f) {
+            tiles += row_block<ROWS, TOKENS>(a, u, v).tiles;
+            if (f + 1 < f1) step(u, v);
+        }
+    }
+    uint64_t per_head;
+    const uint64_t incl = block_scan<uint64_t, THREADS>(tiles, lm, tid, &per_head);
+    const uint64_t total = per_head * a.kv.kv_heads;
+    *part = max((total + parts - 1) / parts, uint64_t(min_part));
+    const uint64_t at = *part * index;
+    *left = at < total ? min(*part, total - at) : 0;
+    if (*left != 0) {
+        const uint32_t kvh = uint32_t(at / per_head);
+        uint64_t target = at - kvh * per_head;
+        if (target >= incl - tiles && target < incl) {
+            target -= incl - tiles;
+            for (;;) {
+                const uint32_t t = row_block<ROWS, TOKENS>(a, s, r0).tiles;
+                if (target < t) break;
+                target -= t;
+                step(s, r0);
+            }
+            lm.at = Place{s, r0, kvh, uint32_t(target)};
+        }
+    }
+    __syncthreads();
+    Place p;
+    p.seq = __builtin_amdgcn_readfirstlane(lm.at.seq);
+    p.r0 = __builtin_amdgcn_readfirstlane(lm.at.r0);
+    p.kvh = __builtin_amdgcn_readfirstlane(lm.at.kvh);
+    p.off = __builtin_amdgcn_readfirstlane(lm.at.off);
+    return p;
+}
+
+// The block of rows behind place p's (p.off = 0). The line does not end there.
+template <int ROWS>
+__device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, uint32_t rows, Place &p) {
+    p.off = 0;
+    p.r0 += ROWS;
+    if (p.r0 < rows) return;
+    p.r0 = 0;
+    uint32_t begin;
+    do {
+        if (++p.seq == a.kv.n_seq) p.seq = 0, ++p.kvh;
+    } while (seq_row_count(a, rg, p.seq, &begin) == 0);
+}
 
 // ---- rows of q --------------------------------------------------------------
 // 32 rows of NP pieces in LDS, [NP][32][DP] 16-bit elements in swizzled chunks, and
@@ -239,6 +469,42 @@ __device__ __forceinline__ void stage_q(const AttnArgs &a, uint32_t begin, uint3
         }
     }
     if (l == 0) factor[r] = ldexpf(1.4426950408889634f * a.scale, e);
+}
+
+// ---- the join ----------------------------------------------------------------
+// Blocks of ROWS rows split over several workgroups: rows [4 y, 4 y + 4) of the
+// block that part x has on the list.
+template <int DP, int ROWS>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, SplitScratch sc) {
+    const SplitJob job = sc.jobs[blockIdx.x];
+    if (job.count == 0) return;
+    uint32_t begin, end;
+    seq_rows(a.kv.start, a.kv.n_tokens, job.seq, &begin, &end);
+    const uint32_t r = 4 * blockIdx.y + threadIdx.x / 64, row = job.r0 + r, lane = threadIdx.x & 63;
+    if (row >= (end - begin) * a.group) return;
+    auto slot = [&](uint32_t i) { return i == 0 ? job.slot : 2 * (blockIdx.x + i); };
+    float top = kNegInf;
+    for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[(slot(i) * ROWS + r) * 2]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    constexpr int N = DP / 64;
+    float x[N], all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = 0.0f;
+#pragma unroll 8
+    for (uint32_t i = 0; i < job.count; ++i) {
+        const uint32_t sl = slot(i);
+        const float m = sc.ml[(sl * ROWS + r) * 2], l = sc.ml[(sl * ROWS + r) * 2 + 1];
+        const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
+        all = fmaf(w, l, all);
+        const float *p = sc.o + (uint64_t(sl) * ROWS + r) * DP + N * lane;
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = fmaf(w, p[k], x[k]);
+    }
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (N * lane + k < a.kv.dim) store1(a, begin, job.kvh, row, N * lane + k, x[k] * inv);
 }
 
 }  // namespace

@@ -2,9 +2,8 @@
 // drafted tokens. HBM-bound: every cached key and value of a head is read once for
 // up to 32 rows.
 //
-// The tiles (32 tokens of one key/value head for one block of 32 rows) of all
-// sequences form one line, which is cut into equal parts, one per workgroup,
-// however long each sequence is. The waves of a workgroup take its tiles in turn,
+// The line of tiles (32 tokens for 32 rows) is cut into equal parts, one per
+// workgroup. The waves of a workgroup take its tiles in turn,
 // each through LDS of its own and without barriers: keys of the next tile are on
 // their way while the values of this one are multiplied, and the other way round.
 // Where a sequence's tiles end or the part does, the waves join their sums. Blocks
@@ -17,30 +16,6 @@
 namespace tc {
 namespace {
 
-// A block of 32 rows of a sequence: its positions, and its tiles.
-struct RowBlock {
-    uint32_t begin, n, rows;  // first token row, tokens, rows (tokens * group)
-    int64_t pos0;             // position of the first token
-    int64_t first, last;      // positions of the block's first and last row
-    int64_t lo, hi;           // tokens it may see
-    uint32_t tiles;           // at least 1
-};
-__device__ __forceinline__ RowBlock row_block(const AttnArgs &a, uint32_t s, uint32_t r0) {
-    RowBlock b;
-    uint32_t end;
-    seq_rows(a.kv.start, a.kv.n_tokens, s, &b.begin, &end);
-    b.n = end - b.begin;
-    b.rows = b.n * a.group;
-    b.pos0 = int64_t(a.kv.len[s]) - b.n;
-    b.first = b.pos0 + r0 / a.group;
-    b.last = b.pos0 + (min(r0 + 32, max(b.rows, 1u)) - 1) / a.group;
-    const int64_t cap = min(int64_t(a.kv.table_pages) * a.kv.page, int64_t(kMaxPos));
-    b.hi = max(int64_t(0), min(b.last + 1, cap));
-    b.lo = a.window != 0 ? max(int64_t(0), min(b.hi, b.first - a.window + 1)) & ~int64_t(31) : 0;
-    b.tiles = max(1u, uint32_t((b.hi - b.lo + 31) / 32));
-    return b;
-}
-
 // Shape of a launch for one cache type, number of pieces and padded head size.
 template <int CT, int NP, int DP>
 struct SplitShape {
@@ -52,7 +27,7 @@ struct SplitShape {
     static constexpr int Q = NP * 32 * 2 * DP;
     static constexpr bool QREG = NP * DP <= 256;  // rows of q in registers (64 of them at most)
     // (the first MISC bytes of LDS hold the small things)
-    static constexpr int MISC = 2560;
+    static constexpr int MISC = 4096;
     static constexpr int NW = MISC + (QREG ? 0 : Q) + 4 * WAVE <= 160 * 1024 ? 4 : 3;
     static constexpr int LDS = MISC + (QREG ? (NW * WAVE > Q ? NW * WAVE : Q) : Q + NW * WAVE);
     // workgroups per CU: what LDS and, at this size of the sums, the registers allow
@@ -63,16 +38,13 @@ struct SplitShape {
 struct SplitMisc {
     float factor[32];
     float m[4][32], l[4][32];
-    uint64_t sums[4];
-    uint64_t total;
-    uint32_t seq, r0, kvh, off;
-    uint32_t pad[4];
+    LineMisc line;
 };
-static_assert(sizeof(SplitMisc) <= 2560, "");
+static_assert(sizeof(SplitMisc) <= 4096, "");
 
 template <int CT, int NP, int DP>
 __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, NP, DP>::OCC)) void k_attn_split(
-    AttnArgs a, SplitScratch sc) {
+    AttnArgs a, RowRange rg, SplitScratch sc) {
     using Sh = SplitShape<CT, NP, DP>;
     constexpr int ES = Sh::ES, RB = Sh::RB, NW = Sh::NW, KS = DP / 16, DB = DP / 32;
     constexpr bool SCALED = scaled_type(CT);
@@ -88,63 +60,14 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
     const uint32_t kvh_n = a.kv.kv_heads, D = a.kv.dim, rowbytes = D * ES, nch = rowbytes / 16;
 
     // ---- this workgroup's part of the line of tiles ----
-    auto cost = [&](uint32_t s) {
-        const RowBlock b0 = row_block(a, s, 0);
-        uint64_t c = 0;
-        for (uint32_t r0 = 0; r0 < b0.rows; r0 += 32) c += row_block(a, s, r0).tiles;
-        return c * kvh_n;
-    };
-    const uint32_t per = (a.kv.n_seq + 64 * NW - 1) / (64 * NW);
-    const uint32_t s0 = min(tid * per, a.kv.n_seq), s1 = min(s0 + per, a.kv.n_seq);
-    uint64_t sum = 0;
-    for (uint32_t s = s0; s < s1; ++s) sum += cost(s);
-    uint64_t incl = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t v = __shfl_up(incl, o);
-        if (lane >= uint32_t(o)) incl += v;
-    }
-    if (lane == 63) ms.sums[wave] = incl;
-    __syncthreads();
-    uint64_t base = 0, total = 0;
-    for (int w = 0; w < NW; ++w) {
-        if (uint32_t(w) < wave) base += ms.sums[w];
-        total += ms.sums[w];
-    }
-    // (a tile for each wave at least)
-    const uint64_t part = max((total + gridDim.x - 1) / gridDim.x, uint64_t(NW));
-    uint64_t at = part * blockIdx.x;
+    uint64_t part, left;
+    Place pl = line_part<32, kTileTokens, 64 * NW>(a, rg, blockIdx.x, gridDim.x, NW, ms.line, tid, &part, &left);
     if (tid == 0) sc.jobs[blockIdx.x].count = 0;
-    if (at >= total) return;
-    uint64_t left = min(part, total - at);
-    uint64_t target = at - (base + incl - sum);
-    if (at >= base + incl - sum && target < sum)
-        for (uint32_t s = s0; s < s1; ++s) {
-            const uint64_t c = cost(s);
-            if (target >= c) {
-                target -= c;
-                continue;
-            }
-            for (uint32_t r0 = 0;; r0 += 32) {
-                const uint64_t t = row_block(a, s, r0).tiles;
-                if (target < t * kvh_n) {
-                    ms.seq = s;
-                    ms.r0 = r0;
-                    ms.kvh = uint32_t(target / t);
-                    ms.off = uint32_t(target % t);
-                    break;
-                }
-                target -= t * kvh_n;
-            }
-            break;
-        }
-    __syncthreads();
-    uint32_t seq = __builtin_amdgcn_readfirstlane(ms.seq), r0 = __builtin_amdgcn_readfirstlane(ms.r0);
-    uint32_t kvh = __builtin_amdgcn_readfirstlane(ms.kvh), off = __builtin_amdgcn_readfirstlane(ms.off);
 
     bool first_seg = true;
     while (left != 0) {
-        const RowBlock b = row_block(a, seq, r0);
+        const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
+        const RowBlock b = row_block<32, kTileTokens>(a, seq, r0);
         const uint32_t seg = uint32_t(min(uint64_t(b.tiles - off), left));
 
         // ---- rows of q ----
@@ -168,8 +91,8 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         if (DP != D)  // dims past the row's: zeros, which no load touches
             for (uint32_t i = lane; i < 2 * Sh::TILE / 16; i += 64) *reinterpret_cast<u32x4 *>(mine + 16 * i) = u32x4{0, 0, 0, 0};
         const uint32_t row = r0 + col;
-        const int64_t pos = row < b.rows ? b.pos0 + row / a.group : -1;  // the lane's row sees tokens up to here
-        const int64_t from = a.window != 0 ? pos - a.window + 1 : 0;
+        const int32_t pos = row < b.rows ? b.pos0 + int32_t(row / a.group) : -1;  // the lane's row sees tokens up to here
+        const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
 
         // ---- tiles ----
         // Cache rows of a tile's two runs of 16 tokens (each in one page), and
@@ -182,7 +105,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             Where w;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const int64_t r = cache_row(a.kv, seq, b.lo + 32 * int64_t(t) + 16 * g, kvh);
+                const int64_t r = cache_row(a.kv, seq, b.lo + 32 * int32_t(t) + 16 * g, kvh);
                 w.held[g] = r >= 0;
                 w.row[g] = r >= 0 ? r : 0;
             }
@@ -292,15 +215,15 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     for (int j = 0; j < 4; ++j) kf[i + j] = x[j], lf[i + j] = y[j], rf[i + j] = z[j];
                 }
             }
-            const int64_t j0 = b.lo + 32 * int64_t(t);
+            const int32_t j0 = b.lo + 32 * int32_t(t);
             // whether every row of the block sees every token of the tile
-            const bool full = now.held[0] && now.held[1] && j0 + 31 <= b.first && (a.window == 0 || j0 > b.last - a.window);
+            const bool full = now.held[0] && now.held[1] && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
             uint32_t seen = 0xFFFF;
             if (!full) {
                 seen = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int64_t j = j0 + token_of_reg(i, half);
+                    const int32_t j = j0 + int32_t(token_of_reg(i, half));
                     if (j <= pos && j >= from && now.held[i / 8]) seen |= 1u << i;
                 }
             }
@@ -341,14 +264,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             else
                 wait_loads<0>();
             bool odd = false;  // values that are not finite where some row must not see them
-            if (CT != kI8 && !full) {
-                uint32_t bad = 0;
-                for (uint32_t i = lane; i < Sh::TILE / 16; i += 64) {
-                    const u32x4 w = *reinterpret_cast<const u32x4 *>(vtile + 16 * i);
-                    bad |= not_finite<CT>(w[0]) | not_finite<CT>(w[1]) | not_finite<CT>(w[2]) | not_finite<CT>(w[3]);
-                }
-                odd = __ballot(bad != 0) != 0;
-            }
+            if (CT != kI8 && !full) odd = tile_not_finite<CT, Sh::TILE>(vtile, lane);
             if (!odd) {
                 // P^T of 16 tokens: the registers as they are
                 u32x4 pw[2][NP];
@@ -360,22 +276,15 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
 #pragma unroll
                         for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<CT>(x, y);
                     }
-                const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         u32x4 v;
                         if constexpr (ES == 2) {
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const uint32_t r = 16 * k + 8 * half + 4 * u + l16 / 4, e = 32 * d + 16 * g16 + 4 * (l16 % 4);
-                                const unsigned char *p = vtile + r * RB + (((e / 8) ^ value_swizzle<RB, ES>(r)) << 4) + (e & 4) * 2;
-                                const u32x2 w = __builtin_bit_cast(
-                                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
-                                v[2 * u] = w[0], v[2 * u + 1] = w[1];
-                            }
+                            v = value_frag<CT, RB>(vtile, d, k, lane);
                         } else {
+                            const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1;
                             const uint32_t r = 16 * k + 8 * half + l16 / 2, e = 32 * d + 16 * g16 + 8 * (l16 % 2);
                             const unsigned char *p = vtile + r * RB + (((e / 16) ^ value_swizzle<RB, ES>(r)) << 4) + (e & 8);
                             const u32x2 w = __builtin_bit_cast(
@@ -387,26 +296,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                         for (int p = NP - 1; p >= 0; --p) o[d] = mfma<CT>(v, pw[k][p], o[d]);
                     }
             } else {
-                // token by token, those that the row sees alone
-                for (uint32_t i = 0; i < 16; ++i)
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        float p = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) p = i == uint32_t(j) ? s[j] : p;
-                        const bool sees = (__shfl(seen, int(col + 32 * h)) >> i) & 1;
-                        p = __shfl(p, int(col + 32 * h));
-                        const uint32_t r = token_of_reg(i, h);
-#pragma unroll
-                        for (int d = 0; d < DB; ++d)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t e = 32 * d + 8 * k + 4 * half, byte = e * ES;
-                                float x[4];
-                                value4<CT>(vtile + r * RB + (((byte / 16) ^ value_swizzle<RB, ES>(r)) << 4) + byte % 16, x);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) o[d][4 * k + j] = sees ? fmaf(p, x[j], o[d][4 * k + j]) : o[d][4 * k + j];
-                            }
-                    }
+                add_values_one_by_one<CT, RB, DB>(vtile, s, seen, lane, o);
             }
             wait_lds();
             if (more) {
@@ -467,60 +357,10 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         if (off == 0 && !whole && tid == 0)
             sc.jobs[blockIdx.x] = SplitJob{seq, r0, kvh, 1 + uint32_t((b.tiles - seg + part - 1) / part), slot};
 
-        // ---- the next block of rows ----
         left -= seg;
         first_seg = false;
-        off = 0;
-        if (++kvh == kvh_n) {
-            kvh = 0;
-            r0 += 32;
-            if (r0 >= b.rows) {
-                r0 = 0;
-                if (left != 0) {
-                    uint32_t x, y;
-                    do {
-                        ++seq;
-                        seq_rows(a.kv.start, a.kv.n_tokens, seq, &x, &y);
-                    } while (x == y);
-                }
-            }
-        }
+        if (left != 0) next_block<32>(a, rg, b.rows, pl);
     }
-}
-
-// Blocks of rows split over several workgroups: rows [4 y, 4 y + 4) of the block
-// that workgroup x has on the list.
-template <int DP>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, SplitScratch sc) {
-    const SplitJob job = sc.jobs[blockIdx.x];
-    if (job.count == 0) return;
-    uint32_t begin, end;
-    seq_rows(a.kv.start, a.kv.n_tokens, job.seq, &begin, &end);
-    const uint32_t r = 4 * blockIdx.y + threadIdx.x / 64, row = job.r0 + r, lane = threadIdx.x & 63;
-    if (row >= (end - begin) * a.group) return;
-    auto slot = [&](uint32_t i) { return i == 0 ? job.slot : 2 * (blockIdx.x + i); };
-    float top = kNegInf;
-    for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[(slot(i) * 32 + r) * 2]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    constexpr int N = DP / 64;
-    float x[N], all = 0.0f;
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = 0.0f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < job.count; ++i) {
-        const uint32_t sl = slot(i);
-        const float m = sc.ml[(sl * 32 + r) * 2], l = sc.ml[(sl * 32 + r) * 2 + 1];
-        const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
-        all = fmaf(w, l, all);
-        const float *p = sc.o + (uint64_t(sl) * 32 + r) * DP + N * lane;
-#pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = fmaf(w, p[k], x[k]);
-    }
-    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-        if (N * lane + k < a.kv.dim) store1(a, begin, job.kvh, row, N * lane + k, x[k] * inv);
 }
 
 }  // namespace

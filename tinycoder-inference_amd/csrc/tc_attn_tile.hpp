@@ -1,0 +1,383 @@
+// tc_attn_tile.hpp -- attention of many rows per key/value head: prompts. Bound by
+// the matrix cores and the exponentials between their products.
+//
+// A workgroup takes 32 rows per wave of one key/value head, which go over its tiles
+// of 32 tokens together: tiles come into LDS two steps ahead (8-bit ones through
+// registers, widened to fp16 once for all waves), rows of q stay in registers. A
+// step's score products belong to the tile behind the one whose weights are being
+// formed, so that a wave's matrix and vector work do not wait for each other. The
+// line of tiles is cut into one part per CU; blocks that a cut goes through leave
+// their sums for k_attn_join.
+#pragma once
+
+#include "tc_attn_kernel.hpp"
+
+namespace tc {
+namespace {
+
+template <int CT, int NP, int DP>
+struct TileShape {
+    static constexpr int LT = CT == kBF16 ? kBF16 : kF16;  // element type in LDS
+    static constexpr int RB = 2 * DP;
+    static constexpr int TILE = kTileTokens * RB;
+    // registers of the sums and of q: beyond 128, one wave per SIMD
+    static constexpr int NW = DP / 2 + NP * DP / 4 > 128 ? 4 : 8;
+    static constexpr int ROWS = 32 * NW;
+    static constexpr int NBUF = 4;
+    static constexpr int MISC = 4096;
+    static constexpr int LDS = MISC + 2 * NBUF * TILE;
+};
+
+struct TileMisc {
+    float kf[4][32], lv[4][32], iv[4][32];  // factors of a tile's keys; log2 and reciprocal of the values'
+    LineMisc line;
+};
+static_assert(sizeof(TileMisc) <= 4096, "");
+
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int CT, int NP, int DP>
+__global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_tile(AttnArgs a, RowRange rg, SplitScratch sc) {
+    using Sh = TileShape<CT, NP, DP>;
+    constexpr int LT = Sh::LT, RB = Sh::RB, NW = Sh::NW, KS = DP / 16, DB = DP / 32, TILE = Sh::TILE, NBUF = Sh::NBUF;
+    constexpr int THREADS = 64 * NW;
+    constexpr bool SCALED = scaled_type(CT);
+    extern __shared__ __align__(1024) unsigned char lds[];
+    TileMisc &ms = *reinterpret_cast<TileMisc *>(lds);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31, half = lane >> 5;
+    unsigned char *const kbuf = lds + Sh::MISC, *const vbuf = kbuf + NBUF * TILE;
+    const uint32_t D = a.kv.dim, rowbytes = D * (SCALED ? 1 : 2);
+
+    // workgroups of one XCD (every eighth) take parts next to each other
+    const uint32_t n_parts = gridDim.x, eighth = n_parts / 8;
+    const uint32_t index = n_parts % 8 == 0 ? blockIdx.x % 8 * eighth + blockIdx.x / 8 : blockIdx.x;
+    uint64_t part, left;
+    Place pl = line_part<Sh::ROWS, kTileTokens, THREADS>(a, rg, index, n_parts, 4, ms.line, tid, &part, &left);
+    if (tid == 0) sc.jobs[index].count = 0;
+
+    bool first_seg = true;
+    while (left != 0) {
+        const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
+        const RowBlock b = row_block<Sh::ROWS, kTileTokens>(a, seq, r0);
+        const uint32_t seg = uint32_t(min(uint64_t(b.tiles - off), left));
+        const uint32_t t0 = off, t1 = off + seg;
+
+        // ---- the wave's rows of q ----
+        const uint32_t wr0 = r0 + 32 * wave, row = wr0 + col;
+        const bool active = wr0 < b.rows;  // the wave has rows
+        const uint32_t tok = row / a.group;
+        const int32_t pos = row < b.rows ? b.pos0 + int32_t(tok) : -1;  // the lane's row sees tokens up to here
+        const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
+        const int32_t wfirst = b.pos0 + int32_t(wr0 / a.group);
+        const int32_t wlast = b.pos0 + int32_t((min(wr0 + 32, b.rows) - 1) / a.group);
+        u32x4 q[NP][KS];
+        float factor = 1.4426950408889634f * a.scale;
+        {
+            float x[KS][8], mx = 0.0f;
+            const uint64_t at =
+                uint64_t(b.begin + tok) * a.q_stride + uint64_t(kvh * a.group + row - tok * a.group) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t d = 16 * ks + 8 * half;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
+                if (row < b.rows && d < D) load8(a.xtype, a.q, at + d, x[ks]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+            }
+            const int e = row_exponent<CT>(fmaxf(mx, other_half(mx)));
+            factor = ldexpf(factor, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (CT != kBF16)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[ks][i] = ldexpf(x[ks][i], -e);
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) q[p][ks][i] = piece2<CT>(x[ks][2 * i], x[ks][2 * i + 1]);
+            }
+        }
+        __syncthreads();  // (the last block's tiles are no longer read)
+        if (DP != D) {  // dims past the row's: zeros, which no load touches
+            for (uint32_t i = tid; i < uint32_t(2 * NBUF * TILE / 16); i += THREADS)
+                *reinterpret_cast<u32x4 *>(kbuf + 16 * i) = u32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
+
+        // ---- tiles into LDS ----
+        // Runs of 16 tokens lie in one page each; where none holds one, page 0 is
+        // read instead. Bit 2 i + g of `held`: run g of the tile i steps from now.
+        uint32_t held = 0;
+        constexpr int LPR = RB / 16, RPI = 64 / LPR, LOADS = kTileTokens / RPI;  // direct loads of keys or values
+        constexpr int MINE = 2 * LOADS / NW;                                   // a wave's
+        static_assert(2 * LOADS % NW == 0, "");
+        constexpr uint32_t CHUNKS = 2 * kTileTokens * DP / 16;  // 16-byte loads of a tile, 8-bit types
+        constexpr int RAW = SCALED ? (CHUNKS + THREADS - 1) / THREADS : 1;  // a thread's
+        static_assert(CHUNKS < THREADS || CHUNKS % THREADS == 0, "");
+        u32x4 raw[RAW];
+        float raw_scale = 0.0f;
+        auto run_row = [&](uint32_t t, uint32_t g, uint32_t *ok) __attribute__((always_inline)) {
+            const int64_t r = cache_row(a.kv, seq, b.lo + 32 * int32_t(t) + 16 * int32_t(g), kvh);
+            *ok |= r >= 0 ? 1u << g : 0u;
+            return r >= 0 ? r : int64_t(0);
+        };
+        auto load = [&](uint32_t t, uint32_t ahead) __attribute__((always_inline)) {
+            uint32_t ok = 0;
+            const int64_t run[2] = {run_row(t, 0, &ok), run_row(t, 1, &ok)};
+            held |= ok << (2 * ahead);
+            const uint32_t buf = (t - t0) % NBUF;
+            if constexpr (!SCALED) {
+#pragma unroll
+                for (int j = 0; j < MINE; ++j) {
+                    const uint32_t f = wave + NW * j;
+                    const bool val = f >= uint32_t(LOADS);
+                    const uint32_t i = val ? f - LOADS : f, g = i * RPI / 16, rg = i * RPI % 16 + lane / LPR;
+                    const uint32_t r = 16 * g + rg;
+                    const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<RB, 2>(r) : key_swizzle<RB>(r));
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + (g != 0 ? run[1] : run[0]) * rowbytes;
+                    unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + i * 1024;
+                    if (DP == D || 16 * c < rowbytes) dma16(lds_addr(dst), src, rg * rowbytes + 16 * c);
+                }
+            } else {
+                // 16 bytes (16 dims) of one row per load: THREADS / (DP / 16) rows at a time, keys then values
+#pragma unroll
+                for (int j = 0; j < RAW; ++j) {
+                    const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
+                    const bool val = rr >= kTileTokens;
+                    const uint32_t r = rr % kTileTokens;
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + ((r >= 16 ? run[1] : run[0]) + r % 16) * rowbytes;
+                    raw[j] = u32x4{0, 0, 0, 0};
+                    if ((CHUNKS >= THREADS || f < CHUNKS) && (DP == D || 16 * c < rowbytes)) raw[j] = *reinterpret_cast<const u32x4 *>(src + 16 * c);
+                }
+                if (tid < 64) raw_scale = (half ? a.kv.vs : a.kv.ks)[(col >= 16 ? run[1] : run[0]) + col % 16];
+            }
+        };
+        // (8-bit types) what load() fetched, widened, into its tile
+        auto put = [&](uint32_t t) __attribute__((always_inline)) {
+            const uint32_t buf = (t - t0) % NBUF;
+#pragma unroll
+            for (int j = 0; j < RAW; ++j) {
+                const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
+                if (CHUNKS < THREADS && f >= CHUNKS) break;
+                const bool val = rr >= kTileTokens;
+                const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<RB, 2>(r) : key_swizzle<RB>(r);
+                unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + r * RB;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const u32x2 x = widen<CT>(raw[j][2 * e]), y = widen<CT>(raw[j][2 * e + 1]);
+                    *reinterpret_cast<u32x4 *>(dst + (((2 * c + e) ^ sw) << 4)) = u32x4{x[0], x[1], y[0], y[1]};
+                }
+            }
+            if (tid < 64) {
+                if (half == 0) {
+                    ms.kf[buf][col] = raw_scale;
+                } else {
+                    // (a factor of 0: values of next to nothing; NaN stays)
+                    const float x = raw_scale == raw_scale ? fmaxf(raw_scale, 0x1p-126f) : raw_scale;
+                    ms.lv[buf][col] = __builtin_amdgcn_logf(x);
+                    ms.iv[buf][col] = __builtin_amdgcn_rcpf(x);
+                }
+            }
+        };
+
+        v16f o[DB], s;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+        float m = kNegInf, l = 0.0f, tmax = kNegInf;
+        uint32_t seen = 0xFFFF;
+
+        auto key = [&](uint32_t t, int ks) __attribute__((always_inline)) {
+            const uint32_t r = token_of_row(col);
+            return *reinterpret_cast<const u32x4 *>(kbuf + (t - t0) % NBUF * TILE + r * RB +
+                                                    (((2 * ks + half) ^ key_swizzle<RB>(r)) << 4));
+        };
+        // whether some row of the wave sees a token of tile t, and whether all see all
+        auto any_seen = [&](uint32_t t) {
+            const int32_t j0 = b.lo + 32 * int32_t(t);
+            return active && j0 <= wlast && (a.window == 0 || int64_t(j0) + 31 + a.window > int64_t(wfirst));
+        };
+        // scores to exponents of 2, unseen ones to -inf, and their maximum
+        auto finish_scores = [&](uint32_t t, uint32_t ok, v16f &x) __attribute__((always_inline)) {
+            const int32_t j0 = b.lo + 32 * int32_t(t);
+            const bool full = ok == 3 && j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
+            seen = 0xFFFF;
+            if (!full) {
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int32_t j = j0 + int32_t(token_of_reg(i, half));
+                    if (j <= pos && j >= from && (ok >> (i / 8)) & 1) seen |= 1u << i;
+                }
+            }
+            if constexpr (SCALED) {
+                const uint32_t buf = (t - t0) % NBUF;
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg(i, half));
+                    const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg(i, half));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] *= factor;
+            }
+            if (!full)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = (seen >> i) & 1 ? x[i] : kNegInf;
+            float y = x[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) y = fmaxf(y, x[i]);
+            tmax = fmaxf(y, other_half(y));
+        };
+
+        // ---- the first tiles ----
+        load(t0, 0);
+        if constexpr (SCALED) put(t0);
+        if (t0 + 1 < t1) {
+            load(t0 + 1, 1);
+            if constexpr (SCALED) put(t0 + 1);
+        }
+        if (t0 + 2 < t1) load(t0 + 2, 2);
+        if constexpr (!SCALED) wait_loads<0>();
+        tile_barrier();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+        if (any_seen(t0)) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 k = key(t0, ks);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) s = mfma<LT>(k, q[p][ks], s);
+            }
+            finish_scores(t0, held & 3, s);
+        }
+
+        for (uint32_t t = t0; t < t1; ++t) {
+            // tile t + 1 is in LDS once every wave is here
+            if constexpr (!SCALED) {
+                if (t + 2 < t1)
+                    wait_loads<MINE>();
+                else
+                    wait_loads<0>();
+            }
+            tile_barrier();
+            if constexpr (SCALED)
+                if (t + 2 < t1) put(t + 2);
+            if (t + 3 < t1) load(t + 3, 3);
+
+            const bool now = any_seen(t), more = t + 1 < t1 && any_seen(t + 1);
+            v16f sn;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
+            if (now && __ballot(tmax > m + kLazy) != 0) {
+                const float up = tmax > m + kLazy ? tmax : m;
+                const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= al;
+            }
+            const float ref = (m == kNegInf ? 0.0f : m) - kLift;
+            // next scores, and this tile's weights in between
+            if (more) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const u32x4 k = key(t + 1, ks);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) sn = mfma<LT>(k, q[p][ks], sn);
+                }
+            }
+            if (now) {
+                if constexpr (SCALED) {
+                    const uint32_t buf = (t - t0) % NBUF;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg(i, half));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = __builtin_amdgcn_exp2f(s[i + j] - ref);
+                            s[i + j] = p;
+                            l += (seen >> (i + j)) & 1 ? p * rf[j] : 0.0f;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+                        l += s[i];
+                    }
+                }
+                const unsigned char *vt = vbuf + (t - t0) % NBUF * TILE;
+                bool odd = false;  // values that are not finite where some row must not see them
+                if (CT != kI8 && __ballot(seen != 0xFFFF) != 0) odd = tile_not_finite<LT, TILE>(vt, lane);
+                if (!odd) {
+                    u32x4 pw[2][NP];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
+#pragma unroll
+                            for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
+                        }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            const u32x4 v = value_frag<LT, RB>(vt, d, k, lane);
+#pragma unroll
+                            for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
+                        }
+                } else {
+                    add_values_one_by_one<LT, RB, DB>(vt, s, seen, lane, o);
+                }
+            }
+            held >>= 2;
+            if (more) finish_scores(t + 1, held & 3, sn);
+            s = sn;
+        }
+
+        // ---- the sums ----
+        l += other_half(l);
+        const bool whole = off == 0 && seg == b.tiles;
+        const uint32_t slot = 2 * index + (first_seg ? 0 : 1);
+        if (row < b.rows) {
+            if (whole) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t e = 32 * d + 8 * k + 4 * half;
+                        const f32x4 x = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+                        if (e < D) store4(a, b.begin, kvh, row, e, x * inv);
+                    }
+            } else {
+                const uint64_t at = uint64_t(slot) * Sh::ROWS + row - r0;
+                if (half == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<f32x4 *>(sc.o + at * DP + 32 * d + 8 * k + 4 * half) =
+                            f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+            }
+        }
+        // this workgroup has the block's first tiles but not its last: the join is on its list
+        if (off == 0 && !whole && tid == 0)
+            sc.jobs[index] = SplitJob{seq, r0, kvh, 1 + uint32_t((b.tiles - seg + part - 1) / part), slot};
+        left -= seg;
+        first_seg = false;
+        if (left != 0) next_block<Sh::ROWS>(a, rg, b.rows, pl);
+    }
+}
+
+}  // namespace
+}  // namespace tc
