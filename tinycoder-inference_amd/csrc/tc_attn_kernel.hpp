@@ -173,24 +173,63 @@ __device__ __forceinline__ void value4(const unsigned char *p, float (&x)[4]) {
     }
 }
 
-// v of the lane 32 away.
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// The two halves' values of a lane's column: in both halves the lower's and the
+// upper's.
+__device__ __forceinline__ f32x2 both_halves(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return f32x2{__builtin_bit_cast(float, uint32_t(r[0])), __builtin_bit_cast(float, uint32_t(r[1]))};
+}
+__device__ __forceinline__ float halves_max(float v) {
+    const f32x2 h = both_halves(v);
+    return fmaxf(h[0], h[1]);
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const f32x2 h = both_halves(v);
+    return h[0] + h[1];
+}
+
+// (fmaxf would first quiet its operands, an instruction each)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max16(const v16f &x) {
+    const float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]), c = max3(x[6], x[7], x[8]);
+    const float d = max3(x[9], x[10], x[11]), e = max3(x[12], x[13], x[14]);
+    return max3(max3(a, b, c), max3(d, e, x[15]), x[15]);
+}
+
+// 16 bytes of LDS at an address of lds_addr's.
+typedef const __attribute__((address_space(3))) u32x4 *lds_u32x4;
+__device__ __forceinline__ u32x4 lds_at(uint32_t addr) { return *reinterpret_cast<lds_u32x4>(addr); }
+__device__ __forceinline__ u32x2 lds_transposed16(uint32_t addr) {
+    return __builtin_bit_cast(u32x2,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4 *>(addr)));
+}
 
 // Operand of o^T += V^T P^T for dims 32 d + 0 .. 31 and tokens 16 k + 0 .. 15 of a
-// 16-bit tile in LDS.
-template <int LT, int RB>
-__device__ __forceinline__ u32x4 value_frag(const unsigned char *vt, uint32_t d, uint32_t k, uint32_t lane) {
+// 16-bit tile at LDS address vt. The lane's place depends on d alone (the rows 16 k
+// + 8 half + 4 u + l16 / 4 are alike in the bits that the swizzle takes), so a loop
+// holds one register per d.
+template <int RB>
+__device__ __forceinline__ uint32_t value_place(uint32_t d, uint32_t lane) {
     const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1, half = lane >> 5;
-    u32x4 v;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const uint32_t r = 16 * k + 8 * half + 4 * u + l16 / 4, e = 32 * d + 16 * g16 + 4 * (l16 % 4);
-        const unsigned char *p = vt + r * RB + (((e / 8) ^ value_swizzle<RB, 2>(r)) << 4) + (e & 4) * 2;
-        const u32x2 w =
-            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
-        v[2 * u] = w[0], v[2 * u + 1] = w[1];
-    }
-    return v;
+    const uint32_t r = 8 * half + l16 / 4, e = 32 * d + 16 * g16 + 4 * (l16 % 4);
+    return r * RB + (((e / 8) ^ value_swizzle<RB, 2>(r)) << 4) + (e & 4) * 2;
+}
+template <int RB>
+__device__ __forceinline__ u32x4 value_frag(uint32_t vt_place, uint32_t k) {
+    const u32x2 a = lds_transposed16(vt_place + 16 * k * RB), b = lds_transposed16(vt_place + (16 * k + 4) * RB);
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+// ... and of scores = K Q^T for contraction step ks: the keys' place for step 0,
+// which step ks changes by an exclusive or.
+template <int RB>
+__device__ __forceinline__ uint32_t key_place(uint32_t lane) {
+    const uint32_t r = token_of_row(lane & 31);
+    return r * RB + (((lane >> 5) ^ key_swizzle<RB>(r)) << 4);
 }
 
 // Whether a tile in LDS holds a value that is not finite.

@@ -227,16 +227,15 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     if (j <= pos && j >= from && now.held[i / 8]) seen |= 1u << i;
                 }
             }
-            float tmax = kNegInf;
+            float tmax;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float x = s[i] * factor;
                 if constexpr (SCALED) x = fmaf(x, kf[i], lf[i]);
                 if (!full) x = (seen >> i) & 1 ? x : kNegInf;
                 s[i] = x;
-                tmax = fmaxf(tmax, x);
             }
-            tmax = fmaxf(tmax, other_half(tmax));
+            tmax = halves_max(max16(s));
             if (__ballot(tmax > m + kLazy) != 0) {
                 const float up = tmax > m + kLazy ? tmax : m;
                 const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
@@ -282,7 +281,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     for (int k = 0; k < 2; ++k) {
                         u32x4 v;
                         if constexpr (ES == 2) {
-                            v = value_frag<CT, RB>(vtile, d, k, lane);
+                            v = value_frag<RB>(lds_addr(vtile) + value_place<RB>(d, lane), k);
                         } else {
                             const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1;
                             const uint32_t r = 16 * k + 8 * half + l16 / 2, e = 32 * d + 16 * g16 + 8 * (l16 % 2);
@@ -307,7 +306,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         }
 
         // ---- the waves' sums joined ----
-        l += other_half(l);
+        l = halves_sum(l);
         if (half == 0) ms.m[wave][col] = m, ms.l[wave][col] = l;
         __syncthreads();
         float top = kNegInf, all = 0.0f;

@@ -10,6 +10,8 @@
 // their sums for k_attn_join.
 #pragma once
 
+#include <type_traits>
+
 #include "tc_attn_kernel.hpp"
 
 namespace tc {
@@ -86,8 +88,9 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
 #pragma unroll
                 for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
             }
-            const int e = row_exponent<CT>(fmaxf(mx, other_half(mx)));
-            factor = ldexpf(factor, e);
+            const int e = row_exponent<CT>(halves_max(mx));
+            // (not 0: times an unseen score, -inf, it stays that)
+            factor = fmaxf(ldexpf(factor, e), 0x1p-126f);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if constexpr (CT != kBF16)
@@ -190,49 +193,66 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         float m = kNegInf, l = 0.0f, tmax = kNegInf;
         uint32_t seen = 0xFFFF;
 
-        auto key = [&](uint32_t t, int ks) __attribute__((always_inline)) {
-            const uint32_t r = token_of_row(col);
-            return *reinterpret_cast<const u32x4 *>(kbuf + (t - t0) % NBUF * TILE + r * RB +
-                                                    (((2 * ks + half) ^ key_swizzle<RB>(r)) << 4));
-        };
+        const uint32_t kplace = lds_addr(kbuf) + key_place<RB>(lane);
+        uint32_t vplace[DB];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<RB>(d, lane);
+        auto key = [&](uint32_t buf, int ks) __attribute__((always_inline)) { return lds_at((kplace ^ (32 * ks)) + buf * TILE); };
         // whether some row of the wave sees a token of tile t, and whether all see all
         auto any_seen = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
             return active && j0 <= wlast && (a.window == 0 || int64_t(j0) + 31 + a.window > int64_t(wfirst));
         };
-        // scores to exponents of 2, unseen ones to -inf, and their maximum
+        // Scores as they come from the matrix cores to what the weights are formed
+        // from: as they are (times `factor` later), or with a token's factors the
+        // exponents of 2 already; unseen ones to -inf; and the largest exponent.
+        auto token_factors = [&](uint32_t buf, v16f &x) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg(i, half));
+                const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg(i, half));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
+            }
+        };
+        auto largest = [&](const v16f &x) __attribute__((always_inline)) {
+            const float y = halves_max(max16(x));
+            return SCALED ? y : y * factor;
+        };
+        auto full_tile = [&](uint32_t t) {
+            const int32_t j0 = b.lo + 32 * int32_t(t);
+            return j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
+        };
         auto finish_scores = [&](uint32_t t, uint32_t ok, v16f &x) __attribute__((always_inline)) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
-            const bool full = ok == 3 && j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
             seen = 0xFFFF;
-            if (!full) {
+            if constexpr (SCALED) token_factors((t - t0) % NBUF, x);
+            if (ok != 3 || !full_tile(t)) {
                 seen = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int32_t j = j0 + int32_t(token_of_reg(i, half));
                     if (j <= pos && j >= from && (ok >> (i / 8)) & 1) seen |= 1u << i;
+                    x[i] = (seen >> i) & 1 ? x[i] : kNegInf;
                 }
             }
-            if constexpr (SCALED) {
-                const uint32_t buf = (t - t0) % NBUF;
+            tmax = largest(x);
+        };
+        auto raise = [&]() __attribute__((always_inline)) {
+            if (__ballot(tmax > m + kLazy) != 0) {
+                const float up = tmax > m + kLazy ? tmax : m;
+                const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= al;
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg(i, half));
-                    const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg(i, half));
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] *= factor;
+                    for (int i = 0; i < 16; ++i) o[d][i] *= al;
             }
-            if (!full)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = (seen >> i) & 1 ? x[i] : kNegInf;
-            float y = x[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) y = fmaxf(y, x[i]);
-            tmax = fmaxf(y, other_half(y));
+        };
+        // the weight of a score
+        auto exponential = [&](float x, float ref) __attribute__((always_inline)) {
+            return __builtin_amdgcn_exp2f(SCALED ? x - ref : fmaf(x, factor, -ref));
         };
 
         // ---- the first tiles ----
@@ -250,14 +270,87 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         if (any_seen(t0)) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 k = key(t0, ks);
+                const u32x4 k = key(0, ks);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p) s = mfma<LT>(k, q[p][ks], s);
             }
             finish_scores(t0, held & 3, s);
         }
 
-        for (uint32_t t = t0; t < t1; ++t) {
+        // Four tiles at a time, each in its own buffer, so that no address is formed in
+        // the loop, as long as every row of the wave sees all of them and the one behind.
+        // A tile's score products are issued among the weights of the one before, its
+        // value products among the maxima of the one behind.
+        auto fast = [&](auto buf_c, uint32_t t, v16f &s, v16f &sn) __attribute__((always_inline)) {
+            constexpr uint32_t buf = decltype(buf_c)::value, nbuf = (buf + 1) % NBUF;
+            if constexpr (!SCALED) wait_loads<MINE>();
+            tile_barrier();
+            if constexpr (SCALED) put(t + 2);
+            load(t + 3, 3);
+            raise();
+            const float ref = (m == kNegInf ? 0.0f : m) - kLift;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 k = key(nbuf, ks);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) sn = mfma<LT>(k, q[p][ks], sn);
+            }
+            u32x4 pw[2][NP];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = exponential(s[i], ref);
+            if constexpr (SCALED) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg(i, half));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) l = fmaf(s[i + j], rf[j], l);
+                }
+            } else {
+                l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) + ((s[8] + s[9]) + (s[10] + s[11])) +
+                     ((s[12] + s[13]) + (s[14] + s[15]));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
+                }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
+                }
+            held >>= 2;
+            if constexpr (SCALED) token_factors(nbuf, sn);
+            tmax = largest(sn);
+        };
+
+        for (uint32_t t = t0; t < t1;) {
+            if (active && (t - t0) % NBUF == 0 && t + 6 < t1 && full_tile(t) && full_tile(t + 4) && (held & 63) == 63) {
+                uint32_t ok = 0;
+                run_row(t + 3, 0, &ok);
+                run_row(t + 3, 1, &ok);
+                uint32_t ok4 = 0;
+                run_row(t + 4, 0, &ok4);
+                run_row(t + 4, 1, &ok4);
+                if ((ok & ok4) == 3) {
+                    v16f sn;
+                    seen = 0xFFFF;
+                    fast(std::integral_constant<uint32_t, 0>{}, t, s, sn);
+                    fast(std::integral_constant<uint32_t, 1>{}, t + 1, sn, s);
+                    fast(std::integral_constant<uint32_t, 2>{}, t + 2, s, sn);
+                    fast(std::integral_constant<uint32_t, 3>{}, t + 3, sn, s);
+                    t += 4;
+                    continue;
+                }
+            }
             // tile t + 1 is in LDS once every wave is here
             if constexpr (!SCALED) {
                 if (t + 2 < t1)
@@ -270,53 +363,19 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 if (t + 2 < t1) put(t + 2);
             if (t + 3 < t1) load(t + 3, 3);
 
-            const bool now = any_seen(t), more = t + 1 < t1 && any_seen(t + 1);
-            v16f sn;
+            const uint32_t buf = (t - t0) % NBUF;
+            if (any_seen(t)) {
+                raise();
+                const float ref = (m == kNegInf ? 0.0f : m) - kLift;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
-            if (now && __ballot(tmax > m + kLazy) != 0) {
-                const float up = tmax > m + kLazy ? tmax : m;
-                const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
-                m = up;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= al;
-            }
-            const float ref = (m == kNegInf ? 0.0f : m) - kLift;
-            // next scores, and this tile's weights in between
-            if (more) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const u32x4 k = key(t + 1, ks);
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; --p) sn = mfma<LT>(k, q[p][ks], sn);
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = exponential(s[i], ref);
+                    // (the factor of a token that is not seen may be anything)
+                    const float p = SCALED ? s[i] * ms.iv[buf][token_of_reg(i, half)] : s[i];
+                    l += (seen >> i) & 1 ? p : 0.0f;
                 }
-            }
-            if (now) {
-                if constexpr (SCALED) {
-                    const uint32_t buf = (t - t0) % NBUF;
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg(i, half));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(s[i + j] - ref);
-                            s[i + j] = p;
-                            l += (seen >> (i + j)) & 1 ? p * rf[j] : 0.0f;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-                        l += s[i];
-                    }
-                }
-                const unsigned char *vt = vbuf + (t - t0) % NBUF * TILE;
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && __ballot(seen != 0xFFFF) != 0) odd = tile_not_finite<LT, TILE>(vt, lane);
+                if (CT != kI8 && __ballot(seen != 0xFFFF) != 0) odd = tile_not_finite<LT, TILE>(vbuf + buf * TILE, lane);
                 if (!odd) {
                     u32x4 pw[2][NP];
 #pragma unroll
@@ -331,21 +390,31 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
                         for (int d = 0; d < DB; ++d) {
-                            const u32x4 v = value_frag<LT, RB>(vt, d, k, lane);
+                            const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
 #pragma unroll
                             for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
                         }
                 } else {
-                    add_values_one_by_one<LT, RB, DB>(vt, s, seen, lane, o);
+                    add_values_one_by_one<LT, RB, DB>(vbuf + buf * TILE, s, seen, lane, o);
                 }
             }
             held >>= 2;
-            if (more) finish_scores(t + 1, held & 3, sn);
-            s = sn;
+            if (t + 1 < t1 && any_seen(t + 1)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const u32x4 k = key((buf + 1) % NBUF, ks);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) s = mfma<LT>(k, q[p][ks], s);
+                }
+                finish_scores(t + 1, held & 3, s);
+            }
+            ++t;
         }
 
         // ---- the sums ----
-        l += other_half(l);
+        l = halves_sum(l);
         const bool whole = off == 0 && seg == b.tiles;
         const uint32_t slot = 2 * index + (first_seg ? 0 : 1);
         if (row < b.rows) {
