@@ -40,6 +40,10 @@ int kv_args(const tc_kv_cache *c, const tc_kv_batch *b, int xtype, tc::KvArgs *a
     if (uint64_t(b->n_tokens) * 2 * c->kv_heads * 32 >= (uint64_t(1) << 39) ||
         uint64_t(b->n_tokens) * 2 * c->kv_heads >= (uint64_t(1) << 31))
         return refuse(TC_E_UNSUPPORTED, "too many rows");
+    // (runs of 16 rows are numbered in 32 bits)
+    if (uint64_t(c->n_pages) * c->kv_heads > (uint64_t(1) << 48) / c->page_tokens ||
+        uint64_t(c->n_pages) * c->kv_heads * (c->page_tokens / 16) >= 0xFFFFFFFFu)
+        return refuse(TC_E_UNSUPPORTED, "2^36 cache rows or more");
     for (const void *p : {c->k, c->v})
         if (!aligned16(p)) return refuse(TC_E_UNSUPPORTED, "the cache must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) |

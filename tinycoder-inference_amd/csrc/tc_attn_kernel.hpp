@@ -468,6 +468,45 @@ __device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, uint3
     } while (seq_row_count(a, rg, p.seq, &begin) == 0);
 }
 
+// ---- pages --------------------------------------------------------------------
+// The cache rows of a stretch of tiles in LDS: for each run of 16 tokens, which lies
+// in one page, its first cache row / 16 (kNoRun where no page holds it), looked up by
+// all threads at once. (Looked up tile by tile, the chain of scalar loads took two
+// thirds of the prompt kernel's step.)
+constexpr uint32_t kNoRun = 0xFFFFFFFFu;
+constexpr uint32_t kStretch = 512;  // tiles
+struct RunMisc {
+    uint32_t run[2 * kStretch];
+    uint32_t missing;  // whether a run with tokens to be seen is not held (set to 0 a barrier earlier)
+};
+// For the tiles from position pos on (a multiple of 16), up to position hi.
+template <int THREADS>
+__device__ __forceinline__ void find_runs(const AttnArgs &a, uint32_t seq, uint32_t kvh, int32_t pos, int32_t hi, uint32_t tiles,
+                                          RunMisc &rm, uint32_t tid) {
+    for (uint32_t i = tid; i < 2 * tiles; i += THREADS) {
+        const int32_t p = pos + 16 * int32_t(i);
+        const uint32_t pi = div_fast(uint32_t(p), a.kv.page_div);
+        const int32_t pg = page_at(a.kv, seq, pi);
+        const uint32_t per = a.kv.page / 16;
+        rm.run[i] = pg < 0 ? kNoRun : (uint32_t(pg) * a.kv.kv_heads + kvh) * per + (uint32_t(p) / 16 - pi * per);
+        if (pg < 0 && p < hi) rm.missing = 1;
+    }
+}
+// The two runs of a tile, wave-uniform, and which are held; run 0 takes a missing
+// one's place in the loads.
+struct TileRuns {
+    uint32_t run[2];
+    uint32_t held;  // bit g: run g
+};
+__device__ __forceinline__ TileRuns tile_runs(const RunMisc &rm, uint32_t t) {
+    const uint32_t x = __builtin_amdgcn_readfirstlane(rm.run[2 * t]), y = __builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]);
+    TileRuns r;
+    r.held = (x != kNoRun ? 1u : 0u) | (y != kNoRun ? 2u : 0u);
+    r.run[0] = x != kNoRun ? x : 0;
+    r.run[1] = y != kNoRun ? y : 0;
+    return r;
+}
+
 // ---- rows of q --------------------------------------------------------------
 // 32 rows of NP pieces in LDS, [NP][32][DP] 16-bit elements in swizzled chunks, and
 // each row's factor log2(e) * scale * 2^e. Row r is query head (r0 + r) % group of

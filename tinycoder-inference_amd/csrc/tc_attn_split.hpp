@@ -27,7 +27,7 @@ struct SplitShape {
     static constexpr int Q = NP * 32 * 2 * DP;
     static constexpr bool QREG = NP * DP <= 256;  // rows of q in registers (64 of them at most)
     // (the first MISC bytes of LDS hold the small things)
-    static constexpr int MISC = 4096;
+    static constexpr int MISC = 8192;
     static constexpr int NW = MISC + (QREG ? 0 : Q) + 4 * WAVE <= 160 * 1024 ? 4 : 3;
     static constexpr int LDS = MISC + (QREG ? (NW * WAVE > Q ? NW * WAVE : Q) : Q + NW * WAVE);
     // workgroups per CU: what LDS and, at this size of the sums, the registers allow
@@ -39,8 +39,9 @@ struct SplitMisc {
     float factor[32];
     float m[4][32], l[4][32];
     LineMisc line;
+    RunMisc runs;
 };
-static_assert(sizeof(SplitMisc) <= 4096, "");
+static_assert(sizeof(SplitMisc) <= 8192, "");
 
 template <int CT, int NP, int DP>
 __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, NP, DP>::OCC)) void k_attn_split(
@@ -95,28 +96,13 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
 
         // ---- tiles ----
-        // Cache rows of a tile's two runs of 16 tokens (each in one page), and
-        // whether pages hold them; where none does, page 0 is read instead.
-        struct Where {
-            int64_t row[2];
-            bool held[2];
-        };
-        auto where = [&](uint32_t t) __attribute__((always_inline)) {
-            Where w;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int64_t r = cache_row(a.kv, seq, b.lo + 32 * int32_t(t) + 16 * g, kvh);
-                w.held[g] = r >= 0;
-                w.row[g] = r >= 0 ? r : 0;
-            }
-            return w;
-        };
+        const uint32_t run_bytes = 16 * rowbytes;
         constexpr int LPR = RB / 16, RPI = 64 / LPR;  // lanes per row, rows per load
         constexpr int LOADS = 2 * (16 / RPI);         // loads of a tile of keys or values
-        auto load = [&](unsigned char *dst, const uint8_t *src, const Where &w, auto swizzle) __attribute__((always_inline)) {
+        auto load = [&](unsigned char *dst, const uint8_t *src, const TileRuns &w, auto swizzle) __attribute__((always_inline)) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const uint8_t *from = src + w.row[g] * rowbytes;
+                const uint8_t *from = src + uint64_t(w.run[g]) * run_bytes;
 #pragma unroll
                 for (int j = 0; j < 16 / RPI; ++j) {
                     const uint32_t r = j * RPI + lane / LPR, c = (lane % LPR) ^ swizzle(16 * g + r);
@@ -124,17 +110,15 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 }
             }
         };
-        auto load_k = [&](const Where &w) __attribute__((always_inline)) {
+        auto load_k = [&](const TileRuns &w) __attribute__((always_inline)) {
             load(ktile, a.kv.k, w, key_swizzle<RB>);
         };
-        auto load_v = [&](const Where &w) __attribute__((always_inline)) {
+        auto load_v = [&](const TileRuns &w) __attribute__((always_inline)) {
             load(vtile, a.kv.v, w, value_swizzle<RB, ES>);
         };
         // lanes 0-31 the keys' factors of the 32 tokens, the others the values'
-        auto load_scales = [&](const Where &w) __attribute__((always_inline)) {
-            const int64_t r = (col >> 4 ? w.row[1] : w.row[0]) + (col & 15);
-            const float *p = (half ? a.kv.vs : a.kv.ks) + r;
-            return *p;
+        auto load_scales = [&](const TileRuns &w) __attribute__((always_inline)) {
+            return (half ? a.kv.vs : a.kv.ks)[16 * uint64_t(col >> 4 ? w.run[1] : w.run[0]) + (col & 15)];
         };
 
         v16f o[DB];
@@ -144,12 +128,18 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
         float m = kNegInf, l = 0.0f;
 
-        uint32_t t = off + wave;
-        const uint32_t t_end = off + seg;
-        Where now{};
+        for (uint32_t c0 = off; c0 < off + seg; c0 += kStretch) {
+        const uint32_t t_end = min(off + seg, c0 + kStretch);
+        __syncthreads();
+        if (tid == 0) ms.runs.missing = 0;
+        __syncthreads();
+        find_runs<64 * NW>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
+        __syncthreads();
+        uint32_t t = c0 + wave;
+        TileRuns now{};
         float next_scale = 0.0f;
         if (t < t_end) {
-            now = where(t);
+            now = tile_runs(ms.runs, t - c0);
             wait_lds();
             load_k(now);
             load_v(now);
@@ -157,8 +147,8 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         }
         for (; t < t_end; t += NW) {
             const bool more = t + NW < t_end;
-            Where next = now;
-            if (more) next = where(t + NW);
+            TileRuns next = now;
+            if (more) next = tile_runs(ms.runs, t + NW - c0);
             if constexpr (SCALED) {
                 raw[lane] = next_scale;
                 const float vsc = fmaxf(next_scale, 0x1p-126f);  // (a factor of 0: values of next to nothing)
@@ -217,14 +207,14 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             }
             const int32_t j0 = b.lo + 32 * int32_t(t);
             // whether every row of the block sees every token of the tile
-            const bool full = now.held[0] && now.held[1] && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
+            const bool full = now.held == 3 && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
             uint32_t seen = 0xFFFF;
             if (!full) {
                 seen = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int32_t j = j0 + int32_t(token_of_reg(i, half));
-                    if (j <= pos && j >= from && now.held[i / 8]) seen |= 1u << i;
+                    if (j <= pos && j >= from && (now.held >> (i / 8)) & 1) seen |= 1u << i;
                 }
             }
             float tmax;
@@ -303,6 +293,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 if constexpr (SCALED) next_scale = load_scales(next);
             }
             now = next;
+        }
         }
 
         // ---- the waves' sums joined ----

@@ -26,15 +26,16 @@ struct TileShape {
     static constexpr int NW = DP / 2 + NP * DP / 4 > 128 ? 4 : 8;
     static constexpr int ROWS = 32 * NW;
     static constexpr int NBUF = 4;
-    static constexpr int MISC = 4096;
+    static constexpr int MISC = 8192;
     static constexpr int LDS = MISC + 2 * NBUF * TILE;
 };
 
 struct TileMisc {
     float kf[4][32], lv[4][32], iv[4][32];  // factors of a tile's keys; log2 and reciprocal of the values'
     LineMisc line;
+    RunMisc runs;
 };
-static_assert(sizeof(TileMisc) <= 4096, "");
+static_assert(sizeof(TileMisc) <= 8192, "");
 
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -63,7 +64,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
         const RowBlock b = row_block<Sh::ROWS, kTileTokens>(a, seq, r0);
         const uint32_t seg = uint32_t(min(uint64_t(b.tiles - off), left));
-        const uint32_t t0 = off, t1 = off + seg;
 
         // ---- the wave's rows of q ----
         const uint32_t wr0 = r0 + 32 * wave, row = wr0 + col;
@@ -102,6 +102,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     for (int i = 0; i < 4; ++i) q[p][ks][i] = piece2<CT>(x[ks][2 * i], x[ks][2 * i + 1]);
             }
         }
+        if (tid == 0) ms.runs.missing = 0;
         __syncthreads();  // (the last block's tiles are no longer read)
         if (DP != D) {  // dims past the row's: zeros, which no load touches
             for (uint32_t i = tid; i < uint32_t(2 * NBUF * TILE / 16); i += THREADS)
@@ -109,10 +110,29 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             __syncthreads();
         }
 
+        v16f o[DB], s;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+        float m = kNegInf, l = 0.0f, tmax = kNegInf;
+        uint32_t seen = 0xFFFF;
+
+        const uint32_t kplace = lds_addr(kbuf) + key_place<RB>(lane);
+        uint32_t vplace[DB];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<RB>(d, lane);
+        auto key = [&](uint32_t buf, int ks) __attribute__((always_inline)) { return lds_at((kplace ^ (32 * ks)) + buf * TILE); };
+        for (uint32_t t0 = off; t0 < off + seg; t0 += kStretch) {
+        const uint32_t t1 = min(off + seg, t0 + kStretch);
+        find_runs<THREADS>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.hi, t1 - t0, ms.runs, tid);
+        __syncthreads();
+        const bool missing = ms.runs.missing != 0;
+
         // ---- tiles into LDS ----
-        // Runs of 16 tokens lie in one page each; where none holds one, page 0 is
-        // read instead. Bit 2 i + g of `held`: run g of the tile i steps from now.
+        // Bit 2 i + g of `held`: whether a page holds run g of the tile i steps from now.
         uint32_t held = 0;
+        const uint32_t run_bytes = 16 * rowbytes;
         constexpr int LPR = RB / 16, RPI = 64 / LPR, LOADS = kTileTokens / RPI;  // direct loads of keys or values
         constexpr int MINE = 2 * LOADS / NW;                                   // a wave's
         static_assert(2 * LOADS % NW == 0, "");
@@ -121,15 +141,9 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         static_assert(CHUNKS < THREADS || CHUNKS % THREADS == 0, "");
         u32x4 raw[RAW];
         float raw_scale = 0.0f;
-        auto run_row = [&](uint32_t t, uint32_t g, uint32_t *ok) __attribute__((always_inline)) {
-            const int64_t r = cache_row(a.kv, seq, b.lo + 32 * int32_t(t) + 16 * int32_t(g), kvh);
-            *ok |= r >= 0 ? 1u << g : 0u;
-            return r >= 0 ? r : int64_t(0);
-        };
         auto load = [&](uint32_t t, uint32_t ahead) __attribute__((always_inline)) {
-            uint32_t ok = 0;
-            const int64_t run[2] = {run_row(t, 0, &ok), run_row(t, 1, &ok)};
-            held |= ok << (2 * ahead);
+            const TileRuns w = tile_runs(ms.runs, t - t0);
+            held |= w.held << (2 * ahead);
             const uint32_t buf = (t - t0) % NBUF;
             if constexpr (!SCALED) {
 #pragma unroll
@@ -139,7 +153,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     const uint32_t i = val ? f - LOADS : f, g = i * RPI / 16, rg = i * RPI % 16 + lane / LPR;
                     const uint32_t r = 16 * g + rg;
                     const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<RB, 2>(r) : key_swizzle<RB>(r));
-                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + (g != 0 ? run[1] : run[0]) * rowbytes;
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(g != 0 ? w.run[1] : w.run[0]) * run_bytes;
                     unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + i * 1024;
                     if (DP == D || 16 * c < rowbytes) dma16(lds_addr(dst), src, rg * rowbytes + 16 * c);
                 }
@@ -150,11 +164,11 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
                     const bool val = rr >= kTileTokens;
                     const uint32_t r = rr % kTileTokens;
-                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + ((r >= 16 ? run[1] : run[0]) + r % 16) * rowbytes;
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(r >= 16 ? w.run[1] : w.run[0]) * run_bytes + r % 16 * rowbytes;
                     raw[j] = u32x4{0, 0, 0, 0};
                     if ((CHUNKS >= THREADS || f < CHUNKS) && (DP == D || 16 * c < rowbytes)) raw[j] = *reinterpret_cast<const u32x4 *>(src + 16 * c);
                 }
-                if (tid < 64) raw_scale = (half ? a.kv.vs : a.kv.ks)[(col >= 16 ? run[1] : run[0]) + col % 16];
+                if (tid < 64) raw_scale = (half ? a.kv.vs : a.kv.ks)[16 * uint64_t(col >= 16 ? w.run[1] : w.run[0]) + col % 16];
             }
         };
         // (8-bit types) what load() fetched, widened, into its tile
@@ -185,19 +199,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             }
         };
 
-        v16f o[DB], s;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-        float m = kNegInf, l = 0.0f, tmax = kNegInf;
-        uint32_t seen = 0xFFFF;
-
-        const uint32_t kplace = lds_addr(kbuf) + key_place<RB>(lane);
-        uint32_t vplace[DB];
-#pragma unroll
-        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<RB>(d, lane);
-        auto key = [&](uint32_t buf, int ks) __attribute__((always_inline)) { return lds_at((kplace ^ (32 * ks)) + buf * TILE); };
         // whether some row of the wave sees a token of tile t, and whether all see all
         auto any_seen = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
@@ -333,23 +334,15 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         };
 
         for (uint32_t t = t0; t < t1;) {
-            if (active && (t - t0) % NBUF == 0 && t + 6 < t1 && full_tile(t) && full_tile(t + 4) && (held & 63) == 63) {
-                uint32_t ok = 0;
-                run_row(t + 3, 0, &ok);
-                run_row(t + 3, 1, &ok);
-                uint32_t ok4 = 0;
-                run_row(t + 4, 0, &ok4);
-                run_row(t + 4, 1, &ok4);
-                if ((ok & ok4) == 3) {
-                    v16f sn;
-                    seen = 0xFFFF;
-                    fast(std::integral_constant<uint32_t, 0>{}, t, s, sn);
-                    fast(std::integral_constant<uint32_t, 1>{}, t + 1, sn, s);
-                    fast(std::integral_constant<uint32_t, 2>{}, t + 2, s, sn);
-                    fast(std::integral_constant<uint32_t, 3>{}, t + 3, sn, s);
-                    t += 4;
-                    continue;
-                }
+            if (active && (t - t0) % NBUF == 0 && t + 6 < t1 && full_tile(t) && full_tile(t + 4) && !missing) {
+                v16f sn;
+                seen = 0xFFFF;
+                fast(std::integral_constant<uint32_t, 0>{}, t, s, sn);
+                fast(std::integral_constant<uint32_t, 1>{}, t + 1, sn, s);
+                fast(std::integral_constant<uint32_t, 2>{}, t + 2, s, sn);
+                fast(std::integral_constant<uint32_t, 3>{}, t + 3, sn, s);
+                t += 4;
+                continue;
             }
             // tile t + 1 is in LDS once every wave is here
             if constexpr (!SCALED) {
@@ -411,6 +404,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 finish_scores(t + 1, held & 3, s);
             }
             ++t;
+        }
+        __syncthreads();  // (the stretch's runs are no longer read)
         }
 
         // ---- the sums ----
