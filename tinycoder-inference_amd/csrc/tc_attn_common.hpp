@@ -121,11 +121,11 @@ inline SplitScratch split_scratch(void *scratch, uint32_t parts, uint32_t rows) 
 }
 // Sequences of at most this many rows (new tokens * query heads per key/value
 // head) go to the kernel for few rows.
-constexpr uint32_t kSplitRows = 64;
-// ... for any call: two workgroups per CU with 32 rows, one with 256 of up to 128
-// dims or 128 of up to 256.
+constexpr uint32_t kSplitRows = 16;
+// For any call: four workgroups per CU with 16 rows, one with 256 of up to 128 dims
+// or 128 of up to 256.
 inline size_t attn_part_bytes(int num_cu) {
-    const size_t cu = num_cu, jobs = (2 * cu * sizeof(SplitJob) + 255) & ~size_t(255);
+    const size_t cu = num_cu, jobs = (4 * cu * sizeof(SplitJob) + 255) & ~size_t(255);
     return jobs + cu * 2 * 256 * 2 * 4 + cu * 2 * 256 * 128 * 4;
 }
 

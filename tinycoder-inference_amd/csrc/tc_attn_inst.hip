@@ -17,11 +17,11 @@ hipError_t split(const AttnArgs &a, RowRange rg, int num_cu, void *scratch, hipS
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS);
     if (attr != hipSuccess) return attr;
     const uint32_t grid = Sh::OCC * num_cu;
-    const SplitScratch sc = split_scratch(scratch, grid, 32);
+    const SplitScratch sc = split_scratch(scratch, grid, Sh::R);
     k_attn_split<CT, NP, DP><<<grid, 64 * Sh::NW, Sh::LDS, st>>>(a, rg, sc);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_attn_join<DP, 32><<<dim3(grid, 8), 256, 0, st>>>(a, sc);
+    k_attn_join<DP, Sh::R><<<dim3(grid, Sh::R / 4), 256, 0, st>>>(a, sc);
     return hipGetLastError();
 }
 

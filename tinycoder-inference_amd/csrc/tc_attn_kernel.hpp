@@ -7,15 +7,16 @@
 // for any reference m_r, so one pass over the cache does, with m_r raised (and the
 // sums so far multiplied) only where a score exceeds it by 2^kLazy.
 //
-// On the matrix cores, 32 rows at a time as columns: scores = K Q^T (tokens by
-// rows, v_mfma_f32_32x32x16), o^T += V^T P^T (dims by rows). A lane then holds one
-// row's scores of 16 tokens and the same row's sums, so maxima, exponentials and
-// the raising of m need one exchange between the wave's halves and no other. The
-// scores come out of the first product in the registers in which the second one
-// takes them, if the tokens are numbered 16 (i / 8) + 8 half + i % 8 for register
-// i: the first product's operand rows are read in that order (token_of_row). V is
-// stored by rows and enters by columns: ds_read_b64_tr_b16 / _b8 transpose on the
-// way out of LDS.
+// On the matrix cores, R = 16 or 32 rows at a time as columns: scores = K Q^T (tokens
+// by rows), o^T += V^T P^T (dims by rows), v_mfma_f32_16x16x32 or _32x32x16. A lane
+// then holds scores of one row (its column, lane % R) and the same row's sums;
+// maxima and sums over a row's lanes, one in each of the 64 / R groups, take an
+// exchange or two. The scores come out of the first product in the registers in
+// which the second one takes them, if score register i of group g is the token
+// token_of_reg(i, g): the first product's operand rows are read in that order. V is
+// stored by rows and enters by columns: ds_read_b64_tr_b16 / _b8 transpose on the way
+// out of LDS. 32 rows halve the LDS reads per product, 16 the registers of the sums
+// and of q, and the work where there are no more rows.
 //
 // Operands: F16 and the 8-bit caches as fp16 (both exact there), BF16 as bf16. Rows
 // and weights of more bits go as several pieces, each exact product accumulated in
@@ -35,46 +36,76 @@ namespace {
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int s32x2 __attribute__((ext_vector_type(2)));
-typedef int s32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLazy = 4.0f, kLift = 11.0f;
-constexpr uint32_t kTileTokens = 32;  // tokens of one score product
+constexpr uint32_t kTileTokens = 32;
 constexpr float kNegInf = -__builtin_inff();
+
+// Shapes of the products for R rows and a padded head size.
+template <int R, int DP>
+struct Geo {
+    static constexpr int G = 64 / R;                // groups of lanes
+    static constexpr int NS = R / 2;                // scores of a lane: 32 tokens by R rows
+    static constexpr int AE = R == 32 ? 16 : 4;     // registers of an accumulator
+    static constexpr int NA = NS / AE;              // score accumulators
+    static constexpr int KS = DP * R / 512;         // contraction steps over the dims: 16 or 32 each
+    static constexpr int KT = R == 32 ? 2 : 1;      // ... over the tokens: 16 or 32 each
+    static constexpr int DB = DP / R;               // blocks of R dims
+};
+template <int R>
+struct AccOf {
+    typedef v16f type;
+};
+template <>
+struct AccOf<16> {
+    typedef f32x4 type;
+};
+template <int R>
+using Acc = typename AccOf<R>::type;
 
 // ---- LDS tiles --------------------------------------------------------------
 // Rows of RB bytes in 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so
-// that the lanes of one LDS cycle (256 bytes) fall on different banks: 16
-// consecutive rows of one chunk (keys, rows of q), or 4 (16-bit) or 8 (8-bit)
-// consecutive rows of 64 or 32 bytes each (values, read transposed).
-template <int RB>
+// that the lanes of one LDS cycle (256 bytes) fall on different banks. Keys: 16
+// lanes read one chunk of as many rows, consecutive ones (R = 32), or four runs of
+// four, 8 apart (R = 16). Values, read transposed by 32 lanes: R = 32: 64 bytes of 4
+// consecutive rows; R = 16: 32 bytes of two such runs, 8 apart (8-bit: 16 bytes of 16
+// consecutive rows).
+template <int R, int RB>
 __device__ __forceinline__ constexpr uint32_t key_swizzle(uint32_t r) {
-    return RB >= 256 ? r & 15 : (r / (256 / RB)) & (RB / 16 - 1);
+    const uint32_t x = R == 32 ? r & 15 : (r & 3) | ((r >> 1) & 12);  // 16 rows told apart
+    return RB >= 256 ? x : (x / (256 / RB)) & (RB / 16 - 1);
 }
-template <int RB, int ES>
+template <int R, int RB, int ES>
 __device__ __forceinline__ constexpr uint32_t value_swizzle(uint32_t r) {
-    constexpr uint32_t rp = RB >= 256 ? 1 : 256 / RB, rows = ES == 2 ? 4 : 8, cw = ES == 2 ? 4 : 2;
-    return cw * ((r / rp) & (rows / rp - 1));
+    constexpr uint32_t rp = RB >= 256 ? 1 : 256 / RB;  // rows of one LDS cycle
+    if (ES == 1) return (r / rp) & (16 / rp - 1);
+    const uint32_t x = R == 32 ? r & 3 : (r & 3) | ((r >> 1) & 4);
+    return (R == 32 ? 4 : 2) * ((x / rp) & ((R == 32 ? 4 : 8) / rp - 1));
 }
 
 __device__ __forceinline__ uint32_t lds_addr(const void *p) {
     return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)(p)));
 }
 
-// Lane l's 16 (4) bytes at base + off to LDS byte dst + 16 l (4 l), asynchronously:
+// Lane l's 16 (4) bytes to LDS byte dst + 16 l (4 l), asynchronously:
 // the kernel waits (vmcnt) before it reads them. Inline, so that the compiler does
 // not wait for these at every LDS read in between; m0 is restored.
 __device__ __forceinline__ void dma16(uint32_t dst, const void *base, uint32_t off) {
     uint32_t saved;
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    // (readfirstlane gives an int: widened as one, its sign would fill the upper half)
+    const uint32_t blo = __builtin_amdgcn_readfirstlane(uint32_t(b)), bhi = __builtin_amdgcn_readfirstlane(uint32_t(b >> 32));
+    const uint64_t ub = uint64_t(bhi) << 32 | blo;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(saved)
-                 : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(base)
+                 : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
                  : "memory");
 }
-__device__ __forceinline__ void dma4(uint32_t dst, const void *base, uint32_t off) {
+__device__ __forceinline__ void dma4(uint32_t dst, const void *p) {  // (4 bytes of each lane's own)
     uint32_t saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dword %2, %3\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(saved)
-                 : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(base)
+                 : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(p)
                  : "memory");
 }
 template <int N>
@@ -92,6 +123,13 @@ __device__ __forceinline__ v16f mfma(u32x4 a, u32x4 b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <int CT>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (CT == kBF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // 4 cache bytes as 4 fp16, exactly. I8: b ^ 0x80 under the exponent of 1024 is
@@ -111,16 +149,25 @@ __device__ __forceinline__ u32x2 widen(uint32_t w) {
     }
 }
 
-// The token (of 32) whose key is row m of the first product.
-__device__ __forceinline__ uint32_t token_of_row(uint32_t m) { return (m & 19) | ((m & 4) << 1) | ((m & 8) >> 1); }
-// The token of score register i in a half of the wave.
-__device__ __forceinline__ uint32_t token_of_reg(uint32_t i, uint32_t half) { return 16 * (i / 8) + 8 * half + i % 8; }
+// The token (of 32) whose key is operand row m of score accumulator a.
+template <int R>
+__device__ __forceinline__ uint32_t token_of_row(uint32_t m, uint32_t a) {
+    return R == 32 ? (m & 19) | ((m & 4) << 1) | ((m & 8) >> 1) : 8 * (m / 4) + 4 * a + m % 4;
+}
+// The token of score register i in group g.
+template <int R>
+__device__ __forceinline__ uint32_t token_of_reg(uint32_t i, uint32_t g) {
+    return R == 32 ? 16 * (i / 8) + 8 * g + i % 8 : 8 * g + i;
+}
+// The dims of quad k (registers 4 k to 4 k + 3) of a block of R dims in group g.
+__device__ __forceinline__ uint32_t dim_of_quad(uint32_t k, uint32_t g) { return 8 * k + 4 * g; }
 
-// First of the 8 dims of contraction step ks in a half of the wave: 16-bit rows
-// are read in 16-byte chunks of 8 dims, 8-bit ones in chunks of 16, for two steps.
-template <int ES>
-__device__ __forceinline__ uint32_t step_dim(uint32_t ks, uint32_t half) {
-    return ES == 2 ? 16 * ks + 8 * half : 32 * (ks / 2) + 16 * half + 8 * (ks % 2);
+// First of the 8 dims of contraction step ks in group g: 16-bit rows are read in
+// 16-byte chunks of 8 dims, 8-bit ones in chunks of 16, for two steps.
+template <int R, int ES>
+__device__ __forceinline__ uint32_t step_dim(uint32_t ks, uint32_t g) {
+    constexpr uint32_t G = 64 / R;
+    return ES == 2 ? 8 * (G * ks + g) : 16 * (G * (ks / 2) + g) + 8 * (ks % 2);
 }
 
 // One or more 16-bit pieces of x: x = sum of the pieces but for what is below them.
@@ -173,20 +220,26 @@ __device__ __forceinline__ void value4(const unsigned char *p, float (&x)[4]) {
     }
 }
 
-// The two halves' values of a lane's column: in both halves the lower's and the
-// upper's.
-__device__ __forceinline__ f32x2 both_halves(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return f32x2{__builtin_bit_cast(float, uint32_t(r[0])), __builtin_bit_cast(float, uint32_t(r[1]))};
+// Over a row's lanes, one in each group; the result in all of them.
+template <int R, class F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+    uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto h = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    v = f(__builtin_bit_cast(float, uint32_t(h[0])), __builtin_bit_cast(float, uint32_t(h[1])));
+    if constexpr (R == 16) {
+        b = __builtin_bit_cast(uint32_t, v);
+        const auto q = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        v = f(__builtin_bit_cast(float, uint32_t(q[0])), __builtin_bit_cast(float, uint32_t(q[1])));
+    }
+    return v;
 }
-__device__ __forceinline__ float halves_max(float v) {
-    const f32x2 h = both_halves(v);
-    return fmaxf(h[0], h[1]);
+template <int R>
+__device__ __forceinline__ float groups_max(float v) {
+    return over_groups<R>(v, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ float halves_sum(float v) {
-    const f32x2 h = both_halves(v);
-    return h[0] + h[1];
+template <int R>
+__device__ __forceinline__ float groups_sum(float v) {
+    return over_groups<R>(v, [](float a, float b) { return a + b; });
 }
 
 // (fmaxf would first quiet its operands, an instruction each)
@@ -195,10 +248,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-__device__ __forceinline__ float max16(const v16f &x) {
-    const float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]), c = max3(x[6], x[7], x[8]);
-    const float d = max3(x[9], x[10], x[11]), e = max3(x[12], x[13], x[14]);
-    return max3(max3(a, b, c), max3(d, e, x[15]), x[15]);
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+    float m = max3(x[0], x[1], x[2]), n = max3(x[3], x[4], x[5]);
+#pragma unroll
+    for (int i = 6; i + 3 < N; i += 4) m = max3(m, x[i], x[i + 1]), n = max3(n, x[i + 2], x[i + 3]);
+    return max3(m, max3(n, x[N - 2], x[N - 1]), n);
 }
 
 // 16 bytes of LDS at an address of lds_addr's.
@@ -209,27 +264,30 @@ __device__ __forceinline__ u32x2 lds_transposed16(uint32_t addr) {
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4 *>(addr)));
 }
 
-// Operand of o^T += V^T P^T for dims 32 d + 0 .. 31 and tokens 16 k + 0 .. 15 of a
-// 16-bit tile at LDS address vt. The lane's place depends on d alone (the rows 16 k
-// + 8 half + 4 u + l16 / 4 are alike in the bits that the swizzle takes), so a loop
-// holds one register per d.
-template <int RB>
+// Operands from 16-bit tiles at LDS addresses. Scores: the lane's place for
+// accumulator a and step 0, which step ks changes by an exclusive or (the step's
+// chunk number and the group's share no bits).
+template <int R, int RB>
+__device__ __forceinline__ uint32_t key_place(uint32_t a, uint32_t lane) {
+    const uint32_t r = token_of_row<R>(lane % R, a);
+    return r * RB + (((lane / R) ^ key_swizzle<R, RB>(r)) << 4);
+}
+template <int R>
+__device__ __forceinline__ uint32_t key_step(uint32_t ks) {
+    return ks * (64 / R) * 16;
+}
+// Values: the lane's place for dims R d to R d + R - 1; the rows of step k differ from
+// those of step 0 in no bit that the swizzle takes.
+template <int R, int RB>
 __device__ __forceinline__ uint32_t value_place(uint32_t d, uint32_t lane) {
-    const uint32_t l16 = lane & 15, g16 = (lane >> 4) & 1, half = lane >> 5;
-    const uint32_t r = 8 * half + l16 / 4, e = 32 * d + 16 * g16 + 4 * (l16 % 4);
-    return r * RB + (((e / 8) ^ value_swizzle<RB, 2>(r)) << 4) + (e & 4) * 2;
+    const uint32_t l16 = lane & 15, g = lane / R;
+    const uint32_t r = 8 * g + l16 / 4, e = R * d + (lane % R) / 16 * 16 + 4 * (l16 % 4);
+    return r * RB + (((e / 8) ^ value_swizzle<R, RB, 2>(r)) << 4) + (e & 4) * 2;
 }
 template <int RB>
 __device__ __forceinline__ u32x4 value_frag(uint32_t vt_place, uint32_t k) {
     const u32x2 a = lds_transposed16(vt_place + 16 * k * RB), b = lds_transposed16(vt_place + (16 * k + 4) * RB);
     return u32x4{a[0], a[1], b[0], b[1]};
-}
-// ... and of scores = K Q^T for contraction step ks: the keys' place for step 0,
-// which step ks changes by an exclusive or.
-template <int RB>
-__device__ __forceinline__ uint32_t key_place(uint32_t lane) {
-    const uint32_t r = token_of_row(lane & 31);
-    return r * RB + (((lane >> 5) ^ key_swizzle<RB>(r)) << 4);
 }
 
 // Whether a tile in LDS holds a value that is not finite.
@@ -246,26 +304,26 @@ __device__ __forceinline__ bool tile_not_finite(const unsigned char *vt, uint32_
 // o += weights * values token by token, of those that the lane's row sees alone: for
 // tiles with infinities or NaN that some row must not see, which a product with a
 // weight of 0 would bring in.
-template <int CT, int RB, int DB>
-__device__ __forceinline__ void add_values_one_by_one(const unsigned char *vt, const v16f &s, uint32_t seen, uint32_t lane,
-                                                      v16f (&o)[DB]) {
-    constexpr uint32_t ES = scaled_type(CT) ? 1 : 2;
-    const uint32_t col = lane & 31, half = lane >> 5;
-    for (uint32_t i = 0; i < 16; ++i)
-        for (uint32_t h = 0; h < 2; ++h) {
+template <int CT, int R, int RB, int DP>
+__device__ __forceinline__ void add_values_one_by_one(const unsigned char *vt, const float (&s)[R / 2], uint32_t seen, uint32_t lane,
+                                                      Acc<R> (&o)[DP / R]) {
+    constexpr uint32_t ES = scaled_type(CT) ? 1 : 2, G = 64 / R;
+    const uint32_t col = lane % R, g = lane / R;
+    for (uint32_t i = 0; i < R / 2; ++i)
+        for (uint32_t h = 0; h < G; ++h) {
             float p = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) p = i == uint32_t(j) ? s[j] : p;
-            const bool sees = (__shfl(seen, int(col + 32 * h)) >> i) & 1;
-            p = __shfl(p, int(col + 32 * h));
-            const uint32_t r = token_of_reg(i, h);
+            for (int j = 0; j < R / 2; ++j) p = i == uint32_t(j) ? s[j] : p;
+            const bool sees = (__shfl(seen, int(col + R * h)) >> i) & 1;
+            p = __shfl(p, int(col + R * h));
+            const uint32_t r = token_of_reg<R>(i, h);
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DP / R; ++d)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t byte = (32 * d + 8 * k + 4 * half) * ES;
+                for (int k = 0; k < (R == 32 ? 4 : 1); ++k) {
+                    const uint32_t byte = (R * d + dim_of_quad(k, g)) * ES;
                     float x[4];
-                    value4<CT>(vt + r * RB + (((byte / 16) ^ value_swizzle<RB, ES>(r)) << 4) + byte % 16, x);
+                    value4<CT>(vt + r * RB + (((byte / 16) ^ value_swizzle<R, RB, ES>(r)) << 4) + byte % 16, x);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[d][4 * k + j] = sees ? fmaf(p, x[j], o[d][4 * k + j]) : o[d][4 * k + j];
                 }
@@ -474,15 +532,15 @@ __device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, uint3
 // all threads at once. (Looked up tile by tile, the chain of scalar loads took two
 // thirds of the prompt kernel's step.)
 constexpr uint32_t kNoRun = 0xFFFFFFFFu;
-constexpr uint32_t kStretch = 512;  // tiles
+template <int STRETCH>
 struct RunMisc {
-    uint32_t run[2 * kStretch];
+    uint32_t run[2 * STRETCH];
     uint32_t missing;  // whether a run with tokens to be seen is not held (set to 0 a barrier earlier)
 };
 // For the tiles from position pos on (a multiple of 16), up to position hi.
-template <int THREADS>
+template <int THREADS, int STRETCH>
 __device__ __forceinline__ void find_runs(const AttnArgs &a, uint32_t seq, uint32_t kvh, int32_t pos, int32_t hi, uint32_t tiles,
-                                          RunMisc &rm, uint32_t tid) {
+                                          RunMisc<STRETCH> &rm, uint32_t tid) {
     for (uint32_t i = tid; i < 2 * tiles; i += THREADS) {
         const int32_t p = pos + 16 * int32_t(i);
         const uint32_t pi = div_fast(uint32_t(p), a.kv.page_div);
@@ -498,7 +556,8 @@ struct TileRuns {
     uint32_t run[2];
     uint32_t held;  // bit g: run g
 };
-__device__ __forceinline__ TileRuns tile_runs(const RunMisc &rm, uint32_t t) {
+template <int STRETCH>
+__device__ __forceinline__ TileRuns tile_runs(const RunMisc<STRETCH> &rm, uint32_t t) {
     const uint32_t x = __builtin_amdgcn_readfirstlane(rm.run[2 * t]), y = __builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]);
     TileRuns r;
     r.held = (x != kNoRun ? 1u : 0u) | (y != kNoRun ? 2u : 0u);
@@ -508,45 +567,43 @@ __device__ __forceinline__ TileRuns tile_runs(const RunMisc &rm, uint32_t t) {
 }
 
 // ---- rows of q --------------------------------------------------------------
-// 32 rows of NP pieces in LDS, [NP][32][DP] 16-bit elements in swizzled chunks, and
-// each row's factor log2(e) * scale * 2^e. Row r is query head (r0 + r) % group of
-// token row (r0 + r) / group; rows at n_rows or above are zeros. THREADS threads.
-template <int CT, int NP, int DP, int THREADS>
-__device__ __forceinline__ void stage_q(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t r0, uint32_t n_rows,
-                                        unsigned char *lds, float *factor, uint32_t tid) {
-    constexpr uint32_t QB = 2 * DP, per = THREADS / 32, chunks = DP / 8;
-    static_assert(chunks % per == 0, "");
-    const uint32_t r = tid / per, l = tid % per, row = r0 + r;
+// The lane's row, in NP pieces of the operands' type, and its factor log2(e) * scale *
+// 2^e. `row` is query head row % group of the sequence's token row / group; rows at
+// n_rows or above are zeros.
+template <int CT, int NP, int R, int DP, int ES>
+__device__ __forceinline__ float load_q(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row, uint32_t n_rows, uint32_t g,
+                                        u32x4 (&q)[NP][Geo<R, DP>::KS]) {
+    constexpr int KS = Geo<R, DP>::KS;
     const uint32_t tok = row / a.group;
     const uint64_t at = uint64_t(begin + tok) * a.q_stride + uint64_t(kvh * a.group + row - tok * a.group) * a.kv.dim;
-    float x[chunks / per][8];
-    float m = 0.0f;
+    float x[KS][8], m = 0.0f;
 #pragma unroll
-    for (uint32_t k = 0; k < chunks / per; ++k) {
-        const uint32_t d = 8 * (l + per * k);
+    for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t d = step_dim<R, ES>(ks, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[k][i] = 0.0f;
-        if (row < n_rows && d < a.kv.dim) load8(a.xtype, a.q, at + d, x[k]);
+        for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
+        if (row < n_rows && d < a.kv.dim) load8(a.xtype, a.q, at + d, x[ks]);
+    }
+    int e = 0;
+    if constexpr (CT != kBF16) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[k][i]));
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[ks][i]));
+        e = row_exponent<CT>(groups_max<R>(m));
     }
 #pragma unroll
-    for (uint32_t o = 1; o < per; o <<= 1) m = fmaxf(m, __shfl_xor(m, int(o)));
-    const int e = row_exponent<CT>(m);
+    for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (CT != kBF16)
 #pragma unroll
-    for (uint32_t k = 0; k < chunks / per; ++k) {
+            for (int i = 0; i < 8; ++i) x[ks][i] = ldexpf(x[ks][i], -e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[k][i] = ldexpf(x[k][i], -e);
-        const uint32_t c = l + per * k;
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = piece2<CT>(x[k][2 * i], x[k][2 * i + 1]);
-            *reinterpret_cast<u32x4 *>(lds + (p * 32 + r) * QB + ((c ^ key_swizzle<QB>(r)) << 4)) = w;
-        }
+            for (int i = 0; i < 4; ++i) q[p][ks][i] = piece2<CT>(x[ks][2 * i], x[ks][2 * i + 1]);
     }
-    if (l == 0) factor[r] = ldexpf(1.4426950408889634f * a.scale, e);
+    // (not 0: times an unseen score, -inf, it stays that)
+    return fmaxf(ldexpf(1.4426950408889634f * a.scale, e), 0x1p-126f);
 }
 
 // ---- the join ----------------------------------------------------------------

@@ -1,7 +1,7 @@
 // tc_attn_tile.hpp -- attention of many rows per key/value head: prompts. Bound by
 // the matrix cores and the exponentials between their products.
 //
-// A workgroup takes 32 rows per wave of one key/value head, which go over its tiles
+// A workgroup takes 32 (or 16) rows per wave of one key/value head, which go over its tiles
 // of 32 tokens together: tiles come into LDS two steps ahead (8-bit ones through
 // registers, widened to fp16 once for all waves), rows of q stay in registers. A
 // step's score products belong to the tile behind the one whose weights are being
@@ -22,9 +22,11 @@ struct TileShape {
     static constexpr int LT = CT == kBF16 ? kBF16 : kF16;  // element type in LDS
     static constexpr int RB = 2 * DP;
     static constexpr int TILE = kTileTokens * RB;
-    // registers of the sums and of q: beyond 128, one wave per SIMD
-    static constexpr int NW = DP / 2 + NP * DP / 4 > 128 ? 4 : 8;
-    static constexpr int ROWS = 32 * NW;
+    // 32 rows per wave where the sums and q leave room in the registers, else 16
+    static constexpr int R = NP == 1 && DP <= 128 ? 32 : 16;
+    static constexpr int NW = 8;
+    static constexpr int ROWS = R * NW;
+    static constexpr int STRETCH = 512;
     static constexpr int NBUF = 4;
     static constexpr int MISC = 8192;
     static constexpr int LDS = MISC + 2 * NBUF * TILE;
@@ -33,7 +35,7 @@ struct TileShape {
 struct TileMisc {
     float kf[4][32], lv[4][32], iv[4][32];  // factors of a tile's keys; log2 and reciprocal of the values'
     LineMisc line;
-    RunMisc runs;
+    RunMisc<512> runs;
 };
 static_assert(sizeof(TileMisc) <= 8192, "");
 
@@ -42,13 +44,16 @@ __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt
 template <int CT, int NP, int DP>
 __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_tile(AttnArgs a, RowRange rg, SplitScratch sc) {
     using Sh = TileShape<CT, NP, DP>;
-    constexpr int LT = Sh::LT, RB = Sh::RB, NW = Sh::NW, KS = DP / 16, DB = DP / 32, TILE = Sh::TILE, NBUF = Sh::NBUF;
+    constexpr int R = Sh::R, LT = Sh::LT, RB = Sh::RB, NW = Sh::NW, TILE = Sh::TILE, NBUF = Sh::NBUF;
+    using Ge = Geo<R, DP>;
+    constexpr int KS = Ge::KS, DB = Ge::DB, NS = Ge::NS, NA = Ge::NA, AE = Ge::AE;
+    constexpr uint32_t ALL = (1u << NS) - 1;
     constexpr int THREADS = 64 * NW;
     constexpr bool SCALED = scaled_type(CT);
     extern __shared__ __align__(1024) unsigned char lds[];
     TileMisc &ms = *reinterpret_cast<TileMisc *>(lds);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t col = lane & 31, half = lane >> 5;
+    const uint32_t col = lane % R, g = lane / R;
     unsigned char *const kbuf = lds + Sh::MISC, *const vbuf = kbuf + NBUF * TILE;
     const uint32_t D = a.kv.dim, rowbytes = D * (SCALED ? 1 : 2);
 
@@ -66,42 +71,14 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         const uint32_t seg = uint32_t(min(uint64_t(b.tiles - off), left));
 
         // ---- the wave's rows of q ----
-        const uint32_t wr0 = r0 + 32 * wave, row = wr0 + col;
+        const uint32_t wr0 = r0 + R * wave, row = wr0 + col;
         const bool active = wr0 < b.rows;  // the wave has rows
-        const uint32_t tok = row / a.group;
-        const int32_t pos = row < b.rows ? b.pos0 + int32_t(tok) : -1;  // the lane's row sees tokens up to here
+        const int32_t pos = row < b.rows ? b.pos0 + int32_t(row / a.group) : -1;  // the lane's row sees tokens up to here
         const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
         const int32_t wfirst = b.pos0 + int32_t(wr0 / a.group);
-        const int32_t wlast = b.pos0 + int32_t((min(wr0 + 32, b.rows) - 1) / a.group);
+        const int32_t wlast = b.pos0 + int32_t((min(wr0 + R, b.rows) - 1) / a.group);
         u32x4 q[NP][KS];
-        float factor = 1.4426950408889634f * a.scale;
-        {
-            float x[KS][8], mx = 0.0f;
-            const uint64_t at =
-                uint64_t(b.begin + tok) * a.q_stride + uint64_t(kvh * a.group + row - tok * a.group) * D;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t d = 16 * ks + 8 * half;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
-                if (row < b.rows && d < D) load8(a.xtype, a.q, at + d, x[ks]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
-            }
-            const int e = row_exponent<CT>(halves_max(mx));
-            // (not 0: times an unseen score, -inf, it stays that)
-            factor = fmaxf(ldexpf(factor, e), 0x1p-126f);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if constexpr (CT != kBF16)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[ks][i] = ldexpf(x[ks][i], -e);
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) q[p][ks][i] = piece2<CT>(x[ks][2 * i], x[ks][2 * i + 1]);
-            }
-        }
+        const float factor = load_q<CT, NP, R, DP, 2>(a, b.begin, kvh, row, b.rows, g, q);
         if (tid == 0) ms.runs.missing = 0;
         __syncthreads();  // (the last block's tiles are no longer read)
         if (DP != D) {  // dims past the row's: zeros, which no load touches
@@ -110,21 +87,59 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             __syncthreads();
         }
 
-        v16f o[DB], s;
+        Acc<R> o[DB];
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d) o[d] = Acc<R>{};
+        float s[NS];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+        for (int i = 0; i < NS; ++i) s[i] = 0.0f;
         float m = kNegInf, l = 0.0f, tmax = kNegInf;
-        uint32_t seen = 0xFFFF;
+        uint32_t seen = ALL;
 
-        const uint32_t kplace = lds_addr(kbuf) + key_place<RB>(lane);
-        uint32_t vplace[DB];
+        uint32_t kplace[NA], vplace[DB];
 #pragma unroll
-        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<RB>(d, lane);
-        auto key = [&](uint32_t buf, int ks) __attribute__((always_inline)) { return lds_at((kplace ^ (32 * ks)) + buf * TILE); };
-        for (uint32_t t0 = off; t0 < off + seg; t0 += kStretch) {
-        const uint32_t t1 = min(off + seg, t0 + kStretch);
+        for (int i = 0; i < NA; ++i) kplace[i] = lds_addr(kbuf) + key_place<R, RB>(i, lane);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<R, RB>(d, lane);
+        // scores of the tile in a buffer
+        auto products = [&](uint32_t buf, float (&x)[NS]) __attribute__((always_inline)) {
+            Acc<R> y[NA];
+#pragma unroll
+            for (int i = 0; i < NA; ++i) y[i] = Acc<R>{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    const u32x4 k = lds_at((kplace[i] ^ key_step<R>(ks)) + buf * TILE);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) y[i] = mfma<LT>(k, q[p][ks], y[i]);
+                }
+#pragma unroll
+            for (int i = 0; i < NS; ++i) x[i] = y[i / AE][i % AE];
+        };
+        // o += weights * values of the tile in a buffer
+        auto add_values = [&](uint32_t buf) __attribute__((always_inline)) {
+            u32x4 pw[Ge::KT][NP];
+#pragma unroll
+            for (int k = 0; k < Ge::KT; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
+                }
+#pragma unroll
+            for (int k = 0; k < Ge::KT; ++k)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
+                }
+        };
+
+        for (uint32_t t0 = off; t0 < off + seg; t0 += Sh::STRETCH) {
+        const uint32_t t1 = min(off + seg, t0 + Sh::STRETCH);
         find_runs<THREADS>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.hi, t1 - t0, ms.runs, tid);
         __syncthreads();
         const bool missing = ms.runs.missing != 0;
@@ -150,12 +165,12 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 for (int j = 0; j < MINE; ++j) {
                     const uint32_t f = wave + NW * j;
                     const bool val = f >= uint32_t(LOADS);
-                    const uint32_t i = val ? f - LOADS : f, g = i * RPI / 16, rg = i * RPI % 16 + lane / LPR;
-                    const uint32_t r = 16 * g + rg;
-                    const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<RB, 2>(r) : key_swizzle<RB>(r));
-                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(g != 0 ? w.run[1] : w.run[0]) * run_bytes;
+                    const uint32_t i = val ? f - LOADS : f, h = i * RPI / 16, rh = i * RPI % 16 + lane / LPR;
+                    const uint32_t r = 16 * h + rh;
+                    const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r));
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(h != 0 ? w.run[1] : w.run[0]) * run_bytes;
                     unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + i * 1024;
-                    if (DP == D || 16 * c < rowbytes) dma16(lds_addr(dst), src, rg * rowbytes + 16 * c);
+                    if (DP == D || 16 * c < rowbytes) dma16(lds_addr(dst), src, rh * rowbytes + 16 * c);
                 }
             } else {
                 // 16 bytes (16 dims) of one row per load: THREADS / (DP / 16) rows at a time, keys then values
@@ -168,7 +183,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     raw[j] = u32x4{0, 0, 0, 0};
                     if ((CHUNKS >= THREADS || f < CHUNKS) && (DP == D || 16 * c < rowbytes)) raw[j] = *reinterpret_cast<const u32x4 *>(src + 16 * c);
                 }
-                if (tid < 64) raw_scale = (half ? a.kv.vs : a.kv.ks)[16 * uint64_t(col >= 16 ? w.run[1] : w.run[0]) + col % 16];
+                if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + lane % 16];
             }
         };
         // (8-bit types) what load() fetched, widened, into its tile
@@ -179,7 +194,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
                 if (CHUNKS < THREADS && f >= CHUNKS) break;
                 const bool val = rr >= kTileTokens;
-                const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<RB, 2>(r) : key_swizzle<RB>(r);
+                const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r);
                 unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + r * RB;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -188,13 +203,13 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 }
             }
             if (tid < 64) {
-                if (half == 0) {
-                    ms.kf[buf][col] = raw_scale;
+                if (lane < 32) {
+                    ms.kf[buf][lane] = raw_scale;
                 } else {
                     // (a factor of 0: values of next to nothing; NaN stays)
                     const float x = raw_scale == raw_scale ? fmaxf(raw_scale, 0x1p-126f) : raw_scale;
-                    ms.lv[buf][col] = __builtin_amdgcn_logf(x);
-                    ms.iv[buf][col] = __builtin_amdgcn_rcpf(x);
+                    ms.lv[buf][lane - 32] = __builtin_amdgcn_logf(x);
+                    ms.iv[buf][lane - 32] = __builtin_amdgcn_rcpf(x);
                 }
             }
         };
@@ -207,33 +222,34 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         // Scores as they come from the matrix cores to what the weights are formed
         // from: as they are (times `factor` later), or with a token's factors the
         // exponents of 2 already; unseen ones to -inf; and the largest exponent.
-        auto token_factors = [&](uint32_t buf, v16f &x) __attribute__((always_inline)) {
+        auto token_factors = [&](uint32_t buf, float (&x)[NS]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg(i, half));
-                const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg(i, half));
+            for (int i = 0; i < NS; i += 4) {
+                const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg<R>(i, g));
+                const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg<R>(i, g));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
             }
         };
-        auto largest = [&](const v16f &x) __attribute__((always_inline)) {
-            const float y = halves_max(max16(x));
+        auto largest = [&](const float (&x)[NS]) __attribute__((always_inline)) {
+            const float y = groups_max<R>(max_of(x));
             return SCALED ? y : y * factor;
         };
         auto full_tile = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
             return j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
         };
-        auto finish_scores = [&](uint32_t t, uint32_t ok, v16f &x) __attribute__((always_inline)) {
+        auto finish_scores = [&](uint32_t t, uint32_t ok, float (&x)[NS]) __attribute__((always_inline)) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
-            seen = 0xFFFF;
+            seen = ALL;
             if constexpr (SCALED) token_factors((t - t0) % NBUF, x);
             if (ok != 3 || !full_tile(t)) {
                 seen = 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int32_t j = j0 + int32_t(token_of_reg(i, half));
-                    if (j <= pos && j >= from && (ok >> (i / 8)) & 1) seen |= 1u << i;
+                for (int i = 0; i < NS; ++i) {
+                    const uint32_t tok = token_of_reg<R>(i, g);
+                    const int32_t j = j0 + int32_t(tok);
+                    if (j <= pos && j >= from && (ok >> (tok / 16)) & 1) seen |= 1u << i;
                     x[i] = (seen >> i) & 1 ? x[i] : kNegInf;
                 }
             }
@@ -246,9 +262,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 m = up;
                 l *= al;
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= al;
+                for (int d = 0; d < DB; ++d) o[d] *= al;
             }
         };
         // the weight of a score
@@ -266,15 +280,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         if (t0 + 2 < t1) load(t0 + 2, 2);
         if constexpr (!SCALED) wait_loads<0>();
         tile_barrier();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
         if (any_seen(t0)) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 k = key(0, ks);
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p) s = mfma<LT>(k, q[p][ks], s);
-            }
+            products(0, s);
             finish_scores(t0, held & 3, s);
         }
 
@@ -282,7 +289,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         // the loop, as long as every row of the wave sees all of them and the one behind.
         // A tile's score products are issued among the weights of the one before, its
         // value products among the maxima of the one behind.
-        auto fast = [&](auto buf_c, uint32_t t, v16f &s, v16f &sn) __attribute__((always_inline)) {
+        auto fast = [&](auto buf_c, uint32_t t) __attribute__((always_inline)) {
             constexpr uint32_t buf = decltype(buf_c)::value, nbuf = (buf + 1) % NBUF;
             if constexpr (!SCALED) wait_loads<MINE>();
             tile_barrier();
@@ -290,57 +297,38 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             load(t + 3, 3);
             raise();
             const float ref = (m == kNegInf ? 0.0f : m) - kLift;
+            float sn[NS];
+            products(nbuf, sn);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 k = key(nbuf, ks);
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p) sn = mfma<LT>(k, q[p][ks], sn);
-            }
-            u32x4 pw[2][NP];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exponential(s[i], ref);
+            for (int i = 0; i < NS; ++i) s[i] = exponential(s[i], ref);
             if constexpr (SCALED) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg(i, half));
+                for (int i = 0; i < NS; i += 4) {
+                    const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg<R>(i, g));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) l = fmaf(s[i + j], rf[j], l);
                 }
             } else {
-                l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) + ((s[8] + s[9]) + (s[10] + s[11])) +
-                     ((s[12] + s[13]) + (s[14] + s[15]));
+                float x = 0.0f, y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NS; i += 2) x += s[i], y += s[i + 1];
+                l += x + y;
             }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
-                }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
-                }
+            add_values(buf);
             held >>= 2;
             if constexpr (SCALED) token_factors(nbuf, sn);
             tmax = largest(sn);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) s[i] = sn[i];
         };
 
         for (uint32_t t = t0; t < t1;) {
             if (active && (t - t0) % NBUF == 0 && t + 6 < t1 && full_tile(t) && full_tile(t + 4) && !missing) {
-                v16f sn;
-                seen = 0xFFFF;
-                fast(std::integral_constant<uint32_t, 0>{}, t, s, sn);
-                fast(std::integral_constant<uint32_t, 1>{}, t + 1, sn, s);
-                fast(std::integral_constant<uint32_t, 2>{}, t + 2, s, sn);
-                fast(std::integral_constant<uint32_t, 3>{}, t + 3, sn, s);
+                seen = ALL;
+                fast(std::integral_constant<uint32_t, 0>{}, t);
+                fast(std::integral_constant<uint32_t, 1>{}, t + 1);
+                fast(std::integral_constant<uint32_t, 2>{}, t + 2);
+                fast(std::integral_constant<uint32_t, 3>{}, t + 3);
                 t += 4;
                 continue;
             }
@@ -361,46 +349,22 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 raise();
                 const float ref = (m == kNegInf ? 0.0f : m) - kLift;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < NS; ++i) {
                     s[i] = exponential(s[i], ref);
                     // (the factor of a token that is not seen may be anything)
-                    const float p = SCALED ? s[i] * ms.iv[buf][token_of_reg(i, half)] : s[i];
+                    const float p = SCALED ? s[i] * ms.iv[buf][token_of_reg<R>(i, g)] : s[i];
                     l += (seen >> i) & 1 ? p : 0.0f;
                 }
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && __ballot(seen != 0xFFFF) != 0) odd = tile_not_finite<LT, TILE>(vbuf + buf * TILE, lane);
-                if (!odd) {
-                    u32x4 pw[2][NP];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
-#pragma unroll
-                            for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
-                        }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int d = 0; d < DB; ++d) {
-                            const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
-#pragma unroll
-                            for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
-                        }
-                } else {
-                    add_values_one_by_one<LT, RB, DB>(vbuf + buf * TILE, s, seen, lane, o);
-                }
+                if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(vbuf + buf * TILE, lane);
+                if (!odd)
+                    add_values(buf);
+                else
+                    add_values_one_by_one<LT, R, RB, DP>(vbuf + buf * TILE, s, seen, lane, o);
             }
             held >>= 2;
             if (t + 1 < t1 && any_seen(t + 1)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const u32x4 k = key((buf + 1) % NBUF, ks);
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; --p) s = mfma<LT>(k, q[p][ks], s);
-                }
+                products((buf + 1) % NBUF, s);
                 finish_scores(t + 1, held & 3, s);
             }
             ++t;
@@ -409,7 +373,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         }
 
         // ---- the sums ----
-        l = halves_sum(l);
+        l = groups_sum<R>(l);
         const bool whole = off == 0 && seg == b.tiles;
         const uint32_t slot = 2 * index + (first_seg ? 0 : 1);
         if (row < b.rows) {
@@ -418,19 +382,19 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t e = 32 * d + 8 * k + 4 * half;
+                    for (int k = 0; k < AE / 4; ++k) {
+                        const uint32_t e = R * d + dim_of_quad(k, g);
                         const f32x4 x = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
                         if (e < D) store4(a, b.begin, kvh, row, e, x * inv);
                     }
             } else {
                 const uint64_t at = uint64_t(slot) * Sh::ROWS + row - r0;
-                if (half == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
+                if (g == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        *reinterpret_cast<f32x4 *>(sc.o + at * DP + 32 * d + 8 * k + 4 * half) =
+                    for (int k = 0; k < AE / 4; ++k)
+                        *reinterpret_cast<f32x4 *>(sc.o + at * DP + R * d + dim_of_quad(k, g)) =
                             f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
             }
         }
