@@ -63,6 +63,14 @@ struct AccOf<16> {
 template <int R>
 using Acc = typename AccOf<R>::type;
 
+// The lane's index recomputed where it is used (v_mbcnt on an opaque zero): what rare
+// paths derive from it is then not held in registers across the loops.
+__device__ __forceinline__ uint32_t lane_now() {
+    uint32_t z = 0;
+    asm volatile("" : "+s"(z));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, z));
+}
+
 // ---- LDS tiles --------------------------------------------------------------
 // Rows of RB bytes in 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so
 // that the lanes of one LDS cycle (256 bytes) fall on different banks. Keys: 16
@@ -130,6 +138,20 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Keeps a product where it stands among what follows (nothing is emitted): the
+// accumulator counts as changed here.
+template <class T>
+__device__ __forceinline__ void pin(T &acc) {
+    asm volatile("" : "+v"(acc));
+}
+
+// A value that the compiler cannot form ahead of this point, nor hold what it would
+// form from it in registers of the paths around.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // 4 cache bytes as 4 fp16, exactly. I8: b ^ 0x80 under the exponent of 1024 is
@@ -242,11 +264,10 @@ __device__ __forceinline__ float groups_sum(float v) {
     return over_groups<R>(v, [](float a, float b) { return a + b; });
 }
 
-// (fmaxf would first quiet its operands, an instruction each)
+// (maximum, which keeps NaN, is one instruction for three; fmaxf would first quiet its
+// operands, an instruction each)
 __device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 template <int N>
 __device__ __forceinline__ float max_of(const float (&x)[N]) {
@@ -276,13 +297,17 @@ template <int R>
 __device__ __forceinline__ uint32_t key_step(uint32_t ks) {
     return ks * (64 / R) * 16;
 }
-// Values: the lane's place for dims R d to R d + R - 1; the rows of step k differ from
-// those of step 0 in no bit that the swizzle takes.
+// Values: the lane's place for dims 0 to R - 1, which block d changes by an exclusive
+// or; the rows of step k differ from those of step 0 in no bit that the swizzle takes.
 template <int R, int RB>
-__device__ __forceinline__ uint32_t value_place(uint32_t d, uint32_t lane) {
+__device__ __forceinline__ uint32_t value_place(uint32_t lane) {
     const uint32_t l16 = lane & 15, g = lane / R;
-    const uint32_t r = 8 * g + l16 / 4, e = R * d + (lane % R) / 16 * 16 + 4 * (l16 % 4);
+    const uint32_t r = 8 * g + l16 / 4, e = (lane % R) / 16 * 16 + 4 * (l16 % 4);
     return r * RB + (((e / 8) ^ value_swizzle<R, RB, 2>(r)) << 4) + (e & 4) * 2;
+}
+template <int R>
+__device__ __forceinline__ uint32_t value_block(uint32_t d) {
+    return 2 * R * d;
 }
 template <int RB>
 __device__ __forceinline__ u32x4 value_frag(uint32_t vt_place, uint32_t k) {

@@ -52,7 +52,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane % R, g = lane / R;
     unsigned char *const mine = lds + Sh::MISC + wave * Sh::WAVE;
-    unsigned char *const ktile = mine, *const vtile = mine + Sh::TILE;
+    const uint32_t ktile = lds_addr(lds) + Sh::MISC + wave * Sh::WAVE, vtile = ktile + Sh::TILE;
     float *const raw = reinterpret_cast<float *>(mine + 2 * Sh::TILE);  // [2][64] a tile's factors: keys', values'
     float *const lv = raw + 128, *const iv = raw + 160;                 // [32] log2 and reciprocal of the values'
     const uint32_t D = a.kv.dim, rowbytes = D * ES, run_bytes = 16 * rowbytes, nch = rowbytes / 16;
@@ -75,14 +75,15 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
 
         constexpr int LPR = RB / 16, RPI = 64 / LPR;  // lanes per row, rows per load
         constexpr int LOADS = 2 * (16 / RPI);         // loads of a tile of keys or values
-        auto load = [&](unsigned char *dst, const uint8_t *src, const TileRuns &w, auto swizzle) __attribute__((always_inline)) {
+        auto load = [&](uint32_t dst, const uint8_t *src, const TileRuns &w, auto swizzle) __attribute__((always_inline)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint8_t *at = src + uint64_t(w.run[h]) * run_bytes;
 #pragma unroll
                 for (int j = 0; j < 16 / RPI; ++j) {
                     const uint32_t r = j * RPI + lane / LPR, c = (lane % LPR) ^ swizzle(16 * h + r);
-                    if (DP == D || c < nch) dma16(lds_addr(dst + (16 * h + j * RPI) * RB), at, r * rowbytes + 16 * c);
+                    // (dims past the row's: others of it, which meet zeros of q, or go nowhere)
+                    dma16(dst + (16 * h + j * RPI) * RB, at, r * rowbytes + (c < nch ? 16 * c : 0));
                 }
             }
         };
@@ -91,7 +92,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         // lanes 0-31 the keys' factors of the 32 tokens, the others the values'
         auto load_scales = [&](const TileRuns &w, uint32_t odd) __attribute__((always_inline)) {
             const float *p = lane >= 32 ? a.kv.vs : a.kv.ks;
-            dma4(lds_addr(raw + 64 * odd), p + 16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + (lane & 15));
+            dma4(ktile + 2 * Sh::TILE + 256 * odd, p + 16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + (lane & 15));
         };
 
         Acc<R> o[DB];
@@ -103,9 +104,6 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             const uint32_t t_end = min(off + seg, c0 + Sh::STRETCH);
             __syncthreads();
             find_runs<64 * NW>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
-            if (DP != D)  // dims past the row's: zeros, which no load touches
-                for (uint32_t i = lane; i < 2 * Sh::TILE / 16; i += 64)
-                    *reinterpret_cast<u32x4 *>(mine + 16 * i) = u32x4{0, 0, 0, 0};
             __syncthreads();
             uint32_t t = c0 + wave;
             TileRuns now{};
@@ -133,7 +131,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                             for (int i = 0; i < Ge::NA; ++i) {
-                                const u32x4 k = lds_at((lds_addr(ktile) + key_place<R, RB>(i, lane)) ^ key_step<R>(ks));
+                                const u32x4 k = lds_at((ktile + key_place<R, RB>(i, lane)) ^ key_step<R>(ks));
 #pragma unroll
                                 for (int p = NP - 1; p >= 0; --p) x[i] = mfma<CT>(k, q[p][ks], x[i]);
                             }
@@ -142,7 +140,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                         for (int k2 = 0; k2 < KS / 2; ++k2)
 #pragma unroll
                             for (int i = 0; i < Ge::NA; ++i) {
-                                const u32x4 w = lds_at((lds_addr(ktile) + key_place<R, RB>(i, lane)) ^ key_step<R>(k2));
+                                const u32x4 w = lds_at((ktile + key_place<R, RB>(i, lane)) ^ key_step<R>(k2));
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     const u32x2 y = widen<CT>(w[2 * e]), z = widen<CT>(w[2 * e + 1]);
@@ -203,7 +201,8 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     }
                 }
                 const float tmax = groups_max<R>(max_of(s));
-                if (__ballot(tmax > m + kLazy) != 0) {
+                if (__builtin_expect(__ballot(tmax > m + kLazy) != 0, 0)) {
+                    asm volatile("; raise");  // (a branch, not a product by 1 of every sum in every step)
                     const float up = tmax > m + kLazy ? tmax : m;
                     const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
                     m = up;
@@ -225,7 +224,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 else
                     wait_loads<0>();
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && !full) odd = tile_not_finite<CT, Sh::TILE>(vtile, lane);
+                if (CT != kI8 && !full) odd = tile_not_finite<CT, Sh::TILE>(mine + Sh::TILE, lane);
                 if (!odd) {
                     u32x4 pw[NP];
 #pragma unroll
@@ -238,13 +237,13 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     for (int d = 0; d < DB; ++d) {
                         u32x4 v;
                         if constexpr (ES == 2) {
-                            v = value_frag<RB>(lds_addr(vtile) + value_place<R, RB>(d, lane), 0);
+                            v = value_frag<RB>((vtile + value_place<R, RB>(lane)) ^ value_block<R>(d), 0);
                         } else {
                             // 8 tokens of one dim: 16 lanes give 8 rows of 16 bytes
                             const uint32_t r = 8 * g + (lane & 15) / 2;
                             const u32x2 w = __builtin_bit_cast(
                                 u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) s32x2 *>(
-                                           lds_addr(vtile) + r * RB + ((d ^ value_swizzle<R, RB, 1>(r)) << 4) + 8 * (lane & 1))));
+                                           vtile + r * RB + ((d ^ value_swizzle<R, RB, 1>(r)) << 4) + 8 * (lane & 1))));
                             const u32x2 x = widen<CT>(w[0]), y = widen<CT>(w[1]);
                             v = u32x4{x[0], x[1], y[0], y[1]};
                         }
@@ -252,7 +251,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                         for (int p = NP - 1; p >= 0; --p) o[d] = mfma<CT>(v, pw[p], o[d]);
                     }
                 } else {
-                    add_values_one_by_one<CT, R, RB, DP>(vtile, s, seen, lane, o);
+                    add_values_one_by_one<CT, R, RB, DP>(mine + Sh::TILE, s, seen, lane, o);
                 }
                 wait_lds();
                 if (more) load_v(next);

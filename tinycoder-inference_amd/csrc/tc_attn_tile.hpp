@@ -54,7 +54,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
     TileMisc &ms = *reinterpret_cast<TileMisc *>(lds);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane % R, g = lane / R;
-    unsigned char *const kbuf = lds + Sh::MISC, *const vbuf = kbuf + NBUF * TILE;
+    const uint32_t kbuf = lds_addr(lds) + Sh::MISC, vbuf = kbuf + NBUF * TILE;
     const uint32_t D = a.kv.dim, rowbytes = D * (SCALED ? 1 : 2);
 
     // workgroups of one XCD (every eighth) take parts next to each other
@@ -81,12 +81,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         const float factor = load_q<CT, NP, R, DP, 2>(a, b.begin, kvh, row, b.rows, g, q);
         if (tid == 0) ms.runs.missing = 0;
         __syncthreads();  // (the last block's tiles are no longer read)
-        if (DP != D) {  // dims past the row's: zeros, which no load touches
-            for (uint32_t i = tid; i < uint32_t(2 * NBUF * TILE / 16); i += THREADS)
-                *reinterpret_cast<u32x4 *>(kbuf + 16 * i) = u32x4{0, 0, 0, 0};
-            __syncthreads();
-        }
-
         Acc<R> o[DB];
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = Acc<R>{};
@@ -96,21 +90,20 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         float m = kNegInf, l = 0.0f, tmax = kNegInf;
         uint32_t seen = ALL;
 
-        uint32_t kplace[NA], vplace[DB];
+        uint32_t kplace[NA], vplace = vbuf + value_place<R, RB>(lane);
 #pragma unroll
-        for (int i = 0; i < NA; ++i) kplace[i] = lds_addr(kbuf) + key_place<R, RB>(i, lane);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) vplace[d] = lds_addr(vbuf) + value_place<R, RB>(d, lane);
+        for (int i = 0; i < NA; ++i) kplace[i] = kbuf + key_place<R, RB>(i, lane);
         // scores of the tile in a buffer
         auto products = [&](uint32_t buf, float (&x)[NS]) __attribute__((always_inline)) {
             Acc<R> y[NA];
+            uint32_t place[NA];
 #pragma unroll
-            for (int i = 0; i < NA; ++i) y[i] = Acc<R>{};
+            for (int i = 0; i < NA; ++i) y[i] = Acc<R>{}, place[i] = here(kplace[i]);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
-                    const u32x4 k = lds_at((kplace[i] ^ key_step<R>(ks)) + buf * TILE);
+                    const u32x4 k = lds_at((place[i] ^ key_step<R>(ks)) + buf * TILE);
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) y[i] = mfma<LT>(k, q[p][ks], y[i]);
                 }
@@ -128,11 +121,12 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
 #pragma unroll
                     for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
                 }
+            const uint32_t place = here(vplace);
 #pragma unroll
             for (int k = 0; k < Ge::KT; ++k)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    const u32x4 v = value_frag<RB>(vplace[d] + buf * TILE, k);
+                    const u32x4 v = value_frag<RB>((place ^ value_block<R>(d)) + buf * TILE, k);
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) o[d] = mfma<LT>(v, pw[k][p], o[d]);
                 }
@@ -164,13 +158,13 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
 #pragma unroll
                 for (int j = 0; j < MINE; ++j) {
                     const uint32_t f = wave + NW * j;
-                    const bool val = f >= uint32_t(LOADS);
+                    const bool val = LOADS % NW == 0 ? j >= LOADS / NW : f >= uint32_t(LOADS);
                     const uint32_t i = val ? f - LOADS : f, h = i * RPI / 16, rh = i * RPI % 16 + lane / LPR;
                     const uint32_t r = 16 * h + rh;
                     const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r));
                     const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(h != 0 ? w.run[1] : w.run[0]) * run_bytes;
-                    unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + i * 1024;
-                    if (DP == D || 16 * c < rowbytes) dma16(lds_addr(dst), src, rh * rowbytes + 16 * c);
+                    // (dims past the row's: others of it, which meet zeros of q, or go nowhere)
+                    dma16((val ? vbuf : kbuf) + buf * TILE + i * 1024, src, rh * rowbytes + (16 * c < rowbytes ? 16 * c : 0));
                 }
             } else {
                 // 16 bytes (16 dims) of one row per load: THREADS / (DP / 16) rows at a time, keys then values
@@ -180,8 +174,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     const bool val = rr >= kTileTokens;
                     const uint32_t r = rr % kTileTokens;
                     const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(r >= 16 ? w.run[1] : w.run[0]) * run_bytes + r % 16 * rowbytes;
-                    raw[j] = u32x4{0, 0, 0, 0};
-                    if ((CHUNKS >= THREADS || f < CHUNKS) && (DP == D || 16 * c < rowbytes)) raw[j] = *reinterpret_cast<const u32x4 *>(src + 16 * c);
+                    if (CHUNKS >= THREADS || f < CHUNKS) raw[j] = *reinterpret_cast<const u32x4 *>(src + (16 * c < rowbytes ? 16 * c : 0));
                 }
                 if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + lane % 16];
             }
@@ -195,7 +188,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 if (CHUNKS < THREADS && f >= CHUNKS) break;
                 const bool val = rr >= kTileTokens;
                 const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r);
-                unsigned char *dst = (val ? vbuf : kbuf) + buf * TILE + r * RB;
+                unsigned char *dst = lds + Sh::MISC + ((val ? NBUF : 0) + buf) * TILE + r * RB;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const u32x2 x = widen<CT>(raw[j][2 * e]), y = widen<CT>(raw[j][2 * e + 1]);
@@ -245,9 +238,10 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             if constexpr (SCALED) token_factors((t - t0) % NBUF, x);
             if (ok != 3 || !full_tile(t)) {
                 seen = 0;
+                const uint32_t gn = lane_now() / R;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    const uint32_t tok = token_of_reg<R>(i, g);
+                    const uint32_t tok = token_of_reg<R>(i, gn);
                     const int32_t j = j0 + int32_t(tok);
                     if (j <= pos && j >= from && (ok >> (tok / 16)) & 1) seen |= 1u << i;
                     x[i] = (seen >> i) & 1 ? x[i] : kNegInf;
@@ -256,7 +250,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             tmax = largest(x);
         };
         auto raise = [&]() __attribute__((always_inline)) {
-            if (__ballot(tmax > m + kLazy) != 0) {
+            if (__builtin_expect(__ballot(tmax > m + kLazy) != 0, 0)) {
+                asm volatile("; raise");  // (a branch, not 64 products by 1 in every step)
                 const float up = tmax > m + kLazy ? tmax : m;
                 const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
                 m = up;
@@ -288,49 +283,104 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         // Four tiles at a time, each in its own buffer, so that no address is formed in
         // the loop, as long as every row of the wave sees all of them and the one behind.
         // A tile's score products are issued among the weights of the one before, its
-        // value products among the maxima of the one behind.
-        auto fast = [&](auto buf_c, uint32_t t) __attribute__((always_inline)) {
+        // value products among the sums and maxima of the one behind, operands
+        // kAhead products ahead of their use. The order is pinned: left to itself the
+        // compiler puts the vector work behind the products, and each product right
+        // behind its operands.
+        auto fast = [&](auto buf_c, uint32_t t, const uint32_t (&kp)[NA], uint32_t vp) __attribute__((always_inline)) {
             constexpr uint32_t buf = decltype(buf_c)::value, nbuf = (buf + 1) % NBUF;
+            constexpr int KEYS = NA * KS, VALS = Ge::KT * DB, AHEAD = 4;
             if constexpr (!SCALED) wait_loads<MINE>();
             tile_barrier();
             if constexpr (SCALED) put(t + 2);
             load(t + 3, 3);
             raise();
             const float ref = (m == kNegInf ? 0.0f : m) - kLift;
-            float sn[NS];
-            products(nbuf, sn);
+            u32x4 op[AHEAD];
+            // operand i of the step: keys, then values
+            auto operand = [&](int i) __attribute__((always_inline)) {
+                if (i < KEYS)
+                    op[i % AHEAD] = lds_at((kp[i % NA] ^ key_step<R>(i / NA)) + nbuf * TILE);
+                else if (i < KEYS + VALS)
+                    op[i % AHEAD] = value_frag<RB>((vp ^ value_block<R>((i - KEYS) % DB)) + buf * TILE, (i - KEYS) / DB);
+            };
+            Acc<R> y[NA];
 #pragma unroll
-            for (int i = 0; i < NS; ++i) s[i] = exponential(s[i], ref);
-            if constexpr (SCALED) {
+            for (int i = 0; i < NA; ++i) y[i] = Acc<R>{};
 #pragma unroll
-                for (int i = 0; i < NS; i += 4) {
-                    const f32x4 rf = *reinterpret_cast<const f32x4 *>(ms.iv[buf] + token_of_reg<R>(i, g));
+            for (int i = 0; i < AHEAD; ++i) operand(i);
+            int done = 0;  // weights formed
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) l = fmaf(s[i + j], rf[j], l);
-                }
-            } else {
-                float x = 0.0f, y = 0.0f;
+            for (int i = 0; i < KEYS; ++i) {
 #pragma unroll
-                for (int i = 0; i < NS; i += 2) x += s[i], y += s[i + 1];
-                l += x + y;
+                for (int p = NP - 1; p >= 0; --p) y[i % NA] = mfma<LT>(op[i % AHEAD], q[p][i / NA], y[i % NA]);
+                pin(y[i % NA]);
+                operand(i + AHEAD);
+#pragma unroll
+                for (; done < NS * (i + 1) / KEYS; ++done) s[done] = exponential(s[done], ref);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            add_values(buf);
+            u32x4 pw[Ge::KT][NP];
+            auto pack = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float a = s[8 * k + 2 * j], c = s[8 * k + 2 * j + 1];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(a, c);
+                }
+            };
+            float sn[NS], most = kNegInf, sum[2] = {0.0f, 0.0f};
+            pack(0);
+            int added = 0;
+#pragma unroll
+            for (int i = 0; i < VALS; ++i) {
+                constexpr int half = VALS / 2;
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) o[i % DB] = mfma<LT>(op[(KEYS + i) % AHEAD], pw[i / DB][p], o[i % DB]);
+                pin(o[i % DB]);
+                operand(KEYS + i + AHEAD);
+                if (Ge::KT == 2 && i == 0) pack(1);
+#pragma unroll
+                for (; added < NS * (i + 1) / VALS; ++added)
+                    if constexpr (SCALED)
+                        sum[added % 2] = fmaf(s[added], ms.iv[buf][token_of_reg<R>(added, g)], sum[added % 2]);
+                    else
+                        sum[added % 2] += s[added];
+                if (i == half) {
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) sn[j] = y[j / AE][j % AE];
+                    if constexpr (SCALED) token_factors(nbuf, sn);
+                }
+                if (i >= half) {
+                    constexpr int per = NS / (VALS - half);
+#pragma unroll
+                    for (int j = (i - half) * per; j < (i - half + 1) * per; j += 2) most = max3(most, sn[j], sn[j + 1]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l += sum[0] + sum[1];
             held >>= 2;
-            if constexpr (SCALED) token_factors(nbuf, sn);
-            tmax = largest(sn);
+            most = groups_max<R>(most);
+            tmax = SCALED ? most : most * factor;
 #pragma unroll
             for (int i = 0; i < NS; ++i) s[i] = sn[i];
         };
 
         for (uint32_t t = t0; t < t1;) {
-            if (active && (t - t0) % NBUF == 0 && t + 6 < t1 && full_tile(t) && full_tile(t + 4) && !missing) {
+            if (active && (t - t0) % NBUF == 0 && full_tile(t) && !missing) {
                 seen = ALL;
-                fast(std::integral_constant<uint32_t, 0>{}, t);
-                fast(std::integral_constant<uint32_t, 1>{}, t + 1);
-                fast(std::integral_constant<uint32_t, 2>{}, t + 2);
-                fast(std::integral_constant<uint32_t, 3>{}, t + 3);
-                t += 4;
-                continue;
+                while (t + 6 < t1 && full_tile(t + 4)) {
+                    uint32_t kp[NA];
+#pragma unroll
+                    for (int i = 0; i < NA; ++i) kp[i] = here(kplace[i]);
+                    const uint32_t vp = here(vplace);
+                    fast(std::integral_constant<uint32_t, 0>{}, t, kp, vp);
+                    fast(std::integral_constant<uint32_t, 1>{}, t + 1, kp, vp);
+                    fast(std::integral_constant<uint32_t, 2>{}, t + 2, kp, vp);
+                    fast(std::integral_constant<uint32_t, 3>{}, t + 3, kp, vp);
+                    t += 4;
+                }
             }
             // tile t + 1 is in LDS once every wave is here
             if constexpr (!SCALED) {
@@ -356,11 +406,11 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                     l += (seen >> i) & 1 ? p : 0.0f;
                 }
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(vbuf + buf * TILE, lane);
+                if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(lds + Sh::MISC + (NBUF + buf) * TILE, lane_now());
                 if (!odd)
                     add_values(buf);
                 else
-                    add_values_one_by_one<LT, R, RB, DP>(vbuf + buf * TILE, s, seen, lane, o);
+                    add_values_one_by_one<LT, R, RB, DP>(lds + Sh::MISC + (NBUF + buf) * TILE, s, seen, lane_now(), o);
             }
             held >>= 2;
             if (t + 1 < t1 && any_seen(t + 1)) {
@@ -374,6 +424,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
 
         // ---- the sums ----
         l = groups_sum<R>(l);
+        const uint32_t gn = lane_now() / R;
         const bool whole = off == 0 && seg == b.tiles;
         const uint32_t slot = 2 * index + (first_seg ? 0 : 1);
         if (row < b.rows) {
@@ -383,18 +434,18 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < AE / 4; ++k) {
-                        const uint32_t e = R * d + dim_of_quad(k, g);
+                        const uint32_t e = R * d + dim_of_quad(k, gn);
                         const f32x4 x = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
                         if (e < D) store4(a, b.begin, kvh, row, e, x * inv);
                     }
             } else {
                 const uint64_t at = uint64_t(slot) * Sh::ROWS + row - r0;
-                if (g == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
+                if (gn == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int k = 0; k < AE / 4; ++k)
-                        *reinterpret_cast<f32x4 *>(sc.o + at * DP + R * d + dim_of_quad(k, g)) =
+                        *reinterpret_cast<f32x4 *>(sc.o + at * DP + R * d + dim_of_quad(k, gn)) =
                             f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
             }
         }
