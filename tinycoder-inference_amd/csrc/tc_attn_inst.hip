@@ -31,11 +31,12 @@ hipError_t tile(const AttnArgs &a, RowRange rg, int num_cu, void *scratch, hipSt
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn_tile<CT, NP, DP>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS);
     if (attr != hipSuccess) return attr;
-    const SplitScratch sc = split_scratch(scratch, num_cu, Sh::ROWS);
-    k_attn_tile<CT, NP, DP><<<num_cu, 64 * Sh::NW, Sh::LDS, st>>>(a, rg, sc);
+    const uint32_t grid = Sh::OCC * num_cu;
+    const SplitScratch sc = split_scratch(scratch, grid, Sh::ROWS);
+    k_attn_tile<CT, NP, DP><<<grid, 64 * Sh::NW, Sh::LDS, st>>>(a, rg, sc);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_attn_join<DP, Sh::ROWS><<<dim3(num_cu, Sh::ROWS / 4), 256, 0, st>>>(a, sc);
+    k_attn_join<DP, Sh::ROWS><<<dim3(grid, Sh::ROWS / 4), 256, 0, st>>>(a, sc);
     return hipGetLastError();
 }
 

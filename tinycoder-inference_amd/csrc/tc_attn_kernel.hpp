@@ -97,24 +97,22 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 
 // Lane l's 16 (4) bytes to LDS byte dst + 16 l (4 l), asynchronously:
 // the kernel waits (vmcnt) before it reads them. Inline, so that the compiler does
-// not wait for these at every LDS read in between; m0 is restored.
+// not wait for these at every LDS read in between.
 __device__ __forceinline__ void dma16(uint32_t dst, const void *base, uint32_t off) {
-    uint32_t saved;
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     // (readfirstlane gives an int: widened as one, its sign would fill the upper half)
     const uint32_t blo = __builtin_amdgcn_readfirstlane(uint32_t(b)), bhi = __builtin_amdgcn_readfirstlane(uint32_t(b >> 32));
     const uint64_t ub = uint64_t(bhi) << 32 | blo;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
                  : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(uint32_t dst, const void *p) {  // (4 bytes of each lane's own)
-    uint32_t saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+                 :
                  : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(p)
-                 : "memory");
+                 : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -269,6 +267,19 @@ __device__ __forceinline__ float groups_sum(float v) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
+// a.x * b.x + a.y * b.y + c of 16-bit pairs; b is two ones: the sum of two weights as
+// they enter the products.
+template <int CT>
+__device__ __forceinline__ float add_pair(uint32_t w, float c) {
+    if constexpr (CT == kBF16) {
+        const bf16x2 one = {__bf16(1.0f), __bf16(1.0f)};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), one, c, false);
+    } else {
+        const f16x2 one = {_Float16(1.0f), _Float16(1.0f)};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), one, c, false);
+    }
+}
+
 template <int N>
 __device__ __forceinline__ float max_of(const float (&x)[N]) {
     float m = max3(x[0], x[1], x[2]), n = max3(x[3], x[4], x[5]);
@@ -553,42 +564,42 @@ __device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, uint3
 
 // ---- pages --------------------------------------------------------------------
 // The cache rows of a stretch of tiles in LDS: for each run of 16 tokens, which lies
-// in one page, its first cache row / 16 (kNoRun where no page holds it), looked up by
-// all threads at once. (Looked up tile by tile, the chain of scalar loads took two
-// thirds of the prompt kernel's step.)
-constexpr uint32_t kNoRun = 0xFFFFFFFFu;
+// in one page, its first cache row / 16, looked up by all threads at once (tile by
+// tile, the chain of scalar loads took two thirds of the prompt kernel's step), and
+// whether a page holds it: where none does, run 0 takes its place in the loads.
 template <int STRETCH>
 struct RunMisc {
     uint32_t run[2 * STRETCH];
-    uint32_t missing;  // whether a run with tokens to be seen is not held (set to 0 a barrier earlier)
+    uint64_t held[STRETCH / 32];  // bit i % 64 of word i / 64: run i
+    uint32_t missing;             // whether a run with tokens to be seen is not held (set to 0 a barrier earlier)
 };
 // For the tiles from position pos on (a multiple of 16), up to position hi.
 template <int THREADS, int STRETCH>
 __device__ __forceinline__ void find_runs(const AttnArgs &a, uint32_t seq, uint32_t kvh, int32_t pos, int32_t hi, uint32_t tiles,
                                           RunMisc<STRETCH> &rm, uint32_t tid) {
-    for (uint32_t i = tid; i < 2 * tiles; i += THREADS) {
+    const uint32_t per = a.kv.page / 16;
+    for (uint32_t i = tid; i / 64 * 64 < 2 * tiles; i += THREADS) {  // (whole waves)
         const int32_t p = pos + 16 * int32_t(i);
         const uint32_t pi = div_fast(uint32_t(p), a.kv.page_div);
-        const int32_t pg = page_at(a.kv, seq, pi);
-        const uint32_t per = a.kv.page / 16;
-        rm.run[i] = pg < 0 ? kNoRun : (uint32_t(pg) * a.kv.kv_heads + kvh) * per + (uint32_t(p) / 16 - pi * per);
-        if (pg < 0 && p < hi) rm.missing = 1;
+        const int32_t pg = i < 2 * tiles ? page_at(a.kv, seq, pi) : -1;
+        rm.run[i] = pg < 0 ? 0 : (uint32_t(pg) * a.kv.kv_heads + kvh) * per + (uint32_t(p) / 16 - pi * per);
+        const uint64_t held = __ballot(pg >= 0);
+        if (i % 64 == 0) rm.held[i / 64] = held;
+        if (pg < 0 && p < hi && i < 2 * tiles) rm.missing = 1;
     }
 }
-// The two runs of a tile, wave-uniform, and which are held; run 0 takes a missing
-// one's place in the loads.
+// The two runs of a tile, wave-uniform.
 struct TileRuns {
     uint32_t run[2];
-    uint32_t held;  // bit g: run g
 };
 template <int STRETCH>
 __device__ __forceinline__ TileRuns tile_runs(const RunMisc<STRETCH> &rm, uint32_t t) {
-    const uint32_t x = __builtin_amdgcn_readfirstlane(rm.run[2 * t]), y = __builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]);
-    TileRuns r;
-    r.held = (x != kNoRun ? 1u : 0u) | (y != kNoRun ? 2u : 0u);
-    r.run[0] = x != kNoRun ? x : 0;
-    r.run[1] = y != kNoRun ? y : 0;
-    return r;
+    return TileRuns{{uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t])), uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]))}};
+}
+// Which of them pages hold: bit g for run g.
+template <int STRETCH>
+__device__ __forceinline__ uint32_t tile_held(const RunMisc<STRETCH> &rm, uint32_t t) {
+    return uint32_t(rm.held[t / 32] >> (2 * (t % 32))) & 3;
 }
 
 // ---- rows of q --------------------------------------------------------------

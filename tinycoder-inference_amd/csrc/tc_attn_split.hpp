@@ -106,17 +106,16 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
             find_runs<64 * NW>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
             __syncthreads();
             uint32_t t = c0 + wave;
-            TileRuns now{};
             uint32_t odd_turn = 0;
             if (t < t_end) {
-                now = tile_runs(ms.runs, t - c0);
+                const TileRuns now = tile_runs(ms.runs, t - c0);
                 if constexpr (SCALED) load_scales(now, 0);
                 load_k(now);
                 load_v(now);
             }
             for (; t < t_end; t += NW) {
                 const bool more = t + NW < t_end;
-                TileRuns next = now;
+                TileRuns next{};
                 if (more) next = tile_runs(ms.runs, t + NW - c0);
                 wait_loads<LOADS>();  // (the values', issued behind the keys')
 
@@ -188,7 +187,8 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 }
                 const int32_t j0 = b.lo + 32 * int32_t(t);
                 // whether every row sees every token of the tile
-                const bool full = now.held == 3 && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
+                const uint32_t held = tile_held(ms.runs, t - c0);
+                const bool full = held == 3 && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
                 uint32_t seen = (1u << NS) - 1;
                 if (!full) {
                     seen = 0;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                     for (int i = 0; i < NS; ++i) {
                         const uint32_t tok = token_of_reg<R>(i, g);
                         const int32_t j = j0 + int32_t(tok);
-                        if (j <= pos && j >= from && (now.held >> (tok / 16)) & 1) seen |= 1u << i;
+                        if (j <= pos && j >= from && (held >> (tok / 16)) & 1) seen |= 1u << i;
                         s[i] = (seen >> i) & 1 ? s[i] : kNegInf;
                     }
                 }
@@ -255,7 +255,6 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 }
                 wait_lds();
                 if (more) load_v(next);
-                now = next;
             }
         }
 

@@ -25,6 +25,7 @@ struct TileShape {
     // 32 rows per wave where the sums and q leave room in the registers, else 16
     static constexpr int R = NP == 1 && DP <= 128 ? 32 : 16;
     static constexpr int NW = 8;
+    static constexpr int OCC = 1;
     static constexpr int ROWS = R * NW;
     static constexpr int STRETCH = 512;
     static constexpr int NBUF = 4;
@@ -42,7 +43,7 @@ static_assert(sizeof(TileMisc) <= 8192, "");
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int CT, int NP, int DP>
-__global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_tile(AttnArgs a, RowRange rg, SplitScratch sc) {
+__global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP, DP>::OCC)) void k_attn_tile(AttnArgs a, RowRange rg, SplitScratch sc) {
     using Sh = TileShape<CT, NP, DP>;
     constexpr int R = Sh::R, LT = Sh::LT, RB = Sh::RB, NW = Sh::NW, TILE = Sh::TILE, NBUF = Sh::NBUF;
     using Ge = Geo<R, DP>;
@@ -139,8 +140,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         const bool missing = ms.runs.missing != 0;
 
         // ---- tiles into LDS ----
-        // Bit 2 i + g of `held`: whether a page holds run g of the tile i steps from now.
-        uint32_t held = 0;
         const uint32_t run_bytes = 16 * rowbytes;
         constexpr int LPR = RB / 16, RPI = 64 / LPR, LOADS = kTileTokens / RPI;  // direct loads of keys or values
         constexpr int MINE = 2 * LOADS / NW;                                   // a wave's
@@ -150,9 +149,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         static_assert(CHUNKS < THREADS || CHUNKS % THREADS == 0, "");
         u32x4 raw[RAW];
         float raw_scale = 0.0f;
-        auto load = [&](uint32_t t, uint32_t ahead) __attribute__((always_inline)) {
+        auto load = [&](uint32_t t) __attribute__((always_inline)) {
             const TileRuns w = tile_runs(ms.runs, t - t0);
-            held |= w.held << (2 * ahead);
             const uint32_t buf = (t - t0) % NBUF;
             if constexpr (!SCALED) {
 #pragma unroll
@@ -224,19 +222,18 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
             }
         };
-        auto largest = [&](const float (&x)[NS]) __attribute__((always_inline)) {
-            const float y = groups_max<R>(max_of(x));
-            return SCALED ? y : y * factor;
-        };
+        // (of the lane's own scores: what is above a row's reference shows in one lane)
+        auto largest = [&](const float (&x)[NS]) __attribute__((always_inline)) { return SCALED ? max_of(x) : max_of(x) * factor; };
         auto full_tile = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
             return j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
         };
-        auto finish_scores = [&](uint32_t t, uint32_t ok, float (&x)[NS]) __attribute__((always_inline)) {
+        auto finish_scores = [&](uint32_t t, float (&x)[NS]) __attribute__((always_inline)) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
             seen = ALL;
             if constexpr (SCALED) token_factors((t - t0) % NBUF, x);
-            if (ok != 3 || !full_tile(t)) {
+            if (missing || !full_tile(t)) {
+                const uint32_t ok = tile_held(ms.runs, t - t0);
                 seen = 0;
                 const uint32_t gn = lane_now() / R;
 #pragma unroll
@@ -252,7 +249,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         auto raise = [&]() __attribute__((always_inline)) {
             if (__builtin_expect(__ballot(tmax > m + kLazy) != 0, 0)) {
                 asm volatile("; raise");  // (a branch, not 64 products by 1 in every step)
-                const float up = tmax > m + kLazy ? tmax : m;
+                const float most = groups_max<R>(tmax);
+                const float up = most > m + kLazy ? most : m;
                 const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
                 m = up;
                 l *= al;
@@ -266,18 +264,18 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
         };
 
         // ---- the first tiles ----
-        load(t0, 0);
+        load(t0);
         if constexpr (SCALED) put(t0);
         if (t0 + 1 < t1) {
-            load(t0 + 1, 1);
+            load(t0 + 1);
             if constexpr (SCALED) put(t0 + 1);
         }
-        if (t0 + 2 < t1) load(t0 + 2, 2);
+        if (t0 + 2 < t1) load(t0 + 2);
         if constexpr (!SCALED) wait_loads<0>();
         tile_barrier();
         if (any_seen(t0)) {
             products(0, s);
-            finish_scores(t0, held & 3, s);
+            finish_scores(t0, s);
         }
 
         // Four tiles at a time, each in its own buffer, so that no address is formed in
@@ -293,7 +291,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             if constexpr (!SCALED) wait_loads<MINE>();
             tile_barrier();
             if constexpr (SCALED) put(t + 2);
-            load(t + 3, 3);
             raise();
             const float ref = (m == kNegInf ? 0.0f : m) - kLift;
             u32x4 op[AHEAD];
@@ -319,6 +316,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 operand(i + AHEAD);
 #pragma unroll
                 for (; done < NS * (i + 1) / KEYS; ++done) s[done] = exponential(s[done], ref);
+                if (i == KEYS / 2) load(t + 3);
                 __builtin_amdgcn_sched_barrier(0);
             }
             u32x4 pw[Ge::KT][NP];
@@ -345,8 +343,10 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 for (; added < NS * (i + 1) / VALS; ++added)
                     if constexpr (SCALED)
                         sum[added % 2] = fmaf(s[added], ms.iv[buf][token_of_reg<R>(added, g)], sum[added % 2]);
-                    else
+                    else if constexpr (NP > 1)
                         sum[added % 2] += s[added];
+                    else if (added % 2 == 1)
+                        sum[added / 2 % 2] = add_pair<LT>(pw[added / 8][0][added % 8 / 2], sum[added / 2 % 2]);
                 if (i == half) {
 #pragma unroll
                     for (int j = 0; j < NS; ++j) sn[j] = y[j / AE][j % AE];
@@ -360,8 +360,6 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 __builtin_amdgcn_sched_barrier(0);
             }
             l += sum[0] + sum[1];
-            held >>= 2;
-            most = groups_max<R>(most);
             tmax = SCALED ? most : most * factor;
 #pragma unroll
             for (int i = 0; i < NS; ++i) s[i] = sn[i];
@@ -392,7 +390,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
             tile_barrier();
             if constexpr (SCALED)
                 if (t + 2 < t1) put(t + 2);
-            if (t + 3 < t1) load(t + 3, 3);
+            if (t + 3 < t1) load(t + 3);
 
             const uint32_t buf = (t - t0) % NBUF;
             if (any_seen(t)) {
@@ -412,10 +410,9 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), 1) void k_attn_ti
                 else
                     add_values_one_by_one<LT, R, RB, DP>(lds + Sh::MISC + (NBUF + buf) * TILE, s, seen, lane_now(), o);
             }
-            held >>= 2;
             if (t + 1 < t1 && any_seen(t + 1)) {
                 products((buf + 1) % NBUF, s);
-                finish_scores(t + 1, held & 3, s);
+                finish_scores(t + 1, s);
             }
             ++t;
         }
