@@ -96,14 +96,16 @@ hipError_t launch_attn_cache<kI8>(const AttnArgs &a, int num_cu, void *scratch, 
 template <>
 hipError_t launch_attn_cache<kE4M3>(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st);
 
-// A block of rows whose tiles lie in several workgroups' parts.
+// A block of rows whose tiles lie in several parts.
 struct SplitJob {
     uint32_t seq, r0, kvh;
-    uint32_t count;  // workgroups, from this one on (0: none)
-    uint32_t slot;   // where the first one's sums are; the others': 2 * workgroup
+    uint32_t rows;   // of the block
+    uint32_t count;  // parts, from this one on (0: none)
+    uint32_t slot;   // where the first one's sums are; the others': 2 * part
 };
 
-// Sums that workgroups leave for k_attn_join: two blocks of rows each.
+// Sums that workgroups leave for k_attn_join: two blocks of rows each, in slots of as
+// many rows as the larger kind of block has.
 struct SplitScratch {
     SplitJob *jobs;  // [parts]
     float *ml;       // [2 * parts][rows][2] reference and sum of weights
@@ -120,12 +122,12 @@ inline SplitScratch split_scratch(void *scratch, uint32_t parts, uint32_t rows) 
     return s;
 }
 // Sequences of at most this many rows (new tokens * query heads per key/value
-// head) go to the kernel for few rows.
-constexpr uint32_t kSplitRows = 16;
-// For any call: four workgroups per CU with 16 rows, one with 256 of up to 128 dims
-// or 128 of up to 256.
+// head) are served in blocks of 16, the others in blocks of 128 or 256.
+constexpr uint32_t kFewRows = 64;
+// For any call: a part per CU, with slots of 256 rows of up to 128 dims or 128 of up
+// to 256.
 inline size_t attn_part_bytes(int num_cu) {
-    const size_t cu = num_cu, jobs = (4 * cu * sizeof(SplitJob) + 255) & ~size_t(255);
+    const size_t cu = num_cu, jobs = (cu * sizeof(SplitJob) + 255) & ~size_t(255);
     return jobs + cu * 2 * 256 * 2 * 4 + cu * 2 * 256 * 128 * 4;
 }
 

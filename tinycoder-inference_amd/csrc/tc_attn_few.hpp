@@ -1,13 +1,12 @@
-// tc_attn_split.hpp -- attention of up to 16 rows per key/value head: decode steps and
-// a few drafted tokens. HBM-bound: every cached key and value of a head is read once
-// for all its rows.
+// tc_attn_few.hpp -- attention of up to kFewRows rows per key/value head: decode steps
+// and drafted tokens. HBM-bound: every cached key and value of a head is read once for
+// 16 rows.
 //
-// The line of tiles (32 tokens for 16 rows) is cut into equal parts, one per
-// workgroup. The waves of a workgroup take its tiles in turn, each through LDS of its
-// own and without barriers: keys of the next tile are on their way while the values
-// of this one are multiplied, and the other way round. Where a sequence's tiles end or
-// the part does, the waves join their sums. Rows whose tiles lie in several parts
-// leave unnormalised sums, which k_attn_join adds up.
+// The waves of a workgroup take the tiles of its part (32 tokens for 16 rows) in turn,
+// each through LDS of its own and without barriers: while one tile is multiplied, the
+// keys and values of the next ones are on their way. Where a block's tiles end or the
+// part does, the waves join their sums. Blocks whose tiles lie in several parts leave
+// unnormalised sums, which k_attn_join adds up.
 #pragma once
 
 #include "tc_attn_kernel.hpp"
@@ -15,52 +14,39 @@
 namespace tc {
 namespace {
 
-// Shape of a launch for one cache type, number of pieces and padded head size.
 template <int CT, int NP, int DP>
-struct SplitShape {
-    static constexpr int R = 16, NW = 4, STRETCH = 128;
+struct FewShape {
+    static constexpr int R = 16;
     static constexpr int ES = scaled_type(CT) ? 1 : 2;
-    static constexpr int RB = DP * ES;                        // bytes of a cache row in LDS
-    static constexpr int TILE = kTileTokens * RB;             // of a tile of keys or values
-    static constexpr int SCALES = scaled_type(CT) ? 768 : 0;  // factors, two tiles'; log2 and reciprocal
-    static constexpr int WAVE = 2 * TILE + SCALES;
-    static constexpr int MISC = 6144;  // (the first bytes of LDS hold the small things)
-    static constexpr int LDS = MISC + NW * WAVE;
-    // workgroups per CU: what LDS allows, up to 4 (128 registers a lane)
-    static constexpr int BY_LDS = 160 * 1024 / LDS;
-    static constexpr int BY_REG = DP == 256 || NP == 3 ? 2 : 3;
-    static constexpr int OCC = BY_LDS < BY_REG ? BY_LDS : BY_REG;
+    static constexpr int RB = DP * ES;             // bytes of a cache row in LDS
+    static constexpr int TILE = kTileTokens * RB;  // of a tile of keys or values
+    // tiles in flight per wave, and waves at work: 16 KB each, or 4 of 32
+    static constexpr int NB = 2 * TILE <= 16384 ? 16384 / (2 * TILE) : 1;
+    static constexpr int NW = 2 * TILE <= 16384 ? kWaves : 4;
+    static constexpr int SCALES = scaled_type(CT) ? 256 * (NB + 2) : 0;  // factors of NB + 1 tiles; log2 and reciprocal
+    static constexpr int WAVE = 2 * TILE * NB + SCALES;
+    static constexpr int LDS = kMisc + NW * WAVE;
+    static_assert(LDS <= kLds, "");
 };
 
-struct SplitMisc {
-    float m[4][16], l[4][16], inv[16];
-    LineMisc line;
-    RunMisc<128> runs;
-};
-static_assert(sizeof(SplitMisc) <= 6144, "");
-
-template <int CT, int NP, int DP>
-__global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, NP, DP>::OCC)) void k_attn_split(
-    AttnArgs a, RowRange rg, SplitScratch sc) {
-    using Sh = SplitShape<CT, NP, DP>;
-    constexpr int R = Sh::R, ES = Sh::ES, RB = Sh::RB, NW = Sh::NW;
+template <int CT, int NP, int DP, int SLOT>
+__device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
+    using Sh = FewShape<CT, NP, DP>;
+    constexpr int R = Sh::R, ES = Sh::ES, RB = Sh::RB, NW = Sh::NW, NB = Sh::NB, TILE = Sh::TILE;
     using Ge = Geo<R, DP>;
     constexpr int KS = Ge::KS, DB = Ge::DB, NS = Ge::NS;
     constexpr bool SCALED = scaled_type(CT);
-    extern __shared__ __align__(1024) unsigned char lds[];
-    SplitMisc &ms = *reinterpret_cast<SplitMisc *>(lds);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane % R, g = lane / R;
-    unsigned char *const mine = lds + Sh::MISC + wave * Sh::WAVE;
-    const uint32_t ktile = lds_addr(lds) + Sh::MISC + wave * Sh::WAVE, vtile = ktile + Sh::TILE;
-    float *const raw = reinterpret_cast<float *>(mine + 2 * Sh::TILE);  // [2][64] a tile's factors: keys', values'
-    float *const lv = raw + 128, *const iv = raw + 160;                 // [32] log2 and reciprocal of the values'
+    // LDS of the wave: NB tiles of keys, NB of values, factors (waves without work: the last one's)
+    unsigned char *const mine = lds + kMisc + min(wave, NW - 1u) * Sh::WAVE;
+    const uint32_t kring = lds_addr(lds) + kMisc + min(wave, NW - 1u) * Sh::WAVE, vring = kring + NB * TILE;
+    float *const raw = reinterpret_cast<float *>(mine + 2 * NB * TILE);       // [NB + 1][64] a tile's factors: keys', values'
+    float *const lv = raw + 64 * (NB + 1), *const iv = lv + 32;               // [32] log2 and reciprocal of the values'
     const uint32_t D = a.kv.dim, rowbytes = D * ES, run_bytes = 16 * rowbytes, nch = rowbytes / 16;
 
-    uint64_t part, left;
-    Place pl = line_part<R, kTileTokens, 64 * NW>(a, rg, blockIdx.x, gridDim.x, NW, ms.line, tid, &part, &left);
-    if (tid == 0) sc.jobs[blockIdx.x].count = 0;
-
+    Place pl = work.at;
+    uint64_t left = work.left;
     bool first_seg = true;
     while (left != 0) {
         const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
@@ -87,12 +73,17 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 }
             }
         };
-        auto load_k = [&](const TileRuns &w) __attribute__((always_inline)) { load(ktile, a.kv.k, w, key_swizzle<R, RB>); };
-        auto load_v = [&](const TileRuns &w) __attribute__((always_inline)) { load(vtile, a.kv.v, w, value_swizzle<R, RB, ES>); };
+        // tile number i of the wave
+        auto load_k = [&](const TileRuns &w, uint32_t i) __attribute__((always_inline)) {
+            load(kring + i % NB * TILE, a.kv.k, w, key_swizzle<R, RB>);
+        };
+        auto load_v = [&](const TileRuns &w, uint32_t i) __attribute__((always_inline)) {
+            load(vring + i % NB * TILE, a.kv.v, w, value_swizzle<R, RB, ES>);
+        };
         // lanes 0-31 the keys' factors of the 32 tokens, the others the values'
-        auto load_scales = [&](const TileRuns &w, uint32_t odd) __attribute__((always_inline)) {
+        auto load_scales = [&](const TileRuns &w, uint32_t i) __attribute__((always_inline)) {
             const float *p = lane >= 32 ? a.kv.vs : a.kv.ks;
-            dma4(ktile + 2 * Sh::TILE + 256 * odd, p + 16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + (lane & 15));
+            dma4(kring + 2 * NB * TILE + i % (NB + 1) * 256, p + 16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + (lane & 15));
         };
 
         Acc<R> o[DB];
@@ -100,24 +91,32 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
         for (int d = 0; d < DB; ++d) o[d] = Acc<R>{};
         float m = kNegInf, l = 0.0f;
 
-        for (uint32_t c0 = off; c0 < off + seg; c0 += Sh::STRETCH) {
-            const uint32_t t_end = min(off + seg, c0 + Sh::STRETCH);
+        for (uint32_t c0 = off; c0 < off + seg; c0 += 512) {
+            const uint32_t t_end = min(off + seg, c0 + 512);
             __syncthreads();
-            find_runs<64 * NW>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
+            find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
             __syncthreads();
-            uint32_t t = c0 + wave;
-            uint32_t odd_turn = 0;
-            if (t < t_end) {
-                const TileRuns now = tile_runs(ms.runs, t - c0);
-                if constexpr (SCALED) load_scales(now, 0);
-                load_k(now);
-                load_v(now);
-            }
-            for (; t < t_end; t += NW) {
-                const bool more = t + NW < t_end;
+            const uint32_t mine_n = wave < uint32_t(NW) && t_end - c0 > wave ? (t_end - c0 - wave + NW - 1) / NW : 0;  // the wave's tiles
+            wait_lds();
+#pragma unroll
+            for (uint32_t i = 0; i < NB; ++i)
+                if (i < mine_n) {
+                    const TileRuns w = tile_runs(ms.runs, wave + NW * i);
+                    if constexpr (SCALED) load_scales(w, i);
+                    load_k(w, i);
+                    load_v(w, i);
+                }
+            for (uint32_t n = 0; n < mine_n; ++n) {
+                const uint32_t t = c0 + wave + NW * n;
+                const uint32_t ktile = kring + n % NB * TILE, vtile = vring + n % NB * TILE;
+                const bool more = n + NB < mine_n;
                 TileRuns next{};
-                if (more) next = tile_runs(ms.runs, t + NW - c0);
-                wait_loads<LOADS>();  // (the values', issued behind the keys')
+                if (more) next = tile_runs(ms.runs, t + NW * NB - c0);
+                // (all loads behind the keys', where NB - 1 further tiles are under way)
+                if (n + NB <= mine_n)
+                    wait_loads<(2 * NB - 1) * LOADS + (SCALED ? NB - 1 : 0)>();
+                else
+                    wait_loads<0>();
 
                 // ---- scores ----
                 float s[NS];
@@ -154,21 +153,20 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                 }
                 wait_lds();
                 if (more) {
-                    if constexpr (SCALED) load_scales(next, odd_turn ^ 1);
-                    load_k(next);
+                    if constexpr (SCALED) load_scales(next, n + NB);
+                    load_k(next, n + NB);
                 }
 
                 // ---- weights ----
                 float rf[NS];
                 if constexpr (SCALED) {
-                    const float *const kfac = raw + 64 * odd_turn;
+                    const float *const kfac = raw + n % (NB + 1) * 64;
                     if (lane >= 32) {
                         // (a factor of 0: values of next to nothing; NaN stays)
                         const float y = kfac[lane], x = y == y ? fmaxf(y, 0x1p-126f) : y;
                         lv[lane - 32] = __builtin_amdgcn_logf(x);
                         iv[lane - 32] = __builtin_amdgcn_rcpf(x);
                     }
-                    odd_turn ^= 1;
 #pragma unroll
                     for (int i = 0; i < NS; i += 4) {
                         const uint32_t tok = token_of_reg<R>(i, g);
@@ -220,11 +218,11 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
 
                 // ---- values ----
                 if (more)
-                    wait_loads<LOADS + (SCALED ? 1 : 0)>();
+                    wait_loads<(2 * NB - 1) * LOADS + (SCALED ? NB : 0)>();
                 else
                     wait_loads<0>();
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && !full) odd = tile_not_finite<CT, Sh::TILE>(mine + Sh::TILE, lane);
+                if (CT != kI8 && !full) odd = tile_not_finite<CT, TILE>(mine + (NB + n % NB) * TILE, lane);
                 if (!odd) {
                     u32x4 pw[NP];
 #pragma unroll
@@ -251,55 +249,58 @@ __global__ __launch_bounds__((64 * SplitShape<CT, NP, DP>::NW), (SplitShape<CT, 
                         for (int p = NP - 1; p >= 0; --p) o[d] = mfma<CT>(v, pw[p], o[d]);
                     }
                 } else {
-                    add_values_one_by_one<CT, R, RB, DP>(mine + Sh::TILE, s, seen, lane, o);
+                    add_values_one_by_one<CT, R, RB, DP>(mine + (NB + n % NB) * TILE, s, seen, lane, o);
                 }
                 wait_lds();
-                if (more) load_v(next);
+                if (more) load_v(next, n + NB);
             }
         }
 
         // ---- the waves' sums joined ----
         l = groups_sum<R>(l);
-        if (g == 0) ms.m[wave][col] = m, ms.l[wave][col] = l;
+        if (g == 0 && wave < uint32_t(NW)) ms.few.m[wave][col] = m, ms.few.l[wave][col] = l;
         __syncthreads();
         float top = kNegInf, all = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) top = fmaxf(top, ms.m[w][col]);
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, ms.few.m[w][col]);
         const float weight = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
         for (int w = 0; w < NW; ++w)
-            all += ms.m[w][col] == kNegInf ? ms.l[w][col] : ms.l[w][col] * __builtin_amdgcn_exp2f(ms.m[w][col] - top);
+            all += ms.few.m[w][col] == kNegInf ? ms.few.l[w][col] : ms.few.l[w][col] * __builtin_amdgcn_exp2f(ms.few.m[w][col] - top);
         const bool whole = off == 0 && seg == b.tiles;
-        const uint32_t slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+        const uint32_t slot = 2 * work.id + (first_seg ? 0 : 1);
         if (wave == 0 && g == 0) {
-            ms.inv[col] = !whole ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
+            ms.few.inv[col] = !whole ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
             if (!whole) {
-                sc.ml[(slot * R + col) * 2] = top;
-                sc.ml[(slot * R + col) * 2 + 1] = all;
+                sc.ml[(slot * SLOT + col) * 2] = top;
+                sc.ml[(slot * SLOT + col) * 2 + 1] = all;
             }
         }
-        // 64 dims at a time: a wave's [16][64] floats in swizzled chunks of 4
+        // up to 128 dims at a time: a wave's [16][128] floats in swizzled chunks of 4
+        constexpr int DS = DB < 8 ? DB : 8;
 #pragma unroll
-        for (int d0 = 0; d0 < DB; d0 += 4) {
+        for (int d0 = 0; d0 < DB; d0 += DS) {
+            if (wave < uint32_t(NW))
 #pragma unroll
-            for (int d = 0; d < 4; ++d) *reinterpret_cast<f32x4 *>(mine + col * 256 + (((4 * d + g) ^ col) << 4)) = o[d0 + d] * weight;
+                for (int d = 0; d < DS; ++d)
+                    *reinterpret_cast<f32x4 *>(mine + col * 64 * DS + (((4 * d + g) ^ col) << 4)) = o[d0 + d] * weight;
             __syncthreads();
-            const uint32_t r = tid / 16, c = tid % 16, e = R * d0 + 4 * c;
-            f32x4 x = {0, 0, 0, 0};
+            const uint32_t r = tid / (4 * DS), c = tid % (4 * DS), e = R * d0 + 4 * c;
+            if (r0 + r < b.rows && r < R) {
+                f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < NW; ++w)
-                x += *reinterpret_cast<const f32x4 *>(lds + Sh::MISC + w * Sh::WAVE + r * 256 + ((c ^ r) << 4));
-            if (r0 + r < b.rows) {
+                for (int w = 0; w < NW; ++w)
+                    x += *reinterpret_cast<const f32x4 *>(lds + kMisc + w * Sh::WAVE + r * 64 * DS + ((c ^ r) << 4));
                 if (!whole)
-                    *reinterpret_cast<f32x4 *>(sc.o + (uint64_t(slot) * R + r) * DP + e) = x;
+                    *reinterpret_cast<f32x4 *>(sc.o + (uint64_t(slot) * SLOT + r) * DP + e) = x;
                 else if (e < D)
-                    store4(a, b.begin, kvh, r0 + r, e, x * ms.inv[r]);
+                    store4(a, b.begin, kvh, r0 + r, e, x * ms.few.inv[r]);
             }
             __syncthreads();
         }
         // this workgroup has the rows' first tiles but not their last: the join is on its list
         if (off == 0 && !whole && tid == 0)
-            sc.jobs[blockIdx.x] = SplitJob{seq, r0, kvh, 1 + uint32_t((b.tiles - seg + part - 1) / part), slot};
+            sc.jobs[work.id] = SplitJob{seq, r0, kvh, R, 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= seg;
         first_seg = false;
         if (left != 0) next_block<R>(a, rg, b.rows, pl);

@@ -1,7 +1,7 @@
 // tc_attn_inst.hip -- the attention kernels for one cache type (TC_ATTN_CACHE, one
 // object each), and the choice of the number of pieces and the padded head size.
-#include "tc_attn_split.hpp"
-#include "tc_attn_tile.hpp"
+#include "tc_attn_few.hpp"
+#include "tc_attn_many.hpp"
 
 #ifndef TC_ATTN_CACHE
 #define TC_ATTN_CACHE 30
@@ -10,54 +10,71 @@
 namespace tc {
 namespace {
 
+// One launch for a batch of any mix: sequences of few rows make one line of tiles,
+// those of many another, and the workgroups are shared out between the two as their
+// tiles are (a tile of either takes about as long: 16 KB through HBM on one of 256
+// CUs, or 256 rows' products). `kinds`: bit 0 and 1, which of them the call's size
+// allows at all.
 template <int CT, int NP, int DP>
-hipError_t split(const AttnArgs &a, RowRange rg, int num_cu, void *scratch, hipStream_t st) {
-    using Sh = SplitShape<CT, NP, DP>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn_split<CT, NP, DP>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS);
-    if (attr != hipSuccess) return attr;
-    const uint32_t grid = Sh::OCC * num_cu;
-    const SplitScratch sc = split_scratch(scratch, grid, Sh::R);
-    k_attn_split<CT, NP, DP><<<grid, 64 * Sh::NW, Sh::LDS, st>>>(a, rg, sc);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    k_attn_join<DP, Sh::R><<<dim3(grid, Sh::R / 4), 256, 0, st>>>(a, sc);
-    return hipGetLastError();
-}
-
-template <int CT, int NP, int DP>
-hipError_t tile(const AttnArgs &a, RowRange rg, int num_cu, void *scratch, hipStream_t st) {
-    using Sh = TileShape<CT, NP, DP>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn_tile<CT, NP, DP>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS);
-    if (attr != hipSuccess) return attr;
-    const uint32_t grid = Sh::OCC * num_cu;
-    const SplitScratch sc = split_scratch(scratch, grid, Sh::ROWS);
-    k_attn_tile<CT, NP, DP><<<grid, 64 * Sh::NW, Sh::LDS, st>>>(a, rg, sc);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    k_attn_join<DP, Sh::ROWS><<<dim3(grid, Sh::ROWS / 4), 256, 0, st>>>(a, sc);
-    return hipGetLastError();
-}
-
-// Sequences of few rows and of many go to different kernels. The lengths are the
-// device's, so both are launched unless the call's size rules one out; a kernel
-// without work ends at once.
-template <int CT, int NP, int DP>
-hipError_t both(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
-    const uint64_t most = uint64_t(a.kv.n_tokens) * a.group;
-    if (a.kv.n_seq > 1 || most <= kSplitRows) {
-        const hipError_t e = split<CT, NP, DP>(a, RowRange{1, kSplitRows}, num_cu, scratch, st);
-        if (e != hipSuccess || most <= kSplitRows) return e;
+__global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, SplitScratch sc) {
+    using Many = ManyShape<CT, NP, DP>;
+    constexpr int SLOT = Many::ROWS;
+    constexpr RowRange few{1, kFewRows}, many{kFewRows + 1, ~0u};
+    extern __shared__ __align__(1024) unsigned char lds[];
+    Misc &ms = *reinterpret_cast<Misc *>(lds);
+    const uint32_t tid = threadIdx.x, b = blockIdx.x, parts = gridDim.x;
+    Line lf{}, lm{};
+    if (kinds & 1) lf = line_scan<16, kTileTokens, kThreads>(a, few, ms.line, tid);
+    if (kinds & 2) lm = line_scan<Many::ROWS, kTileTokens, kThreads>(a, many, ms.line, tid);
+    const uint64_t all = lf.per_head + lm.per_head;
+    if (all == 0) {
+        if (tid == 0) sc.jobs[b].count = 0;
+        return;
     }
-    return tile<CT, NP, DP>(a, RowRange{a.kv.n_seq > 1 ? kSplitRows + 1 : 1, ~0u}, num_cu, scratch, st);
+    uint32_t nm = uint32_t((lm.per_head * parts + all / 2) / all);  // workgroups for the second line, spread evenly
+    if (lf.per_head != 0 && nm == parts) nm = parts - 1;
+    if (lm.per_head != 0 && nm == 0) nm = 1;
+    const uint32_t before = uint32_t(uint64_t(b) * nm / parts);
+    Part w;
+    if (uint64_t(b + 1) * nm / parts == before) {
+        const uint32_t index = b - before;
+        w.at = line_part<16, kTileTokens>(a, few, lf, index, parts - nm, FewShape<CT, NP, DP>::NW, ms.line, &w.part, &w.left);
+        w.id = index;
+        if (tid == 0) sc.jobs[w.id].count = 0;
+        attn_few<CT, NP, DP, SLOT>(a, few, sc, w, lds, ms);
+    } else {
+        // (workgroups of one XCD, every eighth, take parts next to each other)
+        const uint32_t index = nm == parts && parts % 8 == 0 ? b % 8 * (parts / 8) + b / 8 : before;
+        w.at = line_part<Many::ROWS, kTileTokens>(a, many, lm, index, nm, 4, ms.line, &w.part, &w.left);
+        w.id = parts - nm + index;
+        if (tid == 0) sc.jobs[w.id].count = 0;
+        attn_many<CT, NP, DP, SLOT>(a, many, sc, w, lds, ms);
+    }
+}
+
+template <int CT, int NP, int DP>
+hipError_t launch(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
+    constexpr int SLOT = ManyShape<CT, NP, DP>::ROWS;
+    constexpr int few = FewShape<CT, NP, DP>::LDS, many = ManyShape<CT, NP, DP>::LDS, lds = few > many ? few : many;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn<CT, NP, DP>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (attr != hipSuccess) return attr;
+    // a sequence has up to n_tokens rows' tokens, the only one all of them
+    const uint64_t most = uint64_t(a.kv.n_tokens) * a.group;
+    const int kinds = (a.kv.n_seq > 1 || most <= kFewRows ? 1 : 0) | (most > kFewRows ? 2 : 0);
+    const SplitScratch sc = split_scratch(scratch, num_cu, SLOT);
+    k_attn<CT, NP, DP><<<num_cu, kThreads, lds, st>>>(a, kinds, sc);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_attn_join<DP, SLOT><<<dim3(num_cu, 8), kThreads, 0, st>>>(a, sc);
+    return hipGetLastError();
 }
 
 template <int CT, int NP>
 hipError_t by_dim(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) {
-    if (a.kv.dim <= 64) return both<CT, NP, 64>(a, num_cu, scratch, st);
-    if (a.kv.dim <= 128) return both<CT, NP, 128>(a, num_cu, scratch, st);
-    return both<CT, NP, 256>(a, num_cu, scratch, st);
+    if (a.kv.dim <= 64) return launch<CT, NP, 64>(a, num_cu, scratch, st);
+    if (a.kv.dim <= 128) return launch<CT, NP, 128>(a, num_cu, scratch, st);
+    return launch<CT, NP, 256>(a, num_cu, scratch, st);
 }
 
 }  // namespace

@@ -471,22 +471,36 @@ __device__ __forceinline__ T block_scan(T v, LineMisc &lm, uint32_t tid, T *all)
     return v;
 }
 
-// This workgroup's part: where it starts and its number of tiles (0: none); *part:
-// that of every workgroup but the last ones, at least min_part.
+// A line as one thread sees it: its blocks' tiles, and where they lie.
+struct Line {
+    uint32_t s, r0;      // its first block
+    uint64_t tiles, incl;  // its tiles; with those of the threads before it
+    uint64_t per_head;   // all of one head
+};
+template <int ROWS>
+__device__ __forceinline__ void line_step(const AttnArgs &a, RowRange rg, uint32_t &s, uint32_t &r0) {  // to the next block, if any
+    uint32_t begin;
+    r0 += ROWS;
+    if (r0 >= seq_row_count(a, rg, s, &begin)) {
+        r0 = 0;
+        do ++s;
+        while (s < a.kv.n_seq && seq_row_count(a, rg, s, &begin) == 0);
+    }
+}
 template <int ROWS, int TOKENS, int THREADS>
-__device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, uint32_t index, uint32_t parts, uint32_t min_part,
-                                           LineMisc &lm, uint32_t tid, uint64_t *part, uint64_t *left) {
+__device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMisc &lm, uint32_t tid) {
     const uint32_t per = (a.kv.n_seq + THREADS - 1) / THREADS;
     const uint32_t s0 = min(tid * per, a.kv.n_seq), s1 = min(s0 + per, a.kv.n_seq);
     uint32_t mine = 0, begin;
     for (uint32_t s = s0; s < s1; ++s) mine += (seq_row_count(a, rg, s, &begin) + ROWS - 1) / ROWS;
     uint32_t n_blocks;
-    lm.blocks[tid] = block_scan<uint32_t, THREADS>(mine, lm, tid, &n_blocks);
+    const uint32_t upto = block_scan<uint32_t, THREADS>(mine, lm, tid, &n_blocks);
+    lm.blocks[tid] = upto;
     __syncthreads();
+    Line ln{0, 0, 0, 0, 0};
     // the tiles of this thread's blocks
     const uint32_t q = (n_blocks + THREADS - 1) / THREADS;
     const uint32_t f0 = min(tid * q, n_blocks), f1 = min(f0 + q, n_blocks);
-    uint32_t s = 0, r0 = 0;
     if (f0 < f1) {
         uint32_t x = 0, y = THREADS - 1;  // the first thread whose sequences reach past block f0
         while (x < y) {
@@ -497,45 +511,42 @@ __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, uint3
                 x = mid + 1;
         }
         uint32_t skip = f0 - (x != 0 ? lm.blocks[x - 1] : 0);
-        for (s = x * per;; ++s) {
-            const uint32_t nb = (seq_row_count(a, rg, s, &begin) + ROWS - 1) / ROWS;
+        for (ln.s = x * per;; ++ln.s) {
+            const uint32_t nb = (seq_row_count(a, rg, ln.s, &begin) + ROWS - 1) / ROWS;
             if (skip < nb) break;
             skip -= nb;
         }
-        r0 = skip * ROWS;
-    }
-    auto step = [&](uint32_t &s, uint32_t &r0) {  // to the next block, where there is one
-        r0 += ROWS;
-        if (r0 >= seq_row_count(a, rg, s, &begin)) {
-            r0 = 0;
-            do ++s;
-            while (s < a.kv.n_seq && seq_row_count(a, rg, s, &begin) == 0);
-        }
-    };
-    uint64_t tiles = 0;
-    {
-        uint32_t u = s, v = r0;
+        ln.r0 = skip * ROWS;
+        uint32_t u = ln.s, v = ln.r0;
         for (uint32_t f = f0; f < f1; ++f) {
-            tiles += row_block<ROWS, TOKENS>(a, u, v).tiles;
-            if (f + 1 < f1) step(u, v);
+            ln.tiles += row_block<ROWS, TOKENS>(a, u, v).tiles;
+            if (f + 1 < f1) line_step<ROWS>(a, rg, u, v);
         }
     }
-    uint64_t per_head;
-    const uint64_t incl = block_scan<uint64_t, THREADS>(tiles, lm, tid, &per_head);
-    const uint64_t total = per_head * a.kv.kv_heads;
+    ln.incl = block_scan<uint64_t, THREADS>(ln.tiles, lm, tid, &ln.per_head);
+    return ln;
+}
+
+// Part `index` of `parts` (of at least min_part tiles each): where it starts, and its
+// number of tiles (0: none); *part: that of every part but the last ones.
+template <int ROWS, int TOKENS>
+__device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const Line &ln, uint32_t index, uint32_t parts,
+                                           uint32_t min_part, LineMisc &lm, uint64_t *part, uint64_t *left) {
+    const uint64_t total = ln.per_head * a.kv.kv_heads;
     *part = max((total + parts - 1) / parts, uint64_t(min_part));
     const uint64_t at = *part * index;
     *left = at < total ? min(*part, total - at) : 0;
     if (*left != 0) {
-        const uint32_t kvh = uint32_t(at / per_head);
-        uint64_t target = at - kvh * per_head;
-        if (target >= incl - tiles && target < incl) {
-            target -= incl - tiles;
+        const uint32_t kvh = uint32_t(at / ln.per_head);
+        uint64_t target = at - kvh * ln.per_head;
+        if (target >= ln.incl - ln.tiles && target < ln.incl) {
+            target -= ln.incl - ln.tiles;
+            uint32_t s = ln.s, r0 = ln.r0;
             for (;;) {
                 const uint32_t t = row_block<ROWS, TOKENS>(a, s, r0).tiles;
                 if (target < t) break;
                 target -= t;
-                step(s, r0);
+                line_step<ROWS>(a, rg, s, r0);
             }
             lm.at = Place{s, r0, kvh, uint32_t(target)};
         }
@@ -642,40 +653,84 @@ __device__ __forceinline__ float load_q(const AttnArgs &a, uint32_t begin, uint3
     return fmaxf(ldexpf(1.4426950408889634f * a.scale, e), 0x1p-126f);
 }
 
+// ---- the kernel's shape ---------------------------------------------------------
+// 8 waves, one workgroup per CU; the small things first in LDS.
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kMisc = 8192, kLds = 160 * 1024;
+struct Misc {
+    LineMisc line;
+    RunMisc<512> runs;
+    union {
+        struct {
+            float m[kWaves][16], l[kWaves][16], inv[16];
+        } few;
+        struct {
+            float kf[4][32], lv[4][32], iv[4][32];  // factors of a tile's keys; log2 and reciprocal of the values'
+        } many;
+    };
+};
+static_assert(sizeof(Misc) <= kMisc, "");
+
+// What a workgroup has to do: a part of a line.
+struct Part {
+    Place at;
+    uint64_t part, left;
+    uint32_t id;  // of all parts
+};
+
 // ---- the join ----------------------------------------------------------------
-// Blocks of ROWS rows split over several workgroups: rows [4 y, 4 y + 4) of the
-// block that part x has on the list.
-template <int DP, int ROWS>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, SplitScratch sc) {
+// Blocks of rows split over several parts: of the block that part x has on the list
+// the rows y, y + 8, ... A wave takes a row where there are few parts to add, all of
+// them share one where there are many.
+template <int DP, int SLOT>
+__global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, SplitScratch sc) {
     const SplitJob job = sc.jobs[blockIdx.x];
     if (job.count == 0) return;
+    __shared__ float part_x[kWaves][DP], part_l[kWaves];
     uint32_t begin, end;
     seq_rows(a.kv.start, a.kv.n_tokens, job.seq, &begin, &end);
-    const uint32_t r = 4 * blockIdx.y + threadIdx.x / 64, row = job.r0 + r, lane = threadIdx.x & 63;
-    if (row >= (end - begin) * a.group) return;
-    auto slot = [&](uint32_t i) { return i == 0 ? job.slot : 2 * (blockIdx.x + i); };
-    float top = kNegInf;
-    for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[(slot(i) * ROWS + r) * 2]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t rows = min(job.rows, (end - begin) * a.group - job.r0);
+    const bool shared = job.count > 16;
     constexpr int N = DP / 64;
-    float x[N], all = 0.0f;
+    auto slot = [&](uint32_t i) { return i == 0 ? job.slot : 2 * (blockIdx.x + i); };
+    for (uint32_t r0 = blockIdx.y; r0 < rows; r0 += shared ? 8 : 8 * kWaves) {
+        const uint32_t r = shared ? r0 : r0 + 8 * wave;
+        if (!shared && r >= rows) break;
+        float top = kNegInf;
+        for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[(slot(i) * SLOT + r) * 2]);
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = 0.0f;
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        float x[N], all = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = 0.0f;
 #pragma unroll 8
-    for (uint32_t i = 0; i < job.count; ++i) {
-        const uint32_t sl = slot(i);
-        const float m = sc.ml[(sl * ROWS + r) * 2], l = sc.ml[(sl * ROWS + r) * 2 + 1];
-        const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
-        all = fmaf(w, l, all);
-        const float *p = sc.o + (uint64_t(sl) * ROWS + r) * DP + N * lane;
+        for (uint32_t i = shared ? wave : 0; i < job.count; i += shared ? kWaves : 1) {
+            const uint32_t at = slot(i) * SLOT + r;
+            const float m = sc.ml[at * 2], l = sc.ml[at * 2 + 1];
+            const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
+            all = fmaf(w, l, all);
+            const float *p = sc.o + uint64_t(at) * DP + N * lane;
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = fmaf(w, p[k], x[k]);
+            for (int k = 0; k < N; ++k) x[k] = fmaf(w, p[k], x[k]);
+        }
+        if (shared) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k) part_x[wave][N * lane + k] = x[k];
+            if (lane == 0) part_l[wave] = all;
+            __syncthreads();
+            if (wave != 0) continue;
+            for (int w = 1; w < kWaves; ++w) {
+                all += part_l[w];
+#pragma unroll
+                for (int k = 0; k < N; ++k) x[k] += part_x[w][N * lane + k];
+            }
+        }
+        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (N * lane + k < a.kv.dim) store1(a, begin, job.kvh, job.r0 + r, N * lane + k, x[k] * inv);
     }
-    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-        if (N * lane + k < a.kv.dim) store1(a, begin, job.kvh, row, N * lane + k, x[k] * inv);
 }
 
 }  // namespace

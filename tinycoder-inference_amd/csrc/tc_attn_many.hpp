@@ -1,4 +1,4 @@
-// tc_attn_tile.hpp -- attention of many rows per key/value head: prompts. Bound by
+// tc_attn_many.hpp -- attention of many rows per key/value head: prompts. Bound by
 // the matrix cores and the exponentials between their products.
 //
 // A workgroup takes 32 (or 16) rows per wave of one key/value head, which go over its tiles
@@ -18,53 +18,34 @@ namespace tc {
 namespace {
 
 template <int CT, int NP, int DP>
-struct TileShape {
+struct ManyShape {
     static constexpr int LT = CT == kBF16 ? kBF16 : kF16;  // element type in LDS
     static constexpr int RB = 2 * DP;
     static constexpr int TILE = kTileTokens * RB;
     // 32 rows per wave where the sums and q leave room in the registers, else 16
     static constexpr int R = NP == 1 && DP <= 128 ? 32 : 16;
-    static constexpr int NW = 8;
-    static constexpr int OCC = 1;
-    static constexpr int ROWS = R * NW;
-    static constexpr int STRETCH = 512;
+    static constexpr int ROWS = R * kWaves;
     static constexpr int NBUF = 4;
-    static constexpr int MISC = 8192;
-    static constexpr int LDS = MISC + 2 * NBUF * TILE;
+    static constexpr int LDS = kMisc + 2 * NBUF * TILE;
 };
-
-struct TileMisc {
-    float kf[4][32], lv[4][32], iv[4][32];  // factors of a tile's keys; log2 and reciprocal of the values'
-    LineMisc line;
-    RunMisc<512> runs;
-};
-static_assert(sizeof(TileMisc) <= 8192, "");
 
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int CT, int NP, int DP>
-__global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP, DP>::OCC)) void k_attn_tile(AttnArgs a, RowRange rg, SplitScratch sc) {
-    using Sh = TileShape<CT, NP, DP>;
-    constexpr int R = Sh::R, LT = Sh::LT, RB = Sh::RB, NW = Sh::NW, TILE = Sh::TILE, NBUF = Sh::NBUF;
+template <int CT, int NP, int DP, int SLOT>
+__device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
+    using Sh = ManyShape<CT, NP, DP>;
+    constexpr int R = Sh::R, LT = Sh::LT, RB = Sh::RB, NW = kWaves, TILE = Sh::TILE, NBUF = Sh::NBUF, STRETCH = 512;
     using Ge = Geo<R, DP>;
     constexpr int KS = Ge::KS, DB = Ge::DB, NS = Ge::NS, NA = Ge::NA, AE = Ge::AE;
     constexpr uint32_t ALL = (1u << NS) - 1;
-    constexpr int THREADS = 64 * NW;
     constexpr bool SCALED = scaled_type(CT);
-    extern __shared__ __align__(1024) unsigned char lds[];
-    TileMisc &ms = *reinterpret_cast<TileMisc *>(lds);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane % R, g = lane / R;
-    const uint32_t kbuf = lds_addr(lds) + Sh::MISC, vbuf = kbuf + NBUF * TILE;
+    const uint32_t kbuf = lds_addr(lds) + kMisc, vbuf = kbuf + NBUF * TILE;
     const uint32_t D = a.kv.dim, rowbytes = D * (SCALED ? 1 : 2);
 
-    // workgroups of one XCD (every eighth) take parts next to each other
-    const uint32_t n_parts = gridDim.x, eighth = n_parts / 8;
-    const uint32_t index = n_parts % 8 == 0 ? blockIdx.x % 8 * eighth + blockIdx.x / 8 : blockIdx.x;
-    uint64_t part, left;
-    Place pl = line_part<Sh::ROWS, kTileTokens, THREADS>(a, rg, index, n_parts, 4, ms.line, tid, &part, &left);
-    if (tid == 0) sc.jobs[index].count = 0;
-
+    Place pl = work.at;
+    uint64_t left = work.left;
     bool first_seg = true;
     while (left != 0) {
         const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
@@ -133,9 +114,9 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
                 }
         };
 
-        for (uint32_t t0 = off; t0 < off + seg; t0 += Sh::STRETCH) {
-        const uint32_t t1 = min(off + seg, t0 + Sh::STRETCH);
-        find_runs<THREADS>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.hi, t1 - t0, ms.runs, tid);
+        for (uint32_t t0 = off; t0 < off + seg; t0 += STRETCH) {
+        const uint32_t t1 = min(off + seg, t0 + STRETCH);
+        find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.hi, t1 - t0, ms.runs, tid);
         __syncthreads();
         const bool missing = ms.runs.missing != 0;
 
@@ -145,8 +126,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
         constexpr int MINE = 2 * LOADS / NW;                                   // a wave's
         static_assert(2 * LOADS % NW == 0, "");
         constexpr uint32_t CHUNKS = 2 * kTileTokens * DP / 16;  // 16-byte loads of a tile, 8-bit types
-        constexpr int RAW = SCALED ? (CHUNKS + THREADS - 1) / THREADS : 1;  // a thread's
-        static_assert(CHUNKS < THREADS || CHUNKS % THREADS == 0, "");
+        constexpr int RAW = SCALED ? (CHUNKS + kThreads - 1) / kThreads : 1;  // a thread's
+        static_assert(CHUNKS < kThreads || CHUNKS % kThreads == 0, "");
         u32x4 raw[RAW];
         float raw_scale = 0.0f;
         auto load = [&](uint32_t t) __attribute__((always_inline)) {
@@ -165,14 +146,14 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
                     dma16((val ? vbuf : kbuf) + buf * TILE + i * 1024, src, rh * rowbytes + (16 * c < rowbytes ? 16 * c : 0));
                 }
             } else {
-                // 16 bytes (16 dims) of one row per load: THREADS / (DP / 16) rows at a time, keys then values
+                // 16 bytes (16 dims) of one row per load: kThreads / (DP / 16) rows at a time, keys then values
 #pragma unroll
                 for (int j = 0; j < RAW; ++j) {
-                    const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
+                    const uint32_t f = tid + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
                     const bool val = rr >= kTileTokens;
                     const uint32_t r = rr % kTileTokens;
                     const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(r >= 16 ? w.run[1] : w.run[0]) * run_bytes + r % 16 * rowbytes;
-                    if (CHUNKS >= THREADS || f < CHUNKS) raw[j] = *reinterpret_cast<const u32x4 *>(src + (16 * c < rowbytes ? 16 * c : 0));
+                    if (CHUNKS >= kThreads || f < CHUNKS) raw[j] = *reinterpret_cast<const u32x4 *>(src + (16 * c < rowbytes ? 16 * c : 0));
                 }
                 if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + lane % 16];
             }
@@ -182,11 +163,11 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
             const uint32_t buf = (t - t0) % NBUF;
 #pragma unroll
             for (int j = 0; j < RAW; ++j) {
-                const uint32_t f = tid + THREADS * j, c = f % (DP / 16), rr = f / (DP / 16);
-                if (CHUNKS < THREADS && f >= CHUNKS) break;
+                const uint32_t f = tid + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
+                if (CHUNKS < kThreads && f >= CHUNKS) break;
                 const bool val = rr >= kTileTokens;
                 const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r);
-                unsigned char *dst = lds + Sh::MISC + ((val ? NBUF : 0) + buf) * TILE + r * RB;
+                unsigned char *dst = lds + kMisc + ((val ? NBUF : 0) + buf) * TILE + r * RB;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const u32x2 x = widen<CT>(raw[j][2 * e]), y = widen<CT>(raw[j][2 * e + 1]);
@@ -195,12 +176,12 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
             }
             if (tid < 64) {
                 if (lane < 32) {
-                    ms.kf[buf][lane] = raw_scale;
+                    ms.many.kf[buf][lane] = raw_scale;
                 } else {
                     // (a factor of 0: values of next to nothing; NaN stays)
                     const float x = raw_scale == raw_scale ? fmaxf(raw_scale, 0x1p-126f) : raw_scale;
-                    ms.lv[buf][lane - 32] = __builtin_amdgcn_logf(x);
-                    ms.iv[buf][lane - 32] = __builtin_amdgcn_rcpf(x);
+                    ms.many.lv[buf][lane - 32] = __builtin_amdgcn_logf(x);
+                    ms.many.iv[buf][lane - 32] = __builtin_amdgcn_rcpf(x);
                 }
             }
         };
@@ -216,8 +197,8 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
         auto token_factors = [&](uint32_t buf, float (&x)[NS]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < NS; i += 4) {
-                const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.kf[buf] + token_of_reg<R>(i, g));
-                const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.lv[buf] + token_of_reg<R>(i, g));
+                const f32x4 kf = *reinterpret_cast<const f32x4 *>(ms.many.kf[buf] + token_of_reg<R>(i, g));
+                const f32x4 lf = *reinterpret_cast<const f32x4 *>(ms.many.lv[buf] + token_of_reg<R>(i, g));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[i + j] = fmaf(x[i + j] * factor, kf[j], lf[j]);
             }
@@ -330,7 +311,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
             };
             float sn[NS], most = kNegInf, sum[2] = {0.0f, 0.0f};
             pack(0);
-            int added = 0;
+            int added = 0, compared = 0;
 #pragma unroll
             for (int i = 0; i < VALS; ++i) {
                 constexpr int half = VALS / 2;
@@ -342,7 +323,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
 #pragma unroll
                 for (; added < NS * (i + 1) / VALS; ++added)
                     if constexpr (SCALED)
-                        sum[added % 2] = fmaf(s[added], ms.iv[buf][token_of_reg<R>(added, g)], sum[added % 2]);
+                        sum[added % 2] = fmaf(s[added], ms.many.iv[buf][token_of_reg<R>(added, g)], sum[added % 2]);
                     else if constexpr (NP > 1)
                         sum[added % 2] += s[added];
                     else if (added % 2 == 1)
@@ -352,11 +333,10 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
                     for (int j = 0; j < NS; ++j) sn[j] = y[j / AE][j % AE];
                     if constexpr (SCALED) token_factors(nbuf, sn);
                 }
-                if (i >= half) {
-                    constexpr int per = NS / (VALS - half);
+                if (i >= half)
 #pragma unroll
-                    for (int j = (i - half) * per; j < (i - half + 1) * per; j += 2) most = max3(most, sn[j], sn[j + 1]);
-                }
+                    for (; compared + 2 <= NS * (i - half + 1) / (VALS - half); compared += 2)
+                        most = max3(most, sn[compared], sn[compared + 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             l += sum[0] + sum[1];
@@ -400,15 +380,15 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
                 for (int i = 0; i < NS; ++i) {
                     s[i] = exponential(s[i], ref);
                     // (the factor of a token that is not seen may be anything)
-                    const float p = SCALED ? s[i] * ms.iv[buf][token_of_reg<R>(i, g)] : s[i];
+                    const float p = SCALED ? s[i] * ms.many.iv[buf][token_of_reg<R>(i, g)] : s[i];
                     l += (seen >> i) & 1 ? p : 0.0f;
                 }
                 bool odd = false;  // values that are not finite where some row must not see them
-                if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(lds + Sh::MISC + (NBUF + buf) * TILE, lane_now());
+                if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(lds + kMisc + (NBUF + buf) * TILE, lane_now());
                 if (!odd)
                     add_values(buf);
                 else
-                    add_values_one_by_one<LT, R, RB, DP>(lds + Sh::MISC + (NBUF + buf) * TILE, s, seen, lane_now(), o);
+                    add_values_one_by_one<LT, R, RB, DP>(lds + kMisc + (NBUF + buf) * TILE, s, seen, lane_now(), o);
             }
             if (t + 1 < t1 && any_seen(t + 1)) {
                 products((buf + 1) % NBUF, s);
@@ -423,7 +403,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
         l = groups_sum<R>(l);
         const uint32_t gn = lane_now() / R;
         const bool whole = off == 0 && seg == b.tiles;
-        const uint32_t slot = 2 * index + (first_seg ? 0 : 1);
+        const uint32_t slot = 2 * work.id + (first_seg ? 0 : 1);
         if (row < b.rows) {
             if (whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -436,7 +416,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
                         if (e < D) store4(a, b.begin, kvh, row, e, x * inv);
                     }
             } else {
-                const uint64_t at = uint64_t(slot) * Sh::ROWS + row - r0;
+                const uint64_t at = uint64_t(slot) * SLOT + row - r0;
                 if (gn == 0) sc.ml[2 * at] = m, sc.ml[2 * at + 1] = l;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -448,7 +428,7 @@ __global__ __launch_bounds__((64 * TileShape<CT, NP, DP>::NW), (TileShape<CT, NP
         }
         // this workgroup has the block's first tiles but not its last: the join is on its list
         if (off == 0 && !whole && tid == 0)
-            sc.jobs[index] = SplitJob{seq, r0, kvh, 1 + uint32_t((b.tiles - seg + part - 1) / part), slot};
+            sc.jobs[work.id] = SplitJob{seq, r0, kvh, Sh::ROWS, 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= seg;
         first_seg = false;
         if (left != 0) next_block<Sh::ROWS>(a, rg, b.rows, pl);
