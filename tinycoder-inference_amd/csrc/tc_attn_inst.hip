@@ -17,6 +17,7 @@ namespace {
 // allows at all.
 template <int CT, int NP, int DP>
 __global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, SplitScratch sc) {
+    using Few = FewShape<CT, NP, DP>;
     using Many = ManyShape<CT, NP, DP>;
     constexpr int SLOT = Many::ROWS;
     constexpr RowRange few{1, kFewRows}, many{kFewRows + 1, ~0u};
@@ -24,8 +25,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, Spl
     Misc &ms = *reinterpret_cast<Misc *>(lds);
     const uint32_t tid = threadIdx.x, b = blockIdx.x, parts = gridDim.x;
     Line lf{}, lm{};
-    if (kinds & 1) lf = line_scan<16, kTileTokens, kThreads>(a, few, ms.line, tid);
-    if (kinds & 2) lm = line_scan<Many::ROWS, kTileTokens, kThreads>(a, many, ms.line, tid);
+    if (kinds & 1) lf = line_scan<Few::R, kTileTokens, Few::START, kThreads>(a, few, ms.line, tid);
+    if (kinds & 2) lm = line_scan<Many::ROWS, kTileTokens, Many::START, kThreads>(a, many, ms.line, tid);
     const uint64_t all = lf.per_head + lm.per_head;
     if (all == 0) {
         if (tid == 0) sc.jobs[b].count = 0;
@@ -38,14 +39,14 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, Spl
     Part w;
     if (uint64_t(b + 1) * nm / parts == before) {
         const uint32_t index = b - before;
-        w.at = line_part<16, kTileTokens>(a, few, lf, index, parts - nm, FewShape<CT, NP, DP>::NW, ms.line, &w.part, &w.left);
+        w.at = line_part<Few::R, kTileTokens, Few::START>(a, few, lf, index, parts - nm, Few::NW, ms.line, &w.part, &w.left);
         w.id = index;
         if (tid == 0) sc.jobs[w.id].count = 0;
         attn_few<CT, NP, DP, SLOT>(a, few, sc, w, lds, ms);
     } else {
         // (workgroups of one XCD, every eighth, take parts next to each other)
         const uint32_t index = nm == parts && parts % 8 == 0 ? b % 8 * (parts / 8) + b / 8 : before;
-        w.at = line_part<Many::ROWS, kTileTokens>(a, many, lm, index, nm, 4, ms.line, &w.part, &w.left);
+        w.at = line_part<Many::ROWS, kTileTokens, Many::START>(a, many, lm, index, nm, 4, ms.line, &w.part, &w.left);
         w.id = parts - nm + index;
         if (tid == 0) sc.jobs[w.id].count = 0;
         attn_many<CT, NP, DP, SLOT>(a, many, sc, w, lds, ms);

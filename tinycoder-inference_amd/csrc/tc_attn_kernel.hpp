@@ -98,15 +98,22 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 // Lane l's 16 (4) bytes to LDS byte dst + 16 l (4 l), asynchronously:
 // the kernel waits (vmcnt) before it reads them. Inline, so that the compiler does
 // not wait for these at every LDS read in between.
+template <bool ONCE = false>
 __device__ __forceinline__ void dma16(uint32_t dst, const void *base, uint32_t off) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     // (readfirstlane gives an int: widened as one, its sign would fill the upper half)
     const uint32_t blo = __builtin_amdgcn_readfirstlane(uint32_t(b)), bhi = __builtin_amdgcn_readfirstlane(uint32_t(b >> 32));
     const uint64_t ub = uint64_t(bhi) << 32 | blo;
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
-                 : "memory", "m0");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
+                     : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(uint32_t dst, const void *p) {  // (4 bytes of each lane's own)
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
@@ -395,7 +402,8 @@ __device__ __forceinline__ void store1(const AttnArgs &a, uint32_t begin, uint32
 // after head, in each sequence after sequence, block after block, tile after tile.
 // Workgroups take equal parts of the line, so that the load is even whatever the
 // lengths are, and blocks next to each other, which read the same keys, run on one
-// XCD at about the same time.
+// XCD at about the same time. A block begins with START places without a tile, for what
+// it costs besides its tiles (its rows, its pages, the first loads, its results).
 
 // Which sequences a launch serves: those of `least` to `most` rows (new tokens *
 // group) per key/value head.
@@ -440,8 +448,22 @@ __device__ __forceinline__ RowBlock row_block(const AttnArgs &a, uint32_t s, uin
 
 // A place on the line.
 struct Place {
-    uint32_t seq, r0, kvh, off;  // off: tiles of the block that lie before it
+    uint32_t seq, r0, kvh, off;  // off: places of the block that lie before it
 };
+
+// The stretch of a block that a part with `left` places takes from place `off` on.
+struct Segment {
+    uint32_t places, off, tiles;  // of them, the first tile and the tiles
+};
+template <int START>
+__device__ __forceinline__ Segment segment(uint32_t tiles, uint32_t off, uint64_t left) {
+    Segment g;
+    g.places = uint32_t(min(uint64_t(tiles + START - off), left));
+    const uint32_t end = off + g.places;
+    g.off = off > START ? off - START : 0;
+    g.tiles = (end > START ? end - START : 0) - g.off;
+    return g;
+}
 
 struct LineMisc {
     uint32_t blocks[512];  // blocks of the sequences up to a thread's last
@@ -471,10 +493,10 @@ __device__ __forceinline__ T block_scan(T v, LineMisc &lm, uint32_t tid, T *all)
     return v;
 }
 
-// A line as one thread sees it: its blocks' tiles, and where they lie.
+// A line as one thread sees it: its blocks' places, and where they lie.
 struct Line {
     uint32_t s, r0;      // its first block
-    uint64_t tiles, incl;  // its tiles; with those of the threads before it
+    uint64_t places, incl;  // its places; with those of the threads before it
     uint64_t per_head;   // all of one head
 };
 template <int ROWS>
@@ -487,7 +509,7 @@ __device__ __forceinline__ void line_step(const AttnArgs &a, RowRange rg, uint32
         while (s < a.kv.n_seq && seq_row_count(a, rg, s, &begin) == 0);
     }
 }
-template <int ROWS, int TOKENS, int THREADS>
+template <int ROWS, int TOKENS, int START, int THREADS>
 __device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMisc &lm, uint32_t tid) {
     const uint32_t per = (a.kv.n_seq + THREADS - 1) / THREADS;
     const uint32_t s0 = min(tid * per, a.kv.n_seq), s1 = min(s0 + per, a.kv.n_seq);
@@ -498,7 +520,7 @@ __device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMi
     lm.blocks[tid] = upto;
     __syncthreads();
     Line ln{0, 0, 0, 0, 0};
-    // the tiles of this thread's blocks
+    // the places of this thread's blocks
     const uint32_t q = (n_blocks + THREADS - 1) / THREADS;
     const uint32_t f0 = min(tid * q, n_blocks), f1 = min(f0 + q, n_blocks);
     if (f0 < f1) {
@@ -519,17 +541,17 @@ __device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMi
         ln.r0 = skip * ROWS;
         uint32_t u = ln.s, v = ln.r0;
         for (uint32_t f = f0; f < f1; ++f) {
-            ln.tiles += row_block<ROWS, TOKENS>(a, u, v).tiles;
+            ln.places += row_block<ROWS, TOKENS>(a, u, v).tiles + START;
             if (f + 1 < f1) line_step<ROWS>(a, rg, u, v);
         }
     }
-    ln.incl = block_scan<uint64_t, THREADS>(ln.tiles, lm, tid, &ln.per_head);
+    ln.incl = block_scan<uint64_t, THREADS>(ln.places, lm, tid, &ln.per_head);
     return ln;
 }
 
-// Part `index` of `parts` (of at least min_part tiles each): where it starts, and its
-// number of tiles (0: none); *part: that of every part but the last ones.
-template <int ROWS, int TOKENS>
+// Part `index` of `parts` (of at least min_part places each): where it starts, and its
+// number of places (0: none); *part: that of every part but the last ones.
+template <int ROWS, int TOKENS, int START>
 __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const Line &ln, uint32_t index, uint32_t parts,
                                            uint32_t min_part, LineMisc &lm, uint64_t *part, uint64_t *left) {
     const uint64_t total = ln.per_head * a.kv.kv_heads;
@@ -539,11 +561,11 @@ __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const
     if (*left != 0) {
         const uint32_t kvh = uint32_t(at / ln.per_head);
         uint64_t target = at - kvh * ln.per_head;
-        if (target >= ln.incl - ln.tiles && target < ln.incl) {
-            target -= ln.incl - ln.tiles;
+        if (target >= ln.incl - ln.places && target < ln.incl) {
+            target -= ln.incl - ln.places;
             uint32_t s = ln.s, r0 = ln.r0;
             for (;;) {
-                const uint32_t t = row_block<ROWS, TOKENS>(a, s, r0).tiles;
+                const uint32_t t = row_block<ROWS, TOKENS>(a, s, r0).tiles + START;
                 if (target < t) break;
                 target -= t;
                 line_step<ROWS>(a, rg, s, r0);
@@ -678,58 +700,74 @@ struct Part {
 };
 
 // ---- the join ----------------------------------------------------------------
-// Blocks of rows split over several parts: of the block that part x has on the list
-// the rows y, y + 8, ... A wave takes a row where there are few parts to add, all of
-// them share one where there are many.
+// Blocks of rows split over several parts: the rows of the block that part x has on the
+// list. Where many parts share a block a workgroup takes a row and its waves the
+// parts; where few do, DP / 4 lanes take a row.
 template <int DP, int SLOT>
 __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, SplitScratch sc) {
     const SplitJob job = sc.jobs[blockIdx.x];
     if (job.count == 0) return;
-    __shared__ float part_x[kWaves][DP], part_l[kWaves];
+    __shared__ f32x4 part_x[kWaves][64];
+    __shared__ float part_l[kWaves];
     uint32_t begin, end;
     seq_rows(a.kv.start, a.kv.n_tokens, job.seq, &begin, &end);
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t rows = min(job.rows, (end - begin) * a.group - job.r0);
-    const bool shared = job.count > 16;
-    constexpr int N = DP / 64;
-    auto slot = [&](uint32_t i) { return i == 0 ? job.slot : 2 * (blockIdx.x + i); };
-    for (uint32_t r0 = blockIdx.y; r0 < rows; r0 += shared ? 8 : 8 * kWaves) {
-        const uint32_t r = shared ? r0 : r0 + 8 * wave;
-        if (!shared && r >= rows) break;
+    constexpr uint32_t L = DP / 4;  // lanes of a row
+    const uint32_t e = 4 * (tid % L);
+    auto at_slot = [&](uint32_t i, uint32_t r) { return (i == 0 ? job.slot : 2 * (blockIdx.x + i)) * SLOT + r; };
+    auto add = [&](uint32_t i, uint32_t r, float top, f32x4 &x, float &all) __attribute__((always_inline)) {
+        const uint32_t at = at_slot(i, r);
+        const float m = sc.ml[at * 2], l = sc.ml[at * 2 + 1];
+        const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
+        all = fmaf(w, l, all);
+        const f32x4 p = *reinterpret_cast<const f32x4 *>(sc.o + uint64_t(at) * DP + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = fmaf(w, p[k], x[k]);
+    };
+    auto store = [&](uint32_t r, f32x4 x, float all) __attribute__((always_inline)) {
+        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+        if (e < a.kv.dim) store4(a, begin, job.kvh, job.r0 + r, e, x * inv);
+    };
+    if (job.count <= 8) {
+        for (uint32_t r = blockIdx.y * (kThreads / L) + tid / L; r < rows; r += gridDim.y * (kThreads / L)) {
+            float top = kNegInf, all = 0.0f;
+            for (uint32_t i = 0; i < job.count; ++i) top = fmaxf(top, sc.ml[at_slot(i, r) * 2]);
+            f32x4 x = {0, 0, 0, 0};
+#pragma unroll 4
+            for (uint32_t i = 0; i < job.count; ++i) add(i, r, top, x, all);
+            store(r, x, all);
+        }
+        return;
+    }
+    // (64 / L parts at a time in a wave)
+    constexpr uint32_t P = 64 / L;
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
         float top = kNegInf;
-        for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[(slot(i) * SLOT + r) * 2]);
+        for (uint32_t i = lane; i < job.count; i += 64) top = fmaxf(top, sc.ml[at_slot(i, r) * 2]);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        float x[N], all = 0.0f;
+        f32x4 x = {0, 0, 0, 0};
+        float all = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = wave * P + lane / L; i < job.count; i += kWaves * P) add(i, r, top, x, all);
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = 0.0f;
-#pragma unroll 8
-        for (uint32_t i = shared ? wave : 0; i < job.count; i += shared ? kWaves : 1) {
-            const uint32_t at = slot(i) * SLOT + r;
-            const float m = sc.ml[at * 2], l = sc.ml[at * 2 + 1];
-            const float w = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top);  // (no tokens: zeros)
-            all = fmaf(w, l, all);
-            const float *p = sc.o + uint64_t(at) * DP + N * lane;
+        for (uint32_t o = L; o < 64; o <<= 1) {
+            all += __shfl_xor(all, int(o));
 #pragma unroll
-            for (int k = 0; k < N; ++k) x[k] = fmaf(w, p[k], x[k]);
+            for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], int(o));
         }
-        if (shared) {
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < N; ++k) part_x[wave][N * lane + k] = x[k];
-            if (lane == 0) part_l[wave] = all;
-            __syncthreads();
-            if (wave != 0) continue;
+        __syncthreads();
+        part_x[wave][lane] = x;
+        if (lane == 0) part_l[wave] = all;
+        __syncthreads();
+        if (tid < L) {
             for (int w = 1; w < kWaves; ++w) {
                 all += part_l[w];
-#pragma unroll
-                for (int k = 0; k < N; ++k) x[k] += part_x[w][N * lane + k];
+                x += part_x[w][lane];
             }
+            store(r, x, all);
         }
-        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (N * lane + k < a.kv.dim) store1(a, begin, job.kvh, job.r0 + r, N * lane + k, x[k] * inv);
     }
 }
 

@@ -26,6 +26,7 @@ struct ManyShape {
     static constexpr int R = NP == 1 && DP <= 128 ? 32 : 16;
     static constexpr int ROWS = R * kWaves;
     static constexpr int NBUF = 4;
+    static constexpr int START = 10;  // places of a block without a tile
     static constexpr int LDS = kMisc + 2 * NBUF * TILE;
 };
 
@@ -48,9 +49,11 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
     uint64_t left = work.left;
     bool first_seg = true;
     while (left != 0) {
-        const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh, off = pl.off;
+        const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh;
         const RowBlock b = row_block<Sh::ROWS, kTileTokens>(a, seq, r0);
-        const uint32_t seg = uint32_t(min(uint64_t(b.tiles - off), left));
+        const Segment sg = segment<Sh::START>(b.tiles, pl.off, left);
+        const uint32_t off = sg.off, seg = sg.tiles;
+        if (seg == 0) break;  // (the part ends among the block's first places)
 
         // ---- the wave's rows of q ----
         const uint32_t wr0 = r0 + R * wave, row = wr0 + col;
@@ -269,9 +272,15 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         auto fast = [&](auto buf_c, uint32_t t, const uint32_t (&kp)[NA], uint32_t vp) __attribute__((always_inline)) {
             constexpr uint32_t buf = decltype(buf_c)::value, nbuf = (buf + 1) % NBUF;
             constexpr int KEYS = NA * KS, VALS = Ge::KT * DB, AHEAD = 4;
-            if constexpr (!SCALED) wait_loads<MINE>();
+            if constexpr (!SCALED) {
+                if (t + 2 < t1)
+                    wait_loads<MINE>();
+                else
+                    wait_loads<0>();
+            }
             tile_barrier();
-            if constexpr (SCALED) put(t + 2);
+            if constexpr (SCALED)
+                if (t + 2 < t1) put(t + 2);
             raise();
             const float ref = (m == kNegInf ? 0.0f : m) - kLift;
             u32x4 op[AHEAD];
@@ -297,7 +306,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
                 operand(i + AHEAD);
 #pragma unroll
                 for (; done < NS * (i + 1) / KEYS; ++done) s[done] = exponential(s[done], ref);
-                if (i == KEYS / 2) load(t + 3);
+                if (i == KEYS / 2 && t + 3 < t1) load(t + 3);
                 __builtin_amdgcn_sched_barrier(0);
             }
             u32x4 pw[Ge::KT][NP];
@@ -348,7 +357,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         for (uint32_t t = t0; t < t1;) {
             if (active && (t - t0) % NBUF == 0 && full_tile(t) && !missing) {
                 seen = ALL;
-                while (t + 6 < t1 && full_tile(t + 4)) {
+                while (t + 4 < t1 && full_tile(t + 4)) {
                     uint32_t kp[NA];
 #pragma unroll
                     for (int i = 0; i < NA; ++i) kp[i] = here(kplace[i]);
@@ -429,7 +438,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         // this workgroup has the block's first tiles but not its last: the join is on its list
         if (off == 0 && !whole && tid == 0)
             sc.jobs[work.id] = SplitJob{seq, r0, kvh, Sh::ROWS, 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
-        left -= seg;
+        left -= sg.places;
         first_seg = false;
         if (left != 0) next_block<Sh::ROWS>(a, rg, b.rows, pl);
     }
