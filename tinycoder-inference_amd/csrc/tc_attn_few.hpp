@@ -25,7 +25,7 @@ struct FewShape {
     static constexpr int NW = 2 * TILE <= 16384 ? kWaves : 4;
     static constexpr int SCALES = scaled_type(CT) ? 256 * (NB + 2) : 0;  // factors of NB + 1 tiles; log2 and reciprocal
     static constexpr int WAVE = 2 * TILE * NB + SCALES;
-    static constexpr int START = 6;  // places of a block without a tile
+    static constexpr int START = 12;  // places of a block without a tile
     static constexpr int LDS = kMisc + NW * WAVE;
     static_assert(LDS <= kLds, "");
 };

@@ -97,29 +97,34 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 
 // Lane l's 16 (4) bytes to LDS byte dst + 16 l (4 l), asynchronously:
 // the kernel waits (vmcnt) before it reads them. Inline, so that the compiler does
-// not wait for these at every LDS read in between.
+// not wait for these at every LDS read in between; m0 (the LDS address) is restored:
+// the compiler may hold a value there. The s_nop: a load takes an LDS address one wait
+// state after a scalar write of m0, and a scalar operand five after a vector instruction
+// (readfirstlane) wrote it; the compiler counts neither for inline code. ONCE: the line is not read again soon.
 template <bool ONCE = false>
 __device__ __forceinline__ void dma16(uint32_t dst, const void *base, uint32_t off) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     // (readfirstlane gives an int: widened as one, its sign would fill the upper half)
     const uint32_t blo = __builtin_amdgcn_readfirstlane(uint32_t(b)), bhi = __builtin_amdgcn_readfirstlane(uint32_t(b >> 32));
     const uint64_t ub = uint64_t(bhi) << 32 | blo;
+    uint32_t saved;
     if constexpr (ONCE)
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
-                     :
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %2, %3 nt\n\ts_mov_b32 m0, %0"
+                     : "=&s"(saved)
                      : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
-                     : "memory", "m0");
+                     : "memory");
     else
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(saved)
                      : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(ub)
-                     : "memory", "m0");
+                     : "memory");
 }
 __device__ __forceinline__ void dma4(uint32_t dst, const void *p) {  // (4 bytes of each lane's own)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
-                 :
+    uint32_t saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
                  : "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(p)
-                 : "memory", "m0");
+                 : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {

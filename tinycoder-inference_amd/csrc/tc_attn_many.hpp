@@ -26,7 +26,7 @@ struct ManyShape {
     static constexpr int R = NP == 1 && DP <= 128 ? 32 : 16;
     static constexpr int ROWS = R * kWaves;
     static constexpr int NBUF = 4;
-    static constexpr int START = 10;  // places of a block without a tile
+    static constexpr int START = 20;  // places of a block without a tile
     static constexpr int LDS = kMisc + 2 * NBUF * TILE;
 };
 
