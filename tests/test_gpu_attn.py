@@ -223,6 +223,54 @@ def test_attn_rows_that_see_nothing(tc, dev):
 
 
 @pytest.mark.parametrize("ctype", CTYPES)
+@pytest.mark.parametrize("n", [2, 120])
+def test_attn_table_ends_inside_a_tile(tc, dev, ctype, n):
+    """Lengths past what the table has room for, which ends in the middle of 32 tokens; a page missing between others."""
+    rng = np.random.default_rng(11)
+    b = Batch(rng, [(n, 200), (n, 190), (n, 150)], 16, 1, 64, ctype, width=5)
+    b.table[1, 2] = -1
+    b.table[2, 1:3] = b.n_pages + 7
+    check_attn(tc, dev, b.to(dev), 4, "F32", 0.125)
+
+
+@pytest.mark.parametrize("n_seq", [511, 512, 513, 1300])
+def test_attn_many_sequences(tc, dev, n_seq):
+    """Sequences of no, one and several rows among many; two of them prompts."""
+    rng = np.random.default_rng(n_seq)
+    new = rng.choice([0, 1, 1, 1, 3], n_seq)
+    new[[2, n_seq - 1]] = 40, 36
+    seqs = [(int(n), int(n + rng.integers(0, 30))) for n in new]
+    b = Batch(rng, seqs, 16, 2, 32, "F16", pad_rows=3).to(dev)
+    check_attn(tc, dev, b, 4, "F32", 0.2)
+    none = Batch(rng, [(0, 5)] * n_seq, 16, 2, 32, "F16", pad_rows=4).to(dev)
+    check_attn(tc, dev, none, 4, "F32", 0.2)
+
+
+@pytest.mark.parametrize("ctype", ["F16", "I8"])
+@pytest.mark.parametrize("n", [1, 80])
+def test_attn_long_parts(tc, dev, ctype, n):
+    """As many heads as there are compute units, so that each takes thousands of tokens."""
+    rng = np.random.default_rng(12)
+    H, D, total = 256, 16, 20001
+    b = Batch(rng, [(n, total)], 48, H, D, ctype).to(dev)
+    q = rows_of(rng, n, H, D, "F32")
+    got = tc.attn(b.cache, b.batch, q.to(dev), 0.25).double().cpu().numpy()
+    at = np.arange(total)
+    pg, sl = torch.from_numpy(b.table[0, at // 48].astype(np.int64)).to(dev), torch.from_numpy(at % 48).to(dev)
+    seen = torch.arange(total, device=dev)[None] <= torch.arange(total - n, total, device=dev)[:, None]
+    for h in range(0, H, 37):
+        k, v = (b.dev[x][pg, h, sl].double() for x in ("k", "v"))
+        if ctype == "I8":
+            k, v = (x * b.dev[c][pg, h, sl].double()[:, None] for x, c in ((k, "k_scale"), (v, "v_scale")))
+        x = q[:, h].double().to(dev)
+        p = torch.softmax((x @ k.T * 0.25).masked_fill(~seen, float("-inf")), 1)
+        absv = seen.double() @ v.abs()
+        terms = (x.abs() @ k.abs().T * 0.25).masked_fill(~seen, 0).amax(1, keepdim=True)
+        want, mass, absv, terms = (y.cpu().numpy() for y in (p @ v, p @ v.abs(), absv, terms))
+        assert (np.abs(got[:, h] - want) <= attn_bound("F32", ctype, D, total, want, mass, terms, absv)).all(), h
+
+
+@pytest.mark.parametrize("ctype", CTYPES)
 @pytest.mark.parametrize("n", [1, 3, 70])
 def test_attn_ignores_what_it_does_not_see(tc, dev, ctype, n):
     """Infinities and NaN behind a sequence's end, in free pages and in tokens that a row does not see change

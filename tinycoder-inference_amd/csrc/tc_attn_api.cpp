@@ -127,9 +127,11 @@ int tc_attn(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, const
     a.out = out;
     a.heads = heads;
     a.group = heads / a.kv.kv_heads;
+    a.group_div = tc::make_divmod(a.group);
     a.q_stride = n > 1 ? q_stride : heads * a.kv.dim;
     a.scale = scale;
-    a.window = window;
+    a.cap = int32_t(std::min(uint64_t(a.kv.table_pages) * a.kv.page, uint64_t(tc::kMaxPos - 64)));
+    a.span = window == 0 ? INT32_MAX : int32_t(std::min(window, uint32_t(INT32_MAX)));
     a.xtype = xtype;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int num_cu = tc::device_cu_count();

@@ -77,9 +77,11 @@ struct AttnArgs {
     const void *q;
     void *out;
     uint32_t heads, group;  // query heads, query heads per key/value head
+    DivMod group_div;
     uint32_t q_stride;
     float scale;
-    uint32_t window;
+    int32_t cap;   // tokens that the table has room for
+    int32_t span;  // tokens that a row sees at most: the window
     int xtype;
 };
 size_t attn_scratch_bytes(uint32_t heads, uint32_t n_tokens, int num_cu);
@@ -98,7 +100,7 @@ hipError_t launch_attn_cache<kE4M3>(const AttnArgs &a, int num_cu, void *scratch
 
 // A block of rows whose tiles lie in several parts.
 struct SplitJob {
-    uint32_t seq, r0, kvh;
+    uint32_t begin, r0, kvh;  // the sequence's first token row; the block's first row
     uint32_t rows;   // of the block
     uint32_t count;  // parts, from this one on (0: none)
     uint32_t slot;   // where the first one's sums are; the others': 2 * part

@@ -31,7 +31,7 @@ struct FewShape {
 };
 
 template <int CT, int NP, int DP, int SLOT>
-__device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
+__device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs seqs, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
     using Sh = FewShape<CT, NP, DP>;
     constexpr int R = Sh::R, ES = Sh::ES, RB = Sh::RB, NW = Sh::NW, NB = Sh::NB, TILE = Sh::TILE;
     using Ge = Geo<R, DP>;
@@ -51,16 +51,19 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const S
     bool first_seg = true;
     while (left != 0) {
         const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh;
-        const RowBlock b = row_block<R, kTileTokens>(a, seq, r0);
+        const RowBlock b = row_block<R, kTileTokens>(a, seqs.uniform(a, seq), r0);
         const Segment sg = segment<Sh::START>(b.tiles, pl.off, left);
         const uint32_t off = sg.off, seg = sg.tiles;
         if (seg == 0) break;  // (the part ends among the block's first places)
 
         const uint32_t row = r0 + col;
-        u32x4 q[NP][KS];
-        const float factor = load_q<CT, NP, R, DP, ES>(a, b.begin, kvh, row, b.rows, g, q);
-        const int32_t pos = row < b.rows ? b.pos0 + int32_t(row / a.group) : -1;  // the lane's row sees tokens up to here
-        const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
+        u32x4 raw_q[f32_rows<CT, NP>() ? 2 : 1][KS], q[NP][KS];
+        fetch_q<CT, NP, R, DP, ES>(a, b.begin, kvh, row, b.rows, g, raw_q);
+        find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(off), b.last, min(seg, 512u), ms.runs, tid);
+        __syncthreads();
+        const float factor = make_q<CT, NP, R, DP>(a, raw_q, q);
+        const int32_t pos = row < b.rows ? b.pos0 + int32_t(div_fast(row, a.group_div)) : -1;  // the lane's row sees tokens up to here
+        const int32_t from = max(0, max(pos, -1) + 1 - a.span);
 
         constexpr int LPR = RB / 16, RPI = 64 / LPR;  // lanes per row, rows per load
         constexpr int LOADS = 2 * (16 / RPI);         // loads of a tile of keys or values
@@ -103,9 +106,11 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const S
 
         for (uint32_t c0 = off; c0 < off + seg; c0 += 512) {
             const uint32_t t_end = min(off + seg, c0 + 512);
-            __syncthreads();
-            find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.hi, t_end - c0, ms.runs, tid);
-            __syncthreads();
+            if (c0 != off) {
+                __syncthreads();
+                find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(c0), b.last, t_end - c0, ms.runs, tid);
+                __syncthreads();
+            }
             const uint32_t mine_n = wave < uint32_t(NW) && t_end - c0 > wave ? (t_end - c0 - wave + NW - 1) / NW : 0;  // the wave's tiles
             wait_lds();
 #pragma unroll
@@ -196,7 +201,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const S
                 const int32_t j0 = b.lo + 32 * int32_t(t);
                 // whether every row sees every token of the tile
                 const uint32_t held = tile_held(ms.runs, t - c0);
-                const bool full = held == 3 && j0 + 31 <= b.first && (a.window == 0 || int64_t(j0) + a.window > int64_t(b.last));
+                const bool full = held == 3 && j0 + 31 <= b.first && int64_t(j0) + a.span > int64_t(b.last);
                 uint32_t seen = (1u << NS) - 1;
                 if (!full) {
                     seen = 0;
@@ -310,10 +315,10 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, const S
         }
         // this workgroup has the rows' first tiles but not their last: the join is on its list
         if (off == 0 && !whole && tid == 0)
-            sc.jobs[work.id] = SplitJob{seq, r0, kvh, R, 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
+            sc.jobs[work.id] = SplitJob{b.begin, r0, kvh, min(uint32_t(R), b.rows - r0), 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= sg.places;
         first_seg = false;
-        if (left != 0) next_block<R>(a, rg, b.rows, pl);
+        if (left != 0) next_block<R>(a, rg, seqs, b.rows, pl);
     }
 }
 

@@ -13,10 +13,9 @@ namespace {
 // One launch for a batch of any mix: sequences of few rows make one line of tiles,
 // those of many another, and the workgroups are shared out between the two as their
 // tiles are (a tile of either takes about as long: 16 KB through HBM on one of 256
-// CUs, or 256 rows' products). `kinds`: bit 0 and 1, which of them the call's size
-// allows at all.
+// CUs, or 256 rows' products).
 template <int CT, int NP, int DP>
-__global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, SplitScratch sc) {
+__global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, SplitScratch sc) {
     using Few = FewShape<CT, NP, DP>;
     using Many = ManyShape<CT, NP, DP>;
     constexpr int SLOT = Many::ROWS;
@@ -24,32 +23,37 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, int kinds, Spl
     extern __shared__ __align__(1024) unsigned char lds[];
     Misc &ms = *reinterpret_cast<Misc *>(lds);
     const uint32_t tid = threadIdx.x, b = blockIdx.x, parts = gridDim.x;
+    Seqs seqs;
+    const uint64_t blocks = count_blocks<Few::R, Many::ROWS>(a, few, many, ms.line, seqs, tid);
     Line lf{}, lm{};
-    if (kinds & 1) lf = line_scan<Few::R, kTileTokens, Few::START, kThreads>(a, few, ms.line, tid);
-    if (kinds & 2) lm = line_scan<Many::ROWS, kTileTokens, Many::START, kThreads>(a, many, ms.line, tid);
+    if (uint32_t(blocks) != 0) lf = line_scan<Few::R, kTileTokens, Few::START>(a, few, ms.line, seqs, uint32_t(blocks), 0, tid);
+    if (blocks >> 32 != 0) lm = line_scan<Many::ROWS, kTileTokens, Many::START>(a, many, ms.line, seqs, uint32_t(blocks >> 32), 32, tid);
     const uint64_t all = lf.per_head + lm.per_head;
     if (all == 0) {
         if (tid == 0) sc.jobs[b].count = 0;
         return;
     }
-    uint32_t nm = uint32_t((lm.per_head * parts + all / 2) / all);  // workgroups for the second line, spread evenly
-    if (lf.per_head != 0 && nm == parts) nm = parts - 1;
-    if (lm.per_head != 0 && nm == 0) nm = 1;
-    const uint32_t before = uint32_t(uint64_t(b) * nm / parts);
+    uint32_t nm = lm.per_head != 0 ? parts : 0, before = lm.per_head != 0 ? b : 0;  // workgroups for the second line
+    bool second = lm.per_head != 0;
+    if (lf.per_head != 0 && lm.per_head != 0) {  // (spread evenly)
+        nm = min(max(uint32_t(div_wide(lm.per_head * parts + all / 2, all)), 1u), parts - 1);
+        before = b * nm / parts;
+        second = (b + 1) * nm / parts != before;
+    }
     Part w;
-    if (uint64_t(b + 1) * nm / parts == before) {
+    if (!second) {
         const uint32_t index = b - before;
-        w.at = line_part<Few::R, kTileTokens, Few::START>(a, few, lf, index, parts - nm, Few::NW, ms.line, &w.part, &w.left);
+        w.at = line_part<Few::R, kTileTokens, Few::START>(a, few, lf, index, parts - nm, Few::NW, ms.line, seqs, &w.part, &w.left);
         w.id = index;
         if (tid == 0) sc.jobs[w.id].count = 0;
-        attn_few<CT, NP, DP, SLOT>(a, few, sc, w, lds, ms);
+        attn_few<CT, NP, DP, SLOT>(a, few, seqs, sc, w, lds, ms);
     } else {
         // (workgroups of one XCD, every eighth, take parts next to each other)
         const uint32_t index = nm == parts && parts % 8 == 0 ? b % 8 * (parts / 8) + b / 8 : before;
-        w.at = line_part<Many::ROWS, kTileTokens, Many::START>(a, many, lm, index, nm, 4, ms.line, &w.part, &w.left);
+        w.at = line_part<Many::ROWS, kTileTokens, Many::START>(a, many, lm, index, nm, 4, ms.line, seqs, &w.part, &w.left);
         w.id = parts - nm + index;
         if (tid == 0) sc.jobs[w.id].count = 0;
-        attn_many<CT, NP, DP, SLOT>(a, many, sc, w, lds, ms);
+        attn_many<CT, NP, DP, SLOT>(a, many, seqs, sc, w, lds, ms);
     }
 }
 
@@ -60,11 +64,8 @@ hipError_t launch(const AttnArgs &a, int num_cu, void *scratch, hipStream_t st) 
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&k_attn<CT, NP, DP>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (attr != hipSuccess) return attr;
-    // a sequence has up to n_tokens rows' tokens, the only one all of them
-    const uint64_t most = uint64_t(a.kv.n_tokens) * a.group;
-    const int kinds = (a.kv.n_seq > 1 || most <= kFewRows ? 1 : 0) | (most > kFewRows ? 2 : 0);
     const SplitScratch sc = split_scratch(scratch, num_cu, SLOT);
-    k_attn<CT, NP, DP><<<num_cu, kThreads, lds, st>>>(a, kinds, sc);
+    k_attn<CT, NP, DP><<<num_cu, kThreads, lds, st>>>(a, sc);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     k_attn_join<DP, SLOT><<<dim3(num_cu, 8), kThreads, 0, st>>>(a, sc);

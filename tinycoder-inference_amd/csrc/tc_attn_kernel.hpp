@@ -380,7 +380,7 @@ __device__ __forceinline__ void add_values_one_by_one(const unsigned char *vt, c
 
 // Output dims e .. e + 3 (or e alone) of a row of a sequence's block.
 __device__ __forceinline__ uint64_t out_at(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row) {
-    const uint32_t tok = row / a.group;
+    const uint32_t tok = div_fast(row, a.group_div);
     return (uint64_t(begin + tok) * a.heads + kvh * a.group + row - tok * a.group) * a.kv.dim;
 }
 __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row, uint32_t e, f32x4 x) {
@@ -416,6 +416,37 @@ struct RowRange {
     uint32_t least, most;
 };
 
+// A sequence's first token row, its rows' tokens and its length.
+struct Seq {
+    uint32_t begin, n;
+    int32_t len;
+};
+// The batch's start and len: copies in LDS where there are few sequences (one fetch for
+// the whole workgroup, where every later look would wait for a cache, a microsecond at
+// the kernel's start), else themselves. Pointers that may be either, so that there is one
+// code for both: what a workgroup does once waits for its instructions to be fetched.
+struct Seqs {
+    const int32_t *start, *len;
+    __device__ __forceinline__ Seq at(const AttnArgs &a, uint32_t s) const {
+        Seq q;
+        uint32_t end;
+        seq_rows(start, a.kv.n_tokens, s, &q.begin, &end);
+        q.n = end - q.begin;
+        // (kept where sums with a few 2^24 do not overflow)
+        q.len = min(len[s], int32_t(kMaxPos) - 64);
+        return q;
+    }
+    __device__ __forceinline__ Seq uniform(const AttnArgs &a, uint32_t s) const {
+        const Seq q = at(a, s);
+        return Seq{uint32_t(__builtin_amdgcn_readfirstlane(q.begin)), uint32_t(__builtin_amdgcn_readfirstlane(q.n)),
+                   __builtin_amdgcn_readfirstlane(q.len)};
+    }
+};
+__device__ __forceinline__ uint32_t rows_in(const AttnArgs &a, RowRange rg, uint32_t n) {
+    const uint32_t rows = n * a.group;
+    return rows >= rg.least && rows <= rg.most ? rows : 0;
+}
+
 // A block of rows of a sequence: its positions, and its tiles.
 struct RowBlock {
     uint32_t begin, rows;  // first token row; rows of the sequence (tokens * group)
@@ -424,29 +455,16 @@ struct RowBlock {
     int32_t lo, hi;        // tokens that a row of it may see
     uint32_t tiles;        // at least 1, so that rows which see nothing are written too
 };
-__device__ __forceinline__ uint32_t seq_row_count(const AttnArgs &a, RowRange rg, uint32_t s, uint32_t *begin) {
-    uint32_t end;
-    seq_rows(a.kv.start, a.kv.n_tokens, s, begin, &end);
-    const uint32_t rows = (end - *begin) * a.group;
-    return rows >= rg.least && rows <= rg.most ? rows : 0;
-}
 template <int ROWS, int TOKENS>
-__device__ __forceinline__ RowBlock row_block(const AttnArgs &a, uint32_t s, uint32_t r0) {
+__device__ __forceinline__ RowBlock row_block(const AttnArgs &a, const Seq &q, uint32_t r0) {
     RowBlock b;
-    uint32_t end;
-    seq_rows(a.kv.start, a.kv.n_tokens, s, &b.begin, &end);
-    const uint32_t n = end - b.begin;
-    b.rows = n * a.group;
-    // (kept where sums with a few 2^24 do not overflow)
-    const int32_t len = min(a.kv.len[s], int32_t(kMaxPos) - 64);
-    b.pos0 = max(len, 0) - int32_t(n);
-    b.first = b.pos0 + int32_t(r0 / a.group);
-    b.last = b.pos0 + int32_t((min(r0 + ROWS, max(b.rows, 1u)) - 1) / a.group);
-    const uint64_t cap = uint64_t(a.kv.table_pages) * a.kv.page;
-    b.hi = max(0, int32_t(min(int64_t(b.last) + 1, int64_t(min(cap, uint64_t(kMaxPos - 64))))));
-    b.lo = 0;
-    if (a.window != 0 && int64_t(b.first) + 1 > int64_t(a.window))
-        b.lo = min(b.hi, int32_t(int64_t(b.first) + 1 - a.window)) & ~31;
+    b.begin = q.begin;
+    b.rows = q.n * a.group;
+    b.pos0 = max(q.len, 0) - int32_t(q.n);
+    b.first = b.pos0 + int32_t(div_fast(r0, a.group_div));
+    b.last = b.pos0 + int32_t(div_fast(min(r0 + ROWS, max(b.rows, 1u)) - 1, a.group_div));
+    b.hi = max(0, min(b.last + 1, a.cap));
+    b.lo = min(b.hi, max(0, max(b.first, -1) + 1 - a.span)) & ~31;
     b.tiles = max(1u, uint32_t(b.hi - b.lo + TOKENS - 1) / TOKENS);
     return b;
 }
@@ -470,32 +488,55 @@ __device__ __forceinline__ Segment segment(uint32_t tiles, uint32_t off, uint64_
     return g;
 }
 
+template <int THREADS>
 struct LineMisc {
-    uint32_t blocks[512];  // blocks of the sequences up to a thread's last
-    uint64_t waves[8];
+    int32_t start[THREADS + 1], len[THREADS];  // of up to THREADS sequences
+    uint64_t blocks[THREADS];  // blocks of the sequences up to a thread's last: of few rows, of many << 32
+    uint64_t waves[3][THREADS / 64];
     Place at;
 };
 
-// Inclusive sum over the workgroup's threads, and the sum of all.
-template <class T, int THREADS>
-__device__ __forceinline__ T block_scan(T v, LineMisc &lm, uint32_t tid, T *all) {
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t other_lane(uint64_t v) {  // 0 where there is none
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 15, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 15, false);
+    return uint64_t(hi) << 32 | lo;
+}
+// Inclusive sum over the workgroup's threads, and the sum of all. All threads call it.
+template <int THREADS>
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t (&waves)[THREADS / 64], uint32_t tid, uint64_t *all) {
     const uint32_t lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T u = __shfl_up(v, o);
-        if (lane >= uint32_t(o)) v += u;
-    }
+    v += other_lane<0x111, 15>(v);  // 1, 2, 4, 8 lanes to the left in rows of 16
+    v += other_lane<0x112, 15>(v);
+    v += other_lane<0x114, 15>(v);
+    v += other_lane<0x118, 15>(v);
+    v += other_lane<0x142, 10>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+    v += other_lane<0x143, 12>(v);  // lane 31 to rows 2 and 3
+    if (lane == 63) waves[wave] = v;
     __syncthreads();
-    if (lane == 63) lm.waves[wave] = v;
-    __syncthreads();
-    T sum = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < THREADS / 64; ++w) {
-        if (w < wave) v += T(lm.waves[w]);
-        sum += T(lm.waves[w]);
-    }
-    *all = sum;
-    return v;
+    static_assert(THREADS == 512, "");
+    uint64_t x = waves[lane % 8];
+    x += other_lane<0x111, 15>(x);
+    x += other_lane<0x112, 15>(x);
+    x += other_lane<0x114, 15>(x);  // (lanes 0 to 7: the waves up to this one)
+    auto upto = [&](uint32_t w) {
+        return uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(x >> 32), w))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(x), w));
+    };
+    *all = upto(7);
+    return wave == 0 ? v : v + upto(__builtin_amdgcn_readfirstlane(wave - 1) & 7);
+}
+
+// x / y for x up to 2^53 (the compiler's division of 64-bit integers is 150 instructions,
+// and what a workgroup does once waits for its instructions to be fetched)
+__device__ __forceinline__ uint64_t div_wide(uint64_t x, uint64_t y) {
+    if (__builtin_expect((x | y) >> 32 == 0, 1)) return uint32_t(x) / uint32_t(y);
+    uint64_t q = uint64_t(double(x) / double(y));
+    const int64_t r = int64_t(x - q * y);
+    if (r < 0)
+        --q;
+    else if (uint64_t(r) >= y)
+        ++q;
+    return q;
 }
 
 // A line as one thread sees it: its blocks' places, and where they lie.
@@ -505,75 +546,89 @@ struct Line {
     uint64_t per_head;   // all of one head
 };
 template <int ROWS>
-__device__ __forceinline__ void line_step(const AttnArgs &a, RowRange rg, uint32_t &s, uint32_t &r0) {  // to the next block, if any
-    uint32_t begin;
+__device__ __forceinline__ void line_step(const AttnArgs &a, RowRange rg, Seqs seqs, uint32_t &s, uint32_t &r0) {  // to the next block
     r0 += ROWS;
-    if (r0 >= seq_row_count(a, rg, s, &begin)) {
+    if (r0 >= rows_in(a, rg, seqs.at(a, s).n)) {
         r0 = 0;
         do ++s;
-        while (s < a.kv.n_seq && seq_row_count(a, rg, s, &begin) == 0);
+        while (s + 1 < a.kv.n_seq && rows_in(a, rg, seqs.at(a, s).n) == 0);
     }
 }
-template <int ROWS, int TOKENS, int START, int THREADS>
-__device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMisc &lm, uint32_t tid) {
+// The sequences into LDS where they fit, and their blocks of both kinds counted: few |
+// many << 32.
+template <int FEW, int MANY, int THREADS>
+__device__ __forceinline__ uint64_t count_blocks(const AttnArgs &a, RowRange few, RowRange many, LineMisc<THREADS> &lm, Seqs &seqs, uint32_t tid) {
     const uint32_t per = (a.kv.n_seq + THREADS - 1) / THREADS;
-    const uint32_t s0 = min(tid * per, a.kv.n_seq), s1 = min(s0 + per, a.kv.n_seq);
-    uint32_t mine = 0, begin;
-    for (uint32_t s = s0; s < s1; ++s) mine += (seq_row_count(a, rg, s, &begin) + ROWS - 1) / ROWS;
-    uint32_t n_blocks;
-    const uint32_t upto = block_scan<uint32_t, THREADS>(mine, lm, tid, &n_blocks);
-    lm.blocks[tid] = upto;
+    seqs = Seqs{a.kv.start, a.kv.len};
+    uint64_t mine = 0, all;
+    for (uint32_t i = 0, s = tid * per; i < per && s < a.kv.n_seq; ++i, ++s) {
+        const int32_t x = seqs.start[s], y = seqs.start[s + 1], z = seqs.len[s];
+        if (per == 1) lm.start[s] = x, lm.start[s + 1] = y, lm.len[s] = z;  // (two lanes write the same)
+        const int32_t se[2] = {x, y};
+        uint32_t begin, end;
+        seq_rows(se, a.kv.n_tokens, 0, &begin, &end);
+        mine += (rows_in(a, few, end - begin) + FEW - 1) / FEW + (uint64_t((rows_in(a, many, end - begin) + MANY - 1) / MANY) << 32);
+    }
+    lm.blocks[tid] = block_scan<THREADS>(mine, lm.waves[0], tid, &all);
+    if (per == 1) seqs = Seqs{lm.start, lm.len};
     __syncthreads();
+    return all;
+}
+// The line of the blocks of one kind, `n_blocks` of them, whose counts stand at bit `shift`.
+template <int ROWS, int TOKENS, int START, int THREADS>
+__device__ __forceinline__ Line line_scan(const AttnArgs &a, RowRange rg, LineMisc<THREADS> &lm, Seqs seqs, uint32_t n_blocks, uint32_t shift, uint32_t tid) {
+    const uint32_t per = (a.kv.n_seq + THREADS - 1) / THREADS;
     Line ln{0, 0, 0, 0, 0};
     // the places of this thread's blocks
     const uint32_t q = (n_blocks + THREADS - 1) / THREADS;
     const uint32_t f0 = min(tid * q, n_blocks), f1 = min(f0 + q, n_blocks);
     if (f0 < f1) {
-        uint32_t x = 0, y = THREADS - 1;  // the first thread whose sequences reach past block f0
+        // the first thread whose sequences reach past block f0
+        uint32_t x = 0, y = min(a.kv.n_seq, uint32_t(THREADS)) - 1;
         while (x < y) {
             const uint32_t mid = (x + y) / 2;
-            if (lm.blocks[mid] > f0)
+            if (uint32_t(lm.blocks[mid] >> shift) > f0)
                 y = mid;
             else
                 x = mid + 1;
         }
-        uint32_t skip = f0 - (x != 0 ? lm.blocks[x - 1] : 0);
-        for (ln.s = x * per;; ++ln.s) {
-            const uint32_t nb = (seq_row_count(a, rg, ln.s, &begin) + ROWS - 1) / ROWS;
+        uint32_t skip = f0 - (x != 0 ? uint32_t(lm.blocks[x - 1] >> shift) : 0);
+        for (ln.s = x * per; ln.s + 1 < a.kv.n_seq; ++ln.s) {
+            const uint32_t nb = (rows_in(a, rg, seqs.at(a, ln.s).n) + ROWS - 1) / ROWS;
             if (skip < nb) break;
             skip -= nb;
         }
         ln.r0 = skip * ROWS;
         uint32_t u = ln.s, v = ln.r0;
         for (uint32_t f = f0; f < f1; ++f) {
-            ln.places += row_block<ROWS, TOKENS>(a, u, v).tiles + START;
-            if (f + 1 < f1) line_step<ROWS>(a, rg, u, v);
+            ln.places += row_block<ROWS, TOKENS>(a, seqs.at(a, u), v).tiles + START;
+            if (f + 1 < f1) line_step<ROWS>(a, rg, seqs, u, v);
         }
     }
-    ln.incl = block_scan<uint64_t, THREADS>(ln.places, lm, tid, &ln.per_head);
+    ln.incl = block_scan<THREADS>(ln.places, lm.waves[shift == 0 ? 1 : 2], tid, &ln.per_head);
     return ln;
 }
 
 // Part `index` of `parts` (of at least min_part places each): where it starts, and its
 // number of places (0: none); *part: that of every part but the last ones.
-template <int ROWS, int TOKENS, int START>
+template <int ROWS, int TOKENS, int START, int THREADS>
 __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const Line &ln, uint32_t index, uint32_t parts,
-                                           uint32_t min_part, LineMisc &lm, uint64_t *part, uint64_t *left) {
+                                           uint32_t min_part, LineMisc<THREADS> &lm, Seqs seqs, uint64_t *part, uint64_t *left) {
     const uint64_t total = ln.per_head * a.kv.kv_heads;
-    *part = max((total + parts - 1) / parts, uint64_t(min_part));
+    *part = max(div_wide(total + parts - 1, parts), uint64_t(min_part));
     const uint64_t at = *part * index;
     *left = at < total ? min(*part, total - at) : 0;
     if (*left != 0) {
-        const uint32_t kvh = uint32_t(at / ln.per_head);
+        const uint32_t kvh = min(uint32_t(div_wide(at, ln.per_head)), a.kv.kv_heads - 1);
         uint64_t target = at - kvh * ln.per_head;
         if (target >= ln.incl - ln.places && target < ln.incl) {
             target -= ln.incl - ln.places;
             uint32_t s = ln.s, r0 = ln.r0;
             for (;;) {
-                const uint32_t t = row_block<ROWS, TOKENS>(a, s, r0).tiles + START;
+                const uint32_t t = row_block<ROWS, TOKENS>(a, seqs.at(a, s), r0).tiles + START;
                 if (target < t) break;
                 target -= t;
-                line_step<ROWS>(a, rg, s, r0);
+                line_step<ROWS>(a, rg, seqs, s, r0);
             }
             lm.at = Place{s, r0, kvh, uint32_t(target)};
         }
@@ -589,15 +644,14 @@ __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const
 
 // The block of rows behind place p's (p.off = 0). The line does not end there.
 template <int ROWS>
-__device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, uint32_t rows, Place &p) {
+__device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, Seqs seqs, uint32_t rows, Place &p) {
     p.off = 0;
     p.r0 += ROWS;
     if (p.r0 < rows) return;
     p.r0 = 0;
-    uint32_t begin;
     do {
         if (++p.seq == a.kv.n_seq) p.seq = 0, ++p.kvh;
-    } while (seq_row_count(a, rg, p.seq, &begin) == 0);
+    } while (rows_in(a, rg, seqs.uniform(a, p.seq).n) == 0);
 }
 
 // ---- pages --------------------------------------------------------------------
@@ -609,22 +663,27 @@ template <int STRETCH>
 struct RunMisc {
     uint32_t run[2 * STRETCH];
     uint64_t held[STRETCH / 32];  // bit i % 64 of word i / 64: run i
-    uint32_t missing;             // whether a run with tokens to be seen is not held (set to 0 a barrier earlier)
 };
-// For the tiles from position pos on (a multiple of 16), up to position hi.
+// For the tiles from position pos on (a multiple of 16), whose tokens up to position
+// `last` may be seen (those behind count as held).
 template <int THREADS, int STRETCH>
-__device__ __forceinline__ void find_runs(const AttnArgs &a, uint32_t seq, uint32_t kvh, int32_t pos, int32_t hi, uint32_t tiles,
+__device__ __forceinline__ void find_runs(const AttnArgs &a, uint32_t seq, uint32_t kvh, int32_t pos, int32_t last, uint32_t tiles,
                                           RunMisc<STRETCH> &rm, uint32_t tid) {
     const uint32_t per = a.kv.page / 16;
     for (uint32_t i = tid; i / 64 * 64 < 2 * tiles; i += THREADS) {  // (whole waves)
         const int32_t p = pos + 16 * int32_t(i);
         const uint32_t pi = div_fast(uint32_t(p), a.kv.page_div);
-        const int32_t pg = i < 2 * tiles ? page_at(a.kv, seq, pi) : -1;
+        const bool wanted = i < 2 * tiles && p <= last;
+        const int32_t pg = wanted ? page_at(a.kv, seq, pi) : -1;
         rm.run[i] = pg < 0 ? 0 : (uint32_t(pg) * a.kv.kv_heads + kvh) * per + (uint32_t(p) / 16 - pi * per);
-        const uint64_t held = __ballot(pg >= 0);
+        const uint64_t held = __ballot(pg >= 0 || !wanted);
         if (i % 64 == 0) rm.held[i / 64] = held;
-        if (pg < 0 && p < hi && i < 2 * tiles) rm.missing = 1;
     }
+}
+// Whether all runs of the stretch are held (a barrier after find_runs).
+template <int STRETCH>
+__device__ __forceinline__ bool all_held(const RunMisc<STRETCH> &rm, uint32_t tiles, uint32_t lane) {
+    return __ballot(lane < (2 * tiles + 63) / 64 && rm.held[lane % (STRETCH / 32)] != ~uint64_t(0)) == 0;
 }
 // The two runs of a tile, wave-uniform.
 struct TileRuns {
@@ -644,20 +703,42 @@ __device__ __forceinline__ uint32_t tile_held(const RunMisc<STRETCH> &rm, uint32
 // The lane's row, in NP pieces of the operands' type, and its factor log2(e) * scale *
 // 2^e. `row` is query head row % group of the sequence's token row / group; rows at
 // n_rows or above are zeros.
+template <int CT, int NP>
+constexpr bool f32_rows() { return NP == (CT == kBF16 ? 3 : 2); }
+// its elements as they are, on their way
 template <int CT, int NP, int R, int DP, int ES>
-__device__ __forceinline__ float load_q(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row, uint32_t n_rows, uint32_t g,
-                                        u32x4 (&q)[NP][Geo<R, DP>::KS]) {
-    constexpr int KS = Geo<R, DP>::KS;
-    const uint32_t tok = row / a.group;
+__device__ __forceinline__ void fetch_q(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row, uint32_t n_rows, uint32_t g,
+                                        u32x4 (&raw)[f32_rows<CT, NP>() ? 2 : 1][Geo<R, DP>::KS]) {
+    constexpr int W = f32_rows<CT, NP>() ? 2 : 1;
+    const uint32_t tok = div_fast(row, a.group_div);
     const uint64_t at = uint64_t(begin + tok) * a.q_stride + uint64_t(kvh * a.group + row - tok * a.group) * a.kv.dim;
-    float x[KS][8], m = 0.0f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
+    for (int ks = 0; ks < Geo<R, DP>::KS; ++ks) {
         const uint32_t d = step_dim<R, ES>(ks, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
-        if (row < n_rows && d < a.kv.dim) load8(a.xtype, a.q, at + d, x[ks]);
+        for (int w = 0; w < W; ++w) {
+            raw[w][ks] = u32x4{0, 0, 0, 0};
+            if (row < n_rows && d < a.kv.dim)
+                raw[w][ks] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.q) + (at + d) * (2 * W) + 16 * w);
+        }
     }
+}
+template <int CT, int NP, int R, int DP>
+__device__ __forceinline__ float make_q(const AttnArgs &a, const u32x4 (&raw)[f32_rows<CT, NP>() ? 2 : 1][Geo<R, DP>::KS],
+                                        u32x4 (&q)[NP][Geo<R, DP>::KS]) {
+    constexpr int KS = Geo<R, DP>::KS;
+    float x[KS][8], m = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (f32_rows<CT, NP>()) {
+                x[ks][i] = __builtin_bit_cast(float, uint32_t(raw[i / 4][ks][i % 4]));
+            } else {
+                const uint32_t h = i % 2 ? raw[0][ks][i / 2] >> 16 : raw[0][ks][i / 2] & 0xFFFF;
+                x[ks][i] = a.xtype == kBF16 ? __builtin_bit_cast(float, h << 16) : float(__builtin_bit_cast(_Float16, uint16_t(h)));
+            }
+        }
     int e = 0;
     if constexpr (CT != kBF16) {
 #pragma unroll
@@ -682,9 +763,9 @@ __device__ __forceinline__ float load_q(const AttnArgs &a, uint32_t begin, uint3
 
 // ---- the kernel's shape ---------------------------------------------------------
 // 8 waves, one workgroup per CU; the small things first in LDS.
-constexpr int kWaves = 8, kThreads = 64 * kWaves, kMisc = 8192, kLds = 160 * 1024;
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kMisc = 16384, kLds = 160 * 1024;
 struct Misc {
-    LineMisc line;
+    LineMisc<kThreads> line;
     RunMisc<512> runs;
     union {
         struct {
@@ -714,10 +795,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, SplitScratch
     if (job.count == 0) return;
     __shared__ f32x4 part_x[kWaves][64];
     __shared__ float part_l[kWaves];
-    uint32_t begin, end;
-    seq_rows(a.kv.start, a.kv.n_tokens, job.seq, &begin, &end);
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t rows = min(job.rows, (end - begin) * a.group - job.r0);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = job.rows;
     constexpr uint32_t L = DP / 4;  // lanes of a row
     const uint32_t e = 4 * (tid % L);
     auto at_slot = [&](uint32_t i, uint32_t r) { return (i == 0 ? job.slot : 2 * (blockIdx.x + i)) * SLOT + r; };
@@ -732,7 +810,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, SplitScratch
     };
     auto store = [&](uint32_t r, f32x4 x, float all) __attribute__((always_inline)) {
         const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-        if (e < a.kv.dim) store4(a, begin, job.kvh, job.r0 + r, e, x * inv);
+        if (e < a.kv.dim) store4(a, job.begin, job.kvh, job.r0 + r, e, x * inv);
     };
     if (job.count <= 8) {
         for (uint32_t r = blockIdx.y * (kThreads / L) + tid / L; r < rows; r += gridDim.y * (kThreads / L)) {

@@ -33,7 +33,7 @@ struct ManyShape {
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int CT, int NP, int DP, int SLOT>
-__device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
+__device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs seqs, const SplitScratch &sc, Part work, unsigned char *lds, Misc &ms) {
     using Sh = ManyShape<CT, NP, DP>;
     constexpr int R = Sh::R, LT = Sh::LT, RB = Sh::RB, NW = kWaves, TILE = Sh::TILE, NBUF = Sh::NBUF, STRETCH = 512;
     using Ge = Geo<R, DP>;
@@ -50,7 +50,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
     bool first_seg = true;
     while (left != 0) {
         const uint32_t seq = pl.seq, r0 = pl.r0, kvh = pl.kvh;
-        const RowBlock b = row_block<Sh::ROWS, kTileTokens>(a, seq, r0);
+        const RowBlock b = row_block<Sh::ROWS, kTileTokens>(a, seqs.uniform(a, seq), r0);
         const Segment sg = segment<Sh::START>(b.tiles, pl.off, left);
         const uint32_t off = sg.off, seg = sg.tiles;
         if (seg == 0) break;  // (the part ends among the block's first places)
@@ -58,14 +58,15 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         // ---- the wave's rows of q ----
         const uint32_t wr0 = r0 + R * wave, row = wr0 + col;
         const bool active = wr0 < b.rows;  // the wave has rows
-        const int32_t pos = row < b.rows ? b.pos0 + int32_t(row / a.group) : -1;  // the lane's row sees tokens up to here
-        const int32_t from = a.window != 0 && int64_t(pos) + 1 > int64_t(a.window) ? int32_t(pos + 1 - a.window) : 0;
-        const int32_t wfirst = b.pos0 + int32_t(wr0 / a.group);
-        const int32_t wlast = b.pos0 + int32_t((min(wr0 + R, b.rows) - 1) / a.group);
-        u32x4 q[NP][KS];
-        const float factor = load_q<CT, NP, R, DP, 2>(a, b.begin, kvh, row, b.rows, g, q);
-        if (tid == 0) ms.runs.missing = 0;
-        __syncthreads();  // (the last block's tiles are no longer read)
+        const int32_t pos = row < b.rows ? b.pos0 + int32_t(div_fast(row, a.group_div)) : -1;  // the lane's row sees tokens up to here
+        const int32_t from = max(0, max(pos, -1) + 1 - a.span);
+        const int32_t wfirst = b.pos0 + int32_t(div_fast(wr0, a.group_div));
+        const int32_t wlast = b.pos0 + int32_t(div_fast(min(wr0 + R, b.rows) - 1, a.group_div));
+        u32x4 raw_q[f32_rows<CT, NP>() ? 2 : 1][KS], q[NP][KS];
+        fetch_q<CT, NP, R, DP, 2>(a, b.begin, kvh, row, b.rows, g, raw_q);
+        find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(off), b.last, min(seg, uint32_t(STRETCH)), ms.runs, tid);
+        __syncthreads();
+        const float factor = make_q<CT, NP, R, DP>(a, raw_q, q);
         Acc<R> o[DB];
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = Acc<R>{};
@@ -119,9 +120,11 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
 
         for (uint32_t t0 = off; t0 < off + seg; t0 += STRETCH) {
         const uint32_t t1 = min(off + seg, t0 + STRETCH);
-        find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.hi, t1 - t0, ms.runs, tid);
-        __syncthreads();
-        const bool missing = ms.runs.missing != 0;
+        if (t0 != off) {
+            find_runs<kThreads>(a, seq, kvh, b.lo + 32 * int32_t(t0), b.last, t1 - t0, ms.runs, tid);
+            __syncthreads();
+        }
+        const bool missing = !all_held(ms.runs, t1 - t0, lane_now());
 
         // ---- tiles into LDS ----
         const uint32_t run_bytes = 16 * rowbytes;
@@ -192,7 +195,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         // whether some row of the wave sees a token of tile t, and whether all see all
         auto any_seen = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
-            return active && j0 <= wlast && (a.window == 0 || int64_t(j0) + 31 + a.window > int64_t(wfirst));
+            return active && j0 <= wlast && int64_t(j0) + 31 + a.span > int64_t(wfirst);
         };
         // Scores as they come from the matrix cores to what the weights are formed
         // from: as they are (times `factor` later), or with a token's factors the
@@ -210,7 +213,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         auto largest = [&](const float (&x)[NS]) __attribute__((always_inline)) { return SCALED ? max_of(x) : max_of(x) * factor; };
         auto full_tile = [&](uint32_t t) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
-            return j0 + 31 <= wfirst && (a.window == 0 || int64_t(j0) + a.window > int64_t(wlast));
+            return j0 + 31 <= wfirst && int64_t(j0) + a.span > int64_t(wlast);
         };
         auto finish_scores = [&](uint32_t t, float (&x)[NS]) __attribute__((always_inline)) {
             const int32_t j0 = b.lo + 32 * int32_t(t);
@@ -437,10 +440,10 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, const 
         }
         // this workgroup has the block's first tiles but not its last: the join is on its list
         if (off == 0 && !whole && tid == 0)
-            sc.jobs[work.id] = SplitJob{seq, r0, kvh, Sh::ROWS, 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
+            sc.jobs[work.id] = SplitJob{b.begin, r0, kvh, min(uint32_t(Sh::ROWS), b.rows - r0), 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= sg.places;
         first_seg = false;
-        if (left != 0) next_block<Sh::ROWS>(a, rg, b.rows, pl);
+        if (left != 0) next_block<Sh::ROWS>(a, rg, seqs, b.rows, pl);
     }
 }
 
