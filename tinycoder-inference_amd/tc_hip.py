@@ -113,11 +113,16 @@ def load_library(path=LIB_PATH):
     return lib
 
 
+_ELEM_TYPES = {}
+
+
 def _elem_type(dtype):
     """The tc_attention.h element type of a torch dtype."""
-    import torch
-    t = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8,
-         torch.float8_e4m3fn: E4M3}.get(dtype)
+    if not _ELEM_TYPES:
+        import torch
+        _ELEM_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8,
+                            torch.float8_e4m3fn: E4M3})
+    t = _ELEM_TYPES.get(dtype)
     if t is None:
         raise TCError(TC_E_UNSUPPORTED, f"no element type for {dtype}")
     return t
@@ -154,8 +159,10 @@ class KVCache:
         _need(all(t.is_contiguous() and t.device == k.device for t in held), "a cache is contiguous and on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
+        self.device = k.get_device()  # (-1: the CPU)
         self.c = _CKVCache(_elem_type(k.dtype), self.n_pages, self.kv_heads, self.page_tokens, self.head_dim,
                            *[None if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale)])
+        self.ref = ctypes.byref(self.c)
 
     @classmethod
     def empty(cls, dtype, n_pages, kv_heads, page_tokens, head_dim, device="cuda"):
@@ -181,7 +188,19 @@ class KVBatch:
         _need(start.numel() == n + 1 and table.dim() == 2 and table.shape[0] == n,
               "start has n_seq + 1 entries, table n_seq rows")
         self.start, self.length, self.table = start, length, table
-        self.c = _CKVBatch(n, 0, table.shape[1], start.data_ptr(), length.data_ptr(), table.data_ptr())
+        self.device = start.get_device()
+        self._of = {}  # a struct for each number of rows: calls at once share none that changes
+
+    def of(self, n_tokens):
+        """The C struct of a call with n_tokens rows, by reference."""
+        ref = self._of.get(n_tokens)
+        if ref is None:
+            if len(self._of) >= 64:
+                self._of.clear()
+            c = _CKVBatch(self.length.numel(), n_tokens, self.table.shape[1], self.start.data_ptr(), self.length.data_ptr(),
+                          self.table.data_ptr())
+            ref = self._of[n_tokens] = ctypes.byref(c)
+        return ref
 
 
 def _ptr(t):
@@ -196,7 +215,7 @@ class Library:
         self.path = path
 
     # -- helpers ---------------------------------------------------------------
-    def _stream(self):
+    def _stream(self, device=None):
         # The current device's current stream as a handle: reading it without
         # building a torch.cuda.Stream object takes 0.4 instead of 2.9 us, a
         # quarter of a small call's host time (10.1 -> 7.6 us for tc_gemv).
@@ -204,7 +223,7 @@ class Library:
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if raw is None:
             return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-        return ctypes.c_void_p(raw(torch.cuda.current_device()))
+        return ctypes.c_void_p(raw(torch.cuda.current_device() if device is None else device))
 
     def _check(self, rc):
         if rc != TC_OK:
@@ -367,20 +386,27 @@ class Library:
 
 
     # -- paged cache, attention, drafted tokens ---------------------------------------
-    def _kv_call(self, cache, batch, rows):
-        """The batch's C struct for `rows` [n_tokens][heads][head_dim], checked."""
+    # (a call's host time is a small call's whole time, so its checks cost no more than they must: 10.5 -> 6.9 us
+    # for tc_kv_write)
+    def _kv_call(self, cache, batch, x, y, strided):
+        """Checks of rows x and y [n_tokens][heads][head_dim], of which the first
+        `strided` may have strides; -> n_tokens, current stream."""
         import torch
-        _need(rows[0].dim() == 3 and all(t.shape == rows[0].shape and t.dtype == rows[0].dtype for t in rows),
-              "rows are [n_tokens][heads][head_dim], of one type")
-        T, H, D = rows[0].shape
-        for t in rows:
-            _need(t.shape[2] == cache.head_dim, f"head_dim {t.shape[2]} is not the cache's {cache.head_dim}")
-            _need(T == 0 or (t.stride(2) == 1 and (H == 1 or t.stride(1) == D)), "a row's heads are not contiguous")
+        shape = x.shape
+        if len(shape) != 3 or y.shape != shape or y.dtype != x.dtype:
+            raise TCError(TC_E_ARG, "rows are [n_tokens][heads][head_dim], of one type")
+        T, H, D = shape
+        if D != cache.head_dim:
+            raise TCError(TC_E_ARG, f"head_dim {D} is not the cache's {cache.head_dim}")
+        for i, t in enumerate((x, y)):
+            if not t.is_contiguous():
+                st = t.stride()
+                if i >= strided or T != 0 and (st[2] != 1 or (H != 1 and st[1] != D)):
+                    raise TCError(TC_E_ARG, "a row's heads are not contiguous" if i < strided else "out is not contiguous")
         dev = torch.cuda.current_device()
-        _need(all(t.device.type == "cuda" and t.device.index == dev for t in (*rows, cache.k, batch.start)),
-              "tensors are not on the current device")
-        batch.c.n_tokens = T
-        return batch.c
+        if not x.get_device() == y.get_device() == cache.device == batch.device == dev:
+            raise TCError(TC_E_ARG, "tensors are not on the current device")
+        return T, self._stream(dev)
 
     @staticmethod
     def _row_stride(t):
@@ -389,23 +415,24 @@ class Library:
     def kv_write(self, cache, batch, k, v):
         """Keys and values [n_tokens][kv_heads][head_dim] (rows may be strided)
         into their slots of the cache."""
-        _need(k.dim() == 3 and k.shape[1] == cache.kv_heads, "k is not [n_tokens][kv_heads][head_dim]")
-        b = self._kv_call(cache, batch, (k, v))
-        self._check(self.lib.tc_kv_write(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(k.dtype), _ptr(k), _ptr(v),
-                                         self._row_stride(k), self._row_stride(v), self._stream()))
+        if k.dim() != 3 or k.shape[1] != cache.kv_heads:
+            raise TCError(TC_E_ARG, "k is not [n_tokens][kv_heads][head_dim]")
+        T, stream = self._kv_call(cache, batch, k, v, 2)
+        self._check(self.lib.tc_kv_write(cache.ref, batch.of(T), _elem_type(k.dtype), k.data_ptr(), v.data_ptr(),
+                                         self._row_stride(k), self._row_stride(v), stream))
 
     def kv_read(self, cache, batch, n_tokens, dtype, out=None):
         """The batch's n_tokens rows out of the cache: (k, v)."""
         import torch
         if out is None:
             shape = (n_tokens, cache.kv_heads, cache.head_dim)
-            out = tuple(torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
-        k, v = out
-        _need(k.is_contiguous() and v.is_contiguous() and k.dtype == dtype and k.shape[0] == n_tokens and
-              k.shape[1] == cache.kv_heads, "outputs are contiguous [n_tokens][kv_heads][head_dim] of dtype")
-        b = self._kv_call(cache, batch, (k, v))
-        self._check(self.lib.tc_kv_read(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(dtype), _ptr(k), _ptr(v),
-                                        self._stream()))
+            k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        else:
+            k, v = out
+            if k.dim() != 3 or k.shape[:2] != (n_tokens, cache.kv_heads) or k.dtype != dtype:
+                raise TCError(TC_E_ARG, "outputs are [n_tokens][kv_heads][head_dim] of dtype")
+        T, stream = self._kv_call(cache, batch, k, v, 0)
+        self._check(self.lib.tc_kv_read(cache.ref, batch.of(T), _elem_type(dtype), k.data_ptr(), v.data_ptr(), stream))
         return k, v
 
     def attn(self, cache, batch, q, scale, window=0, out=None):
@@ -414,10 +441,9 @@ class Library:
         import torch
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _need(out.is_contiguous(), "out is not contiguous")
-        b = self._kv_call(cache, batch, (q, out))
-        self._check(self.lib.tc_attn(ctypes.byref(cache.c), ctypes.byref(b), _elem_type(q.dtype), _ptr(q),
-                                     self._row_stride(q), _ptr(out), q.shape[1], scale, window, self._stream()))
+        T, stream = self._kv_call(cache, batch, q, out, 1)
+        self._check(self.lib.tc_attn(cache.ref, batch.of(T), _elem_type(q.dtype), q.data_ptr(), self._row_stride(q),
+                                     out.data_ptr(), q.shape[1], scale, window, stream))
         return out
 
     def attn_reserve(self, heads, n_tokens):
@@ -429,18 +455,20 @@ class Library:
         import torch
         T, V = logits.shape
         S = temperature.numel()
-        floats = [t for t in (logits, temperature, accept_u, sample_u, draft_probs) if t is not None]
-        _need(all(t.dtype == torch.float32 for t in floats) and tokens.dtype == start.dtype == torch.int32,
-              "tokens and start are int32, the others fp32")
         dev = torch.cuda.current_device()
-        _need(all(t.is_contiguous() and t.device.type == "cuda" and t.device.index == dev for t in (*floats, tokens, start)),
-              "tensors are contiguous and on the current device")
-        _need(start.numel() == S + 1 and tokens.numel() == accept_u.numel() == T and sample_u.numel() == S and
-              (draft_probs is None or draft_probs.shape == logits.shape), "sizes do not agree")
+        for t in (logits, temperature, accept_u, sample_u, draft_probs):
+            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.get_device() != dev):
+                raise TCError(TC_E_ARG, "logits, probabilities and random numbers are contiguous fp32 on the current device")
+        for t in (tokens, start):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != dev:
+                raise TCError(TC_E_ARG, "tokens and start are contiguous int32 on the current device")
+        if not (start.numel() == S + 1 and tokens.numel() == accept_u.numel() == T and sample_u.numel() == S and
+                (draft_probs is None or draft_probs.shape == logits.shape)):
+            raise TCError(TC_E_ARG, "sizes do not agree")
         n, tok = (torch.empty(S, dtype=torch.int32, device=logits.device) for _ in range(2))
         self._check(self.lib.tc_spec_verify(_ptr(logits), _ptr(draft_probs), V, S, T, _ptr(start), _ptr(tokens),
                                             _ptr(temperature), _ptr(accept_u), _ptr(sample_u), _ptr(n), _ptr(tok),
-                                            self._stream()))
+                                            self._stream(dev)))
         return n, tok
 
 
