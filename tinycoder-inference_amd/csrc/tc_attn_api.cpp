@@ -37,8 +37,7 @@ int kv_args(const tc_kv_cache *c, const tc_kv_batch *b, int xtype, tc::KvArgs *a
     if (c->n_pages > 0x7FFFFFFFu || b->n_seq > (1u << 20) || b->n_tokens > (1u << 24))
         return refuse(TC_E_UNSUPPORTED, "more than 2^31 - 1 pages, 2^20 sequences or 2^24 rows");
     // (the kernels work on 2^31 parts of rows at most)
-    if (uint64_t(b->n_tokens) * 2 * c->kv_heads * 32 >= (uint64_t(1) << 39) ||
-        uint64_t(b->n_tokens) * 2 * c->kv_heads >= (uint64_t(1) << 31))
+    if ((uint64_t(b->n_tokens) + 15) * 2 * c->kv_heads >= (uint64_t(1) << 31))
         return refuse(TC_E_UNSUPPORTED, "too many rows");
     // (runs of 16 rows are numbered in 32 bits)
     if (uint64_t(c->n_pages) * c->kv_heads > (uint64_t(1) << 48) / c->page_tokens ||

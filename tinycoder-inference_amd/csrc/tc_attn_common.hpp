@@ -72,6 +72,20 @@ hipError_t launch_kv_write(const KvArgs &a, int ctype, int xtype, const void *k,
                            uint32_t v_stride, hipStream_t st);
 hipError_t launch_kv_read(const KvArgs &a, int ctype, int xtype, void *k, void *v, hipStream_t st);
 
+// As find_seq, 64 sequences at a time: one fetch where there are no more.
+__device__ __forceinline__ int wave_find_seq(const int32_t *start, uint32_t n_seq, uint32_t t) {
+    const uint32_t lane = threadIdx.x & 63;
+    const int32_t before = start[0], behind = start[n_seq];
+    uint32_t lo = 0, hi = n_seq;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) / 64, p = lo + lane * step;
+        const uint64_t m = __ballot(p < hi && (p == lo || start[p] <= int32_t(t)));
+        lo += (63 - __builtin_clzll(m)) * step;
+        hi = min(lo + step, hi);
+    }
+    return int32_t(t) >= behind || int32_t(t) < before ? -1 : int(lo);
+}
+
 struct AttnArgs {
     KvArgs kv;
     const void *q;

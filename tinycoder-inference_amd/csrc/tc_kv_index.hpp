@@ -92,10 +92,17 @@ TC_HD int64_t cache_row(const KvArgs &a, uint32_t s, int64_t pos, uint32_t head)
     return (int64_t(pg) * a.kv_heads + head) * a.page + (uint32_t(pos) - pi * a.page);
 }
 
-// Cache row of batch row t of sequence s (-1: none) and head.
+// Cache row of batch row t of sequence s (-1: none) and head. (No branch between the
+// loads: a lane's rows are looked up side by side.)
 TC_HD int64_t slot_of(const KvArgs &a, int s, uint32_t t, uint32_t head) {
-    if (s < 0) return -1;
-    return cache_row(a, uint32_t(s), int64_t(a.len[s]) - a.start[s + 1] + t, head);
+    const uint32_t q = s < 0 ? 0 : uint32_t(s);
+    const int64_t pos = int64_t(a.len[q]) - a.start[q + 1] + t;
+    bool ok = s >= 0 && pos >= 0 && pos < int64_t(kMaxPos);
+    const uint32_t p = ok ? uint32_t(pos) : 0, pi = div_fast(p, a.page_div);
+    ok = ok && pi < a.table_pages;
+    const uint32_t pg = uint32_t(a.table[size_t(q) * a.table_pages + (ok ? pi : 0)]);
+    ok = ok && pg < a.n_pages;
+    return ok ? (int64_t(pg) * a.kv_heads + head) * a.page + (p - pi * a.page) : -1;
 }
 
 }  // namespace tc

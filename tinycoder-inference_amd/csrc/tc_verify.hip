@@ -95,20 +95,6 @@ __device__ __forceinline__ double wave_scan(double v) {
 }
 __device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), 63); }
 
-// As find_seq, 64 sequences at a time: one fetch where there are no more.
-__device__ __forceinline__ int wave_find_seq(const int32_t *start, uint32_t n_seq, uint32_t t) {
-    const uint32_t lane = threadIdx.x & 63;
-    const int32_t before = start[0], behind = start[n_seq];
-    uint32_t lo = 0, hi = n_seq;
-    while (hi - lo > 1) {
-        const uint32_t step = div_up(hi - lo, 64), p = lo + lane * step;
-        const uint64_t m = __ballot(p < hi && (p == lo || start[p] <= int32_t(t)));
-        lo += (63 - __builtin_clzll(m)) * step;
-        hi = min(lo + step, hi);
-    }
-    return int32_t(t) >= behind || int32_t(t) < before ? -1 : int(lo);
-}
-
 // log2(e) / temperature, 0 for the greedy choice; and the difference of logits below
 // which a token's share is taken for 0 (2^-900).
 struct Scale {
