@@ -73,7 +73,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
         auto load = [&](uint32_t dst, const uint8_t *src, const TileRuns &w, auto swizzle) __attribute__((always_inline)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint8_t *at = src + uint64_t(w.run[h]) * run_bytes;
+                const uint8_t *at = src + uint64_t(w.of(h != 0)) * run_bytes;
 #pragma unroll
                 for (int j = 0; j < 16 / RPI; ++j) {
                     const uint32_t r = j * RPI + lane / LPR, c = (lane % LPR) ^ swizzle(16 * h + r);
@@ -96,7 +96,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
         // lanes 0-31 the keys' factors of the 32 tokens, the others the values'
         auto load_scales = [&](const TileRuns &w, uint32_t i) __attribute__((always_inline)) {
             const float *p = lane >= 32 ? a.kv.vs : a.kv.ks;
-            dma4(kring + 2 * NB * TILE + i % (NB + 1) * 256, p + 16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + (lane & 15));
+            dma4(kring + 2 * NB * TILE + i % (NB + 1) * 256, p + 16 * uint64_t(w.of(lane & 16)) + (lane & 15));
         };
 
         Acc<R> o[DB];

@@ -685,13 +685,18 @@ template <int STRETCH>
 __device__ __forceinline__ bool all_held(const RunMisc<STRETCH> &rm, uint32_t tiles, uint32_t lane) {
     return __ballot(lane < (2 * tiles + 63) / 64 && rm.held[lane % (STRETCH / 32)] != ~uint64_t(0)) == 0;
 }
-// The two runs of a tile, wave-uniform.
+// The two runs of a tile, wave-uniform. (Not an array: one that lanes index goes to
+// memory, and waiting for that waits for every tile on its way.)
 struct TileRuns {
-    uint32_t run[2];
+    uint32_t first, second;
+    __device__ __forceinline__ uint32_t of(bool later) const {
+        const uint32_t x = first, y = second;
+        return later ? y : x;
+    }
 };
 template <int STRETCH>
 __device__ __forceinline__ TileRuns tile_runs(const RunMisc<STRETCH> &rm, uint32_t t) {
-    return TileRuns{{uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t])), uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]))}};
+    return TileRuns{uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t])), uint32_t(__builtin_amdgcn_readfirstlane(rm.run[2 * t + 1]))};
 }
 // Which of them pages hold: bit g for run g.
 template <int STRETCH>

@@ -147,7 +147,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                     const uint32_t i = val ? f - LOADS : f, h = i * RPI / 16, rh = i * RPI % 16 + lane / LPR;
                     const uint32_t r = 16 * h + rh;
                     const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r));
-                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(h != 0 ? w.run[1] : w.run[0]) * run_bytes;
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(w.of(h != 0)) * run_bytes;
                     // (dims past the row's: others of it, which meet zeros of q, or go nowhere)
                     dma16((val ? vbuf : kbuf) + buf * TILE + i * 1024, src, rh * rowbytes + (16 * c < rowbytes ? 16 * c : 0));
                 }
@@ -158,10 +158,10 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                     const uint32_t f = tid + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
                     const bool val = rr >= kTileTokens;
                     const uint32_t r = rr % kTileTokens;
-                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(r >= 16 ? w.run[1] : w.run[0]) * run_bytes + r % 16 * rowbytes;
+                    const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(w.of(r >= 16)) * run_bytes + r % 16 * rowbytes;
                     if (CHUNKS >= kThreads || f < CHUNKS) raw[j] = *reinterpret_cast<const u32x4 *>(src + (16 * c < rowbytes ? 16 * c : 0));
                 }
-                if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(lane & 16 ? w.run[1] : w.run[0]) + lane % 16];
+                if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(w.of(lane & 16)) + lane % 16];
             }
         };
         // (8-bit types) what load() fetched, widened, into its tile
