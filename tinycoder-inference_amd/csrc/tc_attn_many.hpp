@@ -45,6 +45,13 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
     const uint32_t kbuf = lds_addr(lds) + kMisc, vbuf = kbuf + NBUF * TILE;
     const uint32_t D = a.kv.dim, rowbytes = D * (SCALED ? 1 : 2);
 
+    // Where rows of q in several pieces and wide sums fill the registers, what a tile's loads
+    // need of the lane is formed for each: kept, it was spilled, and a reload waits for the
+    // tiles on their way (7 sequences, fp32 rows, int8 heads of 256: 157 -> 125 us; narrower
+    // ones lose up to 5% so). Fewer operands are fetched ahead there too.
+    constexpr bool SHORT = NP * DP >= 512;
+    auto place_lane = [&]() __attribute__((always_inline)) { return SHORT ? lane_now() : lane; };
+
     Place pl = work.at;
     uint64_t left = work.left;
     bool first_seg = true;
@@ -139,37 +146,39 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
         auto load = [&](uint32_t t) __attribute__((always_inline)) {
             const TileRuns w = tile_runs(ms.runs, t - t0);
             const uint32_t buf = (t - t0) % NBUF;
+            const uint32_t ln = place_lane();
             if constexpr (!SCALED) {
 #pragma unroll
                 for (int j = 0; j < MINE; ++j) {
                     const uint32_t f = wave + NW * j;
                     const bool val = LOADS % NW == 0 ? j >= LOADS / NW : f >= uint32_t(LOADS);
-                    const uint32_t i = val ? f - LOADS : f, h = i * RPI / 16, rh = i * RPI % 16 + lane / LPR;
+                    const uint32_t i = val ? f - LOADS : f, h = i * RPI / 16, rh = i * RPI % 16 + ln / LPR;
                     const uint32_t r = 16 * h + rh;
-                    const uint32_t c = (lane % LPR) ^ (val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r));
+                    const uint32_t c = (ln % LPR) ^ (val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r));
                     const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(w.of(h != 0)) * run_bytes;
                     // (dims past the row's: others of it, which meet zeros of q, or go nowhere)
                     dma16((val ? vbuf : kbuf) + buf * TILE + i * 1024, src, rh * rowbytes + (16 * c < rowbytes ? 16 * c : 0));
                 }
             } else {
                 // 16 bytes (16 dims) of one row per load: kThreads / (DP / 16) rows at a time, keys then values
+                const uint32_t tn = 64 * wave + ln;
 #pragma unroll
                 for (int j = 0; j < RAW; ++j) {
-                    const uint32_t f = tid + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
+                    const uint32_t f = tn + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
                     const bool val = rr >= kTileTokens;
                     const uint32_t r = rr % kTileTokens;
                     const uint8_t *src = (val ? a.kv.v : a.kv.k) + uint64_t(w.of(r >= 16)) * run_bytes + r % 16 * rowbytes;
                     if (CHUNKS >= kThreads || f < CHUNKS) raw[j] = *reinterpret_cast<const u32x4 *>(src + (16 * c < rowbytes ? 16 * c : 0));
                 }
-                if (tid < 64) raw_scale = (lane >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(w.of(lane & 16)) + lane % 16];
+                if (wave == 0) raw_scale = (ln >= 32 ? a.kv.vs : a.kv.ks)[16 * uint64_t(w.of(ln & 16)) + ln % 16];
             }
         };
         // (8-bit types) what load() fetched, widened, into its tile
         auto put = [&](uint32_t t) __attribute__((always_inline)) {
-            const uint32_t buf = (t - t0) % NBUF;
+            const uint32_t buf = (t - t0) % NBUF, ln = place_lane(), tn = 64 * wave + ln;
 #pragma unroll
             for (int j = 0; j < RAW; ++j) {
-                const uint32_t f = tid + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
+                const uint32_t f = tn + kThreads * j, c = f % (DP / 16), rr = f / (DP / 16);
                 if (CHUNKS < kThreads && f >= CHUNKS) break;
                 const bool val = rr >= kTileTokens;
                 const uint32_t r = rr % kTileTokens, sw = val ? value_swizzle<R, RB, 2>(r) : key_swizzle<R, RB>(r);
@@ -180,14 +189,14 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                     *reinterpret_cast<u32x4 *>(dst + (((2 * c + e) ^ sw) << 4)) = u32x4{x[0], x[1], y[0], y[1]};
                 }
             }
-            if (tid < 64) {
-                if (lane < 32) {
-                    ms.many.kf[buf][lane] = raw_scale;
+            if (wave == 0) {
+                if (ln < 32) {
+                    ms.many.kf[buf][ln] = raw_scale;
                 } else {
                     // (a factor of 0: values of next to nothing; NaN stays)
                     const float x = raw_scale == raw_scale ? fmaxf(raw_scale, 0x1p-126f) : raw_scale;
-                    ms.many.lv[buf][lane - 32] = __builtin_amdgcn_logf(x);
-                    ms.many.iv[buf][lane - 32] = __builtin_amdgcn_rcpf(x);
+                    ms.many.lv[buf][ln - 32] = __builtin_amdgcn_logf(x);
+                    ms.many.iv[buf][ln - 32] = __builtin_amdgcn_rcpf(x);
                 }
             }
         };
@@ -274,7 +283,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
         // behind its operands.
         auto fast = [&](auto buf_c, uint32_t t, const uint32_t (&kp)[NA], uint32_t vp) __attribute__((always_inline)) {
             constexpr uint32_t buf = decltype(buf_c)::value, nbuf = (buf + 1) % NBUF;
-            constexpr int KEYS = NA * KS, VALS = Ge::KT * DB, AHEAD = 4;
+            constexpr int KEYS = NA * KS, VALS = Ge::KT * DB, AHEAD = SHORT ? 2 : 4;
             if constexpr (!SCALED) {
                 if (t + 2 < t1)
                     wait_loads<MINE>();
