@@ -46,6 +46,10 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
     float *const lv = raw + 64 * (NB + 1), *const iv = lv + 32;               // [32] log2 and reciprocal of the values'
     const uint32_t D = a.kv.dim, rowbytes = D * ES, run_bytes = 16 * rowbytes, nch = rowbytes / 16;
 
+    // (as for many rows: formed anew, not kept, where registers are short)
+    constexpr bool SHORT = NP * DP >= 512;
+    auto place_lane = [&]() __attribute__((always_inline)) { return SHORT ? lane_now() : lane; };
+
     Place pl = work.at;
     uint64_t left = work.left;
     bool first_seg = true;
@@ -71,12 +75,13 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
         // decoding sequences 198 -> 175 us, while 4 blocks read 5% slower so)
         const bool once = b.rows <= R;
         auto load = [&](uint32_t dst, const uint8_t *src, const TileRuns &w, auto swizzle) __attribute__((always_inline)) {
+            const uint32_t ln = place_lane();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint8_t *at = src + uint64_t(w.of(h != 0)) * run_bytes;
 #pragma unroll
                 for (int j = 0; j < 16 / RPI; ++j) {
-                    const uint32_t r = j * RPI + lane / LPR, c = (lane % LPR) ^ swizzle(16 * h + r);
+                    const uint32_t r = j * RPI + ln / LPR, c = (ln % LPR) ^ swizzle(16 * h + r);
                     // (dims past the row's: others of it, which meet zeros of q, or go nowhere)
                     const uint32_t lane_off = r * rowbytes + (c < nch ? 16 * c : 0);
                     if (once)
@@ -136,6 +141,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                 // ---- scores ----
                 float s[NS];
                 {
+                    const uint32_t ln = place_lane();
                     Acc<R> x[Ge::NA];
 #pragma unroll
                     for (int i = 0; i < Ge::NA; ++i) x[i] = Acc<R>{};
@@ -144,7 +150,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                             for (int i = 0; i < Ge::NA; ++i) {
-                                const u32x4 k = lds_at((ktile + key_place<R, RB>(i, lane)) ^ key_step<R>(ks));
+                                const u32x4 k = lds_at((ktile + key_place<R, RB>(i, ln)) ^ key_step<R>(ks));
 #pragma unroll
                                 for (int p = NP - 1; p >= 0; --p) x[i] = mfma<CT>(k, q[p][ks], x[i]);
                             }
@@ -153,7 +159,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                         for (int k2 = 0; k2 < KS / 2; ++k2)
 #pragma unroll
                             for (int i = 0; i < Ge::NA; ++i) {
-                                const u32x4 w = lds_at((ktile + key_place<R, RB>(i, lane)) ^ key_step<R>(k2));
+                                const u32x4 w = lds_at((ktile + key_place<R, RB>(i, ln)) ^ key_step<R>(k2));
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     const u32x2 y = widen<CT>(w[2 * e]), z = widen<CT>(w[2 * e + 1]);
@@ -246,17 +252,18 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
 #pragma unroll
                         for (int p = 0; p < NP; ++p) pw[p][j] = piece2<CT>(x, y);
                     }
+                    const uint32_t ln = place_lane();
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
                         u32x4 v;
                         if constexpr (ES == 2) {
-                            v = value_frag<RB>((vtile + value_place<R, RB>(lane)) ^ value_block<R>(d), 0);
+                            v = value_frag<RB>((vtile + value_place<R, RB>(ln)) ^ value_block<R>(d), 0);
                         } else {
                             // 8 tokens of one dim: 16 lanes give 8 rows of 16 bytes
-                            const uint32_t r = 8 * g + (lane & 15) / 2;
+                            const uint32_t r = 8 * (ln / R) + (ln & 15) / 2;
                             const u32x2 w = __builtin_bit_cast(
                                 u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) s32x2 *>(
-                                           vtile + r * RB + ((d ^ value_swizzle<R, RB, 1>(r)) << 4) + 8 * (lane & 1))));
+                                           vtile + r * RB + ((d ^ value_swizzle<R, RB, 1>(r)) << 4) + 8 * (ln & 1))));
                             const u32x2 x = widen<CT>(w[0]), y = widen<CT>(w[1]);
                             v = u32x4{x[0], x[1], y[0], y[1]};
                         }
