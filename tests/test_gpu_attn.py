@@ -246,6 +246,53 @@ def test_attn_many_sequences(tc, dev, n_seq):
     check_attn(tc, dev, none, 4, "F32", 0.2)
 
 
+@pytest.mark.parametrize("ctype,xtype", [("BF16", "BF16"), ("F16", "F32"), ("I8", "F32"), ("E4M3", "F16")])
+@pytest.mark.parametrize("dim", [48, 64, 112, 128, 208, 240])
+def test_attn_block_borders(tc, dev, ctype, xtype, dim):
+    """As many rows as fill blocks of either kind, one less and one more, alone in a head and in groups."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, [(n, n + int(rng.integers(0, 80))) for n in (15, 16, 17, 63, 64, 65, 127, 129)], 48, 1, dim, ctype).to(dev)
+    check_attn(tc, dev, b, 1, xtype, dim ** -0.5)
+    b = Batch(rng, [(n, n + int(rng.integers(0, 80))) for n in (5, 6, 21, 22, 43, 86)], 16, 1, dim, ctype, pad_rows=1).to(dev)
+    check_attn(tc, dev, b, 3, xtype, dim ** -0.5, window=40)
+
+
+@pytest.mark.parametrize("group", [1, 5, 64, 65, 300])
+def test_attn_groups(tc, dev, group):
+    """Groups as large as the blocks of rows and larger: a token's rows lie in several blocks."""
+    rng = np.random.default_rng(group)
+    b = Batch(rng, [(1, 33), (2, 50), (7, 7)], 16, 2, 32, "BF16").to(dev)
+    check_attn(tc, dev, b, 2 * group, "BF16", 0.2)
+
+
+def test_attn_captured_at_first(tc, dev):
+    """The first call of its kind, captured after tc_attn_reserve alone."""
+    rng = np.random.default_rng(13)
+    b = Batch(rng, [(1, 90), (40, 70)], 32, 2, 144, "E4M3").to(dev)
+    q = rows_of(rng, b.T, 4, 144, "F32").to(dev)
+    tc.attn_reserve(4, b.T)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = tc.attn(b.cache, b.batch, q, 0.1)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, tc.attn(b.cache, b.batch, q, 0.1))
+
+
+def test_attn_batch_of_several_calls(tc, dev):
+    """One batch for calls of different numbers of rows, as a program's padded and whole steps make them."""
+    rng = np.random.default_rng(14)
+    b = Batch(rng, [(1, 40), (2, 30)], 16, 2, 64, "F16", pad_rows=5).to(dev)
+    q = rows_of(rng, b.T, 4, 64, "F32").to(dev)
+    whole = tc.attn(b.cache, b.batch, q, 0.125)
+    assert torch.equal(tc.attn(b.cache, b.batch, q[:3].contiguous(), 0.125), whole[:3])
+    k, _ = tc.kv_read(b.cache, b.batch, 3, torch.float32)
+    assert torch.equal(tc.kv_read(b.cache, b.batch, 3, torch.float32)[0], k)
+    assert torch.equal(tc.attn(b.cache, b.batch, q, 0.125)[:3], whole[:3])
+
+
 @pytest.mark.parametrize("ctype", ["F16", "I8"])
 @pytest.mark.parametrize("n", [1, 80])
 def test_attn_long_parts(tc, dev, ctype, n):

@@ -325,7 +325,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
             sc.jobs[work.id] = SplitJob{b.begin, r0, kvh, min(uint32_t(R), b.rows - r0), 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= sg.places;
         first_seg = false;
-        if (left != 0) next_block<R>(a, rg, seqs, b.rows, pl);
+        if (left != 0 && !next_block<R>(a, rg, seqs, b.rows, pl)) break;
     }
 }
 

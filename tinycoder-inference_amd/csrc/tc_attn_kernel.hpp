@@ -552,6 +552,7 @@ __device__ __forceinline__ void line_step(const AttnArgs &a, RowRange rg, Seqs s
         r0 = 0;
         do ++s;
         while (s + 1 < a.kv.n_seq && rows_in(a, rg, seqs.at(a, s).n) == 0);
+        s = min(s, a.kv.n_seq - 1);  // (start and len may change under a call that should not run then)
     }
 }
 // The sequences into LDS where they fit, and their blocks of both kinds counted: few |
@@ -642,16 +643,21 @@ __device__ __forceinline__ Place line_part(const AttnArgs &a, RowRange rg, const
     return p;
 }
 
-// The block of rows behind place p's (p.off = 0). The line does not end there.
+// The block of rows behind place p's (p.off = 0); false where the line ends there, as it
+// only does if start or len have changed since.
 template <int ROWS>
-__device__ __forceinline__ void next_block(const AttnArgs &a, RowRange rg, Seqs seqs, uint32_t rows, Place &p) {
+__device__ __forceinline__ bool next_block(const AttnArgs &a, RowRange rg, Seqs seqs, uint32_t rows, Place &p) {
     p.off = 0;
     p.r0 += ROWS;
-    if (p.r0 < rows) return;
+    if (p.r0 < rows) return true;
     p.r0 = 0;
     do {
-        if (++p.seq == a.kv.n_seq) p.seq = 0, ++p.kvh;
+        if (++p.seq == a.kv.n_seq) {
+            p.seq = 0;
+            if (++p.kvh == a.kv.kv_heads) return false;
+        }
     } while (rows_in(a, rg, seqs.uniform(a, p.seq).n) == 0);
+    return true;
 }
 
 // ---- pages --------------------------------------------------------------------

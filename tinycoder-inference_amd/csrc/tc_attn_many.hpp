@@ -452,7 +452,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
             sc.jobs[work.id] = SplitJob{b.begin, r0, kvh, min(uint32_t(Sh::ROWS), b.rows - r0), 1 + uint32_t((b.tiles - seg + work.part - 1) / work.part), slot};
         left -= sg.places;
         first_seg = false;
-        if (left != 0) next_block<Sh::ROWS>(a, rg, seqs, b.rows, pl);
+        if (left != 0 && !next_block<Sh::ROWS>(a, rg, seqs, b.rows, pl)) break;
     }
 }
 
