@@ -39,7 +39,10 @@ enum { TC_F32 = 0, TC_F16 = 1, TC_I8 = 24, TC_BF16 = 30, TC_E4M3 = 100 };
  *                     16-byte aligned
  *   k_scale, v_scale  fp32 [n_pages][kv_heads][page_tokens] for I8 and E4M3 (one
  *                     factor per token and head), NULL for F16 and BF16
- * page_tokens: a multiple of 16. head_dim: a multiple of 16, up to 256. */
+ * page_tokens: a multiple of 16. head_dim: a multiple of 16, up to 256. Factors as
+ * tc_kv_write forms them are above 0; tc_attn takes v_scale for that (one below
+ * 2^-126 as 2^-126). Less than 2^32 runs of 16 tokens (n_pages * kv_heads *
+ * page_tokens / 16). */
 typedef struct tc_kv_cache {
     int32_t type;
     uint32_t n_pages, kv_heads, page_tokens, head_dim;
@@ -55,7 +58,8 @@ typedef struct tc_kv_cache {
  * page_tokens]. Positions below 0, at table_pages * page_tokens or above, or in
  * a page outside [0, n_pages) hold no token: not written, read as zeros, not
  * attended to. Rows past start[n_seq] are not touched. Pages may be shared
- * between sequences; one slot is to be written by one row of a call. */
+ * between sequences; one slot is to be written by one row of a call. At most 2^20
+ * sequences, 2^24 rows, 2^31 - 65 tokens of a sequence. */
 typedef struct tc_kv_batch {
     uint32_t n_seq, n_tokens, table_pages;
     const int32_t *start, *len, *table;
@@ -85,8 +89,11 @@ int tc_kv_read(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, vo
  * [n_tokens][heads][head_dim] of `xtype`, 16-byte aligned. Sums and the softmax are
  * held in fp32; q and the softmax's weights enter the matrix cores as F16 or BF16
  * (the 16-bit cache's own type; F16 for the 8-bit ones) in as many pieces as
- * `xtype` has bits for, so that fp32 rows keep fp32 results. heads: a multiple of
- * kv_heads. scale: finite, not negative. */
+ * `xtype` has bits for, so that fp32 rows keep fp32 results (as F16 a weight is held
+ * to half a step or 2^-36 of its row's largest, whichever is more). Infinities and
+ * NaN in the cache reach only the rows that see them. The same call gives the same
+ * bits. heads: a multiple of kv_heads, up to 4096; n_tokens * heads < 2^31. scale:
+ * finite, not negative. start, len and table are not to change while a call runs. */
 int tc_attn(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, const void *q, uint32_t q_stride, void *out,
             uint32_t heads, float scale, uint32_t window, void *stream);
 
@@ -110,7 +117,9 @@ int tc_attn_reserve(uint32_t heads, uint32_t n_tokens);
  * p = 1 and needs no random numbers. Drafts outside [0, vocab) are rejected.
  * Probabilities and sums are formed in fp64. n_accepted[s] (drafts taken) and
  * next_token[s] are int32; a sequence without rows gives 0 and -1, one whose row
- * has a NaN or no finite largest logit the rejection of that draft and -1 as the token. */
+ * has a NaN or no finite largest logit the rejection of that draft and -1 as the token.
+ * (Shares below 2^-900 of the largest count as 0.) 1 to 65535 rows, up to 65535
+ * sequences, vocab up to 2^30. */
 int tc_spec_verify(const float *logits, const float *draft_probs, uint32_t vocab, uint32_t n_seq, uint32_t n_tokens,
                    const int32_t *start, const int32_t *tokens, const float *temperature, const float *accept_u,
                    const float *sample_u, int32_t *n_accepted, int32_t *next_token, void *stream);

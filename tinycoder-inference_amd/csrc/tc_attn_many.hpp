@@ -8,6 +8,13 @@
 // formed, so that a wave's matrix and vector work do not wait for each other. The
 // line of tiles is cut into one part per CU; blocks that a cut goes through leave
 // their sums for k_attn_join.
+//
+// Measured: 2048 rows of 28 heads of 128 at 8193 tokens (bf16, 210 GFLOP) 230 to 245 us,
+// 860 to 915 TFLOP/s, where a large library product reaches 1190: matrix cores busy 41%
+// of the time, vector instructions 39%, no LDS conflicts; the two of a SIMD hardly overlap
+// although their order is pinned side by side. As fast: two workgroups of 4 waves per
+// CU; a barrier between the two products. Slower: a barrier at every second tile (247
+// against 241). Seven sequences of fp32 rows (two pieces) over int8 heads of 256, 125 us.
 #pragma once
 
 #include <type_traits>
@@ -278,7 +285,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
         // the loop, as long as every row of the wave sees all of them and the one behind.
         // A tile's score products are issued among the weights of the one before, its
         // value products among the sums and maxima of the one behind, operands
-        // kAhead products ahead of their use. The order is pinned: left to itself the
+        // AHEAD products ahead of their use. The order is pinned: left to itself the
         // compiler puts the vector work behind the products, and each product right
         // behind its operands.
         auto fast = [&](auto buf_c, uint32_t t, const uint32_t (&kp)[NA], uint32_t vp) __attribute__((always_inline)) {
