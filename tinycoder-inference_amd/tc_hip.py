@@ -398,10 +398,10 @@ class Library:
         T, H, D = shape
         if D != cache.head_dim:
             raise TCError(TC_E_ARG, f"head_dim {D} is not the cache's {cache.head_dim}")
-        for i, t in enumerate((x, y)):
-            if not t.is_contiguous():
+        if not (x.is_contiguous() and y.is_contiguous()):
+            for i, t in enumerate((x, y)):
                 st = t.stride()
-                if i >= strided or T != 0 and (st[2] != 1 or (H != 1 and st[1] != D)):
+                if not t.is_contiguous() and (i >= strided or T != 0 and (st[2] != 1 or (H != 1 and st[1] != D))):
                     raise TCError(TC_E_ARG, "a row's heads are not contiguous" if i < strided else "out is not contiguous")
         dev = torch.cuda.current_device()
         if not x.get_device() == y.get_device() == cache.device == batch.device == dev:
@@ -425,8 +425,8 @@ class Library:
         """The batch's n_tokens rows out of the cache: (k, v)."""
         import torch
         if out is None:
-            shape = (n_tokens, cache.kv_heads, cache.head_dim)
-            k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+            k = torch.empty((n_tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.k.device)
+            v = torch.empty_like(k)
         else:
             k, v = out
             if k.dim() != 3 or k.shape[:2] != (n_tokens, cache.kv_heads) or k.dtype != dtype:
@@ -440,7 +440,7 @@ class Library:
         over the cache."""
         import torch
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         T, stream = self._kv_call(cache, batch, q, out, 1)
         self._check(self.lib.tc_attn(cache.ref, batch.of(T), _elem_type(q.dtype), q.data_ptr(), self._row_stride(q),
                                      out.data_ptr(), q.shape[1], scale, window, stream))
@@ -465,10 +465,11 @@ class Library:
         if not (start.numel() == S + 1 and tokens.numel() == accept_u.numel() == T and sample_u.numel() == S and
                 (draft_probs is None or draft_probs.shape == logits.shape)):
             raise TCError(TC_E_ARG, "sizes do not agree")
-        n, tok = (torch.empty(S, dtype=torch.int32, device=logits.device) for _ in range(2))
-        self._check(self.lib.tc_spec_verify(_ptr(logits), _ptr(draft_probs), V, S, T, _ptr(start), _ptr(tokens),
-                                            _ptr(temperature), _ptr(accept_u), _ptr(sample_u), _ptr(n), _ptr(tok),
-                                            self._stream(dev)))
+        n = torch.empty(S, dtype=torch.int32, device=logits.device)
+        tok = torch.empty_like(n)
+        self._check(self.lib.tc_spec_verify(logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), V, S, T,
+                                            start.data_ptr(), tokens.data_ptr(), temperature.data_ptr(), accept_u.data_ptr(),
+                                            sample_u.data_ptr(), n.data_ptr(), tok.data_ptr(), self._stream(dev)))
         return n, tok
 
 
