@@ -89,6 +89,26 @@ def test_kv_read(tc, dev, xtype, ctype, kv_heads, dim, page):
         assert (got[-3:] == 7).all()
 
 
+@pytest.mark.parametrize("n_seq", [63, 64, 65, 5000])
+@pytest.mark.parametrize("ctype", ["BF16", "I8"])
+def test_kv_many_sequences(tc, dev, ctype, n_seq):
+    """Sequences of no, one and several rows: each row into its own pages and back, more of them than one lane takes."""
+    rng = np.random.default_rng(n_seq)
+    new = rng.choice([0, 0, 1, 1, 2, 17], n_seq)
+    seqs = [(int(n), int(n + rng.integers(0, 40))) for n in new]
+    b = Batch(rng, seqs, 16, 2, 48, ctype, pad_rows=3).to(dev)
+    k, v = (rows_of(rng, b.T, 2, 48, "F32") for _ in range(2))
+    tc.kv_write(b.cache, b.batch, k.to(dev), v.to(dev))
+    got = [t.cpu() for t in tc.kv_read(b.cache, b.batch, b.T, torch.float32,
+                                       out=tuple(torch.full((b.T, 2, 48), 7.0, device=dev) for _ in range(2)))]
+    used = int(b.start[-1])
+    for x, y in zip((k, v), got):
+        # bf16: half a step; int8: half a step of max / 127, and the two roundings of the quotients and of the product
+        top = x.abs().amax(-1, keepdim=True)
+        bound = x.abs() * 2.0 ** -8 if ctype == "BF16" else top / 127 * 0.5 + x.abs() * 2.0 ** -22
+        assert ((x - y).abs() <= bound)[:used].all() and (y[used:] == 7).all()
+
+
 @pytest.mark.parametrize("ctype", ["I8", "E4M3"])
 def test_kv_write_extremes(tc, dev, ctype):
     """A row with an infinity or a NaN reads back as NaNs, its neighbours do not; a row of the smallest

@@ -98,6 +98,12 @@ def test_verify_batches(tc, dev, counts, probs):
 
 
 @pytest.mark.parametrize("probs", [False, True])
+def test_verify_many_sequences(tc, dev, probs):
+    """Thousands of sequences, most of them of no row, one or two."""
+    check(tc, dev, problem(17, [1, 0, 2, 0, 0, 5] * 800, 37, probs, pad=3))
+
+
+@pytest.mark.parametrize("probs", [False, True])
 def test_verify_greedy_and_mixed(tc, dev, probs):
     """Temperature 0, with ties (the lowest token), beside sampled sequences."""
     p = problem(3, [5] * 40, 5000, probs, temps=[0.0, 0.7] * 20)
