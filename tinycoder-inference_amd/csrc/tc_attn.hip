@@ -4,7 +4,7 @@
 
 namespace tc {
 
-size_t attn_scratch_bytes(uint32_t, uint32_t, int num_cu) { return attn_part_bytes(num_cu); }
+size_t attn_scratch_bytes(int num_cu) { return attn_part_bytes(num_cu); }
 
 hipError_t launch_attn(const AttnArgs &a, int ctype, int num_cu, void *scratch, hipStream_t st) {
     switch (ctype) {

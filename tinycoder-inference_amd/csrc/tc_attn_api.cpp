@@ -136,7 +136,7 @@ int tc_attn(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, const
     const int num_cu = tc::device_cu_count();
     if (num_cu == 0) return no_device();
     void *scratch = nullptr;
-    const size_t need = tc::attn_scratch_bytes(heads, n, num_cu);
+    const size_t need = tc::attn_scratch_bytes(num_cu);
     if (need != 0 && !(scratch = tc::aux_scratch(need, st))) return TC_E_LAUNCH;
     return hip_rc(tc::launch_attn(a, cache->type, num_cu, scratch, st), "attention");
 }
@@ -146,7 +146,7 @@ int tc_attn_reserve(uint32_t heads, uint32_t n_tokens) {
     if (heads > 4096 || n_tokens > (1u << 24)) return refuse(TC_E_UNSUPPORTED, "more than 4096 heads or 2^24 rows");
     const int num_cu = tc::device_cu_count();
     if (num_cu == 0) return no_device();
-    size_t need = tc::attn_scratch_bytes(heads, n_tokens, num_cu);
+    size_t need = tc::attn_scratch_bytes(num_cu);
     if (n_tokens <= 65535) need = std::max(need, tc::verify_scratch_bytes(n_tokens, n_tokens));
     return tc::aux_scratch(need, nullptr) ? TC_OK : TC_E_LAUNCH;
 }

@@ -98,7 +98,7 @@ struct AttnArgs {
     int32_t span;  // tokens that a row sees at most: the window
     int xtype;
 };
-size_t attn_scratch_bytes(uint32_t heads, uint32_t n_tokens, int num_cu);
+size_t attn_scratch_bytes(int num_cu);
 hipError_t launch_attn(const AttnArgs &a, int ctype, int num_cu, void *scratch, hipStream_t st);
 // ... for one cache type (tc_attn_inst.hip).
 template <int CT>

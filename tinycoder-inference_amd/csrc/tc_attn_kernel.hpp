@@ -378,7 +378,7 @@ __device__ __forceinline__ void add_values_one_by_one(const unsigned char *vt, c
         }
 }
 
-// Output dims e .. e + 3 (or e alone) of a row of a sequence's block.
+// Output dims e .. e + 3 of a row of a sequence's block.
 __device__ __forceinline__ uint64_t out_at(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row) {
     const uint32_t tok = div_fast(row, a.group_div);
     return (uint64_t(begin + tok) * a.heads + kvh * a.group + row - tok * a.group) * a.kv.dim;
@@ -392,13 +392,6 @@ __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t begin, uint32
                                         : u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
         *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + at) = w;
     }
-}
-__device__ __forceinline__ void store1(const AttnArgs &a, uint32_t begin, uint32_t kvh, uint32_t row, uint32_t e, float x) {
-    const uint64_t at = out_at(a, begin, kvh, row) + e;
-    if (a.xtype == kF32)
-        static_cast<float *>(a.out)[at] = x;
-    else
-        static_cast<uint16_t *>(a.out)[at] = uint16_t(a.xtype == kF16 ? pack_f16(x, x) : pack_bf16(x, x));
 }
 
 // ---- the line of tiles ------------------------------------------------------

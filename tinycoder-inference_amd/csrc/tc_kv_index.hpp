@@ -82,17 +82,8 @@ TC_HD int32_t page_at(const KvArgs &a, uint32_t s, uint32_t pi) {
     return pg < a.n_pages ? int32_t(pg) : -1;
 }
 
-// Cache row (page * kv_heads + head) * page_tokens + slot of position pos of
-// sequence s; -1 where no page holds it. A cache may have more than 2^31 rows.
-TC_HD int64_t cache_row(const KvArgs &a, uint32_t s, int64_t pos, uint32_t head) {
-    if (pos < 0 || pos >= int64_t(kMaxPos)) return -1;
-    const uint32_t pi = div_fast(uint32_t(pos), a.page_div);
-    const int32_t pg = page_at(a, s, pi);
-    if (pg < 0) return -1;
-    return (int64_t(pg) * a.kv_heads + head) * a.page + (uint32_t(pos) - pi * a.page);
-}
-
-// Cache row of batch row t of sequence s (-1: none) and head. (No branch between the
+// Cache row (page * kv_heads + head) * page_tokens + slot of batch row t of sequence s
+// (-1: none) and head; a cache may have more than 2^31 rows. (No branch between the
 // loads: a lane's rows are looked up side by side.)
 TC_HD int64_t slot_of(const KvArgs &a, int s, uint32_t t, uint32_t head) {
     const uint32_t q = s < 0 ? 0 : uint32_t(s);
