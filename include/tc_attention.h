@@ -110,7 +110,8 @@ int tc_attn_reserve(uint32_t heads, uint32_t n_tokens);
  * q_i(x) < p_i(x). At the first that is not, at row i, the next token is drawn from
  * max(p_i - q_i, 0) (from p_i where that is zero everywhere); where all are taken,
  * from the last row's p: the lowest token t whose sum of weights up to t exceeds
- * sample_u[s] times the sum of all (if none: the last of weight above 0).
+ * sample_u[s] times the sum of all (if none: the last of weight above 0; a sample_u
+ * below 0 is taken for 0).
  * draft_probs (fp32 [n_tokens][vocab], row start[s]+i for draft i+1; each
  * sequence's last row is not read) may be NULL: drafted without chance, q is 1 at
  * the draft. temperature[s] = 0 takes the largest logit, lowest token first, for

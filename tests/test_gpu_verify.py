@@ -237,3 +237,68 @@ def test_draft_step(tc, dev):
         assert ((back - rows).abs() <= rows.abs().amax(-1, keepdim=True) / 127 * 0.5001).all()
         if int(lengths.max()) > 90:
             break
+
+
+def verify_into(tc, dev, p):
+    """The C entry into outputs that hold no token yet."""
+    t = [None if a is None else torch.from_numpy(a).to(dev) for a in p]
+    logits, tokens, start, temperature, accept_u, sample_u, probs = t
+    out = [torch.full((len(p[2]) - 1,), -7, dtype=torch.int32, device=dev) for _ in range(2)]
+    ptr = [x.data_ptr() if x is not None else None for x in (logits, probs)]
+    rc = tc.lib.tc_spec_verify(*ptr, logits.shape[1], len(p[2]) - 1, logits.shape[0],
+                               *(x.data_ptr() for x in (start, tokens, temperature, accept_u, sample_u, *out)), tc._stream())
+    assert rc == 0, tc.lib.tc_last_error()
+    return [o.cpu().numpy() for o in out]
+
+
+def draws(logits, u):
+    """One row of each sequence, nothing drafted."""
+    S = len(u)
+    return [logits, np.zeros(S, np.int32), np.arange(S + 1, dtype=np.int32), np.ones(S, np.float32), np.zeros(S, np.float32),
+            np.asarray(u, np.float32), None]
+
+
+def equal_tokens(where, u):
+    """For each random number the tokens it may draw among equal ones: the lowest whose share of the sum up to it
+    exceeds u, and where u is a border, which a rounding of that sum moves to either side, the one before it too."""
+    n = len(where)
+    for x in u:
+        k = int(np.floor(float(x) * n))
+        yield {int(where[k])} | ({int(where[k - 1])} if k and float(x) * n == k else set())
+
+
+@pytest.mark.parametrize("n", [10, 12, 14, 20, 40, 96])
+def test_verify_draws_on_borders_of_few(tc, dev, n):
+    """A few equal tokens of a vocabulary, anywhere: random numbers on the borders between them, each draws a token."""
+    V, u = 32768, np.arange(64) / 64
+    rng = np.random.default_rng(n)
+    for where in [np.arange(n) * (V // n), 512 * np.arange(n) % V + np.arange(n) // 64] + [rng.choice(V, n, False) for _ in range(6)]:
+        where = np.sort(where)
+        logits = np.full((64, V), -np.inf, np.float32)
+        logits[:, where] = 1.25
+        _, got = verify_into(tc, dev, draws(logits, u))
+        for j, may in enumerate(equal_tokens(where, u)):
+            assert got[j] in may, (j, got[j], may)
+        for j in (16, 32, 48):  # alone: other slices
+            _, one = verify_into(tc, dev, draws(logits[:1], u[j:j + 1]))
+            assert one[0] in list(equal_tokens(where, u[j:j + 1]))[0], j
+
+
+@pytest.mark.parametrize("V,S", [(128000, 48), (256000, 48), (50304, 64), (152064, 64), (1000, 1)])
+def test_verify_draws_on_borders_of_flat_rows(tc, dev, V, S):
+    """Vocabularies whose tokens are all alike, random numbers on a grid of 1/64."""
+    where = np.arange(V)
+    for first in range(0, 64, S):
+        u = (first + np.arange(S)) % 64 / 64
+        _, got = verify_into(tc, dev, draws(np.zeros((S, V), np.float32), u))
+        for j, may in enumerate(equal_tokens(where, u)):
+            # (sums of V roundings: a token further at most)
+            assert got[j] in may or abs(got[j] - u[j] * V) <= 1, (u[j], got[j], may)
+
+
+def test_verify_random_numbers_past_the_ends(tc, dev):
+    """Numbers below 0 draw the first token of any weight; 1, more, and NaN the last one."""
+    logits = np.full((7, 5000), -np.inf, np.float32)
+    logits[:, [70, 900, 901, 4321]] = [0.5, -3, 2, 1]
+    _, got = verify_into(tc, dev, draws(logits, [-1e-30, -0.5, -np.inf, 1, 1.5, np.inf, np.nan]))
+    assert got.tolist() == [70, 70, 70, 4321, 4321, 4321, 4321]

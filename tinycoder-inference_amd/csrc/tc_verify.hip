@@ -272,8 +272,10 @@ __device__ __forceinline__ Slice join(const Slice *r, uint32_t n, Scale z) {
 }
 
 // Sampling weight of token i with logit l at the stop: of the residual (over draft
-// probability q, or without the draft itself), and of p alone.
+// probability q, or without the draft itself), and of p alone. (Not contracted: a slice
+// that has a weight in one kernel has it in the other.)
 __device__ __forceinline__ Weight weight(const Stop &st, float l, float q, bool probs, uint32_t i, Scale z) {
+#pragma clang fp contract(off)
     const double p = share(l, st.m, z) * st.inv;
     double r = p;
     if (probs)
@@ -369,7 +371,9 @@ __global__ __launch_bounds__(kThreadsSeq, 6) void k_verify_weights(VerifyArgs a,
 // Twice the same: the first entry whose running sum passes a goal, the last one of any
 // weight where none does (a random number next to 1, and roundings); over the row's
 // slices, by each wave for itself, then over the slice's tokens. A thread's entries lie
-// next to each other.
+// next to each other. Where a lane's sums begin may differ by roundings from where the
+// last lane's ended, so that a goal between the two is passed before the first slice of
+// the next lane: its first weight is the one then, as for random numbers below 0.
 __global__ __launch_bounds__(kThreadsPick) void k_verify_pick(VerifyArgs a, Split sp, const Weight *__restrict__ w,
                                                              const Stop *__restrict__ stops) {
     constexpr uint32_t W = kThreadsPick / 64;
@@ -393,22 +397,27 @@ __global__ __launch_bounds__(kThreadsPick) void k_verify_pick(VerifyArgs a, Spli
     const double rest_to = wave_scan(rest), full_to = wave_scan(full), all_rest = lane_value(rest_to, 63);
     const bool residual = all_rest > 0.0;
     double goal = u * (residual ? all_rest : lane_value(full_to, 63));
-    double before = residual ? rest_to - rest : full_to - full, at = 0.0, least = 0.0;
+    double before = residual ? rest_to - rest : full_to - full, at = 0.0;
     uint32_t hit = 0xFFFFFFFFu, mine = 0;
 #pragma unroll 4
     for (uint32_t i = b0; i < e0; ++i) {
         const double v = residual ? r[i].rest : r[i].full;
         if (v > 0.0) {
             if (hit == 0xFFFFFFFFu && before + v > goal) hit = i, at = before;
-            mine = i + 1, least = before;
+            mine = i + 1;
         }
         before += v;
     }
     const uint64_t hits = __ballot(hit != 0xFFFFFFFFu), any = __ballot(mine != 0);
-    if (any == 0) return;  // (cannot be: the row's weights sum to 1)
+    if (any == 0) {  // (cannot be: the row's weights sum to 1)
+        if (tid == 0) a.next_token[s] = -1;
+        return;
+    }
     const uint32_t from = hits != 0 ? __builtin_ctzll(hits) : 63 - __builtin_clzll(any);
     const uint32_t slice = hits != 0 ? __builtin_amdgcn_readlane(hit, from) : __builtin_amdgcn_readlane(mine, from) - 1;
-    goal -= lane_value(hits != 0 ? at : least, from);
+    // (not below 0, which no weight would be the first to pass; no token of the last slice
+    // passes infinity)
+    goal = hits != 0 ? __builtin_fmax(goal - lane_value(at, from), 0.0) : __builtin_inf();
 
     const float *l = a.logits + size_t(st.row) * a.vocab;
     const float *q = a.draft_probs != nullptr && st.draft >= 0 ? a.draft_probs + size_t(st.row) * a.vocab : nullptr;
