@@ -114,8 +114,9 @@ int tc_attn_reserve(uint32_t heads, uint32_t n_tokens);
  * below 0 is taken for 0).
  * draft_probs (fp32 [n_tokens][vocab], row start[s]+i for draft i+1; each
  * sequence's last row is not read) may be NULL: drafted without chance, q is 1 at
- * the draft. temperature[s] = 0 takes the largest logit, lowest token first, for
- * p = 1 and needs no random numbers. Drafts outside [0, vocab) are rejected.
+ * the draft. temperature[s] = 0 (or below, or NaN) takes the largest logit, lowest
+ * token first, for p = 1 and needs no random numbers; an infinite one makes all
+ * tokens above -infinity alike. Drafts outside [0, vocab) are rejected.
  * Probabilities and sums are formed in fp64. n_accepted[s] (drafts taken) and
  * next_token[s] are int32; a sequence without rows gives 0 and -1, one whose row
  * has a NaN or no finite largest logit the rejection of that draft and -1 as the token.

@@ -302,3 +302,30 @@ def test_verify_random_numbers_past_the_ends(tc, dev):
     logits[:, [70, 900, 901, 4321]] = [0.5, -3, 2, 1]
     _, got = verify_into(tc, dev, draws(logits, [-1e-30, -0.5, -np.inf, 1, 1.5, np.inf, np.nan]))
     assert got.tolist() == [70, 70, 70, 4321, 4321, 4321, 4321]
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_temperature_without_end(tc, dev, probs):
+    """An infinite temperature makes all tokens that are not masked alike, for drafts and draws."""
+    p = problem(12, [4] * 20, 1000, probs, temps=[np.inf, 0.9] * 10)
+    p[0][:, 200:300] = -np.inf
+    p[0][::3, 700] = 3e38
+    p[4][:] *= 2e-3
+    flat = [a if a is None else a.copy() for a in p]
+    for s in range(0, 20, 2):
+        rows = flat[0][flat[2][s]:flat[2][s + 1]]
+        rows[np.isfinite(rows)] = 0  # at temperature 1 the same
+        flat[3][s] = 1
+    got, want = verify_into(tc, dev, p), verify_exact(*flat)
+    assert want[0][::2].max() > 0  # (seeded: some drafts are taken)
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w), (g, w)
+
+
+def test_verify_temperature_below_zero(tc, dev):
+    """Negative temperatures and NaN are taken for 0."""
+    p = problem(13, [3] * 8, 500, True, temps=[0.0, -0.0, -1.0, -np.inf, np.nan, -1e-45, 0.0, -0.7])
+    zero = [a if a is None else a.copy() for a in p]
+    zero[3][:] = 0
+    for g, w in zip(verify_into(tc, dev, p), verify_exact(*zero)):
+        assert np.array_equal(g, w), (g, w)

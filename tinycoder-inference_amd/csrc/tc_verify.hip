@@ -97,13 +97,15 @@ __device__ __forceinline__ double wave_scan(double v) {
 __device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), 63); }
 
 // log2(e) / temperature, 0 for the greedy choice; and the difference of logits below
-// which a token's share is taken for 0 (2^-900).
+// which a token's share is taken for 0 (2^-900). An infinite temperature's factor is not 0:
+// with 1e-60 a difference of finite logits, up to 2^129, is nothing, and -inf still below
+// every difference.
 struct Scale {
     double c, least;
 };
 __device__ __forceinline__ Scale scale_of(float t) {
     if (!(t > 0.0f)) return Scale{0.0, 0.0};
-    const double c = 1.4426950408889634 / double(t);
+    const double c = __builtin_fmax(1.4426950408889634 / double(t), 1e-60);
     return Scale{c, -900.0 / c};
 }
 
