@@ -40,8 +40,8 @@ enum { TC_F32 = 0, TC_F16 = 1, TC_I8 = 24, TC_BF16 = 30, TC_E4M3 = 100 };
  *   k_scale, v_scale  fp32 [n_pages][kv_heads][page_tokens] for I8 and E4M3 (one
  *                     factor per token and head), NULL for F16 and BF16
  * page_tokens: a multiple of 16. head_dim: a multiple of 16, up to 256. Factors as
- * tc_kv_write forms them are above 0; tc_attn takes v_scale for that (one below
- * 2^-126 as 2^-126). Less than 2^32 runs of 16 tokens (n_pages * kv_heads *
+ * tc_kv_write forms them are above 0; tc_attn takes a v_scale below 2^-80 (0 and
+ * negative ones too) for 2^-80. Less than 2^32 runs of 16 tokens (n_pages * kv_heads *
  * page_tokens / 16). */
 typedef struct tc_kv_cache {
     int32_t type;

@@ -460,3 +460,23 @@ def test_attn_cache_beyond_4_gib(tc, dev):
         p = torch.softmax(kd[:, h] @ q[0, h].double() * 0.0625, 0)
         want, mass = p @ vd[:, h], p @ vd[:, h].abs()
         assert ((got[0, h] - want).abs() <= mass * (2.0 ** -8 + 2e-3) + 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+@pytest.mark.parametrize("factor", [0.0, 2.0 ** -126, 2.0 ** -118])
+@pytest.mark.parametrize("size", [1.0, 100.0])
+def test_attn_next_to_no_values(tc, dev, ctype, factor, size):
+    """Tokens whose values are nothing beside the others', as in slots of a fresh cache (factors of 0) that a length
+    reaches: their weights count in the sum, small ones too."""
+    rng = np.random.default_rng(24)
+    b = Batch(rng, [(1, 400), (70, 200), (4, 100)], 16, 2, 64, ctype)
+    b.host["v_scale"] *= size
+    at = torch.from_numpy(rng.random(b.host["v_scale"].shape) < 0.5)
+    b.host["v_scale"][at] = factor
+    if factor == 0:
+        for name in ("k", "v"):
+            b.host[name].view(torch.uint8)[at] = 0
+        b.host["k_scale"][at] = 0
+    b.to(dev)
+    for spread in (1.0, 5.0, 9.0):
+        check_attn(tc, dev, b, 4, "F32", 0.125, spread=spread)

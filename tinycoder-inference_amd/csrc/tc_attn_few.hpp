@@ -191,8 +191,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                 if constexpr (SCALED) {
                     const float *const kfac = raw + n % (NB + 1) * 64;
                     if (lane >= 32) {
-                        // (a factor of 0: values of next to nothing; NaN stays)
-                        const float y = kfac[lane], x = y == y ? fmaxf(y, 0x1p-126f) : y;
+                        const float x = value_factor(kfac[lane]);
                         lv[lane - 32] = __builtin_amdgcn_logf(x);
                         iv[lane - 32] = __builtin_amdgcn_rcpf(x);
                     }

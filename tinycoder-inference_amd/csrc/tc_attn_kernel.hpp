@@ -24,7 +24,7 @@
 // in [2^14, 2^15); weights carry a factor 2^kLift, which keeps those that matter
 // out of fp16's subnormals and cancels in the quotient. A factor per token (8-bit
 // caches): the key's multiplies the score; the value's goes into the weight as
-// 2^(t + log2 v_scale - m), and the sum of weights takes it out again.
+// 2^(t + log2 v_scale - m), and the sum of weights takes it out again (value_factor).
 #pragma once
 
 #include "tc_attn_common.hpp"
@@ -299,6 +299,14 @@ __device__ __forceinline__ float max_of(const float (&x)[N]) {
     for (int i = 6; i + 3 < N; i += 4) m = max3(m, x[i], x[i + 1]), n = max3(n, x[i + 2], x[i + 3]);
     return max3(m, max3(n, x[N - 2], x[N - 1]), n);
 }
+
+// A value's factor as weights take it: at least 2^-80 (NaN stays). A token whose values
+// are nothing, by a factor of 0 as in a slot that was never written, or next to it, still
+// has its weight, 2^(t + log2 factor - m + kLift) divided by the factor, in the sum of
+// weights: from 2^-80 on neither is the one lost below 2^-126 (nor the products that raise m)
+// where it is 2^-24 of the largest beside factors of up to 2^22, nor do 2^31 of the other, up
+// to 2^95 each, pass fp32's end.
+__device__ __forceinline__ float value_factor(float x) { return x == x ? fmaxf(x, 0x1p-80f) : x; }
 
 // 16 bytes of LDS at an address of lds_addr's.
 typedef const __attribute__((address_space(3))) u32x4 *lds_u32x4;

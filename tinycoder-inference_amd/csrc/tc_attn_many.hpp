@@ -200,8 +200,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                 if (ln < 32) {
                     ms.many.kf[buf][ln] = raw_scale;
                 } else {
-                    // (a factor of 0: values of next to nothing; NaN stays)
-                    const float x = raw_scale == raw_scale ? fmaxf(raw_scale, 0x1p-126f) : raw_scale;
+                    const float x = value_factor(raw_scale);
                     ms.many.lv[buf][ln - 32] = __builtin_amdgcn_logf(x);
                     ms.many.iv[buf][ln - 32] = __builtin_amdgcn_rcpf(x);
                 }
