@@ -480,3 +480,71 @@ def test_attn_next_to_no_values(tc, dev, ctype, factor, size):
     b.to(dev)
     for spread in (1.0, 5.0, 9.0):
         check_attn(tc, dev, b, 4, "F32", 0.125, spread=spread)
+
+
+def zero_rows(b, rng, share, factor):
+    """Makes rows of values zeros (of either sign where there are two), with this factor; -> which."""
+    at = torch.from_numpy(rng.random(b.host["v_scale"].shape) < share)
+    v = b.host["v"].view(torch.uint8)
+    v[at] = 0
+    if b.ctype == "E4M3":
+        v[at & torch.from_numpy(rng.random(at.shape) < 0.5)] = 0x80
+    b.host["v_scale"][at] = factor
+    return at
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+@pytest.mark.parametrize("xtype", XTYPES)
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6, 1e-8, 1e-10])
+@pytest.mark.parametrize("dim", [64, 112, 256])
+def test_attn_rows_of_zeros_among_small_values(tc, dev, ctype, xtype, size, dim):
+    """Rows of zeros, to which tc_kv_write gives the factor 1, take nothing of the other rows' precision."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, [(1, 200), (5, 60), (90, 200), (1, 3)], 16, 2, dim, ctype)
+    b.host["v_scale"] *= size
+    zero_rows(b, rng, 0.05, 1.0)
+    check_attn(tc, dev, b.to(dev), 4, xtype, dim ** -0.5)
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+def test_attn_rows_of_zeros_alone(tc, dev, ctype):
+    """Sequences that see rows of zeros first, last, in whole tiles, and nothing else."""
+    rng = np.random.default_rng(21)
+    b = Batch(rng, [(1, 600), (80, 300), (1, 70), (40, 90)], 16, 2, 64, ctype)
+    b.host["v_scale"] *= 1e-6
+    v, sc = b.host["v"].view(torch.uint8), b.host["v_scale"]
+    for s, blocks in ((0, range(0, 20)), (1, range(5, 18)), (2, range(5)), (3, range(6))):
+        for i in blocks:
+            v[int(b.table[s, i])] = 0
+            sc[int(b.table[s, i])] = 1
+    got, _ = check_attn(tc, dev, b.to(dev), 4, "F32", 0.125)
+    assert (got[81] == 0).all() and (got[82:] == 0).all()
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+@pytest.mark.parametrize("xtype", ["F32", "BF16"])
+def test_attn_factors_of_one(tc, dev, ctype, xtype):
+    """Rows of values whose factor is 1 and which are not zeros, beside some which are."""
+    rng = np.random.default_rng(22)
+    b = Batch(rng, [(1, 200), (90, 200)], 16, 2, 64, ctype)
+    at = torch.from_numpy(rng.random(b.host["v_scale"].shape) < 0.5)
+    b.host["v_scale"][at] = 1
+    zero_rows(b, rng, 0.1, 1.0)
+    b.host["v"].view(torch.uint8)[:, :, 3, 1:] = 0  # (one value of a row is enough)
+    b.host["v_scale"][:, :, 3] = 1
+    check_attn(tc, dev, b.to(dev), 4, xtype, 0.125)
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+def test_attn_written_zeros(tc, dev, ctype):
+    """Rows of zeros as tc_kv_write leaves them, through the whole path."""
+    rng = np.random.default_rng(23)
+    b = Batch(rng, [(100, 100), (64, 64)], 16, 2, 64, ctype)
+    b.to(dev)
+    k, v = rows_of(rng, b.T, 2, 64, "F32"), rows_of(rng, b.T, 2, 64, "F32", 1e-7)
+    v[::7] = 0
+    v[3::11] = -0.0
+    tc.kv_write(b.cache, b.batch, k.to(dev), v.to(dev))
+    for name in b.host:
+        b.host[name] = b.dev[name].cpu()
+    check_attn(tc, dev, b, 4, "F32", 0.125)

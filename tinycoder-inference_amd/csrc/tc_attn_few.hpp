@@ -191,7 +191,10 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                 if constexpr (SCALED) {
                     const float *const kfac = raw + n % (NB + 1) * 64;
                     if (lane >= 32) {
-                        const float x = value_factor(kfac[lane]);
+                        const float x = value_factor<CT>(kfac[lane], rowbytes, [&] {
+                            const uint32_t ln = lane_now();
+                            return a.kv.v + (16 * uint64_t(tile_runs(ms.runs, t - c0).of(ln & 16)) + (ln & 15)) * rowbytes;
+                        });
                         lv[lane - 32] = __builtin_amdgcn_logf(x);
                         iv[lane - 32] = __builtin_amdgcn_rcpf(x);
                     }

@@ -306,7 +306,25 @@ __device__ __forceinline__ float max_of(const float (&x)[N]) {
 // weights: from 2^-80 on neither is the one lost below 2^-126 (nor the products that raise m)
 // where it is 2^-24 of the largest beside factors of up to 2^22, nor do 2^31 of the other, up
 // to 2^95 each, pass fp32's end.
-__device__ __forceinline__ float value_factor(float x) { return x == x ? fmaxf(x, 0x1p-80f) : x; }
+//
+// tc_kv_write gives a row of zeros the factor 1. Beside values of 1e-6 that would put m 2^27
+// above what the others' weights reach, and their pieces would lose as many bits; so such a
+// row's factor is 0 here. Rows are looked at only where the factor is 1. `row`: what gives
+// the address of the lane's row.
+template <int CT, class F>
+__device__ __forceinline__ float value_factor(float x, uint32_t rowbytes, F row) {
+    if (__builtin_expect(__ballot(x == 1.0f) != 0, 0)) {
+        asm volatile("; zeros?");
+        if (x == 1.0f) {
+            const u32x4 *p = reinterpret_cast<const u32x4 *>(row());
+            uint32_t any = 0;
+#pragma unroll 1
+            for (uint32_t i = 0; i < rowbytes / 16; ++i) any |= p[i][0] | p[i][1] | p[i][2] | p[i][3];
+            if ((any & (CT == kE4M3 ? 0x7F7F7F7Fu : ~0u)) == 0) x = 0.0f;  // (an 8-bit float's zero has a sign)
+        }
+    }
+    return x == x ? fmaxf(x, 0x1p-80f) : x;
+}
 
 // 16 bytes of LDS at an address of lds_addr's.
 typedef const __attribute__((address_space(3))) u32x4 *lds_u32x4;

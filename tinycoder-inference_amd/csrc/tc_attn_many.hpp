@@ -200,7 +200,9 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                 if (ln < 32) {
                     ms.many.kf[buf][ln] = raw_scale;
                 } else {
-                    const float x = value_factor(raw_scale);
+                    const float x = value_factor<CT>(raw_scale, rowbytes, [&] {
+                        return a.kv.v + (16 * uint64_t(tile_runs(ms.runs, t - t0).of(ln & 16)) + (ln & 15)) * rowbytes;
+                    });
                     ms.many.lv[buf][ln - 32] = __builtin_amdgcn_logf(x);
                     ms.many.iv[buf][ln - 32] = __builtin_amdgcn_rcpf(x);
                 }
