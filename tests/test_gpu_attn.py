@@ -548,3 +548,19 @@ def test_attn_written_zeros(tc, dev, ctype):
     for name in b.host:
         b.host[name] = b.dev[name].cpu()
     check_attn(tc, dev, b, 4, "F32", 0.125)
+
+
+@pytest.mark.parametrize("ctype,xtype", [("BF16", "BF16"), ("F16", "F16"), ("F16", "BF16")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attn_of_values_all_alike(tc, dev, ctype, xtype, dim):
+    """Weights whose sum is not that of the weights that the values were multiplied with would not give them back."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, [(1, 2), (1, 40), (1, 300), (3, 33), (40, 70), (130, 200), (1, 64), (9, 500)], 16, 2, dim, ctype)
+    value = torch.from_numpy(rng.integers(-8, 9, (1, 2, 1, dim)) / 8).to(DT[ctype])
+    b.host["v"] = value.expand(b.host["v"].shape).contiguous()
+    b.to(dev)
+    q = rows_of(rng, b.T, 6, dim, xtype, 2.0)
+    got = tc.attn(b.cache, b.batch, q.to(dev), dim ** -0.5).float().cpu()
+    want = value.float().reshape(1, 2, 1, dim).expand(b.T, 2, 3, dim).reshape(b.T, 6, dim)
+    # (fp32 sums of 500 terms in two orders: 500 * 2^-24, a fraction of half a step of either type)
+    assert torch.equal(got, want), (got - want).abs().max()

@@ -244,7 +244,10 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                 for (int i = 0; i < NS; ++i) {
                     s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
                     // (the factor of a token that is not seen may be anything)
-                    l += SCALED ? ((seen >> i) & 1 ? s[i] * rf[i] : 0.0f) : s[i];
+                    if constexpr (SCALED)
+                        l += (seen >> i) & 1 ? s[i] * rf[i] : 0.0f;
+                    else if constexpr (!rounded_sum<CT, NP>())
+                        l += s[i];
                 }
 
                 // ---- values ----
@@ -261,6 +264,7 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                         float x = s[2 * j], y = s[2 * j + 1];
 #pragma unroll
                         for (int p = 0; p < NP; ++p) pw[p][j] = piece2<CT>(x, y);
+                        if constexpr (rounded_sum<CT, NP>()) l = add_pair<CT>(pw[0][j], l);
                     }
                     const uint32_t ln = place_lane();
 #pragma unroll
@@ -281,6 +285,9 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                         for (int p = NP - 1; p >= 0; --p) o[d] = mfma<CT>(v, pw[p], o[d]);
                     }
                 } else {
+                    if constexpr (rounded_sum<CT, NP>())
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) l += s[i];
                     add_values_one_by_one<CT, R, RB, DP>(mine + (NB + n % NB) * TILE, s, seen, lane, o);
                 }
                 wait_lds();

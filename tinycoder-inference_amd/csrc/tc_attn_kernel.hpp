@@ -292,6 +292,14 @@ __device__ __forceinline__ float add_pair(uint32_t w, float c) {
     }
 }
 
+// Whether the sum of weights is that of the weights as they enter the products. One piece of
+// 16 bits is off by up to half a step, in the sums of values and in that of the weights alike,
+// and the quotient keeps less of it (values that are all alike come out as they are). More
+// pieces hold what fp32 rows ask for. Not with factors: there a token whose values are nothing
+// has a weight below its piece's least, and counts in the sum all the same.
+template <int CT, int NP>
+__device__ constexpr bool rounded_sum() { return NP == 1 && !scaled_type(CT); }
+
 template <int N>
 __device__ __forceinline__ float max_of(const float (&x)[N]) {
     float m = max3(x[0], x[1], x[2]), n = max3(x[3], x[4], x[5]);

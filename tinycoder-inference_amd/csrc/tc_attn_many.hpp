@@ -110,7 +110,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
 #pragma unroll
             for (int i = 0; i < NS; ++i) x[i] = y[i / AE][i % AE];
         };
-        // o += weights * values of the tile in a buffer
+        // o += weights * values of the tile in a buffer (and l += rounded weights)
         auto add_values = [&](uint32_t buf) __attribute__((always_inline)) {
             u32x4 pw[Ge::KT][NP];
 #pragma unroll
@@ -120,6 +120,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                     float x = s[8 * k + 2 * j], y = s[8 * k + 2 * j + 1];
 #pragma unroll
                     for (int p = 0; p < NP; ++p) pw[k][p][j] = piece2<LT>(x, y);
+                    if constexpr (rounded_sum<CT, NP>()) l = add_pair<LT>(pw[k][0][j], l);
                 }
             const uint32_t place = here(vplace);
 #pragma unroll
@@ -353,7 +354,7 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                 for (; added < NS * (i + 1) / VALS; ++added)
                     if constexpr (SCALED)
                         sum[added % 2] = fmaf(s[added], ms.many.iv[buf][token_of_reg<R>(added, g)], sum[added % 2]);
-                    else if constexpr (NP > 1)
+                    else if constexpr (!rounded_sum<CT, NP>())
                         sum[added % 2] += s[added];
                     else if (added % 2 == 1)
                         sum[added / 2 % 2] = add_pair<LT>(pw[added / 8][0][added % 8 / 2], sum[added / 2 % 2]);
@@ -409,15 +410,21 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                 for (int i = 0; i < NS; ++i) {
                     s[i] = exponential(s[i], ref);
                     // (the factor of a token that is not seen may be anything)
-                    const float p = SCALED ? s[i] * ms.many.iv[buf][token_of_reg<R>(i, g)] : s[i];
-                    l += (seen >> i) & 1 ? p : 0.0f;
+                    if constexpr (SCALED)
+                        l += (seen >> i) & 1 ? s[i] * ms.many.iv[buf][token_of_reg<R>(i, g)] : 0.0f;
+                    else if constexpr (!rounded_sum<CT, NP>())
+                        l += s[i];
                 }
                 bool odd = false;  // values that are not finite where some row must not see them
                 if (CT != kI8 && __ballot(seen != ALL) != 0) odd = tile_not_finite<LT, TILE>(lds + kMisc + (NBUF + buf) * TILE, lane_now());
-                if (!odd)
+                if (!odd) {
                     add_values(buf);
-                else
+                } else {
+                    if constexpr (rounded_sum<CT, NP>())
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) l += s[i];
                     add_values_one_by_one<LT, R, RB, DP>(lds + kMisc + (NBUF + buf) * TILE, s, seen, lane_now(), o);
+                }
             }
             if (t + 1 < t1 && any_seen(t + 1)) {
                 products((buf + 1) % NBUF, s);
