@@ -194,3 +194,21 @@ int main() {
     return 0;
 }
 """, "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined")
+
+
+def test_binding_refuses_numbers_beyond_32_bits():
+    """What ctypes would cut to 32 bits."""
+    tc = tc_hip.Library()
+    c = tc_hip.KVCache(*(torch.zeros(2, 1, 16, 32, dtype=torch.float16) for _ in range(2)))
+    b = tc_hip.KVBatch(*(torch.zeros(s, dtype=torch.int32) for s in ((2,), (1,), (1, 2))))
+    q = torch.zeros(1, 1, 32)
+    for window in (-1, 1 << 32):
+        with pytest.raises(tc_hip.TCError, match="window"):
+            tc.attn(c, b, q, 1.0, window=window)
+    for args in ((-1, 4), (4, -1), (1 << 32, 1), (8, 1 << 32)):
+        with pytest.raises(tc_hip.TCError, match="32 bits"):
+            tc.attn_reserve(*args)
+    far = torch.empty_strided((2, 1, 32), ((1 << 32) + 64, 32, 1), device="meta")
+    with pytest.raises(tc_hip.TCError, match="32 bits"):
+        tc._row_stride(far)
+    assert tc._row_stride(far[:1]) == 32 and tc._row_stride(torch.empty(2, 3, 32, device="meta")) == 96

@@ -142,6 +142,13 @@ def _need(ok, what):
         raise TCError(TC_E_ARG, what)
 
 
+def _u32(x, name):
+    """x, which ctypes would cut to 32 bits without a word."""
+    if not 0 <= x <= 0xFFFFFFFF:
+        raise TCError(TC_E_ARG, f"{name}={x} is not a number of 32 bits")
+    return x
+
+
 class KVCache:
     """The buffers of one layer's paged cache (tc_kv_cache): k and v
     [n_pages][kv_heads][page_tokens][head_dim] of float16, bfloat16, int8 or
@@ -410,7 +417,7 @@ class Library:
 
     @staticmethod
     def _row_stride(t):
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+        return _u32(t.stride(0), "row stride") if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
     def kv_write(self, cache, batch, k, v):
         """Keys and values [n_tokens][kv_heads][head_dim] (rows may be strided)
@@ -439,6 +446,7 @@ class Library:
         """Causal attention of q [n_tokens][heads][head_dim] (rows may be strided)
         over the cache."""
         import torch
+        _u32(window, "window")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         T, stream = self._kv_call(cache, batch, q, out, 1)
@@ -447,7 +455,7 @@ class Library:
         return out
 
     def attn_reserve(self, heads, n_tokens):
-        self._check(self.lib.tc_attn_reserve(heads, n_tokens))
+        self._check(self.lib.tc_attn_reserve(_u32(heads, "heads"), _u32(n_tokens, "n_tokens")))
 
     def spec_verify(self, logits, tokens, start, temperature, accept_u, sample_u, draft_probs=None):
         """How many of each sequence's drafted tokens hold against the target's
