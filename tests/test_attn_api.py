@@ -212,3 +212,14 @@ def test_binding_refuses_numbers_beyond_32_bits():
     with pytest.raises(tc_hip.TCError, match="32 bits"):
         tc._row_stride(far)
     assert tc._row_stride(far[:1]) == 32 and tc._row_stride(torch.empty(2, 3, 32, device="meta")) == 96
+
+
+def test_batch_of_no_sequences(lib):
+    """Arrays without an entry have no address: a call for no sequences does nothing, and says so."""
+    none = batch(n_seq=0, n_tokens=0, len=None, table=None)
+    padded = batch(n_seq=0, len=None, table=None)
+    for b in (none, padded):
+        assert write(lib, cache(), b) == tc_hip.TC_OK
+        assert attn(lib, cache(), b) == tc_hip.TC_OK
+        assert lib.tc_kv_read(ctypes.byref(cache()), ctypes.byref(b), 0, P, P, None) == tc_hip.TC_OK
+    assert write(lib, cache(), batch(n_seq=0, start=None, len=None, table=None)) == ARG

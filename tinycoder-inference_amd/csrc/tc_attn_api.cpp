@@ -23,7 +23,8 @@ int kv_args(const tc_kv_cache *c, const tc_kv_batch *b, int xtype, tc::KvArgs *a
     if (c->type != TC_F16 && c->type != TC_BF16 && c->type != TC_I8 && c->type != TC_E4M3)
         return refuse(TC_E_UNSUPPORTED, "unsupported cache type " + std::to_string(c->type));
     if (!row_type(xtype)) return refuse(TC_E_UNSUPPORTED, "unsupported row type " + std::to_string(xtype));
-    if (!c->k || !c->v || !b->start || !b->len || !b->table) return refuse(TC_E_ARG, "null pointer");
+    // (arrays without an entry may have no address)
+    if (!c->k || !c->v || !b->start || (b->n_seq != 0 && (!b->len || !b->table))) return refuse(TC_E_ARG, "null pointer");
     const bool scaled = tc::scaled_type(c->type);
     if (scaled != (c->k_scale != nullptr) || scaled != (c->v_scale != nullptr))
         return refuse(TC_E_ARG, "scales go with the 8-bit types and with these only");
