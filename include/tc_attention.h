@@ -71,13 +71,15 @@ typedef struct tc_kv_batch {
  * bytes' multiples. F16 and BF16 round to nearest even. I8: scale = max|x| / 127
  * (1 for a row of zeros), value = rint(x / scale); E4M3: scale = max|x| / 448,
  * value = x / scale to the nearest, ties to even; both quotients rounded to fp32
- * once. A row with an infinity or NaN reads back as NaNs. */
+ * once, the second held to the type's largest (which it passes where the scale is a
+ * subnormal number). A row with an infinity or NaN reads back as NaNs. */
 int tc_kv_write(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, const void *k, const void *v,
                 uint32_t k_stride, uint32_t v_stride, void *stream);
 
-/* The batch's rows back out of the cache, as `xtype` (value * scale, rounded
- * once): k and v [n_tokens][kv_heads][head_dim], contiguous. A batch whose chunks
- * are whole sequences (start[s+1]-start[s] = len[s]) reads these whole. */
+/* The batch's rows back out of the cache, as `xtype` (8-bit types: value * scale
+ * rounded to fp32, then to xtype): k and v [n_tokens][kv_heads][head_dim],
+ * contiguous. A batch whose chunks are whole sequences (start[s+1]-start[s] =
+ * len[s]) reads these whole. */
 int tc_kv_read(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, void *k, void *v, void *stream);
 
 /* Causal attention of the batch's rows over the cache (which already holds their
@@ -90,10 +92,12 @@ int tc_kv_read(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, vo
  * held in fp32; q and the softmax's weights enter the matrix cores as F16 or BF16
  * (the 16-bit cache's own type; F16 for the 8-bit ones) in as many pieces as
  * `xtype` has bits for, so that fp32 rows keep fp32 results (as F16 a weight is held
- * to half a step or 2^-36 of its row's largest, whichever is more). Infinities and
- * NaN in the cache reach only the rows that see them. The same call gives the same
- * bits. heads: a multiple of kv_heads, up to 4096; n_tokens * heads < 2^31. scale:
- * finite, not negative. start, len and table are not to change while a call runs. */
+ * to half a step or 2^-36 of its row's largest, whichever is more; over 8-bit caches
+ * a weight here is the softmax's times the value's factor, rows of zeros left out).
+ * Infinities and NaN in the cache reach only the rows that see them. The same call
+ * gives the same bits. heads: a multiple of kv_heads, up to 4096; n_tokens * heads
+ * < 2^31. scale: finite, not negative. start, len and table are not to change while
+ * a call runs. */
 int tc_attn(const tc_kv_cache *cache, const tc_kv_batch *batch, int xtype, const void *q, uint32_t q_stride, void *out,
             uint32_t heads, float scale, uint32_t window, void *stream);
 
@@ -111,8 +115,7 @@ int tc_attn_reserve(uint32_t heads, uint32_t n_tokens);
  * max(p_i - q_i, 0) (from p_i where that is zero everywhere); where all are taken,
  * from the last row's p: the lowest token t whose sum of weights up to t exceeds
  * sample_u[s] times the sum of all (if none: the last of weight above 0; a sample_u
- * below 0 is taken for 0).
- * draft_probs (fp32 [n_tokens][vocab], row start[s]+i for draft i+1; each
+ * below 0 is taken for 0). draft_probs (fp32 [n_tokens][vocab], row start[s]+i for draft i+1; each
  * sequence's last row is not read) may be NULL: drafted without chance, q is 1 at
  * the draft. temperature[s] = 0 (or below, or NaN) takes the largest logit, lowest
  * token first, for p = 1 and needs no random numbers; an infinite one makes all

@@ -564,3 +564,17 @@ def test_attn_of_values_all_alike(tc, dev, ctype, xtype, dim):
     want = value.float().reshape(1, 2, 1, dim).expand(b.T, 2, 3, dim).reshape(b.T, 6, dim)
     # (fp32 sums of 500 terms in two orders: 500 * 2^-24, a fraction of half a step of either type)
     assert torch.equal(got, want), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("ctype", ["I8", "E4M3"])
+@pytest.mark.parametrize("xtype", XTYPES)
+def test_kv_read_roundings(tc, dev, ctype, xtype):
+    """value * scale rounded to fp32, and that to the rows' type: bit for bit."""
+    rng = np.random.default_rng(31)
+    b = Batch(rng, [(300, 300), (37, 90)], 16, 3, 96, ctype).to(dev)
+    got = tc.kv_read(b.cache, b.batch, b.T, DT[xtype])
+    at = [b.slot(s, pos) for _, s, pos in b.rows()]
+    pg, sl = (torch.tensor(x) for x in zip(*at))
+    for name, x in zip(("k", "v"), got):
+        want = (b.host[name].float() * b.host[name + "_scale"][..., None])[pg, :, sl].to(DT[xtype])
+        assert torch.equal(x.cpu(), want)
