@@ -9,12 +9,13 @@
 // unnormalised sums, which k_attn_join adds up.
 //
 // Up to 16 KB of tiles per wave are on their way, 128 KB per CU, in LDS directly, so
-// that neither registers nor a barrier bound them. 8 waves, not 4: 61 -> 35 us for 16
-// sequences of drafted tokens. Rows of 16, not 32: 20 -> 16 us for one token at 1000.
+// that neither registers nor a barrier bound them. 8 waves, not 4, together with one launch
+// for a batch of any mix: 61 -> 35 us for 16 sequences of drafted tokens. Rows of 16, not
+// 32: 20 -> 16 us for one token at 1000.
 // Measured: 64 decoding sequences (bf16, 8 heads of 128, 1.04 GB) 166 us, 6.3 TB/s; one
-// token at 131071 (int8, 138 MB) 38 us, 3.6 TB/s, of which 6 are the join; one token at
-// 1001 (2 MB) 13.8 us: launches, 3.5 us until a workgroup knows its part, and what the
-// first instructions and rows take to arrive.
+// token at 131071 (int8, 138 MB) 38 us, 3.6 TB/s, of which 6 are the join and about as
+// many the start and the blocks' sums; one token at 1001 (2 MB) 13.8 us: launches, 3.5 us
+// until a workgroup knows its part, and what the first instructions and rows take to arrive.
 #pragma once
 
 #include "tc_attn_kernel.hpp"

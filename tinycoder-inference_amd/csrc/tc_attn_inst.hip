@@ -14,7 +14,7 @@ namespace {
 // those of many another, and the workgroups are shared out between the two as their
 // tiles are (a tile of either takes about as long: 16 KB through HBM on one of 256
 // CUs, or 256 rows' products): 16 sequences of drafted tokens 61 us in two launches, 35
-// in one.
+// in one (whose few-row part also went from 4 waves to 8).
 template <int CT, int NP, int DP>
 __global__ __launch_bounds__(kThreads, 1) void k_attn(AttnArgs a, SplitScratch sc) {
     using Few = FewShape<CT, NP, DP>;

@@ -4,9 +4,10 @@
 // largest and the sum of exponentials (where the temperature is 0: the largest and its
 // lowest index). k_verify_weights joins a sequence's slices, walks its drafts, and sums
 // the sampling weights of the row where they end, again in slices; k_verify_pick finds
-// the slice and then the token that the random number falls on. The first takes 46 us for
-// 264 rows of 152064 logits (161 MB at 3.5 TB/s; fp64 instructions two thirds of that
-// time), the others 24 and 7 us for their 48 sequences: their latency.
+// the slice and then the token that the random number falls on. The first takes 39 to 44 us
+// for 263 rows of 152064 logits (160 MB at 3.6 to 4.1 TB/s; VALU busy for two thirds of
+// that time, with fp64), the others 19 to 24 and 7 to 8 us for their 48 sequences (each of
+// the second's workgroups walks its sequence's drafts before it reads 53 MB in all).
 //
 // Everything behind the logits is fp64: a token's probability in a vocabulary of
 // 10^5 is 10^-5 and less, so sums in fp32 would move the borders between tokens by
@@ -55,7 +56,7 @@ __host__ __device__ inline uint32_t div_up(uint32_t a, uint32_t b) { return (a +
 
 // As many slices as make about kRowsPerCu workgroups per CU, of 2048 logits or more (8 of
 // a thread); and kPickPerCu waves, of 512 or more (as many as the card holds at a time, for
-// each workgroup walks the drafts: 48 sequences 70 us in all, 74 with 32 waves).
+// each workgroup walks the drafts: 48 sequences of 263 rows 70 us in all, 74 with 32 waves).
 constexpr uint32_t kRowsPerCu = 16, kPickPerCu = 24;
 constexpr int kMostCu = 256;
 Split split(uint32_t vocab, uint32_t n_tokens, uint32_t n_seq, int num_cu) {
@@ -114,7 +115,7 @@ __device__ __forceinline__ Scale scale_of(float t) {
 // in [-1/2, 1/2], is the polynomial of degree 10 through its values at the 11 Chebyshev
 // nodes there: its error is 3e-16 of the value, two roundings' (degree 9: 2e-14), and
 // 2^0 is 1. A third of the library function's instructions, which took more time than the
-// logits' way from HBM (264 rows of 152064 logits 88 us).
+// logits' way from HBM (263 rows of 152064 logits 88 us).
 __device__ __forceinline__ double power(double d, double c) {
     constexpr double kShift = 6755399441055744.0;
     const double k = __builtin_fma(d, c, kShift), f = __builtin_fma(d, c, kShift - k);
