@@ -188,14 +188,12 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                 }
 
                 // ---- weights ----
-                float rf[NS];
+                float rf[NS], vfac = 0.0f;
                 if constexpr (SCALED) {
                     const float *const kfac = raw + n % (NB + 1) * 64;
                     if (lane >= 32) {
-                        const float x = value_factor<CT>(kfac[lane], rowbytes, [&] {
-                            const uint32_t ln = lane_now();
-                            return a.kv.v + (16 * uint64_t(tile_runs(ms.runs, t - c0).of(ln & 16)) + (ln & 15)) * rowbytes;
-                        });
+                        vfac = kfac[lane];
+                        const float x = value_factor(vfac);
                         lv[lane - 32] = __builtin_amdgcn_logf(x);
                         iv[lane - 32] = __builtin_amdgcn_rcpf(x);
                     }
@@ -230,15 +228,29 @@ __device__ __forceinline__ void attn_few(const AttnArgs &a, RowRange rg, Seqs se
                         s[i] = (seen >> i) & 1 ? s[i] : kNegInf;
                     }
                 }
-                const float tmax = groups_max<R>(max_of(s));
+                float tmax = groups_max<R>(max_of(s));
                 if (__builtin_expect(__ballot(tmax > m + kLazy) != 0, 0)) {
                     asm volatile("; raise");  // (a branch, not a product by 1 of every sum in every step)
+                    uint32_t zeros = 0;
+                    if constexpr (SCALED) {
+                        const uint32_t ones = uint32_t(__ballot(vfac == 1.0f) >> 32);
+                        if (__builtin_expect(ones != 0, 0)) {
+                            wait_loads<0>();  // (the tile's values are still on their way)
+                            zeros = rows_of_zeros<CT, RB>(ones, mine + (NB + n % NB) * TILE, lane_now());
+                        }
+                        if (__builtin_expect(zeros != 0, 0)) {
+                            lower_zeros<R>(s, zeros, g);
+                            tmax = groups_max<R>(max_of(s));
+                        }
+                    }
                     const float up = tmax > m + kLazy ? tmax : m;
                     const float al = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);
                     m = up;
                     l *= al;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) o[d] *= al;
+                    if constexpr (SCALED)
+                        if (__builtin_expect(zeros != 0, 0)) l += take_zeros<R>(s, zeros, g, (m == kNegInf ? 0.0f : m) - kLift);
                 }
                 const float ref = (m == kNegInf ? 0.0f : m) - kLift;
 #pragma unroll

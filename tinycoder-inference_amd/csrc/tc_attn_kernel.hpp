@@ -308,30 +308,61 @@ __device__ __forceinline__ float max_of(const float (&x)[N]) {
     return max3(m, max3(n, x[N - 2], x[N - 1]), n);
 }
 
-// A value's factor as weights take it: at least 2^-80 (NaN stays). A token whose values
+// A value's factor as weights take it: at least 2^kLeast (NaN stays). A token whose values
 // are nothing, by a factor of 0 as in a slot that was never written, or next to it, still
 // has its weight, 2^(t + log2 factor - m + kLift) divided by the factor, in the sum of
 // weights: from 2^-80 on neither is the one lost below 2^-126 (nor the products that raise m)
 // where it is 2^-24 of the largest beside factors of up to 2^22, nor do 2^31 of the other, up
 // to 2^95 each, pass fp32's end.
-//
+constexpr float kLeast = -80.0f;
+__device__ __forceinline__ float value_factor(float x) { return x == x ? fmaxf(x, 0x1p-80f) : x; }
+
 // tc_kv_write gives a row of zeros the factor 1. Beside values of 1e-6 that would put m 2^27
-// above what the others' weights reach, and their pieces would lose as many bits; so such a
-// row's factor is 0 here. Rows are looked at only where the factor is 1. `row`: what gives
-// the address of the lane's row.
-template <int CT, class F>
-__device__ __forceinline__ float value_factor(float x, uint32_t rowbytes, F row) {
-    if (__builtin_expect(__ballot(x == 1.0f) != 0, 0)) {
-        asm volatile("; zeros?");
-        if (x == 1.0f) {
-            const u32x4 *p = reinterpret_cast<const u32x4 *>(row());
-            uint32_t any = 0;
+// above what the others' weights reach, and their pieces would lose as many bits; so rows of
+// factor 1 are looked at, and those of zeros count as of factor 2^kLeast. Most show in their
+// first values that they are not, so that caches whose factors are all 1 take 0 to 7% longer
+// (17 to 65% where whole rows were read; 1% where no factor is 1).
+template <int CT>
+__device__ __forceinline__ bool zeros16(u32x4 w) {  // (an 8-bit float's zero has a sign)
+    return ((w[0] | w[1] | w[2] | w[3]) & (CT == kE4M3 ? 0x7F7F7F7Fu : ~0u)) == 0;
+}
+template <int CT>
+__device__ __forceinline__ bool row_of_zeros(const uint8_t *row, uint32_t rowbytes) {
+    bool z = true;
 #pragma unroll 1
-            for (uint32_t i = 0; i < rowbytes / 16; ++i) any |= p[i][0] | p[i][1] | p[i][2] | p[i][3];
-            if ((any & (CT == kE4M3 ? 0x7F7F7F7Fu : ~0u)) == 0) x = 0.0f;  // (an 8-bit float's zero has a sign)
-        }
+    for (uint32_t i = 0; i < rowbytes && z; i += 16) z = zeros16<CT>(*reinterpret_cast<const u32x4 *>(row + i));
+    return z;
+}
+// For few rows the values are on their way to LDS when their factors are wanted, so there the
+// look is taken where m rises, and only there: which of a tile's 32 rows, of those whose bits are set, are zeros.
+template <int CT, int RB>
+__device__ __forceinline__ uint32_t rows_of_zeros(uint32_t may, const unsigned char *vt, uint32_t lane) {
+    const unsigned char *half = vt + lane % 32 * RB + lane / 32 * (RB / 2);
+#pragma unroll 1
+    for (uint32_t i = 0; i < RB / 2 && may != 0; i += 16) {
+        const uint64_t z = __ballot(zeros16<CT>(*reinterpret_cast<const u32x4 *>(half + i)));
+        may &= uint32_t(z) & uint32_t(z >> 32);
     }
-    return x == x ? fmaxf(x, 0x1p-80f) : x;
+    return may;
+}
+// Their scores as exponents of that factor, before m is chosen; ...
+template <int R, int NS>
+__device__ __forceinline__ void lower_zeros(float (&s)[NS], uint32_t zeros, uint32_t g) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+        if ((zeros >> token_of_reg<R>(i, g)) & 1) s[i] += kLeast;
+}
+// ... behind that, their weights' sum, taken out of the scores.
+template <int R, int NS>
+__device__ __forceinline__ float take_zeros(float (&s)[NS], uint32_t zeros, uint32_t g, float ref) {
+    float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+        if ((zeros >> token_of_reg<R>(i, g)) & 1) {
+            l = fmaf(__builtin_amdgcn_exp2f(s[i] - ref), 0x1p80f, l);
+            s[i] = kNegInf;
+        }
+    return l;
 }
 
 // 16 bytes of LDS at an address of lds_addr's.

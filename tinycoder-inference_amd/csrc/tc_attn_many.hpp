@@ -201,9 +201,13 @@ __device__ __forceinline__ void attn_many(const AttnArgs &a, RowRange rg, Seqs s
                 if (ln < 32) {
                     ms.many.kf[buf][ln] = raw_scale;
                 } else {
-                    const float x = value_factor<CT>(raw_scale, rowbytes, [&] {
-                        return a.kv.v + (16 * uint64_t(tile_runs(ms.runs, t - t0).of(ln & 16)) + (ln & 15)) * rowbytes;
-                    });
+                    if (__builtin_expect(__ballot(raw_scale == 1.0f) != 0, 0)) {
+                        asm volatile("; zeros?");
+                        // (from the cache: this tile is on its way to LDS in other waves)
+                        const uint8_t *row = a.kv.v + (16 * uint64_t(tile_runs(ms.runs, t - t0).of(ln & 16)) + (ln & 15)) * rowbytes;
+                        if (raw_scale == 1.0f && row_of_zeros<CT>(row, rowbytes)) raw_scale = 0.0f;
+                    }
+                    const float x = value_factor(raw_scale);
                     ms.many.lv[buf][ln - 32] = __builtin_amdgcn_logf(x);
                     ms.many.iv[buf][ln - 32] = __builtin_amdgcn_rcpf(x);
                 }
