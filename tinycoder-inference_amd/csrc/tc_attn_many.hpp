@@ -14,7 +14,7 @@
 // of the time, vector instructions 39%, no LDS conflicts; the two of a SIMD hardly overlap
 // although their order is pinned side by side. As fast: two workgroups of 4 waves per
 // CU; a barrier between the two products. Slower: a barrier at every second tile (247
-// against 241). Seven sequences of fp32 rows (two pieces) over int8 heads of 256, 125 us.
+// against 241). Seven sequences of fp32 rows (two pieces) over int8 heads of 256, 127 us.
 #pragma once
 
 #include <type_traits>
