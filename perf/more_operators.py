@@ -284,7 +284,9 @@ def import_library(st):
     sys.path.insert(0, os.path.join(os.getcwd(), "tinycoder-inference_amd"))
     import tc_hip
     case, st["lib"] = st["case"], tc_hip.Library()
-    if case["op"] == "rope":
+    if case["op"] == "plan":
+        st["plan"] = tc_hip.KVPlan(st["new"], st["held"], st["pages"], st["table"], st["ring"], st["free"], case["page"], st["T"])
+    elif case["op"] == "rope":
         st["cache"] = tc_hip.KVCache(st["k_cache"], st["v_cache"], st["k_scale"], st["v_scale"])
         st["batch"] = tc_hip.KVBatch(st["start"], st["len"], st["table"])
         st["rope"] = tc_hip.Rope(case["n_rot"], THETA, layout=case["layout"], scaling=case["scaling"], **scaling(case))
@@ -307,8 +309,8 @@ def run(st):
 def run_own(st):
     case, lib = st["case"], st["lib"]
     if case["op"] == "plan":
-        p = lib.kv_plan(st["held"], st["new"], st["pages"], st["table"], st["ring"], st["free"], case["page"], st["T"])
-        return [p.start, p.length, p.pages, p.free, p.sequence, p.position, p.slot, st["table"], st["ring"]]
+        p = lib.kv_plan(st["plan"])
+        return [p.start, p.length, p.pages_out, p.free_out, p.sequence, p.position, p.slot, p.table, p.ring]
     if case["op"] == "rope":
         H, kv = case["heads"], case["kv_heads"]
         q, k, v = st["qkv"][:, :H], st["qkv"][:, H:H + kv], st["qkv"][:, H + kv:]
