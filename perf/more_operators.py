@@ -293,6 +293,7 @@ def import_library(st):
     elif case["op"] == "norm":
         st["pre"], st["post"] = (tc_hip.Norm(st[n + "_weight"], st[n + "_bias"], eps=EPS, kind=case["kind"])
                                  if st[n + "_weight"] is not None else None for n in ("pre", "post"))
+        st["gate_given"] = st["gate"][:, None] if case["gate"] == "row" else st["gate"]
     elif case["op"] == "logits":
         names = ("repetition", "frequency", "presence", "history", "history_start", "prompt", "bias_start", "bias_token",
                  "bias_value", "mask", "mask_of")
@@ -318,7 +319,7 @@ def run_own(st):
                                 k_norm=st["k_weight"], eps=EPS)
         return [out] + cache_of(st)
     if case["op"] == "norm":
-        h, x = lib.norm_add(st["h"], st["y"], pre=st["pre"], post=st["post"], gate=st["gate"], sigmoid=case["sigmoid"],
+        h, x = lib.norm_add(st["h"], st["y"], pre=st["pre"], post=st["post"], gate=st["gate_given"], sigmoid=case["sigmoid"],
                             scale=case["scale"], out_dtype=X[case["o"]], h_out=st["h_out"])
         return [h, x]
     return lib.logits_adjust(st["rules"], st["logits"], st["start"], tokens=st["tokens"])
