@@ -3,21 +3,11 @@
 #include <cmath>
 #include <string>
 
-#include "tc_attention.h"
-#include "tc_attn_common.hpp"
-#include "tc_kernels.hpp"
-#include "tc_qmatmul.h"
+#include "tc_api_util.hpp"
 
-namespace {
+namespace tc {
+namespace api {
 
-int refuse(int code, const std::string &msg) { return tc::fail_code(code, msg.c_str()); }
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int no_device() { return refuse(TC_E_UNSUPPORTED, "no gfx950 device"); }
-bool row_type(int t) { return t == TC_F32 || t == TC_F16 || t == TC_BF16; }
-
-// Cache and batch of a call checked and put together. Nothing of the batch's
-// arrays is read here: they are the device's.
 int kv_args(const tc_kv_cache *c, const tc_kv_batch *b, int xtype, tc::KvArgs *a) {
     if (!c || !b) return refuse(TC_E_ARG, "null pointer");
     if (c->type != TC_F16 && c->type != TC_BF16 && c->type != TC_I8 && c->type != TC_E4M3)
@@ -67,7 +57,6 @@ int kv_args(const tc_kv_cache *c, const tc_kv_batch *b, int xtype, tc::KvArgs *a
     return TC_OK;
 }
 
-// Rows of `width` elements of xtype at a stride.
 int check_rows(const char *name, const void *p, uint32_t stride, uint64_t width, uint32_t n, int xtype) {
     if (!p) return refuse(TC_E_ARG, "null pointer");
     if (n > 1 && stride < width) return refuse(TC_E_ARG, std::string(name) + ": rows overlap");
@@ -76,12 +65,10 @@ int check_rows(const char *name, const void *p, uint32_t stride, uint64_t width,
     return TC_OK;
 }
 
-int hip_rc(hipError_t e, const char *what) {
-    if (e == hipSuccess) return TC_OK;
-    return refuse(TC_E_LAUNCH, std::string(what) + ": " + hipGetErrorString(e));
-}
+}  // namespace api
+}  // namespace tc
 
-}  // namespace
+using namespace tc::api;
 
 extern "C" {
 

@@ -12,19 +12,13 @@
 // The 8-bit types hold one factor per row: scores and the weights of the values
 // then take it as one product per token, after the matrix cores, where factors
 // for parts of a row would have to go into the operands.
-#include "tc_attn_common.hpp"
 #include "tc_kernels.hpp"
+#include "tc_kv_put.hpp"
 
 namespace tc {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-
-// Largest of `lanes` lanes' values (a power of two; no NaN) in each of them.
-__device__ __forceinline__ float group_max(float v, uint32_t lanes) {
-    for (uint32_t o = 1; o < lanes; o <<= 1) v = fmaxf(v, __shfl_xor(v, int(o)));
-    return v;
-}
 
 // How a launch goes over the rows: a block of 2^tokens token rows after the other, in it
 // the keys of head after head, then the values, a token after the other.
@@ -79,58 +73,6 @@ __device__ __forceinline__ void find_slots(const KvArgs &a, const Rows<U> &p, in
     for (int u = 0; u < U; ++u) row[u] = slot_of(a, seq[u], p.r[u].t, p.r[u].h);
 }
 
-// One row to where it belongs.
-template <int CT>
-__device__ __forceinline__ void put(const KvArgs &a, const Row &r, uint32_t at, int64_t row, uint32_t lanes, const float (&x)[8]) {
-    uint8_t *dst = r.second ? a.v : a.k;
-    if constexpr (!scaled_type(CT)) {
-        if (r.live && row >= 0) store8(CT, dst, uint64_t(row) * a.dim + at, x);
-    } else {
-        float m = 0.0f;
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m = fmaxf(m, fabsf(x[i]));
-            odd = odd || x[i] != x[i];
-        }
-        // a NaN makes the factor infinite, as an infinity does: the row reads
-        // back as 0 * inf
-        m = group_max(odd ? __builtin_inff() : m, lanes);
-        constexpr float top = CT == kI8 ? 127.0f : 448.0f;
-        float d = __fdiv_rn(m, top);
-        if (d == 0.0f) d = 1.0f;  // zeros, and what is so small that the factor would be
-        if (!r.live || row < 0) return;
-        uint32_t w[2];
-        if constexpr (CT == kI8) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                w[i] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float q = __builtin_rintf(__fdiv_rn(x[4 * i + j], d));
-                    // (a quotient over an infinite factor may be NaN: 0)
-                    const int n = q == q ? int(fminf(fmaxf(q, -127.0f), 127.0f)) : 0;
-                    w[i] |= (uint32_t(n) & 0xFF) << (8 * j);
-                }
-            }
-        } else {
-            float q[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[i] = __fdiv_rn(x[i], d);
-                q[i] = q[i] == q[i] ? fminf(fmaxf(q[i], -448.0f), 448.0f) : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                int u = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
-                w[i] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], u, true));
-            }
-        }
-        *reinterpret_cast<u32x2 *>(dst + uint64_t(row) * a.dim + at) = u32x2{w[0], w[1]};
-        if (at == 0) (r.second ? a.vs : a.ks)[row] = d;
-    }
-}
-
 template <int CT, int U>
 __global__ __launch_bounds__(kThreads) void k_kv_write(KvArgs a, int xtype, const void *k, const void *v, uint32_t k_stride,
                                                        uint32_t v_stride, Walk w) {
@@ -147,7 +89,10 @@ __global__ __launch_bounds__(kThreads) void k_kv_write(KvArgs a, int xtype, cons
     int64_t row[U];
     find_slots<U>(a, p, seq, row);
 #pragma unroll
-    for (int u = 0; u < U; ++u) put<CT>(a, p.r[u], p.i, row[u], w.lanes, x[u]);
+    for (int u = 0; u < U; ++u) {
+        const Row &r = p.r[u];
+        put_row<CT>(r.second ? a.v : a.k, r.second ? a.vs : a.ks, a.dim, row[u], p.i, r.live, w.lanes, x[u]);
+    }
 }
 
 template <int CT, int U>

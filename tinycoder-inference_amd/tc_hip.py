@@ -1,4 +1,5 @@
-"""Python binding of libtc_hip.so (the C-ABI in include/tc_qmatmul.h).
+"""Python binding of libtc_hip.so (the C-ABI in include/tc_qmatmul.h, tc_gguf.h,
+tc_attention.h and tc_step.h).
 
 The library is the product; this module only passes device pointers, sizes
 and the current HIP stream through ctypes, and raises when a call fails.
@@ -62,6 +63,12 @@ SIGNATURES = {
     "tc_attn": (_I, [_P, _P, _I, _P, _U32, _P, _U32, ctypes.c_float, _U32, _P]),
     "tc_attn_reserve": (_I, [_U32, _U32]),
     "tc_spec_verify": (_I, [_P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "tc_kv_plan": (_I, [_P, _P]),
+    "tc_norm_add": (_I, [_P, _P]),
+    "tc_rope_turns": (_I, [_P, _U32, ctypes.c_double, _P, _P, _P]),
+    "tc_rope_apply": (_I, [_P, _I, _P, _U32, _P, _U32, _P, _U32, _U32, _U32, _P]),
+    "tc_rope_kv_write": (_I, [_P, _P, _P, _I, _P, _U32, _P, _U32, _P, _U32, _P, _U32, _P, _P, ctypes.c_float, _P]),
+    "tc_logits_adjust": (_I, [_P, _I, _P, _U32, _U32, _U32, _U32, _P, _P, _P, _U32, _P]),
     "tc_gguf_open": (_P, [ctypes.c_char_p]),
     "tc_gguf_open_metadata": (_P, [ctypes.c_char_p]),
     "tc_gguf_close": (None, [_P]),
@@ -208,6 +215,182 @@ class KVBatch:
                           self.table.data_ptr())
             ref = self._of[n_tokens] = ctypes.byref(c)
         return ref
+
+
+class _CPlan(ctypes.Structure):
+    _fields_ = [(n, _U32) for n in ("n_seq", "n_tokens", "page_tokens", "table_pages", "ring_pages")] + \
+               [(n, _P) for n in ("new_tokens", "held", "pages", "free", "table", "ring", "start", "len", "pages_out",
+                                  "free_out", "sequence", "position", "slot")]
+
+
+class _CNorm(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("weight", _P), ("bias", _P), ("offset", ctypes.c_float)]
+
+
+class _CNormRows(ctypes.Structure):
+    _fields_ = [("n_rows", _U32), ("cols", _U32), ("h", _P), ("y", _P), ("h_out", _P), ("x", _P),
+                ("h_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("x_type", ctypes.c_int32),
+                ("h_stride", _U32), ("y_stride", _U32), ("h_out_stride", _U32), ("x_stride", _U32),
+                ("post", _P), ("pre", _P), ("gate", _P), ("gate_kind", ctypes.c_int32), ("gate_type", ctypes.c_int32),
+                ("gate_sigmoid", ctypes.c_int32), ("scale", ctypes.c_float), ("act_type", ctypes.c_int32), ("act", _P)]
+
+
+class _CRope(ctypes.Structure):
+    _fields_ = [("n_rot", _U32), ("layout", ctypes.c_int32), ("turns", _P), ("factor", ctypes.c_float)]
+
+
+class _CRopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32)] + [(n, ctypes.c_double) for n in ("factor", "original", "low", "high")] + \
+               [("divisors", _P)]
+
+
+class _CLogitRules(ctypes.Structure):
+    _fields_ = [("repetition", _P), ("frequency", _P), ("presence", _P), ("history", _P), ("history_start", _P), ("prompt", _P),
+                ("n_history", _U32), ("bias_start", _P), ("bias_token", _P), ("bias_value", _P), ("n_bias", _U32), ("mask", _P),
+                ("n_masks", _U32), ("mask_words", _U32), ("mask_of", _P)]
+
+
+def _same_device(ts, what):
+    """The one device index of tensors (or Nones), -1 for the CPU."""
+    ts = [t for t in ts if t is not None]
+    _need(all(t.is_contiguous() and t.device == ts[0].device for t in ts), what)
+    return ts[0].get_device()
+
+
+class KVPlan:
+    """The geometry of a batch's steps (tc_plan): the sequences' state, and what
+    Library.kv_plan makes of it. All int32, contiguous, on one device:
+
+      new     [n_seq]   tokens that each sequence brings to the step, -1: it has ended
+      held    [n_seq]   tokens it has in the cache
+      pages   [n_seq]   pages it has in the table
+      table   [n_seq][table_pages]; new pages are entered
+      ring    [pages]   pages not in use, free[1] of them from ring[free[0]] on
+      free    [2 or 3]
+
+    Behind a call: `batch` (a KVBatch of start, length and table), start [n_seq + 1],
+    length, pages_out [n_seq], free_out [3] (its last entry: pages that were missing),
+    and of each of n_tokens rows its sequence, position (int32) and slot (int64), -1 behind
+    the last sequence. in_place: length, pages_out and free_out are held, pages and free
+    (which has 3 entries then), so that the next call goes on from there."""
+
+    def __init__(self, new, held, pages, table, ring, free, page_tokens, n_tokens, in_place=False):
+        import torch
+        n = new.numel()
+        given = (new, held, pages, table, ring, free)
+        _need(all(t.dtype == torch.int32 for t in given), "a plan's arrays are int32")
+        self.device = _same_device(given, "a plan's arrays are contiguous and on one device")
+        _need(held.numel() == pages.numel() == n and table.dim() == 2 and table.shape[0] == n,
+              "held and pages have an entry for each sequence, table a row")
+        _need(free.numel() == 3 or (free.numel() == 2 and not in_place), "free has 2 entries, or 3")
+        self.new, self.held, self.pages, self.table, self.ring, self.free = given
+
+        def made(n, dtype=torch.int32):
+            return torch.zeros(n, dtype=dtype, device=new.device)
+
+        self.start, self.length, self.pages_out = made(n + 1), held if in_place else made(n), pages if in_place else made(n)
+        self.free_out = free if in_place else made(3)
+        self.sequence, self.position, self.slot = made(n_tokens), made(n_tokens), made(n_tokens, torch.int64)
+        self.n_tokens, self.page_tokens = n_tokens, page_tokens
+        self.batch = KVBatch(self.start, self.length, table)
+        self.c = _CPlan(n, _u32(n_tokens, "n_tokens"), _u32(page_tokens, "page_tokens"), table.shape[1], ring.numel(),
+                        *[t.data_ptr() for t in (new, held, pages, free, table, ring, self.start, self.length, self.pages_out,
+                                                 self.free_out, self.sequence, self.position, self.slot)])
+        self.ref = ctypes.byref(self.c)
+
+
+NORM_KINDS = {"rms": 0, "layer": 1}
+
+
+class Norm:
+    """A norm and its weights (tc_norm): fp32 weight and bias [cols], either None;
+    offset is added to the weights."""
+
+    def __init__(self, weight=None, bias=None, eps=1e-6, kind="rms", offset=0.0):
+        import torch
+        _need(kind in NORM_KINDS, f"a norm is one of {sorted(NORM_KINDS)}")
+        self.weight, self.bias = weight, bias
+        held = [t for t in (weight, bias) if t is not None]
+        _need(all(t.dtype == torch.float32 and t.dim() == 1 for t in held), "a norm's weights are fp32 [cols]")
+        self.device = _same_device(held, "a norm's weights are contiguous and on one device") if held else None
+        _need(len({t.numel() for t in held}) <= 1, "weight and bias differ in size")
+        self.cols = held[0].numel() if held else None
+        self.c = _CNorm(NORM_KINDS[kind], eps, *[None if t is None else t.data_ptr() for t in (weight, bias)], offset)
+        self.ref = ctypes.addressof(self.c)
+
+
+ROPE_LAYOUTS = {"half": 0, "pairs": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+class Rope:
+    """Rotary positions of a head's first n_rot dims (tc_rope), with their table of
+    frequencies on `device`. layout: "half" (dims i and i + n_rot / 2 are a pair) or
+    "pairs" (2i and 2i + 1). scaling: "none", "linear", "ntk", "yarn" or "bands", with the
+    numbers of tc_rope_scaling; divisors: fp32 [n_rot / 2]. factor_of_values: instead of the
+    scaling's own factor of the rotated values."""
+
+    def __init__(self, n_rot, theta=10000.0, layout="half", scaling="none", factor=1.0, original=0.0, low=0.0, high=0.0,
+                 divisors=None, factor_of_values=None, device="cuda"):
+        import torch
+        _need(layout in ROPE_LAYOUTS, f"a layout is one of {sorted(ROPE_LAYOUTS)}")
+        _need(scaling in ROPE_SCALINGS, f"a scaling is one of {sorted(ROPE_SCALINGS)}")
+        _need(n_rot > 0 and n_rot % 2 == 0, "n_rot is even")
+        lib = load_library()
+        self.n_rot, self.layout = n_rot, layout
+        self.turns = torch.empty(n_rot // 2, dtype=torch.float64, device=device)
+        _need(divisors is None or (divisors.dtype == torch.float32 and divisors.is_contiguous() and
+                                   divisors.numel() == n_rot // 2 and divisors.device == self.turns.device),
+              "divisors are contiguous fp32 [n_rot / 2] on the rope's device")
+        self.divisors = divisors
+        self.device = self.turns.get_device()
+        f = ctypes.c_float()
+        c = _CRopeScaling(ROPE_SCALINGS[scaling], factor, original, low, high, None if divisors is None else divisors.data_ptr())
+        with torch.cuda.device(self.device):
+            rc = lib.tc_rope_turns(ctypes.byref(c), n_rot, theta, self.turns.data_ptr(), ctypes.byref(f),
+                                   torch.cuda.current_stream().cuda_stream)
+        if rc != TC_OK:
+            raise TCError(rc, lib.tc_last_error().decode())
+        self.c = _CRope(n_rot, ROPE_LAYOUTS[layout], self.turns.data_ptr(), f.value if factor_of_values is None else factor_of_values)
+        self.ref = ctypes.byref(self.c)
+
+
+class LogitRules:
+    """What is done to a batch's logits (tc_logit_rules), every tensor contiguous, on one
+    device, or None: repetition, frequency, presence fp32 [n_seq]; history int32 (the
+    sequences' tokens one behind the other) with history_start int32 [n_seq + 1] and
+    prompt int32 [n_seq]; bias_token int32, bias_value fp32 with bias_start int32
+    [n_seq + 1]; mask int32 [n_masks][words] (32 tokens a word) with mask_of int32
+    [n_tokens]. Other numbers may be written into the tensors between calls."""
+
+    def __init__(self, repetition=None, frequency=None, presence=None, history=None, history_start=None, prompt=None,
+                 bias_start=None, bias_token=None, bias_value=None, mask=None, mask_of=None):
+        import torch
+        floats, ints = (repetition, frequency, presence, bias_value), (history, history_start, prompt, bias_start, bias_token,
+                                                                       mask, mask_of)
+        _need(all(t is None or t.dtype == torch.float32 for t in floats), "penalties and biases are fp32")
+        _need(all(t is None or t.dtype == torch.int32 for t in ints), "tokens, their places and masks are int32")
+        held = [t for t in floats + ints if t is not None]
+        self.device = _same_device(held, "rules are contiguous and on one device") if held else None
+        _need((history is None) == (history_start is None), "history goes with history_start")
+        _need((bias_start is None) == (bias_token is None) == (bias_value is None), "bias_start, bias_token and bias_value go together")
+        _need(bias_token is None or bias_token.numel() == bias_value.numel(), "bias_token and bias_value differ in size")
+        _need(mask is None or mask.dim() == 2, "a mask is [n_masks][words]")
+        _need(mask_of is None or mask is not None, "mask_of without masks")
+        _need(prompt is None or history is not None, "prompt without a history")
+        self.held = held
+        self.sizes = {t.numel() for t in (repetition, frequency, presence, prompt) if t is not None} | \
+                     {t.numel() - 1 for t in (history_start, bias_start) if t is not None}
+        _need(len(self.sizes) <= 1, "the rules are of different numbers of sequences")
+        # rows that need a mask of their own, or an entry of mask_of
+        self.rows = None if mask_of is None else mask_of.numel()
+        self.words = None if mask is None else mask.shape[1]
+        p = [None if t is None else t.data_ptr() for t in (repetition, frequency, presence, history, history_start, prompt,
+                                                           bias_start, bias_token, bias_value, mask, mask_of)]
+        self.c = _CLogitRules(*p[:6], 0 if history is None else _u32(history.numel(), "history"), *p[6:9],
+                              0 if bias_token is None else _u32(bias_token.numel(), "biases"), p[9],
+                              0 if mask is None else _u32(mask.shape[0], "masks"), 0 if mask is None else mask.shape[1], p[10])
+        self.ref = ctypes.byref(self.c)
 
 
 def _ptr(t):
@@ -479,6 +662,161 @@ class Library:
                                             start.data_ptr(), tokens.data_ptr(), temperature.data_ptr(), accept_u.data_ptr(),
                                             sample_u.data_ptr(), n.data_ptr(), tok.data_ptr(), self._stream(dev)))
         return n, tok
+
+    # -- the rest of a step: geometry, norms, rotary positions, rules on logits ----------
+    def kv_plan(self, plan):
+        """One step's rows, positions, slots and pages (tc_kv_plan): plan, filled."""
+        import torch
+        dev = torch.cuda.current_device()
+        if plan.device != dev:
+            raise TCError(TC_E_ARG, "the plan is not on the current device")
+        self._check(self.lib.tc_kv_plan(plan.ref, self._stream(dev)))
+        return plan
+
+    def _norm_rows(self, h, y, h_out, x, pre, post, gate, sigmoid, scale, act_type, act):
+        import torch
+        if h.dim() != 2:
+            raise TCError(TC_E_ARG, "h is [rows][cols]")
+        shape = T, D = h.shape
+        dev = torch.cuda.current_device()
+        for t in (h, y, h_out, x):
+            if t is not None and (t.shape != shape or (T != 0 and D > 1 and t.stride(1) != 1) or t.get_device() != dev):
+                raise TCError(TC_E_ARG, "rows are [rows][cols], a row's values next to each other, on the current device")
+        if h_out is not None and h_out.dtype != h.dtype:
+            raise TCError(TC_E_ARG, "h_out is not of h's type")
+        for n in (pre, post):
+            if n is not None and n.cols is not None and (n.cols != D or n.device != dev):
+                raise TCError(TC_E_ARG, "a norm's weights are not the rows' or not on the current device")
+        kind = 0
+        if gate is not None:
+            if gate.shape == (T, D):
+                kind = 3
+            elif gate.shape == (T, 1):
+                kind = 2
+            elif gate.shape == (D,):
+                kind = 1
+            else:
+                raise TCError(TC_E_ARG, "a gate is [cols], [rows][1] or [rows][cols]")
+            if not gate.is_contiguous() or gate.get_device() != dev:
+                raise TCError(TC_E_ARG, "a gate is contiguous, on the current device")
+        if act is not None and (not act.is_contiguous() or act.get_device() != dev or
+                                act.numel() * act.element_size() < self.lib.tc_act_bytes(act_type, T, D)):
+            raise TCError(TC_E_ARG, "act is too small, not contiguous or not on the current device")
+
+        def stride(t):
+            return 0 if t is None else _u32(t.stride(0), "row stride") if T > 1 else D
+
+        c = _CNormRows(T, D, h.data_ptr(), y.data_ptr() if y is not None else None,
+                       h_out.data_ptr() if h_out is not None else None, x.data_ptr() if x is not None else None,
+                       _elem_type(h.dtype), _elem_type(y.dtype) if y is not None else 0,
+                       _elem_type(x.dtype) if x is not None else 0, stride(h), stride(y), stride(h_out), stride(x),
+                       post.ref if post is not None else None, pre.ref if pre is not None else None,
+                       gate.data_ptr() if gate is not None else None, kind,
+                       _elem_type(gate.dtype) if gate is not None else 0, sigmoid, scale,
+                       act_type, act.data_ptr() if act is not None else None)
+        self._check(self.lib.tc_norm_add(ctypes.byref(c), self._stream(dev)))
+
+    def norm(self, h, pre, out_dtype=None, out=None):
+        """pre(h): the norm of rows [rows][cols] (which may be strided), of out_dtype (h's)."""
+        import torch
+        if out is None:
+            out = torch.empty(h.shape, dtype=out_dtype or h.dtype, device=h.device)
+        self._norm_rows(h, None, None, out, pre, None, None, False, 1.0, 0, None)
+        return out
+
+    def norm_add(self, h, y, pre=None, post=None, gate=None, sigmoid=False, scale=1.0, out_dtype=None, h_out=None, out=None,
+                 act_type=0, act=None):
+        """h + scale * gate * post(y) into h_out (h itself may be given), and pre of that, of
+        out_dtype (h's) into out: (h_out, out); without `pre` out is None. gate [cols],
+        [rows][1] or [rows][cols]. act: a buffer of
+        tc_act_bytes for the activations quantized for weights of act_type, as act_quantize."""
+        import torch
+        if h_out is None:
+            h_out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        if out is None and pre is not None:
+            out = torch.empty(h.shape, dtype=out_dtype or h.dtype, device=h.device)
+        self._norm_rows(h, y, h_out, out, pre, post, gate, sigmoid, scale, act_type, act)
+        return h_out, out
+
+    def rope(self, rope, x, position, out=None):
+        """Rows [n_tokens][heads][head_dim] (which may be strided) rotated at position int32
+        [n_tokens]; rows below 0 are left as they are in out (which may be x)."""
+        import torch
+        if x.dim() != 3:
+            raise TCError(TC_E_ARG, "rows are [n_tokens][heads][head_dim]")
+        if out is None:
+            out = x.clone(memory_format=torch.contiguous_format) if x.shape[0] else torch.empty_like(x)
+        T, H, D = x.shape
+        dev = torch.cuda.current_device()
+        for t in (x, out):
+            if t.shape != x.shape or t.dtype != x.dtype or t.get_device() != dev or \
+                    (T != 0 and (t.stride(2) != 1 or (H != 1 and t.stride(1) != D))):
+                raise TCError(TC_E_ARG, "rows are of one shape and type, a row's heads contiguous, on the current device")
+        if position.dtype != torch.int32 or position.shape != (T,) or not position.is_contiguous() or \
+                position.get_device() != dev or rope.device != dev:
+            raise TCError(TC_E_ARG, "positions are contiguous int32 [n_tokens], they and the rope on the current device")
+        self._check(self.lib.tc_rope_apply(rope.ref, _elem_type(x.dtype), x.data_ptr(), self._row_stride(x), out.data_ptr(),
+                                           self._row_stride(out), position.data_ptr(), T, H, D, self._stream(dev)))
+        return out
+
+    def rope_kv_write(self, cache, batch, rope, q, k, v, q_norm=None, k_norm=None, eps=1e-6, out=None):
+        """Queries [n_tokens][heads][head_dim] rotated into out (new; contiguous), keys rotated
+        and values as they are into their slots of the cache (tc_rope_kv_write). q_norm, k_norm:
+        fp32 weights [head_dim] of an RMS norm of the heads before. q may be None."""
+        import torch
+        if k.dim() != 3 or k.shape[1] != cache.kv_heads:
+            raise TCError(TC_E_ARG, "k is not [n_tokens][kv_heads][head_dim]")
+        T, stream = self._kv_call(cache, batch, k, v, 2)
+        D, dev = cache.head_dim, cache.device
+        if rope.device != dev:
+            raise TCError(TC_E_ARG, "the rope is not on the current device")
+        for w in (q_norm, k_norm):
+            if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or w.stride(0) != 1 or w.get_device() != dev):
+                raise TCError(TC_E_ARG, "norms of heads are fp32 [head_dim] on the current device")
+        heads = 0
+        if q is not None:
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            if q.dim() != 3 or q.shape[0] != T or q.dtype != k.dtype:
+                raise TCError(TC_E_ARG, "q is not [n_tokens][heads][head_dim] of k's type")
+            self._kv_call(cache, batch, q, out, 1)
+            heads = q.shape[1]
+        elif out is not None:
+            raise TCError(TC_E_ARG, "out without q")
+        self._check(self.lib.tc_rope_kv_write(
+            cache.ref, batch.of(T), rope.ref, _elem_type(k.dtype), None if q is None else q.data_ptr(),
+            0 if q is None else self._row_stride(q), None if q is None else out.data_ptr(), heads, k.data_ptr(), self._row_stride(k),
+            v.data_ptr(), self._row_stride(v), None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, stream))
+        return out
+
+    def logits_adjust(self, rules, logits, start, tokens=None, out=None):
+        """Rules on logits [n_tokens][vocab] (rows may be strided) of the sequences' rows start
+        int32 [n_seq + 1]: fp32 [n_tokens][vocab] in out (which may be logits). tokens int32
+        [n_tokens]: the step's tokens, counted behind the history up to each row's own."""
+        import torch
+        if logits.dim() != 2:
+            raise TCError(TC_E_ARG, "logits are [n_tokens][vocab]")
+        T, V = logits.shape
+        S = start.numel() - 1
+        if out is None:
+            out = torch.empty((T, V), dtype=torch.float32, device=logits.device)
+        dev = torch.cuda.current_device()
+        for t in (start, tokens):
+            if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != dev):
+                raise TCError(TC_E_ARG, "start and tokens are contiguous int32 on the current device")
+        for t in (logits, out):
+            if t.shape != (T, V) or t.get_device() != dev or (T != 0 and V > 1 and t.stride(1) != 1):
+                raise TCError(TC_E_ARG, "logits are [n_tokens][vocab], a row's next to each other, on the current device")
+        if out.dtype != torch.float32 or (tokens is not None and tokens.numel() != T) or S < 0 or \
+                (rules.device is not None and rules.device != dev) or any(n != S for n in rules.sizes) or \
+                (rules.rows is not None and rules.rows < T) or (rules.words is not None and rules.words * 32 < V):
+            raise TCError(TC_E_ARG, "out is not fp32, or sizes or devices do not agree")
+        self._check(self.lib.tc_logits_adjust(
+            rules.ref, _elem_type(logits.dtype), logits.data_ptr(), _u32(logits.stride(0), "row stride") if T > 1 else V, V, S, T,
+            start.data_ptr(), None if tokens is None else tokens.data_ptr(), out.data_ptr(),
+            _u32(out.stride(0), "row stride") if T > 1 else V, self._stream(dev)))
+        return out
 
 
 class TensorRecord:
