@@ -8,8 +8,6 @@
 //
 // No list of tokens is sorted and no counts are kept in HBM: a table of counts of one sequence
 // would be as large as a row of its logits.
-#include <algorithm>
-
 #include "tc_kernels.hpp"
 #include "tc_step.hpp"
 
@@ -37,137 +35,215 @@ __device__ __forceinline__ void part_of(const int32_t *start, uint32_t s, uint32
     *end = uint32_t(e);
 }
 
+// A sequence's penalties. The logit is divided by the repetition's factor as a product with its
+// reciprocal in fp64, a step or two of fp64 from the quotient: where any lane of a wave has a
+// token that was seen, all of them wait for it, and a division takes as long as the rest.
+struct Penalties {
+    double rep, inv_rep, freq, pres;
+};
 // A token's logit where rules change it.
-__device__ __forceinline__ float changed(float l, uint32_t count, float bias, float rep, float freq, float pres) {
+__device__ __forceinline__ float changed(float l, uint32_t count, float bias, const Penalties &p) {
     double v = l;
     if (count != 0) {
         const uint32_t c = count & ~kSeen;
-        v = v > 0.0 ? v / double(rep) : v * double(rep);
-        if (c != 0) v -= double(freq) * double(c) + double(pres);
+        v *= v > 0.0 ? p.inv_rep : p.rep;
+        if (c != 0) v -= __builtin_fma(p.freq, double(c), p.pres);
     }
     return float(v + double(bias));
 }
 
+// 4 logits from token `i` of the chunk on (n: the chunk's), zeros behind its end.
+template <int XT>
+__device__ __forceinline__ void load4(const void *logits, uint64_t from, uint32_t i, uint32_t n, float (&l)[4]) {
+    const bool whole = i + 4 <= n;
+    if constexpr (XT == kF32) {
+        const float *p = static_cast<const float *>(logits) + from + i;
+        if (whole) {
+            const f32x4u v = *reinterpret_cast<const f32x4u *>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] = i + j < n ? p[j] : 0.0f;
+        }
+    } else {
+        const uint16_t *p = static_cast<const uint16_t *>(logits) + from + i;
+        if (whole) {
+            const u16x4u v = *reinterpret_cast<const u16x4u *>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] = widened(XT, v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[j] = i + j < n ? widened(XT, p[j]) : 0.0f;
+        }
+    }
+}
+
+// The words of a row's mask from token lo on, null: no mask.
+__device__ __forceinline__ const uint32_t *mask_of_row(const tc_logit_rules &r, uint32_t row, uint32_t lo) {
+    if (!r.mask) return nullptr;
+    const uint32_t m = r.mask_of ? uint32_t(r.mask_of[row]) : row;
+    return m < r.n_masks ? r.mask + size_t(m) * r.mask_words + (lo >> 5) : nullptr;
+}
+
+// V: vectors of 4 logits that a lane has of its chunk.
+template <int XT, int V>
 __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
+    constexpr uint32_t chunk = kThreads * 4 * V, step = kThreads * 4;
     extern __shared__ uint32_t lds[];
     uint32_t *counts = lds;
-    float *bias = reinterpret_cast<float *>(lds + a.chunk);
-    const uint32_t s = blockIdx.y, lo = blockIdx.x * a.chunk, n = min(a.chunk, a.vocab - lo);
+    float *bias = reinterpret_cast<float *>(lds + chunk);
+    const uint32_t s = blockIdx.y, lo = blockIdx.x * chunk, n = min(chunk, a.vocab - lo);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t row, end;
-    seq_rows(a.start, a.n_tokens, s, &row, &end);
-    if (row == end) return;
+    // everything that other loads wait for, side by side
+    uint32_t begin, end, h0 = 0, h1 = 0, b0 = 0, b1 = 0;
+    seq_rows(a.start, a.n_tokens, s, &begin, &end);
+    uint32_t row = begin + blockIdx.z;
     const float rep = a.r.repetition ? a.r.repetition[s] : 1.0f, freq = a.r.frequency ? a.r.frequency[s] : 0.0f;
     const float pres = a.r.presence ? a.r.presence[s] : 0.0f;
-    const bool counted = rep != 1.0f || freq != 0.0f || pres != 0.0f;
-    uint32_t b0 = 0, b1 = 0;
+    if (a.r.history_start) part_of(a.r.history_start, s, a.r.n_history, &h0, &h1);
     if (a.r.bias_start) part_of(a.r.bias_start, s, a.r.n_bias, &b0, &b1);
-    const bool biased = b0 != b1;
-    if (counted)
-        for (uint32_t i = tid; i < a.chunk; i += kThreads) counts[i] = 0;
-    if (biased)
-        for (uint32_t i = tid; i < a.chunk; i += kThreads) bias[i] = 0.0f;
-    __syncthreads();
-    if (counted && a.r.history_start) {
-        uint32_t h0, h1;
-        part_of(a.r.history_start, s, a.r.n_history, &h0, &h1);
-        const int32_t asked = a.r.prompt ? a.r.prompt[s] : 0;
-        const uint32_t answers = h0 + min(asked < 0 ? 0u : uint32_t(asked), h1 - h0);
-        for (uint32_t i = h0 + tid; i < h1; i += kThreads) {
-            const uint32_t t = uint32_t(a.r.history[i]) - lo;
-            if (t < n) {
-                if (i < answers)
-                    atomicOr(counts + t, kSeen);
-                else
-                    atomicAdd(counts + t, 1u);
-            }
+    const int32_t asked = a.r.prompt ? a.r.prompt[s] : 0;
+    if (row >= end) return;
+    const bool counted = rep != 1.0f || freq != 0.0f || pres != 0.0f, biased = b0 != b1;
+    if (!counted) h1 = h0;
+    const uint32_t answers = h0 + min(asked < 0 ? 0u : uint32_t(asked), h1 - h0);
+    // the first row is on its way while the history is counted, each other one while the row
+    // before it is worked on
+    float l[V][4];
+    uint32_t words[V];
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t i = tid * 4 + v * step;
+            if (i < n) load4<XT>(a.logits, r * a.x_stride + lo, i, n, l[v]);
         }
+        const uint32_t *mask = mask_of_row(a.r, r, lo);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t i = tid * 4 + v * step;
+            words[v] = ~0u;
+            if (mask && i < n) words[v] = mask[i >> 5];
+        }
+    };
+    // each lane's first token of the history and of the biases
+    const int32_t first = h0 + tid < h1 ? a.r.history[h0 + tid] : -1;
+    uint32_t bias_token = b0 + lane < b1 ? uint32_t(a.r.bias_token[b0 + lane]) : ~0u;
+    float bias_value = b0 + lane < b1 ? a.r.bias_value[b0 + lane] : 0.0f;
+    load(row);
+    const u32x4 zero = {0, 0, 0, 0};
+    if (counted)
+#pragma unroll
+        for (int v = 0; v < V; ++v) *reinterpret_cast<u32x4 *>(counts + tid * 4 + v * step) = zero;
+    if (biased)
+#pragma unroll
+        for (int v = 0; v < V; ++v) *reinterpret_cast<u32x4 *>(lds + chunk + tid * 4 + v * step) = zero;
+    __syncthreads();
+    auto count = [&](int32_t token, uint32_t i) {
+        const uint32_t t = uint32_t(token) - lo;
+        if (t < n) {
+            if (i < answers)
+                atomicOr(counts + t, kSeen);
+            else
+                atomicAdd(counts + t, 1u);
+        }
+    };
+    uint32_t i = h0 + tid;
+    count(first, i);
+    // (8 on their way at a time)
+    for (i += kThreads; i + 7 * kThreads < h1; i += 8 * kThreads) {
+        int32_t t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = a.r.history[i + j * kThreads];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) count(t[j], i + j * kThreads);
     }
+    for (; i < h1; i += kThreads) count(a.r.history[i], i);
     if (biased) {
         // each wave has a quarter of the chunk, and adds the biases there one after the other
-        const uint32_t part = a.chunk / kWaves, p0 = lo + wave * part;
-        for (uint32_t i0 = b0; i0 < b1; i0 += 64) {
-            const uint32_t i = i0 + lane;
-            const uint32_t t = i < b1 ? uint32_t(a.r.bias_token[i]) - p0 : part;
-            const float v = i < b1 ? a.r.bias_value[i] : 0.0f;
-            for (uint64_t m = __ballot(t < part && t + p0 < a.vocab); m != 0; m &= m - 1) {
-                const int l = __builtin_ctzll(m);
-                const uint32_t at = wave * part + __builtin_amdgcn_readlane(t, l);
-                const float add = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+        constexpr uint32_t part = chunk / kWaves;
+        const uint32_t p0 = lo + wave * part;
+        for (uint32_t i0 = b0;;) {
+            const uint32_t t = bias_token - p0;
+            for (uint64_t m = __ballot(t < part && bias_token < a.vocab); m != 0; m &= m - 1) {
+                const int b = __builtin_ctzll(m);
+                const uint32_t at = wave * part + __builtin_amdgcn_readlane(t, b);
+                const float add = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bias_value), b));
                 if (lane == 0) bias[at] += add;
             }
+            if ((i0 += 64) >= b1) break;
+            const uint32_t i = i0 + lane;
+            bias_token = i < b1 ? uint32_t(a.r.bias_token[i]) : ~0u;
+            bias_value = i < b1 ? a.r.bias_value[i] : 0.0f;
         }
     }
     __syncthreads();
-    for (; row < end; ++row) {
-        if (counted && a.tokens) {
-            const uint32_t t = uint32_t(a.tokens[row]) - lo;
-            if (tid == 0 && t < n) counts[t] += 1;
+    const Penalties p{double(rep), 1.0 / double(rep), double(freq), double(pres)};
+    const bool own_tokens = counted && a.tokens;
+    for (uint32_t told = begin; row < end; row += gridDim.z) {
+        if (own_tokens) {
+            for (told += tid; told <= row; told += kThreads) {
+                const uint32_t t = uint32_t(a.tokens[told]) - lo;
+                if (t < n) atomicAdd(counts + t, 1u);
+            }
+            told = row + 1;
             __syncthreads();
         }
-        const uint32_t *mask = nullptr;
-        if (a.r.mask) {
-            const uint32_t m = a.r.mask_of ? uint32_t(a.r.mask_of[row]) : row;
-            if (m < a.r.n_masks) mask = a.r.mask + size_t(m) * a.r.mask_words + (lo >> 5);
-        }
-        const uint64_t from = row * a.x_stride + lo, to = row * a.out_stride + lo;
-        for (uint32_t i = tid * 4; i < n; i += kThreads * 4) {
-            float l[4];
-            const bool whole = i + 4 <= n;
-            if (a.xtype == kF32) {
-                const float *p = static_cast<const float *>(a.logits) + from + i;
-                if (whole) {
-                    const f32x4u v = *reinterpret_cast<const f32x4u *>(p);
+        float *out = a.out + row * a.out_stride + lo;
+        float o[V][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) l[j] = v[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) l[j] = i + j < n ? p[j] : 0.0f;
-                }
-            } else {
-                const uint16_t *p = static_cast<const uint16_t *>(a.logits) + from + i;
-                if (whole) {
-                    const u16x4u v = *reinterpret_cast<const u16x4u *>(p);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) l[j] = widened(a.xtype, v[j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) l[j] = i + j < n ? widened(a.xtype, p[j]) : 0.0f;
-                }
-            }
-            uint32_t allowed = 15;
-            if (mask) allowed = mask[i >> 5] >> (i & 31);
-            u32x4 c = {0, 0, 0, 0};
+        for (int v = 0; v < V; ++v) {
+            const uint32_t i = tid * 4 + v * step, allowed = words[v] >> (i & 31);
+            u32x4 c = zero;
             f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
             if (counted) c = *reinterpret_cast<const u32x4 *>(counts + i);
             if (biased) b = *reinterpret_cast<const f32x4 *>(bias + i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (c[j] != 0 || b[j] != 0.0f) l[j] = changed(l[j], c[j], b[j], rep, freq, pres);
-                if (!(allowed >> j & 1)) l[j] = -kInf;
+                o[v][j] = l[v][j];
+                if (c[j] != 0 || b[j] != 0.0f) o[v][j] = changed(l[v][j], c[j], b[j], p);
+                if (!(allowed >> j & 1)) o[v][j] = -kInf;
             }
-            float *o = a.out + to + i;
-            if (whole) {
-                *reinterpret_cast<f32x4u *>(o) = f32x4u{l[0], l[1], l[2], l[3]};
+        }
+        if (row + gridDim.z < end) load(row + gridDim.z);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t i = tid * 4 + v * step;
+            if (i + 4 <= n) {
+                *reinterpret_cast<f32x4u *>(out + i) = f32x4u{o[v][0], o[v][1], o[v][2], o[v][3]};
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (i + j < n) o[j] = l[j];
+                    if (i + j < n) out[i + j] = o[v][j];
             }
         }
-        if (counted && a.tokens) __syncthreads();
+        if (own_tokens) __syncthreads();
     }
+}
+
+template <int XT, int V>
+hipError_t launch(const LogitCall &c, uint32_t parts, hipStream_t st) {
+    const uint32_t chunk = kThreads * 4 * V, bytes = chunk * (c.r.bias_start ? 8 : 4);
+    k_logits<XT, V><<<dim3((c.vocab + chunk - 1) / chunk, c.n_seq, parts), kThreads, bytes, st>>>(c);
+    return hipGetLastError();
+}
+template <int XT>
+hipError_t launch(const LogitCall &c, int num_cu, hipStream_t st) {
+    const uint64_t cu = num_cu, chunks = uint64_t((c.vocab + 1023) / 1024) * c.n_seq;
+    const bool wide = chunks > 4 * cu;
+    const uint64_t most = (c.n_tokens + c.n_seq - 1) / c.n_seq, fill = 8 * cu / (wide ? (chunks + 1) / 2 : chunks);
+    const uint32_t parts = uint32_t(fill < 1 ? 1 : fill < most ? fill : most);
+    return wide ? launch<XT, 2>(c, parts, st) : launch<XT, 1>(c, parts, st);
 }
 
 }  // namespace
 
-hipError_t launch_logits(LogitCall c, int num_cu, hipStream_t st) {
-    // chunks of 1024 to 8192 tokens, as many as make about 8 workgroups per CU
-    const uint64_t want = std::max<uint64_t>(1, uint64_t(c.vocab) * c.n_seq / (8 * uint64_t(num_cu)));
-    c.chunk = want > 4096 ? 8192 : want > 2048 ? 4096 : want > 1024 ? 2048 : 1024;
-    const uint32_t bytes = c.chunk * (c.r.bias_start ? 8 : 4);
-    k_logits<<<dim3((c.vocab + c.chunk - 1) / c.chunk, c.n_seq), kThreads, bytes, st>>>(c);
-    return hipGetLastError();
+hipError_t launch_logits(const LogitCall &c, int num_cu, hipStream_t st) {
+    switch (c.xtype) {
+        case kF32: return launch<kF32>(c, num_cu, st);
+        case kF16: return launch<kF16>(c, num_cu, st);
+        default: return launch<kBF16>(c, num_cu, st);
+    }
 }
 
 }  // namespace tc

@@ -80,8 +80,7 @@ struct LogitCall {
     int32_t xtype;
     uint32_t vocab, n_seq, n_tokens;
     const int32_t *start, *tokens;
-    uint32_t chunk;  // tokens of the vocabulary that a workgroup has, a multiple of 32
 };
-hipError_t launch_logits(LogitCall c, int num_cu, hipStream_t st);
+hipError_t launch_logits(const LogitCall &c, int num_cu, hipStream_t st);
 
 }  // namespace tc

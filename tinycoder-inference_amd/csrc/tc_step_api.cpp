@@ -270,7 +270,7 @@ int tc_logits_adjust(const tc_logit_rules *r, int xtype, const void *logits, uin
         return refuse(TC_E_ARG, "out is logits of another type or stride");
     const int num_cu = tc::device_cu_count();
     if (num_cu == 0) return no_device();
-    const tc::LogitCall c{*r, logits, out, x_stride, out_stride, xtype, vocab, n_seq, n_tokens, start, tokens, 0};
+    const tc::LogitCall c{*r, logits, out, x_stride, out_stride, xtype, vocab, n_seq, n_tokens, start, tokens};
     return hip_rc(tc::launch_logits(c, num_cu, static_cast<hipStream_t>(stream)), "rules on logits");
 }
 
