@@ -109,9 +109,8 @@ typedef struct tc_norm_rows {
 /* One launch. Everything between the inputs and the outputs' rounding is held in fp32: x is
  * the norm of h + scale * gate * post(y) before that is rounded to h's type; act is formed
  * from the fp32 values that an F32 x has, and is tc_act_quantize's of them bit for bit.
- * cols up to 32768. Rows may have any stride that keeps them apart; rows of 8's multiples,
- * strides and bases of 16 bytes' multiples are the fast ones (others take up to three times as
- * long). Outputs do not overlap inputs, apart from h_out = h with the same stride. An
+ * cols up to 32768. Rows may have any stride that keeps them apart and any
+ * alignment that fits their elements (with act: 16 bytes). Outputs do not overlap inputs, apart from h_out = h with the same stride. An
  * infinity or NaN stays in its row; squares that pass fp32's range (values past 10^19) give
  * an infinite mean. */
 int tc_norm_add(const tc_norm_rows *rows, void *stream);

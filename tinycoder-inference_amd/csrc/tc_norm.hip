@@ -8,6 +8,9 @@
 // lane's values, over the wave, over the waves through LDS. So the kernel is bound by HBM for
 // many rows, and for few by the chain of one load, one sum over the row per statistic, and the
 // store; the weights' loads are issued in front of the sums.
+#include <algorithm>
+#include <cmath>
+
 #include "tc_actquant.hpp"
 #include "tc_kernels.hpp"
 #include "tc_step.hpp"
@@ -15,11 +18,6 @@
 namespace tc {
 namespace {
 
-__device__ __forceinline__ float load1(int type, const void *p, uint64_t elem) {
-    if (type == kF32) return static_cast<const float *>(p)[elem];
-    const uint32_t w = static_cast<const uint16_t *>(p)[elem];
-    return type == kF16 ? h2f(w) : __builtin_bit_cast(float, w << 16);
-}
 __device__ __forceinline__ void store1(int type, void *p, uint64_t elem, float x) {
     if (type == kF32)
         static_cast<float *>(p)[elem] = x;
@@ -27,29 +25,92 @@ __device__ __forceinline__ void store1(int type, void *p, uint64_t elem, float x
         static_cast<uint16_t *>(p)[elem] = uint16_t(type == kF16 ? pack_f16(x, 0.0f) : pack_bf16(x, 0.0f));
 }
 
-// A lane's 8 values of a row from column `at` on, zeros behind the row's end. VEC: all 8
-// inside the row or none, and 16-byte aligned; else its columns are `at` + 64 i.
-template <bool VEC>
-__device__ __forceinline__ void row_load(int type, const void *p, uint64_t row, uint32_t at, uint32_t cols, float (&x)[8]) {
+// 16 bytes at any address that fits their elements (rows of odd widths and strides): the
+// hardware takes such accesses whole.
+typedef uint32_t u32x4d __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4h __attribute__((ext_vector_type(4), aligned(2)));
+
+// A lane's 8 columns of a row: from `at` on. The lane at the row's end has the row's last 8,
+// of which the first `off` are the lane's before it; lanes behind it have off = 8. (So every lane
+// loads 16 bytes, and no branch parts the loads: with one for each type and end, a load waited
+// for the one before it.)
+struct Span {
+    uint32_t at, off;
+};
+
+// A lane's 8 values as they are in memory (16-bit types: a alone).
+struct Raw {
+    u32x4 a, b;
+};
+// W: the elements' bytes. TINY: rows of less than 8 columns, all of them the first lane's.
+template <int W, bool TINY>
+__device__ __forceinline__ Raw raw_load(const void *p, uint64_t row, Span s, uint32_t cols) {
+    Raw r;
+    if constexpr (TINY) {
+        r.a = r.b = u32x4{0, 0, 0, 0};
+        if (s.off < 8)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if constexpr (VEC) {
-        if (at < cols) load8(type, p, row + at, x);
+            for (int i = 0; i < 7; ++i)
+                if (uint32_t(i) < cols) {
+                    if constexpr (W == 4)
+                        (i < 4 ? r.a : r.b)[i & 3] = static_cast<const uint32_t *>(p)[row + i];
+                    else
+                        r.a[i >> 1] |= uint32_t(static_cast<const uint16_t *>(p)[row + i]) << (16 * (i & 1));
+                }
+    } else if constexpr (W == 4) {
+        const u32x4d *q = reinterpret_cast<const u32x4d *>(static_cast<const float *>(p) + row + s.at);
+        r.a = q[0], r.b = q[1];
+    } else {
+        r.a = *reinterpret_cast<const u32x4h *>(static_cast<const uint16_t *>(p) + row + s.at);
+    }
+    return r;
+}
+template <int W>
+__device__ __forceinline__ void widen(int type, const Raw &r, float (&x)[8]) {
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(float, uint32_t(r.a[i])), x[4 + i] = __builtin_bit_cast(float, uint32_t(r.b[i]));
+    } else if (type == kF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = h2f(r.a[i] & 0xFFFF), x[2 * i + 1] = h2f(r.a[i] >> 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (at + 64 * i < cols) x[i] = load1(type, p, row + at + 64 * i);
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __builtin_bit_cast(float, uint32_t(r.a[i]) << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, r.a[i] & 0xFFFF0000u);
+        }
     }
 }
-template <bool VEC>
-__device__ __forceinline__ void row_store(int type, void *p, uint64_t row, uint32_t at, uint32_t cols, const float (&x)[8]) {
-    if constexpr (VEC) {
-        if (at < cols) store8(type, p, row + at, x);
-    } else {
+// Zeros in the place of what is not the lane's own.
+template <bool TINY>
+__device__ __forceinline__ void own_only(Span s, uint32_t cols, float (&x)[8]) {
+    if (s.off == 0 && !TINY) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (TINY ? s.off == 8 || uint32_t(i) >= cols : uint32_t(i) < s.off) x[i] = 0.0f;
+}
+template <int W, bool TINY>
+__device__ __forceinline__ void row_store(int type, void *p, uint64_t row, Span s, uint32_t cols, const float (&x)[8]) {
+    if (s.off == 0 && !TINY) {
+        if constexpr (W == 4) {
+            u32x4d *q = reinterpret_cast<u32x4d *>(static_cast<float *>(p) + row + s.at);
+            q[0] = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
+            q[1] = __builtin_bit_cast(u32x4, f32x4{x[4], x[5], x[6], x[7]});
+        } else {
+            u32x4 u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = type == kF16 ? pack_f16(x[2 * i], x[2 * i + 1]) : pack_bf16(x[2 * i], x[2 * i + 1]);
+            *reinterpret_cast<u32x4h *>(static_cast<uint16_t *>(p) + row + s.at) = u;
+        }
+    } else if (s.off != 8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (at + 64 * i < cols) store1(type, p, row + at + 64 * i, x[i]);
+            if (TINY ? uint32_t(i) < cols : uint32_t(i) >= s.off) store1(type, p, row + s.at + i, x[i]);
     }
+}
+template <bool TINY>
+__device__ __forceinline__ void row_store(int type, void *p, uint64_t row, Span s, uint32_t cols, const float (&x)[8]) {
+    type == kF32 ? row_store<4, TINY>(type, p, row, s, cols, x) : row_store<2, TINY>(type, p, row, s, cols, x);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -62,131 +123,169 @@ __device__ __forceinline__ float wave_sum(float v) {
     return (lane(15) + lane(31)) + (lane(47) + lane(63));
 }
 
-// Sum over the row's lanes; `at` counts the sums of a row, so that two barriers are not needed
-// for each: every one has its own place.
-template <bool ONE>
-__device__ __forceinline__ float row_sum(float v, float *lds, int at) {
-    v = wave_sum(v);
-    if constexpr (ONE) return v;
-    const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-    if (lane == 0) lds[16 * at + (threadIdx.x >> 6)] = v;
-    __syncthreads();
-    return wave_sum(lane < waves ? lds[16 * at + lane] : 0.0f);
+// Sum over the row's lanes: LANES of a wave (a power of two), or a workgroup's (0). Every sum of a
+// row has its own place in LDS, so that one barrier is enough for each.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float *lds) {
+    if constexpr (LANES == 64) {
+        return wave_sum(v);
+    } else if constexpr (LANES != 0) {
+        v += dpp_f<0xB1>(v);  // 1, 2, 4, 8 lanes away (as quads, quads' halves and rows mirrored)
+        v += dpp_f<0x4E>(v);
+        v += dpp_f<0x141>(v);
+        if constexpr (LANES >= 16) v += dpp_f<0x140>(v);
+        if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
+        return v;
+    } else {
+        v = wave_sum(v);
+        const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+        if (lane == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return wave_sum(lane < waves ? lds[lane] : 0.0f);
+    }
 }
 
-// One row normed in place; first: the number of its first sum.
-template <bool VEC, bool ONE, int C>
-__device__ __forceinline__ void norm_row(const NormArgs &n, uint32_t cols, uint32_t at, uint32_t step, float *lds, int first,
-                                         float (&z)[C][8]) {
-    // (long rows have no registers for them so early)
-    constexpr bool EARLY = C <= 2;
-    float w[C][8], b[C][8];
-    auto load = [&](int c) {
-        if (n.weight != nullptr) row_load<VEC>(kF32, n.weight, 0, at + c * step, cols, w[c]);
-        if (n.bias != nullptr) row_load<VEC>(kF32, n.bias, 0, at + c * step, cols, b[c]);
-    };
-    if constexpr (EARLY)
-#pragma unroll
-        for (int c = 0; c < C; ++c) load(c);
-    const float inv_n = 1.0f / float(cols);
+// One row normed in place; lds: places of two sums. (The weights are loaded behind the sums: held
+// in registers across them they took more of a CU's rows than their way from L2 costs.)
+template <int LANES, int C, bool TINY>
+__device__ __forceinline__ void norm_row(const NormCall &a, const NormArgs &n, const Span (&at)[C], float *lds, float (&z)[C][8]) {
+    const uint32_t cols = a.cols;
     if (n.kind == TC_NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) s += z[c][i];
-        const float mean = row_sum<ONE>(s, lds, first) * inv_n;
+        const float mean = row_sum<LANES>(s, lds) * a.inv_cols;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                z[c][i] = at + c * step + (VEC ? 0 : 64 * i) < cols ? z[c][i] - mean : 0.0f;
+            for (int i = 0; i < 8; ++i) z[c][i] -= mean;
+            own_only<TINY>(at[c], cols, z[c]);
+        }
     }
     // (squares times a power of two near 1 / cols, so that their sum passes fp32's range no sooner
     // than the largest square does)
-    const float down = __builtin_bit_cast(float, (127u - (32u - __builtin_clz(cols))) << 23);
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(z[c][i] * down, z[c][i], s);
-    const float inv = rsqrtf(__builtin_fmaf(row_sum<ONE>(s, lds, first + 1), inv_n / down, n.eps));
+        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(z[c][i] * a.down, z[c][i], s);
+    const float inv = rsqrtf(__builtin_fmaf(row_sum<LANES>(s, lds + 16), a.inv_cols_down, n.eps));
+    Raw w[C];
+    if (n.weight != nullptr)
+#pragma unroll
+        for (int c = 0; c < C; ++c) w[c] = raw_load<4, TINY>(n.weight, 0, at[c], cols);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        if constexpr (!EARLY) load(c);
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            z[c][i] *= inv;
-            if (n.weight != nullptr) z[c][i] *= w[c][i] + n.offset;
-            if (n.bias != nullptr) z[c][i] += b[c][i];
+        for (int i = 0; i < 8; ++i) z[c][i] *= inv;
+        if (n.weight != nullptr) {
+            widen<4>(kF32, w[c], v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[c][i] *= v[i] + n.offset;
+        }
+        if (n.bias != nullptr) {
+            widen<4>(kF32, raw_load<4, TINY>(n.bias, 0, at[c], cols), v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[c][i] += v[i];
         }
     }
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + expf(-g)); }
 
-// C: blocks of 8 values of a lane. ONE: a wave has a row, a workgroup four; else a
-// workgroup has one. ACT: quantized activations too.
-template <bool VEC, bool ONE, int C, bool ACT>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void k_norm(NormCall a) {
+// YW, HW: bytes of y's (0: none) and h's elements. POST: there may be a norm of y. LANES: lanes
+// that have a row, 0: the workgroup. C: blocks of 8 values of a lane. ACT: quantized activations
+// too. MOST: threads of a workgroup at most (fewer leave more registers to each).
+template <int YW, int HW, bool POST, int LANES, int C, bool ACT, int MOST, bool TINY>
+__global__ __launch_bounds__(MOST) void k_norm(NormCall a) {
     __shared__ float lds[64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t r = ONE ? blockIdx.x * 4 + wave : blockIdx.x;
-    if (r >= a.rows) return;  // (only where no barrier follows)
-    const uint32_t w0 = ONE ? 0 : wave, waves = ONE ? 1 : blockDim.x >> 6;
-    // a lane's blocks lie a row of lanes apart
-    const uint32_t at = w0 * 512 + (VEC ? lane * 8 : lane), step = waves * 512, cols = a.cols;
+    const uint32_t tid = threadIdx.x, lane = LANES ? tid % (LANES ? LANES : 1) : tid & 63, wave = LANES ? 0 : tid >> 6;
+    const uint32_t waves = LANES ? 1 : blockDim.x >> 6, cols = a.cols;
+    const uint32_t r = LANES ? blockIdx.x * (MOST / (LANES ? LANES : 1)) + tid / (LANES ? LANES : 1) : blockIdx.x;
+    if (r >= a.rows) return;  // (only where no barrier follows; a row's lanes go together)
+    Span at[C];  // a lane's blocks lie a row of lanes apart
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t from = (c * waves + wave) * 512 + lane * 8;
+        at[c].at = TINY ? 0 : min(from, cols - 8);
+        at[c].off = TINY ? (lane ? 8 : 0) : min(from - at[c].at, 8u);
+    }
+    Raw y_raw[C], h_raw[C], g_raw[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if constexpr (YW != 0) y_raw[c] = raw_load<YW, TINY>(a.y, r * a.y_stride, at[c], cols);
+        h_raw[c] = raw_load<HW, TINY>(a.h, r * a.h_stride, at[c], cols);
+    }
+    const bool gated = YW != 0 && (a.gate_kind == TC_GATE_CHANNEL || a.gate_kind == TC_GATE_FULL);
+    if (gated) {
+        const uint64_t base = a.gate_kind == TC_GATE_FULL ? uint64_t(r) * cols : 0;
+        if (a.gate_type == kF32) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) g_raw[c] = raw_load<4, TINY>(a.gate, base, at[c], cols);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) g_raw[c] = raw_load<2, TINY>(a.gate, base, at[c], cols);
+        }
+    } else if (YW != 0 && a.gate_kind == TC_GATE_ROW) {  // (one value: the first of a Raw)
+        if (a.gate_type == kF32)
+            g_raw[0].a[0] = static_cast<const uint32_t *>(a.gate)[r];
+        else
+            g_raw[0].a[0] = static_cast<const uint16_t *>(a.gate)[r];
+    }
     float h[C][8];
-    if (a.y != nullptr) {
-        float y[C][8], g[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        widen<HW>(a.h_type, h_raw[c], h[c]);
+        own_only<TINY>(at[c], cols, h[c]);
+    }
+    if constexpr (YW != 0) {
+        float y[C][8];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            row_load<VEC>(a.y_type, a.y, r * a.y_stride, at + c * step, cols, y[c]);
-            row_load<VEC>(a.h_type, a.h, r * a.h_stride, at + c * step, cols, h[c]);
+            widen<YW>(a.y_type, y_raw[c], y[c]);
+            own_only<TINY>(at[c], cols, y[c]);
         }
-        float row_gate = a.scale;
+        if constexpr (POST) {
+            if (a.post.kind >= 0) norm_row<LANES, C, TINY>(a, a.post, at, lds, y);
+        }
+        float f = a.scale;
         if (a.gate_kind == TC_GATE_ROW) {
-            const float v = load1(a.gate_type, a.gate, r);
-            row_gate *= a.gate_sigmoid ? sigmoid(v) : v;
-        } else if (a.gate_kind != TC_GATE_NONE) {
-            const uint64_t base = a.gate_kind == TC_GATE_FULL ? uint64_t(r) * cols : 0;
-#pragma unroll
-            for (int c = 0; c < C; ++c) row_load<VEC>(a.gate_type, a.gate, base, at + c * step, cols, g[c]);
+            const uint32_t bits = g_raw[0].a[0];
+            const float v = a.gate_type == kF32 ? __builtin_bit_cast(float, bits) : a.gate_type == kF16 ? h2f(bits) : __builtin_bit_cast(float, bits << 16);
+            f *= a.gate_sigmoid ? sigmoid(v) : v;
         }
-        if (a.post.kind >= 0) norm_row<VEC, ONE, C>(a.post, cols, at, step, lds, 0, y);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
+            if (gated) {
+                float g[8];
+                if (a.gate_type == kF32)
+                    widen<4>(kF32, g_raw[c], g);
+                else
+                    widen<2>(a.gate_type, g_raw[c], g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float f = row_gate;
-                if (a.gate_kind == TC_GATE_CHANNEL || a.gate_kind == TC_GATE_FULL)
-                    f *= a.gate_sigmoid ? sigmoid(g[c][i]) : g[c][i];
-                h[c][i] = __builtin_fmaf(f, y[c][i], h[c][i]);
+                for (int i = 0; i < 8; ++i) y[c][i] *= a.gate_sigmoid ? sigmoid(g[i]) : g[i];
             }
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (a.h_out != nullptr) row_store<VEC>(a.h_type, a.h_out, r * a.h_out_stride, at + c * step, cols, h[c]);
-            // (a bias of `post` is not to count behind the row's end)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + c * step + (VEC ? 0 : 64 * i) >= cols) h[c][i] = 0.0f;
+            for (int i = 0; i < 8; ++i) h[c][i] = __builtin_fmaf(f, y[c][i], h[c][i]);
+            if (a.h_out != nullptr) row_store<HW, TINY>(a.h_type, a.h_out, r * a.h_out_stride, at[c], cols, h[c]);
+            if constexpr (POST) own_only<TINY>(at[c], cols, h[c]);  // (`post` may have a bias)
         }
-    } else {
-#pragma unroll
-        for (int c = 0; c < C; ++c) row_load<VEC>(a.h_type, a.h, r * a.h_stride, at + c * step, cols, h[c]);
     }
     if (a.pre.kind < 0) return;
-    norm_row<VEC, ONE, C>(a.pre, cols, at, step, lds, 2, h);
+    norm_row<LANES, C, TINY>(a, a.pre, at, lds + 32, h);
     if (a.x != nullptr)
 #pragma unroll
-        for (int c = 0; c < C; ++c) row_store<VEC>(a.x_type, a.x, r * a.x_stride, at + c * step, cols, h[c]);
+        for (int c = 0; c < C; ++c) row_store<TINY>(a.x_type, a.x, r * a.x_stride, at[c], cols, h[c]);
     if constexpr (ACT) {
         // the quantizers want a block of 256 columns in a wave, four to a lane
         extern __shared__ float row[];
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (at + c * step < cols) {
-                f32x4 *p = reinterpret_cast<f32x4 *>(row + at + c * step);
+            if (at[c].off == 0) {
+                f32x4 *p = reinterpret_cast<f32x4 *>(row + at[c].at);
                 p[0] = f32x4{h[c][0], h[c][1], h[c][2], h[c][3]};
                 p[1] = f32x4{h[c][4], h[c][5], h[c][6], h[c][7]};
             }
@@ -203,48 +302,63 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void k_norm(NormCall a) {
     }
 }
 
-template <bool VEC, bool ONE, int C>
-hipError_t launch(const NormCall &a, uint32_t waves, hipStream_t st) {
-    if (a.qs != nullptr) {
-        if constexpr (VEC && !ONE && C <= 2)
-            k_norm<VEC, ONE, C, true><<<a.rows, 64 * waves, a.cols * 4, st>>>(a);
+// Rows of a workgroup, or of its waves' parts.
+template <int YW, int HW, bool POST>
+hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
+    const uint32_t blocks = (a.cols + 511) / 512;  // of a wave's 512 columns
+    const bool many = a.rows > 2u * uint32_t(num_cu);
+    auto waves = [&](uint32_t c) { return 64 * ((blocks + c - 1) / c); };
+    auto grid = [&](uint32_t lanes) { return (a.rows + 256 / lanes - 1) / (256 / lanes); };
+    if (a.cols <= 64)
+        k_norm<YW, HW, POST, 8, 1, false, 256, false><<<grid(8), 256, 0, st>>>(a);
+    else if (a.cols <= 128)
+        k_norm<YW, HW, POST, 16, 1, false, 256, false><<<grid(16), 256, 0, st>>>(a);
+    else if (a.cols <= 256)
+        k_norm<YW, HW, POST, 32, 1, false, 256, false><<<grid(32), 256, 0, st>>>(a);
+    else if (blocks == 1)
+        k_norm<YW, HW, POST, 64, 1, false, 256, false><<<grid(64), 256, 0, st>>>(a);
+    else if (blocks <= 16 && many)
+        k_norm<YW, HW, POST, 0, 2, false, 512, false><<<a.rows, waves(2), 0, st>>>(a);
+    else if (blocks <= 16)
+        k_norm<YW, HW, POST, 0, 1, false, 1024, false><<<a.rows, waves(1), 0, st>>>(a);
+    else if (blocks <= 32)
+        k_norm<YW, HW, POST, 0, 2, false, 1024, false><<<a.rows, waves(2), 0, st>>>(a);
+    else if (blocks <= 48)
+        k_norm<YW, HW, POST, 0, 3, false, 1024, false><<<a.rows, waves(3), 0, st>>>(a);
+    else
+        k_norm<YW, HW, POST, 0, 4, false, 1024, false><<<a.rows, waves(4), 0, st>>>(a);
+    return hipGetLastError();
+}
+template <int YW, int HW>
+hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
+    const uint32_t blocks = (a.cols + 511) / 512;
+    constexpr bool POST = YW != 0;
+    if (a.cols < 8) {
+        k_norm<YW, HW, POST, 64, 1, false, 256, true><<<(a.rows + 3) / 4, 256, 0, st>>>(a);
+    } else if (a.qs != nullptr) {
+        if (blocks <= 16)
+            k_norm<YW, HW, POST, 0, 1, true, 1024, false><<<a.rows, 64 * blocks, a.cols * 4, st>>>(a);
         else
-            return hipErrorInvalidValue;  // (not reached: launch_norm)
-    } else if (ONE) {
-        k_norm<VEC, ONE, C, false><<<(a.rows + 3) / 4, 256, 0, st>>>(a);
+            k_norm<YW, HW, POST, 0, 2, true, 1024, false><<<a.rows, 64 * ((blocks + 1) / 2), a.cols * 4, st>>>(a);
     } else {
-        k_norm<VEC, ONE, C, false><<<a.rows, 64 * waves, 0, st>>>(a);
+        return POST && a.post.kind >= 0 ? launch<YW, HW, POST>(a, num_cu, st) : launch<YW, HW, false>(a, num_cu, st);
     }
     return hipGetLastError();
 }
 
-template <bool VEC>
-hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
-    const uint32_t blocks = (a.cols + 511) / 512;  // of a wave's 512 columns
-    if (blocks == 1 && a.qs == nullptr) return launch<VEC, true, 1>(a, 1, st);
-    const bool many = a.rows > 4u * uint32_t(num_cu);
-    const uint32_t c = blocks > 32 ? 4 : blocks > 16 || (many && blocks > 1) ? 2 : 1;
-    const uint32_t waves = (blocks + c - 1) / c;
-    switch (c) {
-        case 1: return launch<VEC, false, 1>(a, waves, st);
-        case 2: return launch<VEC, false, 2>(a, waves, st);
-        default: return launch<VEC, false, 4>(a, waves, st);
-    }
-}
-
 }  // namespace
 
-hipError_t launch_norm(const NormCall &a, int num_cu, hipStream_t st) {
-    // rows that 16-byte accesses cut into whole parts
-    auto fits = [&](const void *p, uint64_t stride, int type) {
-        return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (a.rows == 1 || stride * elem_bytes(type) % 16 == 0));
-    };
-    const bool gate = a.gate_kind == TC_GATE_CHANNEL || a.gate_kind == TC_GATE_FULL;
-    const bool vec = a.cols % 8 == 0 && fits(a.h, a.h_stride, a.h_type) && fits(a.y, a.y_stride, a.y_type) &&
-                     fits(a.h_out, a.h_out_stride, a.h_type) && fits(a.x, a.x_stride, a.x_type) &&
-                     (!gate || fits(a.gate, a.gate_kind == TC_GATE_FULL ? a.cols : 0, a.gate_type)) && fits(a.post.weight, 0, kF32) &&
-                     fits(a.post.bias, 0, kF32) && fits(a.pre.weight, 0, kF32) && fits(a.pre.bias, 0, kF32);
-    return vec ? launch<true>(a, num_cu, st) : launch<false>(a, num_cu, st);
+hipError_t launch_norm(const NormCall &call, int num_cu, hipStream_t st) {
+    NormCall a = call;
+    int up = 0;
+    while ((2u << up) <= a.cols) ++up;
+    a.inv_cols = 1.0f / float(a.cols);
+    a.down = std::ldexp(1.0f, -up);
+    a.inv_cols_down = std::ldexp(a.inv_cols, up);
+    const bool wide = a.h_type == kF32;
+    if (a.y == nullptr) return wide ? launch<0, 4>(a, num_cu, st) : launch<0, 2>(a, num_cu, st);
+    if (a.y_type == kF32) return wide ? launch<4, 4>(a, num_cu, st) : launch<4, 2>(a, num_cu, st);
+    return wide ? launch<2, 4>(a, num_cu, st) : launch<2, 2>(a, num_cu, st);
 }
 
 }  // namespace tc
