@@ -72,18 +72,29 @@ hipError_t launch_kv_write(const KvArgs &a, int ctype, int xtype, const void *k,
                            uint32_t v_stride, hipStream_t st);
 hipError_t launch_kv_read(const KvArgs &a, int ctype, int xtype, void *k, void *v, hipStream_t st);
 
-// As find_seq, 64 sequences at a time: one fetch where there are no more.
-__device__ __forceinline__ int wave_find_seq(const int32_t *start, uint32_t n_seq, uint32_t t) {
+// As find_seq, 64 sequences at a time: one fetch where there are no more. The first 64 may be
+// fetched ahead.
+struct SeqProbe {
+    int32_t start;
+};
+__device__ __forceinline__ SeqProbe probe_seqs(const int32_t *start, uint32_t n_seq) {
+    return {start[min((threadIdx.x & 63) * ((n_seq + 63) / 64), n_seq)]};
+}
+__device__ __forceinline__ int wave_find_seq(const int32_t *start, uint32_t n_seq, uint32_t t, SeqProbe probe) {
     const uint32_t lane = threadIdx.x & 63;
     const int32_t before = start[0], behind = start[n_seq];
     uint32_t lo = 0, hi = n_seq;
-    while (hi - lo > 1) {
+    for (int32_t v = probe.start; hi - lo > 1;) {
         const uint32_t step = (hi - lo + 63) / 64, p = lo + lane * step;
-        const uint64_t m = __ballot(p < hi && (p == lo || start[p] <= int32_t(t)));
+        const uint64_t m = __ballot(p < hi && (p == lo || v <= int32_t(t)));
         lo += (63 - __builtin_clzll(m)) * step;
         hi = min(lo + step, hi);
+        if (hi - lo > 1) v = start[min(lo + lane * ((hi - lo + 63) / 64), n_seq)];
     }
     return int32_t(t) >= behind || int32_t(t) < before ? -1 : int(lo);
+}
+__device__ __forceinline__ int wave_find_seq(const int32_t *start, uint32_t n_seq, uint32_t t) {
+    return wave_find_seq(start, n_seq, t, probe_seqs(start, n_seq));
 }
 
 struct AttnArgs {

@@ -6,10 +6,23 @@
 
 namespace tc {
 
-// Largest of `lanes` lanes' values (a power of two; no NaN) in each of them.
-__device__ __forceinline__ float group_max(float v, uint32_t lanes) {
-    for (uint32_t o = 1; o < lanes; o <<= 1) v = fmaxf(v, __shfl_xor(v, int(o)));
+// op over the values of `lanes` lanes (a power of two up to 32) in each of them: 1, 2, 4 and 8
+// lanes away as quads, quads' halves and rows mirrored (lane moves that go without LDS), then 16.
+template <class Op>
+__device__ __forceinline__ float group_all(float v, uint32_t lanes, Op op) {
+    v = op(v, dpp_f<0xB1>(v));
+    if (lanes > 2) v = op(v, dpp_f<0x4E>(v));
+    if (lanes > 4) v = op(v, dpp_f<0x141>(v));
+    if (lanes > 8) v = op(v, dpp_f<0x140>(v));
+    if (lanes > 16) v = op(v, __shfl_xor(v, 16));
     return v;
+}
+// (no NaN)
+__device__ __forceinline__ float group_max(float v, uint32_t lanes) {
+    return group_all(v, lanes, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
+    return group_all(v, lanes, [](float a, float b) { return a + b; });
 }
 
 // The lane's 8 values x from dim `at` on of one row to cache row `row` (below 0: none) of

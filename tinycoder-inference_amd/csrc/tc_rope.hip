@@ -48,70 +48,106 @@ struct RopeWalk {
     uint32_t lanes;     // of a head, a power of two
     uint32_t lane_log;  // its logarithm
     uint32_t units;     // of a token
-    DivMod groups;      // of U units in a token
+    DivMod groups;      // of U units in a token, that many units apart
     uint32_t total;     // groups of all tokens
 };
 
-// The 8 factors of a lane's dims from `at` on: out[i] = x[i] * c[i] + other[i] * s[i].
-__device__ __forceinline__ void angles(const RopeArgs &r, uint32_t at, int32_t pos, float (&c)[8], float (&s)[8]) {
+// How a head's dims pair up: neighbours; halves of 8's multiples, so that the other halves of a
+// lane's pairs are one load; any halves.
+enum : int { kPairs, kHalves8, kHalves };
+
+// The turns of the pairs of a lane's dims from `at` on (kPairs: of its 4 pairs).
+template <int L>
+__device__ __forceinline__ void load_turns(const RopeArgs &r, uint32_t at, double (&t)[8]) {
+#pragma unroll
+    for (int i = 0; i < (L == kPairs ? 4 : 8); ++i) {
+        const uint32_t e = L == kPairs ? at / 2 + i : at + i;
+        t[i] = r.turns[min(L == kPairs || e < r.half ? e : e - r.half, r.half - 1)];
+    }
+}
+// The factors of those dims at a position: out[i] = x[i] * c[i] + other[i] * s[i].
+template <int L>
+__device__ __forceinline__ void angles(const RopeArgs &r, uint32_t at, int32_t pos, const double (&t)[8], float (&c)[8], float (&s)[8]) {
     const double p = double(pos);
-    if (r.layout == TC_ROPE_PAIRS) {
+    if constexpr (L == kPairs) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t e = at + 2 * i;
-            float cs = 1.0f, sn = 0.0f;
-            if (e < r.n_rot) {
-                turn(p * r.turns[e >> 1], &cs, &sn);
-                cs *= r.factor, sn *= r.factor;
-            }
-            c[2 * i] = c[2 * i + 1] = cs;
-            s[2 * i] = -sn, s[2 * i + 1] = sn;
+            float cs, sn;
+            turn(p * t[i], &cs, &sn);
+            c[2 * i] = c[2 * i + 1] = cs * r.factor;
+            s[2 * i + 1] = sn * r.factor, s[2 * i] = -s[2 * i + 1];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t e = at + i;
-            const bool second = e >= r.half;
-            c[i] = 1.0f, s[i] = 0.0f;
-            if (e < r.n_rot) {
-                turn(p * r.turns[second ? e - r.half : e], &c[i], &s[i]);
-                c[i] *= r.factor, s[i] *= second ? r.factor : -r.factor;
-            }
+            turn(p * t[i], &c[i], &s[i]);
+            c[i] *= r.factor, s[i] *= at + i < r.half ? -r.factor : r.factor;
         }
     }
 }
 
-__device__ __forceinline__ float load1(int type, const void *p, uint64_t elem) {
-    if (type == kF32) return static_cast<const float *>(p)[elem];
-    const uint32_t w = static_cast<const uint16_t *>(p)[elem];
-    return type == kF16 ? h2f(w) : __builtin_bit_cast(float, w << 16);
+// 8 values as they are in memory. W: an element's bytes.
+template <int W>
+struct Raw {
+    u32x4 v[W / 2];
+};
+template <int W>
+__device__ __forceinline__ Raw<W> raw_load(const void *p, uint64_t elem) {
+    Raw<W> r;
+    const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(p) + elem * W);
+    r.v[0] = q[0];
+    if constexpr (W == 4) r.v[1] = q[1];
+    return r;
 }
-
-// The other halves of the pairs of the row's dims from `at` on (whatever it is where there
-// is none).
-__device__ __forceinline__ void load_others(const RopeArgs &r, int type, const void *p, uint64_t row, uint32_t at,
-                                            const float (&x)[8], float (&y)[8]) {
-    if (r.layout == TC_ROPE_PAIRS) {
+template <int W>
+__device__ __forceinline__ void widen(int type, const Raw<W> &r, float (&x)[8]) {
+    if constexpr (W == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-    } else if ((r.half & 7) == 0) {
-        const uint32_t e = at < r.half ? at + r.half : at < r.n_rot ? at - r.half : at;
-        load8(type, p, row + e, y);
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_bit_cast(float, uint32_t(r.v[i / 4][i & 3]));
+    } else if (type == kF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = h2f(r.v[0][i] & 0xFFFF), x[2 * i + 1] = h2f(r.v[0][i] >> 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t e = at + i, o = e < r.half ? e + r.half : e < r.n_rot ? e - r.half : e;
-            y[i] = load1(type, p, row + o);
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __builtin_bit_cast(float, uint32_t(r.v[0][i]) << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, r.v[0][i] & 0xFFFF0000u);
         }
     }
 }
-__device__ __forceinline__ float weight_of(const RopeArgs &r, const float *w, uint32_t e) {
-    if (r.layout == TC_ROPE_PAIRS) return w[e ^ 1];
-    return w[e < r.half ? e + r.half : e < r.n_rot ? e - r.half : e];
+
+// The dim that dim e is a pair with; e itself behind the rotated ones.
+template <int L>
+__device__ __forceinline__ uint32_t other_of(const RopeArgs &r, uint32_t e) {
+    if constexpr (L == kPairs) return e ^ 1;
+    return e < r.half ? e + r.half : e < r.n_rot ? e - r.half : e;
 }
 
-// CT: the cache's type, kF32 where there is none (positions are given, all units are q's).
-template <int CT, int U>
+// A norm's weights for 8 dims from `at` on, and for those that they are pairs with.
+typedef float f32x4d __attribute__((ext_vector_type(4), aligned(4)));
+template <int L>
+__device__ __forceinline__ void load_norm(const RopeArgs &r, const float *n, uint32_t at, float (&w)[8], float (&o)[8]) {
+    auto load = [&](uint32_t from, float (&x)[8]) {
+        const f32x4d *q = reinterpret_cast<const f32x4d *>(n + from);
+        const f32x4d u = q[0], v = q[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = u[i], x[4 + i] = v[i];
+    };
+    load(at, w);
+    if constexpr (L == kPairs) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = w[i ^ 1];
+    } else if constexpr (L == kHalves8) {
+        load(other_of<L>(r, at), o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = n[other_of<L>(r, at + i)];
+    }
+}
+
+// CT: the cache's type, kF32 where there is none (positions are given, all units are q's). W:
+// bytes of the rows' elements. L: layout. U: units of a lane.
+template <int CT, int W, int L, int U>
 __global__ __launch_bounds__(kThreads) void k_rope(RopeCall a, RopeWalk w) {
     constexpr bool CACHE = CT != kF32;
     const uint32_t dim = a.kv.dim;
@@ -119,76 +155,120 @@ __global__ __launch_bounds__(kThreads) void k_rope(RopeCall a, RopeWalk w) {
     const uint32_t at = (threadIdx.x & (w.lanes - 1)) * 8;
     // lanes without work go through it all the same (the rows' lanes agree on sums and
     // maxima), on the last row, and store nothing
-    const uint32_t gc = min(g, w.total - 1), t = div_fast(gc, w.groups), u0 = (gc - t * w.groups.d) * U;
+    const uint32_t gc = min(g, w.total - 1), t = div_fast(gc, w.groups), u0 = gc - t * w.groups.d;
     const bool mine = g < w.total && at < dim;
     const uint32_t from = at < dim ? at : 0;
-    float x[U][8], y[U][8];
+    // (all loads first, and without branches between them: each would wait for the one before;
+    // what others depend on in front)
+    const uint32_t first = min(div_fast(min(blockIdx.x << (8 - w.lane_log), w.total - 1), w.groups), a.kv.n_tokens - 1);
+    SeqProbe probe;
+    if constexpr (CACHE) probe = probe_seqs(a.kv.start, a.kv.n_seq);
+    Raw<W> x_raw[U], y_raw[U];
+    uint64_t row[U];
+    const void *src[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t n = min(u0 + u, w.units - 1);
+        const uint32_t n = min(u0 + u * w.groups.d, w.units - 1);
         const bool is_q = !CACHE || n < a.q.heads, is_k = CACHE && !is_q && n - a.q.heads < a.k.heads;
         const uint32_t h = is_q ? n : is_k ? n - a.q.heads : n - a.q.heads - a.k.heads;
-        const RopeHeads &src = is_q ? a.q : is_k ? a.k : a.v;
-        const uint64_t row = uint64_t(t) * src.stride + h * dim;
-        load8(a.xtype, src.x, row + from, x[u]);
-        if (is_q || is_k) load_others(a.rope, a.xtype, src.x, row, from, x[u], y[u]);
-        if (at >= dim)  // (of a row's largest magnitude and sum of squares these lanes have nothing)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][i] = y[u][i] = 0.0f;
+        src[u] = is_q ? a.q.x : is_k ? a.k.x : a.v.x;
+        row[u] = uint64_t(t) * (is_q ? a.q.stride : is_k ? a.k.stride : a.v.stride) + h * dim;
+        x_raw[u] = raw_load<W>(src[u], row[u] + from);
+        if constexpr (L == kHalves8) y_raw[u] = raw_load<W>(src[u], row[u] + other_of<L>(a.rope, from));
     }
+    // (the heads' weights of a single unit too, which wait for nothing)
+    float nw[8], no[8];
+    bool normed = false;
+    if constexpr (CACHE && U == 1) {
+        const float *n = u0 < a.q.heads ? a.q.norm : u0 - a.q.heads < a.k.heads ? a.k.norm : nullptr;
+        normed = n != nullptr;
+        if (normed) load_norm<L>(a.rope, n, from, nw, no);
+    }
+    // (long calls have the turns on their way from here, 39 -> 35 us for 8190 rows; short ones'
+    // lookups would wait for them, 6.0 -> 6.7 for 208)
+    double turns[8];
+    if constexpr (U > 1) load_turns<L>(a.rope, from, turns);
     int32_t pos;
     int seq = 0;
     int64_t row0 = -1;  // cache row of head 0
     if constexpr (CACHE) {
-        const uint32_t first = min(div_fast(min(blockIdx.x << (8 - w.lane_log), w.total - 1), w.groups), a.kv.n_tokens - 1);
-        seq = wave_find_seq(a.kv.start, a.kv.n_seq, first);
-        const int32_t end = seq >= 0 ? a.kv.start[seq + 1] : 0;
-        if (int32_t(t) >= end) seq = find_seq(a.kv.start, a.kv.n_seq, t);
-        const uint32_t s = seq < 0 ? 0 : uint32_t(seq);
-        pos = int32_t(int64_t(a.kv.len[s]) - a.kv.start[s + 1] + t);
-        row0 = slot_of(a.kv, seq, t, 0);
+        seq = wave_find_seq(a.kv.start, a.kv.n_seq, first, probe);
+        const uint32_t s0 = seq < 0 ? 0 : uint32_t(seq);
+        int32_t end = a.kv.start[s0 + 1], len = a.kv.len[s0];
+        if (seq < 0 || int32_t(t) >= end) {
+            seq = find_seq(a.kv.start, a.kv.n_seq, t);
+            if (seq >= 0) end = a.kv.start[seq + 1], len = a.kv.len[seq];
+        }
+        const int64_t at = int64_t(len) - end + t;
+        pos = int32_t(at);
+        if (seq >= 0 && at >= 0 && at < int64_t(kMaxPos)) {
+            const uint32_t pi = div_fast(uint32_t(pos), a.kv.page_div);
+            const int32_t page = page_at(a.kv, uint32_t(seq), pi);
+            if (page >= 0) row0 = int64_t(page) * a.kv.kv_heads * a.kv.page + (uint32_t(pos) - pi * a.kv.page);
+        }
     } else {
         pos = a.position[t];
         if (pos < 0) seq = -1;
     }
+    if constexpr (U == 1) load_turns<L>(a.rope, from, turns);
     float c[8], s[8];
-    if (!CACHE || u0 < a.q.heads + a.k.heads) angles(a.rope, from, pos, c, s);
+    if (!CACHE || u0 < a.q.heads + a.k.heads) angles<L>(a.rope, from, pos, turns, c, s);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t n = u0 + u;
+        const uint32_t n = u0 + u * w.groups.d;
         const bool is_q = !CACHE || n < a.q.heads, is_k = CACHE && !is_q && n - a.q.heads < a.k.heads;
         const bool live = mine && n < w.units && seq >= 0;
+        float x[8], y[8];
+        widen<W>(a.xtype, x_raw[u], x);
+        if (at >= dim)  // (of a row's largest magnitude and sum of squares these lanes have nothing)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
         if (is_q || is_k) {
-            if constexpr (CACHE) {
-                const float *nw = is_q ? a.q.norm : a.k.norm;
-                if (nw != nullptr) {  // uniform over the row's lanes, which have the same unit
-                    float m = 0.0f;
+            if constexpr (L == kPairs) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) m = __builtin_fmaf(x[u][i], x[u][i], m);
-                    for (uint32_t o = 1; o < w.lanes; o <<= 1) m += __shfl_xor(m, int(o));
-                    const float inv = rsqrtf(m / float(dim) + a.eps);
+                for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+            } else if constexpr (L == kHalves8) {
+                widen<W>(a.xtype, y_raw[u], y);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[u][i] = x[u][i] * inv * nw[from + i];
-                        y[u][i] = y[u][i] * inv * weight_of(a.rope, nw, from + i);
+                for (int i = 0; i < 8; ++i) {
+                    const uint64_t e = row[u] + other_of<L>(a.rope, from + i);
+                    if constexpr (W == 4) {
+                        y[i] = static_cast<const float *>(src[u])[e];
+                    } else {
+                        const uint32_t bits = static_cast<const uint16_t *>(src[u])[e];
+                        y[i] = a.xtype == kF16 ? h2f(bits) : __builtin_bit_cast(float, bits << 16);
                     }
                 }
             }
-            float o[8];
+            if constexpr (CACHE) {
+                if constexpr (U > 1) {
+                    const float *n = is_q ? a.q.norm : a.k.norm;
+                    normed = n != nullptr;
+                    if (normed) load_norm<L>(a.rope, n, from, nw, no);
+                }
+                if (normed) {  // all of the row's lanes, which have the same unit
+                    float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                o[i] = at + i < a.rope.n_rot ? __builtin_fmaf(x[u][i], c[i], y[u][i] * s[i]) : x[u][i];
+                    for (int i = 0; i < 8; ++i) m = __builtin_fmaf(x[i], x[i], m);
+                    const float inv = rsqrtf(group_sum(m, w.lanes) / float(dim) + a.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][i] = o[i];
+                    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * nw[i], y[i] = y[i] * inv * no[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = at + i < a.rope.n_rot ? __builtin_fmaf(x[i], c[i], y[i] * s[i]) : x[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = y[i];
             if (is_q) {
-                if (live) store8(a.xtype, a.q_out, uint64_t(t) * a.q_out_stride + n * dim + at, x[u]);
+                if (live) store8(a.xtype, a.q_out, uint64_t(t) * a.q_out_stride + n * dim + at, x);
                 continue;
             }
         }
         if constexpr (CACHE) {
             const uint32_t h = is_k ? n - a.q.heads : n - a.q.heads - a.k.heads;
             put_row<CT>(is_k ? a.kv.k : a.kv.v, is_k ? a.kv.ks : a.kv.vs, dim,
-                        row0 < 0 ? -1 : row0 + int64_t(h) * a.kv.page, at, live, w.lanes, x[u]);
+                        row0 < 0 ? -1 : row0 + int64_t(h) * a.kv.page, at, live, w.lanes, x);
         }
     }
 }
@@ -221,17 +301,26 @@ RopeWalk make_walk(const RopeCall &c, uint32_t units, uint32_t per_lane, uint32_
     return w;
 }
 
-template <int CT>
+template <int CT, int W, int L>
 hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
     uint32_t blocks;
     RopeWalk w = make_walk(c, units, 1, &blocks);
-    if (blocks <= 4096) {
-        k_rope<CT, 1><<<blocks, kThreads, 0, st>>>(c, w);
+    if (blocks <= 1024) {
+        k_rope<CT, W, L, 1><<<blocks, kThreads, 0, st>>>(c, w);
     } else {
         w = make_walk(c, units, 4, &blocks);
-        k_rope<CT, 4><<<blocks, kThreads, 0, st>>>(c, w);
+        k_rope<CT, W, L, 4><<<blocks, kThreads, 0, st>>>(c, w);
     }
     return hipGetLastError();
+}
+template <int CT, int W>
+hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
+    if (c.rope.layout == TC_ROPE_PAIRS) return launch<CT, W, kPairs>(c, units, st);
+    return c.rope.half % 8 == 0 ? launch<CT, W, kHalves8>(c, units, st) : launch<CT, W, kHalves>(c, units, st);
+}
+template <int CT>
+hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
+    return c.xtype == kF32 ? launch<CT, 4>(c, units, st) : launch<CT, 2>(c, units, st);
 }
 
 }  // namespace
