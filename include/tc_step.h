@@ -67,7 +67,7 @@ typedef struct tc_plan {
  * positions hold no token for the other calls, and free_out[2] counts the page, as it
  * counts those past table_pages, which no entry is there for: where it is not 0 the step
  * is not to be used. Other entries of the tables and the ring stay as they are. n_seq up to
- * 2^16, n_tokens to 2^24, ring_pages and table_pages to 2^30. free_out[2] says 2^30 at most.
+ * 2^16, n_tokens to 2^24, ring_pages and the tables' entries to 2^30. free_out[2] says 2^30 at most.
  * Lengths past 2^31 - 65 are taken for that. */
 int tc_kv_plan(const tc_plan *plan, void *stream);
 

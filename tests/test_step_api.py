@@ -35,6 +35,7 @@ def plan(lib, **kw):
     (dict(page_tokens=(1 << 30) + 1), UNSUPPORTED, "2^30"),
     (dict(table_pages=(1 << 30) + 1), UNSUPPORTED, "2^30"),
     (dict(ring_pages=(1 << 30) + 1), UNSUPPORTED, "2^30"),
+    (dict(n_seq=1 << 16, table_pages=(1 << 14) + 1), UNSUPPORTED, "tables"),
     (dict(slot=P + 4), UNSUPPORTED, "aligned"),
 ] + [({n: None}, ARG, "null") for n in ("new_tokens", "held", "pages", "free", "table", "ring", "start", "len", "pages_out",
                                         "free_out")] +

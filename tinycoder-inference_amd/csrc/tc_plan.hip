@@ -1,50 +1,56 @@
 // tc_plan.hip -- the geometry of a step from its sequences' lengths.
 //
-// Two sums over the sequences in their order (rows; pages wanted, given back) decide
-// everything, so one workgroup forms them, 1024 sequences at a time, and enters the pages;
-// with it done, a row's sequence, position and slot are looked up as the other kernels do. Few rows
-// are looked up by the same workgroup: a second launch costs 4 us of a decode step's 8 to
-// 10, while one workgroup's stores reach some 60 GB/s, 16 bytes a row.
+// Sums over the sequences in their order decide everything: rows, and pages given back, then
+// pages wanted, which depend on the rows. One workgroup forms them, as many sequences at a time
+// as it has threads, and enters the pages, a thread a page whosever it is; with that done, a row's
+// sequence, position and slot are looked up as the other kernels do. Few rows are looked up by the
+// same workgroup, with the sequences' starts in LDS (1200 rows 5.4 us, 6.3 with a launch of their own;
+// from 4000 on that is the faster, one workgroup's stores reaching some 60 GB/s, 16 bytes a row).
+// Bound by the chain lengths -> sums -> ring -> table -> slots, not by any traffic.
 //
-// Sums of rows saturate at n_tokens, sums of pages at 2^30: both stay in 32 bits whatever the
-// arrays hold, and min(a + b, top) is associative for numbers that are not negative.
+// Sums of rows saturate at n_tokens, and those of missing pages at 2^30, so that they stay in 32
+// bits whatever the arrays hold; min(a + b, top) is associative for numbers that are not negative.
+// The others are at most the tables' entries, 2^30.
 #include "tc_kernels.hpp"
 #include "tc_step.hpp"
 
 namespace tc {
 namespace {
 
-constexpr uint32_t kThreads = 1024;
-constexpr uint32_t kWaves = kThreads / 64;
+// What stands N lanes to the left and the like (DPP); 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t left_lane(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 15, false));
+}
+// The wave's sums up to each lane, saturating at top. All lanes call it.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t top) {
+    v = min(v + left_lane<0x111, 15>(v), top);  // 1, 2, 4, 8 lanes to the left in rows of 16
+    v = min(v + left_lane<0x112, 15>(v), top);
+    v = min(v + left_lane<0x114, 15>(v), top);
+    v = min(v + left_lane<0x118, 15>(v), top);
+    v = min(v + left_lane<0x142, 10>(v), top);  // the last lane of rows 0 and 2 to rows 1 and 3
+    v = min(v + left_lane<0x143, 12>(v), top);  // lane 31 to rows 2 and 3
+    return v;
+}
 
-struct Totals {
-    uint32_t wave[kWaves];
+struct Sum {
+    uint32_t before, all;  // over the threads before this one, over all
 };
-
-// Sum of v over the threads before this one, and over all (in *all); saturating at `top`.
-// Every thread calls it.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t top, Totals &lds, uint32_t *all) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t sum = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t b = uint32_t(__shfl_up(int(sum), o));
-        if (lane >= uint32_t(o)) sum = min(sum + b, top);
-    }
-    __syncthreads();  // (the totals of the call before have been read)
-    if (lane == 63) lds.wave[wave] = sum;
+// Two sums over a workgroup of THREADS, the first saturating at top0, the second at top1. lds:
+// a place that no other scan uses but the one before the last. Every thread calls it.
+template <int THREADS>
+__device__ __forceinline__ void block_scan(uint32_t v0, uint32_t top0, uint32_t v1, uint32_t top1, uint32_t (&lds)[2][THREADS / 64],
+                                           Sum &s0, Sum &s1) {
+    constexpr uint32_t WAVES = THREADS / 64;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t a = wave_scan(v0, top0), b = wave_scan(v1, top1);
+    if (lane == 63) lds[0][wave] = a, lds[1][wave] = b;
     __syncthreads();
-    uint32_t w = lane < kWaves ? lds.wave[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < int(kWaves); o <<= 1) {
-        const uint32_t b = uint32_t(__shfl_up(int(w), o));
-        if (lane >= uint32_t(o)) w = min(w + b, top);
-    }
-    *all = uint32_t(__shfl(int(w), kWaves - 1));
-    uint32_t before = uint32_t(__shfl(int(w), int(wave) - 1 < 0 ? 0 : int(wave) - 1));
-    if (wave == 0) before = 0;
-    const uint32_t mine = uint32_t(__shfl_up(int(sum), 1));
-    return lane == 0 ? before : min(before + mine, top);
+    const uint32_t wa = wave_scan(lane < WAVES ? lds[0][lane] : 0, top0), wb = wave_scan(lane < WAVES ? lds[1][lane] : 0, top1);
+    const uint32_t ba = wave ? __builtin_amdgcn_readlane(wa, wave - 1) : 0, bb = wave ? __builtin_amdgcn_readlane(wb, wave - 1) : 0;
+    // (each lane's sum without its own: the lane's to the left)
+    s0 = {min(ba + uint32_t(__shfl_up(int(a), 1)) * (lane != 0), top0), uint32_t(__builtin_amdgcn_readlane(wa, WAVES - 1))};
+    s1 = {min(bb + uint32_t(__shfl_up(int(b), 1)) * (lane != 0), top1), uint32_t(__builtin_amdgcn_readlane(wb, WAVES - 1))};
 }
 
 __device__ __forceinline__ uint32_t bounded(int32_t v, uint32_t most) { return v < 0 ? 0u : min(uint32_t(v), most); }
@@ -55,85 +61,114 @@ __device__ __forceinline__ uint32_t around(uint32_t at, uint32_t by, uint32_t ri
     return i >= ring ? i % ring : i;
 }
 
-// Sequence, position and slot of a row.
-__device__ __forceinline__ void put_row_maps(const tc_plan &a, const DivMod &page, uint32_t t, int seq) {
-    int32_t pos = -1;
+// Of the first n entries of an ascending list the last that is at most v (list[0] is).
+__device__ __forceinline__ uint32_t find_last(const uint32_t *list, uint32_t n, uint32_t v) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (list[mid] <= v)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// A row's sequence (-1: none), position (below 0: none, where a length was held to the largest)
+// and slot.
+__device__ __forceinline__ void put_row_maps(const tc_plan &a, const DivMod &page, uint32_t t, int seq, int32_t pos) {
     int64_t slot = -1;
-    if (seq >= 0) {
-        pos = a.len[seq] - a.start[seq + 1] + int32_t(t);
-        // (a length that was held to the largest leaves its first rows no position)
-        if (pos >= 0) {
-            const uint32_t pi = div_fast(uint32_t(pos), page);
-            if (pi < a.table_pages) {
-                const int32_t pg = a.table[size_t(seq) * a.table_pages + pi];
-                if (pg >= 0) slot = int64_t(pg) * a.page_tokens + (uint32_t(pos) - pi * a.page_tokens);
-            }
-        } else {
-            pos = -1;
+    if (pos >= 0) {
+        const uint32_t pi = div_fast(uint32_t(pos), page);
+        if (pi < a.table_pages) {
+            const int32_t pg = a.table[size_t(seq) * a.table_pages + pi];
+            if (pg >= 0) slot = int64_t(pg) * a.page_tokens + (uint32_t(pos) - pi * a.page_tokens);
         }
+    } else {
+        pos = -1;
     }
     if (a.sequence) a.sequence[t] = seq;
     if (a.position) a.position[t] = pos;
     if (a.slot) a.slot[t] = slot;
 }
+__device__ __forceinline__ int32_t position_of(const tc_plan &a, uint32_t t, int seq) {
+    return seq < 0 ? -1 : a.len[seq] - a.start[seq + 1] + int32_t(t);
+}
 
-__global__ __launch_bounds__(kThreads) void k_plan(tc_plan a, DivMod page, uint32_t rows) {
-    __shared__ Totals lds;
-    const uint32_t S = a.n_seq, R = a.ring_pages, W = a.table_pages, lane = threadIdx.x & 63;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32_t rows) {
+    __shared__ uint32_t sums[2][2][THREADS / 64];
+    __shared__ uint32_t before[THREADS], had_of[THREADS], begins[THREADS];
+    __shared__ int32_t shift[THREADS];  // of a sequence's rows to their positions
+    const uint32_t S = a.n_seq, R = a.ring_pages, W = a.table_pages, tid = threadIdx.x;
     const uint32_t at = bounded(a.free[0], R - 1), left0 = bounded(a.free[1], R);
-    // pages of ended sequences behind the free ones
-    uint32_t back_all = 0;
-    for (uint32_t s0 = 0; s0 < S; s0 += kThreads) {
-        const uint32_t s = s0 + threadIdx.x;
-        const uint32_t back = s < S && a.new_tokens[s] < 0 ? bounded(a.pages[s], W) : 0;
-        uint32_t all;
-        const uint32_t before = min(back_all + block_scan(back, kPlanMost, lds, &all), kPlanMost);
-        back_all = min(back_all + all, kPlanMost);
-        // a wave takes its sequences one after the other, a lane a page
-        for (uint64_t m = __ballot(back != 0); m != 0; m &= m - 1) {
-            const int l = __builtin_ctzll(m);
-            const uint32_t n = __builtin_amdgcn_readlane(back, l), b = __builtin_amdgcn_readlane(before, l);
-            const uint32_t room = left0 + b < R ? R - left0 - b : 0;
-            const int32_t *row = a.table + size_t(s0 + (threadIdx.x & ~63u) + l) * W;
-            for (uint32_t j = lane; j < min(n, room); j += 64) a.ring[around(at, left0 + b + j, R)] = row[j];
+    int turn = 0;
+    // pages of ended sequences behind the free ones, and where there is one lot of sequences only, their rows
+    uint32_t back_all = 0, row_all = 0;
+    Sum rows_of{0, 0}, back_of, none;
+    int32_t fresh = -1;
+    uint32_t held = 0, had = 0;
+    auto fetch = [&](uint32_t s) {
+        fresh = s < S ? a.new_tokens[s] : -1;
+        held = s < S ? bounded(a.held[s], kLenMost) : 0;
+        had = s < S ? bounded(a.pages[s], W) : 0;
+    };
+    for (uint32_t s0 = 0; s0 < S; s0 += THREADS) {
+        fetch(s0 + tid);
+        const uint32_t back = fresh < 0 ? had : 0;
+        block_scan<THREADS>(back, kPlanMost, bounded(fresh, a.n_tokens), a.n_tokens, sums[turn ^= 1], back_of, rows_of);
+        if (back_of.all != 0) {  // a thread a page
+            before[tid] = back_of.before;
+            __syncthreads();
+            const uint32_t room = left0 + back_all < R ? R - left0 - back_all : 0;
+            for (uint32_t j = tid; j < min(back_of.all, room); j += THREADS) {
+                const uint32_t i = find_last(before, THREADS, j);
+                a.ring[around(at, left0 + back_all + j, R)] = a.table[size_t(s0 + i) * W + (j - before[i])];
+            }
+            __threadfence_block();
+            __syncthreads();
         }
+        back_all += back_of.all;
     }
     const uint32_t left = min(left0 + back_all, R);
-    __threadfence_block();
-    __syncthreads();
-    uint32_t row_all = 0, want_all = 0, short_all = 0;
-    for (uint32_t s0 = 0; s0 < S; s0 += kThreads) {
-        const uint32_t s = s0 + threadIdx.x;
-        const int32_t fresh = s < S ? a.new_tokens[s] : -1;
-        const uint32_t held = s < S ? bounded(a.held[s], kLenMost) : 0, had = s < S ? bounded(a.pages[s], W) : 0;
-        uint32_t all;
-        const uint32_t n = bounded(fresh, a.n_tokens);
-        const uint32_t begin = min(row_all + block_scan(n, a.n_tokens, lds, &all), a.n_tokens);
-        row_all = min(row_all + all, a.n_tokens);
-        const uint32_t got_rows = min(n, a.n_tokens - begin);
+    uint32_t want_all = 0, short_all = 0;
+    for (uint32_t s0 = 0; s0 < S; s0 += THREADS) {
+        const uint32_t s = s0 + tid;
+        if (S > THREADS) {
+            fetch(s);
+            block_scan<THREADS>(bounded(fresh, a.n_tokens), a.n_tokens, 0, 0, sums[turn ^= 1], rows_of, none);
+        }
+        const uint32_t begin = min(row_all + rows_of.before, a.n_tokens);
+        row_all = min(row_all + rows_of.all, a.n_tokens);
+        const uint32_t got_rows = min(bounded(fresh, a.n_tokens), a.n_tokens - begin);
         const uint32_t len = fresh < 0 ? 0 : min(held + got_rows, uint32_t(kLenMost));
         uint32_t need = div_fast(len, page);
         if (need * a.page_tokens < len) ++need;
         const uint32_t fit = min(need, W), want = fresh >= 0 && fit > had ? fit - had : 0;
-        const uint32_t before = min(want_all + block_scan(want, kPlanMost, lds, &all), kPlanMost);
-        want_all = min(want_all + all, kPlanMost);
-        block_scan(need - fit, kPlanMost, lds, &all);
-        short_all = min(short_all + all, kPlanMost);
-        // the first page by the sequence's own lane, more of them by its wave
-        if (want != 0) a.table[size_t(s) * W + had] = before < left ? a.ring[around(at, before, R)] : -1;
-        for (uint64_t m = __ballot(want > 1); m != 0; m &= m - 1) {
-            const int l = __builtin_ctzll(m);
-            const uint32_t k = __builtin_amdgcn_readlane(want, l), b = __builtin_amdgcn_readlane(before, l);
-            int32_t *row = a.table + size_t(s0 + (threadIdx.x & ~63u) + l) * W + __builtin_amdgcn_readlane(had, l);
-            for (uint32_t j = 1 + lane; j < k; j += 64) row[j] = b + j < left ? a.ring[around(at, b + j, R)] : -1;
-        }
+        Sum want_of, short_of;
+        block_scan<THREADS>(want, kPlanMost, need - fit, kPlanMost, sums[turn ^= 1], want_of, short_of);
         if (s < S) {
+            const uint32_t from = want_all + want_of.before;
             a.start[s] = int32_t(begin);
             a.len[s] = int32_t(len);
-            a.pages_out[s] = fresh < 0 ? 0 : int32_t(had + (before < left ? min(want, left - before) : 0));
+            a.pages_out[s] = fresh < 0 ? 0 : int32_t(had + (from < left ? min(want, left - from) : 0));
         }
+        begins[tid] = begin;
+        shift[tid] = int32_t(len) - int32_t(begin + got_rows);
+        if (want_of.all != 0) {  // a thread a page
+            before[tid] = want_of.before;
+            had_of[tid] = had;
+            __syncthreads();
+            for (uint32_t j = tid; j < want_of.all; j += THREADS) {
+                const uint32_t i = find_last(before, THREADS, j), k = want_all + j;
+                a.table[size_t(s0 + i) * W + had_of[i] + (j - before[i])] = k < left ? a.ring[around(at, k, R)] : -1;
+            }
+            __syncthreads();
+        }
+        want_all += want_of.all;
+        short_all = min(short_all + short_of.all, kPlanMost);
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         const uint32_t taken = min(want_all, left);
         a.start[S] = int32_t(row_all);
         a.free_out[0] = int32_t(around(at, taken, R));
@@ -143,7 +178,15 @@ __global__ __launch_bounds__(kThreads) void k_plan(tc_plan a, DivMod page, uint3
     if (rows == 0) return;
     __threadfence_block();
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < rows; t += kThreads) put_row_maps(a, page, t, find_seq(a.start, S, t));
+    for (uint32_t t = tid; t < rows; t += THREADS) {
+        int seq = -1;
+        int32_t pos = -1;
+        if (t < row_all) {
+            seq = S > THREADS ? find_seq(a.start, S, t) : int(find_last(begins, S, t));
+            pos = S > THREADS ? position_of(a, t, seq) : shift[seq] + int32_t(t);
+        }
+        put_row_maps(a, page, t, seq, pos);
+    }
 }
 
 __global__ __launch_bounds__(256) void k_plan_rows(tc_plan a, DivMod page) {
@@ -152,7 +195,7 @@ __global__ __launch_bounds__(256) void k_plan_rows(tc_plan a, DivMod page) {
     const int32_t end = seq >= 0 ? a.start[seq + 1] : 0;
     if (t >= a.n_tokens) return;
     if (int32_t(t) >= end) seq = find_seq(a.start, a.n_seq, t);
-    put_row_maps(a, page, t, seq);
+    put_row_maps(a, page, t, seq, position_of(a, t, seq));
 }
 
 constexpr uint32_t kRowsHere = 4096;
@@ -163,7 +206,13 @@ hipError_t launch_plan(const tc_plan &p, hipStream_t st) {
     const DivMod page = make_divmod(p.page_tokens);
     const bool maps = p.sequence || p.position || p.slot;
     const bool here = maps && p.n_tokens <= kRowsHere;
-    k_plan<<<1, kThreads, 0, st>>>(p, page, here ? p.n_tokens : 0);
+    const uint32_t rows = here ? p.n_tokens : 0;
+    // (barriers of 4 waves cost less than those of 16, 64 sequences 4.6 us and 5.3; many rows and pages
+    // want the threads, 9000 rows 8.5 and 7.2)
+    if (p.n_seq <= 256 && (here ? rows <= 1024 : p.n_tokens <= 8192))
+        k_plan<256><<<1, 256, 0, st>>>(p, page, rows);
+    else
+        k_plan<1024><<<1, 1024, 0, st>>>(p, page, rows);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !maps || here) return e;
     k_plan_rows<<<(p.n_tokens + 255) / 256, 256, 0, st>>>(p, page);

@@ -57,6 +57,7 @@ int tc_kv_plan(const tc_plan *p, void *stream) {
     if (p->n_seq > (1u << 16) || p->n_tokens > (1u << 24)) return refuse(TC_E_UNSUPPORTED, "more than 2^16 sequences or 2^24 rows");
     if (p->page_tokens > (1u << 30) || p->table_pages > (1u << 30) || p->ring_pages > (1u << 30))
         return refuse(TC_E_UNSUPPORTED, "more than 2^30 tokens in a page, pages in a table or in the ring");
+    if (uint64_t(p->n_seq) * p->table_pages > (1u << 30)) return refuse(TC_E_UNSUPPORTED, "more than 2^30 pages in the tables");
     // (arrays without an entry may have no address)
     if (!p->free || !p->free_out || !p->start || !p->ring) return refuse(TC_E_ARG, "null pointer");
     if (p->n_seq != 0 && (!p->new_tokens || !p->held || !p->pages || !p->table || !p->len || !p->pages_out))
