@@ -415,7 +415,9 @@ class Library:
         self.path = path
         import torch
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self._current_device = torch.cuda.current_device
+        # (torch.cuda's own look at whether it is initialised takes longer than the rest of it)
+        quick = getattr(torch._C, "_cuda_getDevice", None)
+        self._current_device = quick if quick is not None and torch.cuda.is_initialized() else torch.cuda.current_device
 
     # -- helpers ---------------------------------------------------------------
     def _stream(self, device=None):
@@ -686,26 +688,37 @@ class Library:
         return plan
 
     # (as above, a small call's host time is its whole time: its struct is packed, not built field by field, and
-    # outputs are made like a tensor that is there: norm_add 9.8 -> 6.9 us, rope_kv_write 15.3 -> 11.6, of which 3.5 are
-    # its caller's three slices)
+    # outputs are made like a tensor that is there)
+    @staticmethod
+    def _stride_of(t, T, width):
+        """Elements between the rows of t [T][...], each of `width` values next to each other."""
+        st, at = t.stride(), 1
+        for n, s in zip(t.shape[:0:-1], st[:0:-1]):
+            if n != 1 and s != at and T != 0:
+                raise TCError(TC_E_ARG, "a row's values are not next to each other")
+            at *= n
+        return _u32(st[0], "row stride") if T > 1 else width
+
     def _norm_rows(self, h, y, h_out, x, pre, post, gate, sigmoid, scale, act_type, act):
-        shape, dev, types = h.shape, self._current_device(), _elem_types()
+        shape, dev, types = h.shape, self._current_device(), _ELEM_TYPES or _elem_types()
         if len(shape) != 2:
             raise TCError(TC_E_ARG, "h is [rows][cols]")
         T, D = shape
-        given = [0] * 12  # addresses, types and strides of h, y, h_out, x
-        for i, t in enumerate((h, y, h_out, x)):
-            if t is None:
-                continue
-            stride = t.stride()
-            if t.shape != shape or (stride[1] != 1 and T != 0 and D > 1) or t.get_device() != dev:
-                raise TCError(TC_E_ARG, "rows are [rows][cols], a row's values next to each other, on the current device")
-            given[i], given[4 + i] = t.data_ptr(), types.get(t.dtype, -1)
-            given[8 + i] = D if T <= 1 else stride[0]
-            if not 0 <= given[8 + i] <= 0xFFFFFFFF:
-                raise TCError(TC_E_ARG, f"row stride={given[8 + i]} is not a number of 32 bits")
-        if h_out is not None and given[6] != given[4]:
-            raise TCError(TC_E_ARG, "h_out is not of h's type")
+        ph = py = po = px = hs = ys = os_ = xs = et_y = et_x = 0
+        et_h = types.get(h.dtype, -1)
+        ph, hs = h.data_ptr(), D if h.is_contiguous() else self._stride_of(h, T, D)
+        good = h.get_device() == dev
+        if y is not None:
+            py, ys, et_y = y.data_ptr(), D if y.is_contiguous() else self._stride_of(y, T, D), types.get(y.dtype, -1)
+            good = good and y.shape == shape and y.get_device() == dev
+        if h_out is not None:
+            po, os_ = h_out.data_ptr(), D if h_out.is_contiguous() else self._stride_of(h_out, T, D)
+            good = good and h_out.shape == shape and h_out.dtype == h.dtype and h_out.get_device() == dev
+        if x is not None:
+            px, xs, et_x = x.data_ptr(), D if x.is_contiguous() else self._stride_of(x, T, D), types.get(x.dtype, -1)
+            good = good and x.shape == shape and x.get_device() == dev
+        if not good:
+            raise TCError(TC_E_ARG, "rows are [rows][cols] on the current device, h_out of h's type")
         for n in (pre, post):
             if n is not None and n.cols is not None and (n.cols != D or n.device != dev):
                 raise TCError(TC_E_ARG, "a norm's weights are not the rows' or not on the current device")
@@ -724,10 +737,10 @@ class Library:
         if act is not None and (not act.is_contiguous() or act.get_device() != dev or
                                 act.numel() * act.element_size() < self.lib.tc_act_bytes(act_type, T, D)):
             raise TCError(TC_E_ARG, "act is too small, not contiguous or not on the current device")
-        p, e, st = given[:4], given[4:8], given[8:]
-        c = _PACK_NORM_ROWS(T, D, *p, e[0], e[1], e[3], *st, 0 if post is None else post.ref, 0 if pre is None else pre.ref,
-                            0 if gate is None else gate.data_ptr(), kind, 0 if gate is None else types.get(gate.dtype, -1),
-                            1 if sigmoid else 0, scale, act_type, 0 if act is None else act.data_ptr())
+        c = _PACK_NORM_ROWS(T, D, ph, py, po, px, et_h, et_y, et_x, hs, ys, os_, xs, 0 if post is None else post.ref,
+                            0 if pre is None else pre.ref, 0 if gate is None else gate.data_ptr(), kind,
+                            0 if gate is None else types.get(gate.dtype, -1), 1 if sigmoid else 0, scale,
+                            act_type, 0 if act is None else act.data_ptr())
         self._check(self.lib.tc_norm_add(c, self._stream(dev)))
 
     def norm(self, h, pre, out_dtype=None, out=None):
@@ -778,38 +791,32 @@ class Library:
         and values as they are into their slots of the cache (tc_rope_kv_write). q_norm, k_norm:
         fp32 weights [head_dim] of an RMS norm of the heads before. q may be None."""
         import torch
-        shape, kv, D, dev = k.shape, cache.kv_heads, cache.head_dim, torch.cuda.current_device()
+        shape, kv, D, dev = k.shape, cache.kv_heads, cache.head_dim, self._current_device()
         if len(shape) != 3 or shape[1] != kv or shape[2] != D or v.shape != shape or v.dtype != k.dtype:
             raise TCError(TC_E_ARG, "k and v are not [n_tokens][kv_heads][head_dim] of the cache, of one type")
-        T, heads, rows = shape[0], 0, [(k, kv), (v, kv)]
+        T, heads, pq, qs, po = shape[0], 0, None, 0, None
+        ks = kv * D if k.is_contiguous() else self._stride_of(k, T, kv * D)
+        vs = kv * D if v.is_contiguous() else self._stride_of(v, T, kv * D)
+        if not k.get_device() == v.get_device() == dev:
+            raise TCError(TC_E_ARG, "tensors are not on the current device")
         if q is not None:
             if out is None:
                 out = torch.empty_like(q, memory_format=torch.contiguous_format)
             shape = q.shape
             if len(shape) != 3 or shape[0] != T or shape[2] != D or q.dtype != k.dtype or out.shape != shape or \
-                    out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != dev:
+                    out.dtype != q.dtype or not out.is_contiguous() or not q.get_device() == out.get_device() == dev:
                 raise TCError(TC_E_ARG, "q is not [n_tokens][heads][head_dim] of k's type, or out not that, contiguous")
             heads = shape[1]
-            rows.append((q, heads))
+            pq, po, qs = q.data_ptr(), out.data_ptr(), heads * D if q.is_contiguous() else self._stride_of(q, T, heads * D)
         elif out is not None:
             raise TCError(TC_E_ARG, "out without q")
-        for i, (t, n) in enumerate(rows):
-            st = t.stride()
-            if T != 0 and (st[2] != 1 or (n != 1 and st[1] != D)):
-                raise TCError(TC_E_ARG, "a row's heads are not contiguous")
-            if t.get_device() != dev:
-                raise TCError(TC_E_ARG, "tensors are not on the current device")
-            rows[i] = n * D if T <= 1 else st[0]
-            if not 0 <= rows[i] <= 0xFFFFFFFF:
-                raise TCError(TC_E_ARG, f"row stride={rows[i]} is not a number of 32 bits")
         if not cache.device == batch.device == rope.device == dev:
             raise TCError(TC_E_ARG, "cache, batch or rope are not on the current device")
         for w in (q_norm, k_norm):
             if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or w.stride(0) != 1 or w.get_device() != dev):
                 raise TCError(TC_E_ARG, "norms of heads are fp32 [head_dim] on the current device")
         self._check(self.lib.tc_rope_kv_write(
-            cache.ref, batch.of(T), rope.ref, _elem_type(k.dtype), None if q is None else q.data_ptr(), 0 if q is None else rows[2],
-            None if q is None else out.data_ptr(), heads, k.data_ptr(), rows[0], v.data_ptr(), rows[1],
+            cache.ref, batch.of(T), rope.ref, _elem_type(k.dtype), pq, qs, po, heads, k.data_ptr(), ks, v.data_ptr(), vs,
             None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps, self._stream(dev)))
         return out
 
@@ -818,7 +825,7 @@ class Library:
         int32 [n_seq + 1]: fp32 [n_tokens][vocab] in out (which may be logits). tokens int32
         [n_tokens]: the step's tokens, counted behind the history up to each row's own."""
         import torch
-        shape, dev = logits.shape, torch.cuda.current_device()
+        shape, dev = logits.shape, self._current_device()
         if out is None:
             out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
         st, to = logits.stride(), out.stride()
