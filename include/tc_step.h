@@ -39,8 +39,8 @@ extern "C" {
  * (more than its tokens need, where drafted tokens were not taken), and brings
  * new_tokens[s] more; below 0: it has ended. Pages not in use stand in a ring of
  * ring_pages entries: free[1] of them from ring[free[0]] on, going round. Lengths are
- * taken for at least 0, and free[1] and pages[s] for at most what the ring and the table
- * have room for. */
+ * taken for at least 0, free[0] for a place of the ring, and free[1] and pages[s] for at most
+ * what the ring and the table have room for. */
 typedef struct tc_plan {
     uint32_t n_seq, n_tokens;         /* n_tokens: rows of the step, those behind the last sequence's too */
     uint32_t page_tokens, table_pages, ring_pages;
@@ -110,7 +110,7 @@ typedef struct tc_norm_rows {
  * the norm of h + scale * gate * post(y) before that is rounded to h's type; act is formed
  * from the fp32 values that an F32 x has, and is tc_act_quantize's of them bit for bit.
  * cols up to 32768. Rows may have any stride that keeps them apart and any
- * alignment that fits their elements (with act: 16 bytes). Outputs do not overlap inputs, apart from h_out = h with the same stride. An
+ * alignment that fits their elements. Outputs do not overlap inputs, apart from h_out = h with the same stride. An
  * infinity or NaN stays in its row; squares that pass fp32's range (values past 10^19) give
  * an infinite mean. */
 int tc_norm_add(const tc_norm_rows *rows, void *stream);
@@ -122,8 +122,8 @@ enum { TC_ROPE_HALF = 0, TC_ROPE_PAIRS = 1 };
 
 /* Pair i of a row at position p is turned by a = 2 pi * p * turns[i]: (u, v) ->
  * factor * (u cos a - v sin a, u sin a + v cos a). The dims behind n_rot stay as they
- * are. Angles are formed in fp64 and reduced there, so that a position of any size is as
- * exact as a near one; cos and sin are off by 2^-23 at most, before the factor. */
+ * are. Angles are formed in fp64 and reduced there: cos and sin are off by 2^-23 at most, before
+ * the factor, at positions up to 2^26 (by 2^-20 at 2^31). */
 typedef struct tc_rope {
     uint32_t n_rot;       /* even, up to the head's size */
     int32_t layout;
@@ -165,7 +165,8 @@ int tc_rope_apply(const tc_rope *rope, int xtype, const void *x, uint32_t x_stri
  * ([n_tokens][heads][head_dim] contiguous, of `xtype`; may be q where q is contiguous); the
  * keys' heads likewise with k_norm, and written to their slots of the cache, as tc_kv_write
  * writes k; the values are written as tc_kv_write writes v. Between loading and the one
- * rounding at the end values are fp32. Rows are laid out as tc_kv_write's k and v, and q
+ * rounding at the end values are fp32 (a norm's squares too: heads with values past 10^18 get an infinite
+ * mean). Rows are laid out as tc_kv_write's k and v, and q
  * as tc_attn's; parts of one fused product's rows are fine. q may be NULL (heads 0): keys and
  * values only. Rows past the last sequence are not touched; q_out is written also for rows
  * whose position has no slot. heads up to 4096. eps: finite, at least 0. */

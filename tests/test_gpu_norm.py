@@ -159,6 +159,20 @@ def test_quantized_activations(tc, dev, qtype, T, D):
         assert torch.equal(out, tc.gemv(qtype, w, x, 40, D))
 
 
+def test_quantized_activations_alone(tc, dev):
+    """act without x and h_out, from rows at any alignment and stride."""
+    rng = np.random.default_rng(1)
+    wide = rows(rng, 3, 1300, "BF16", dev)
+    h, y = wide[:, 1:1025], rows(rng, 3, 1024, "F32", dev)
+    pre, _ = weights(rng, 1024, dev, "rms")
+    size = tc.lib.tc_act_bytes(Q4_K, 3, 1024)
+    act, other = (torch.zeros(size, dtype=torch.uint8, device=dev) for _ in range(2))
+    x = tc.norm_add(h, y, pre=pre, out_dtype=torch.float32)[1]
+    tc._norm_rows(h, y, None, None, pre, None, None, False, 1.0, Q4_K, act)
+    tc._check(tc.lib.tc_act_quantize(Q4_K, tc_hip._ptr(x), 3, 1024, tc_hip._ptr(other), tc._stream()))
+    assert torch.equal(act, other) and act.any()
+
+
 def test_binding_refusals(tc, dev):
     h = torch.zeros(4, 4, device=dev)
     n = tc_hip.Norm(torch.ones(4, device=dev))

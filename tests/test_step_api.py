@@ -102,9 +102,6 @@ NAN, INF = float("nan"), float("inf")
     (dict(act=P, act_type=17, cols=256, h_stride=256, y_stride=256, h_out_stride=256, x_stride=256), UNSUPPORTED, "type 17"),
     (dict(act=P, act_type=12, cols=12544, n_rows=1), UNSUPPORTED, "cols=12544"),
     (dict(act=P + 128, act_type=12, cols=256, n_rows=1), ARG, "256-byte"),
-    (dict(act=P, act_type=12, cols=256, n_rows=1, h=P + 8), UNSUPPORTED, "16-byte"),
-    (dict(act=P, act_type=12, cols=256, n_rows=1, pre=c_norm(weight=P + 4)), UNSUPPORTED, "16-byte"),
-    (dict(act=P, act_type=12, cols=256, h_stride=260, y_stride=256, h_out=None, x=None), UNSUPPORTED, "16-byte"),
 ])
 def test_norm_refusals(lib, kw, code, word):
     assert norm(lib, **kw) == code
@@ -257,6 +254,8 @@ def test_norm_and_rope_class_refusals():
                 dict(n_rot=8, divisors=torch.zeros(4).half()), dict(n_rot=8, divisors=torch.zeros(3))):
         with pytest.raises(tc_hip.TCError):
             tc_hip.Rope(device="cpu", **bad)
+    with pytest.raises(tc_hip.TCError, match="GPU"):
+        tc_hip.Rope(8, device="cpu")
 
 
 def test_rules_class_refusals():

@@ -105,14 +105,6 @@ int tc_norm_add(const tc_norm_rows *r, void *stream) {
         if (r->cols % 256 || r->cols > 12288)
             return refuse(TC_E_UNSUPPORTED, "quantized activations of cols=" + std::to_string(r->cols));
         if (!aligned_to(r->act, 256)) return refuse(TC_E_ARG, "act must be 256-byte aligned");
-        if (!aligned_to(r->h, 16) || (r->y && !aligned_to(r->y, 16)) || (r->n_rows > 1 && (r->h_stride % 8 || (r->y && r->y_stride % 8))) ||
-            (r->y && r->h_out && (!aligned_to(r->h_out, 16) || (r->n_rows > 1 && r->h_out_stride % 8))) ||
-            (r->x && (!aligned_to(r->x, 16) || (r->n_rows > 1 && r->x_stride % 8))) ||
-            ((r->gate_kind == TC_GATE_CHANNEL || r->gate_kind == TC_GATE_FULL) && !aligned_to(r->gate, 16)))
-            return refuse(TC_E_UNSUPPORTED, "quantized activations go with 16-byte aligned rows");
-        for (const tc::NormArgs *n : {&c.post, &c.pre})
-            if (!aligned_to(n->weight, 16) || !aligned_to(n->bias, 16))
-                return refuse(TC_E_UNSUPPORTED, "quantized activations go with 16-byte aligned weights");
         const tc::ActLayout L = tc::act_layout(r->act_type, r->n_rows, r->cols);
         char *const base = static_cast<char *>(r->act);
         c.qs = reinterpret_cast<int8_t *>(base + L.qs_off);

@@ -294,15 +294,15 @@ class KVPlan:
         _need(free.numel() == 3 or (free.numel() == 2 and not in_place), "free has 2 entries, or 3")
         self.new, self.held, self.pages, self.table, self.ring, self.free = given
 
-        def made(n, dtype=torch.int32):
-            return torch.zeros(n, dtype=dtype, device=new.device)
-
-        self.start, self.length, self.pages_out = made(n + 1), held if in_place else made(n), pages if in_place else made(n)
-        self.free_out = free if in_place else made(3)
-        self.sequence, self.position, self.slot = made(n_tokens), made(n_tokens), made(n_tokens, torch.int64)
+        _u32(n_tokens, "n_tokens")
+        self.slot = torch.zeros(n_tokens, dtype=torch.int64, device=new.device)
+        sizes = [n + 1, n_tokens, n_tokens] + ([] if in_place else [n, n, 3])
+        made = torch.zeros(sum(sizes), dtype=torch.int32, device=new.device).split(sizes)
+        self.start, self.sequence, self.position = made[:3]
+        self.length, self.pages_out, self.free_out = (held, pages, free) if in_place else made[3:]
         self.n_tokens, self.page_tokens = n_tokens, page_tokens
         self.batch = KVBatch(self.start, self.length, table)
-        self.c = _CPlan(n, _u32(n_tokens, "n_tokens"), _u32(page_tokens, "page_tokens"), table.shape[1], ring.numel(),
+        self.c = _CPlan(n, n_tokens, _u32(page_tokens, "page_tokens"), table.shape[1], ring.numel(),
                         *[t.data_ptr() for t in (new, held, pages, free, table, ring, self.start, self.length, self.pages_out,
                                                  self.free_out, self.sequence, self.position, self.slot)])
         self.ref = ctypes.byref(self.c)
@@ -345,12 +345,13 @@ class Rope:
         _need(layout in ROPE_LAYOUTS, f"a layout is one of {sorted(ROPE_LAYOUTS)}")
         _need(scaling in ROPE_SCALINGS, f"a scaling is one of {sorted(ROPE_SCALINGS)}")
         _need(n_rot > 0 and n_rot % 2 == 0, "n_rot is even")
+        _need(divisors is None or (divisors.dtype == torch.float32 and divisors.is_contiguous() and divisors.numel() == n_rot // 2),
+              "divisors are contiguous fp32 [n_rot / 2]")
+        _need(torch.device(device).type == "cuda", "a rope's table is on a GPU")
         lib = load_library()
         self.n_rot, self.layout = n_rot, layout
         self.turns = torch.empty(n_rot // 2, dtype=torch.float64, device=device)
-        _need(divisors is None or (divisors.dtype == torch.float32 and divisors.is_contiguous() and
-                                   divisors.numel() == n_rot // 2 and divisors.device == self.turns.device),
-              "divisors are contiguous fp32 [n_rot / 2] on the rope's device")
+        _need(divisors is None or divisors.device == self.turns.device, "divisors are on the rope's device")
         self.divisors = divisors
         self.device = self.turns.get_device()
         f = ctypes.c_float()
@@ -358,8 +359,11 @@ class Rope:
         with torch.cuda.device(self.device):
             rc = lib.tc_rope_turns(ctypes.byref(c), n_rot, theta, self.turns.data_ptr(), ctypes.byref(f),
                                    torch.cuda.current_stream().cuda_stream)
-        if rc != TC_OK:
-            raise TCError(rc, lib.tc_last_error().decode())
+            if rc != TC_OK:
+                raise TCError(rc, lib.tc_last_error().decode())
+            # (made once, used on any stream: the table is there when this returns)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         self.c = _CRope(n_rot, ROPE_LAYOUTS[layout], self.turns.data_ptr(), f.value if factor_of_values is None else factor_of_values)
         self.ref = ctypes.byref(self.c)
 
