@@ -128,7 +128,8 @@ def test_step_against_64_bits(tc, dev):
                 of = lambda q: None if q is None else (f64(q.weight), None, EPS, "rms", 0.0)  # noqa: E731
                 e = norm_add_exact(f64(h), None if y is None else f64(y), of(pre), of(post), None, False, 0.5 if post else 1.0)
                 for got, w, err in ((h2, e[0], e[1]), (x, e[2], e[3])):
-                    assert got is None or (np.abs(f64(got) - w) <= err + U * (np.abs(w) + err)).all()
+                    # (rows past the last sequence hold whatever the memory of attention's output did)
+                    assert got is None or (np.abs(f64(got) - w) <= err + U * (np.abs(w) + err))[:T].all()
             elif kind == "rope":
                 i, q, k, r = a
                 e, err = rope_exact(f64(q)[:T], pos, turns, D, "half", 1.0, f64(m.blocks[i]["qn"].weight), EPS)
