@@ -131,6 +131,26 @@ def test_extreme_rows(tc, dev):
             assert torch.isfinite(h2[0]).sum() == D - 1 and torch.isfinite(h2[1]).sum() == D - 1
 
 
+@pytest.mark.parametrize("cols", [5, 41, 300, 1001, 17407])
+def test_infinite_gates(tc, dev, cols):
+    """A gate's infinity is its own value's: the rest of the row is what it was, and the norm of it 0 (over an infinite mean)."""
+    rng = np.random.default_rng(cols)
+    h, y = rows(rng, 3, cols, "F32", dev), rows(rng, 3, cols, "F32", dev)
+    gate = rows(rng, 3, cols, "F32", dev)
+    want = h + gate * y
+    for at in (cols - 1, cols // 2):
+        g = gate.clone()
+        g[1, at] = float("inf")
+        h2, x = tc.norm_add(h, y, pre=tc_hip.Norm(), gate=g)
+        assert torch.isinf(h2[1, at]) and torch.isnan(x[1, at])
+        keep = torch.ones(cols, dtype=torch.bool, device=dev)
+        keep[at] = False
+        assert (x[1, keep] == 0).all()
+        # (one rounding apart: the kernel's product and sum are one operation)
+        assert ((h2 - want)[:, keep].abs() <= 2.0 ** -23 * (h.abs() + (gate * y).abs())[:, keep]).all()
+        assert torch.isfinite(x[0]).all() and torch.isfinite(x[2]).all()
+
+
 @pytest.mark.parametrize("qtype", [Q4_K, Q6_K, Q8_0])
 @pytest.mark.parametrize("T,D", [(1, 256), (1, 3584), (3, 512), (8, 5120), (5, 12288)])
 def test_quantized_activations(tc, dev, qtype, T, D):

@@ -213,66 +213,79 @@ __global__ __launch_bounds__(MOST) void k_norm(NormCall a) {
         at[c].at = TINY ? 0 : min(from, cols - 8);
         at[c].off = TINY ? (lane ? 8 : 0) : min(from - at[c].at, 8u);
     }
-    Raw y_raw[C], h_raw[C], g_raw[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        if constexpr (YW != 0) y_raw[c] = raw_load<YW, TINY>(a.y, r * a.y_stride, at[c], cols);
-        h_raw[c] = raw_load<HW, TINY>(a.h, r * a.h_stride, at[c], cols);
-    }
+    // What a block needs of h, of the gate and (where no norm comes first) of y. Long rows have two
+    // blocks' on their way at a time, so that a CU has room for two rows (17407 columns 61 -> 56
+    // us), others all of them.
+    constexpr bool WHOLE = C <= 2;
+    constexpr int SLOTS = WHOLE ? C : 2;
+    Raw y_raw[POST ? C : SLOTS], h_raw[SLOTS], g_raw[SLOTS];
     const bool gated = YW != 0 && (a.gate_kind == TC_GATE_CHANNEL || a.gate_kind == TC_GATE_FULL);
-    if (gated) {
-        const uint64_t base = a.gate_kind == TC_GATE_FULL ? uint64_t(r) * cols : 0;
-        if (a.gate_type == kF32) {
+    const uint64_t gate_row = a.gate_kind == TC_GATE_FULL ? uint64_t(r) * cols : 0;
+    auto fetch = [&](int c) {
+        if constexpr (YW != 0 && !POST) y_raw[c % SLOTS] = raw_load<YW, TINY>(a.y, r * a.y_stride, at[c], cols);
+        h_raw[c % SLOTS] = raw_load<HW, TINY>(a.h, r * a.h_stride, at[c], cols);
+        if (gated)
+            g_raw[c % SLOTS] = a.gate_type == kF32 ? raw_load<4, TINY>(a.gate, gate_row, at[c], cols) : raw_load<2, TINY>(a.gate, gate_row, at[c], cols);
+    };
+    if constexpr (POST)
 #pragma unroll
-            for (int c = 0; c < C; ++c) g_raw[c] = raw_load<4, TINY>(a.gate, base, at[c], cols);
-        } else {
+        for (int c = 0; c < C; ++c) y_raw[c] = raw_load<YW, TINY>(a.y, r * a.y_stride, at[c], cols);
+    uint32_t row_gate = 0;
+    if (YW != 0 && a.gate_kind == TC_GATE_ROW)
+        row_gate = a.gate_type == kF32 ? static_cast<const uint32_t *>(a.gate)[r] : static_cast<const uint16_t *>(a.gate)[r];
 #pragma unroll
-            for (int c = 0; c < C; ++c) g_raw[c] = raw_load<2, TINY>(a.gate, base, at[c], cols);
-        }
-    } else if (YW != 0 && a.gate_kind == TC_GATE_ROW) {  // (one value: the first of a Raw)
-        if (a.gate_type == kF32)
-            g_raw[0].a[0] = static_cast<const uint32_t *>(a.gate)[r];
-        else
-            g_raw[0].a[0] = static_cast<const uint16_t *>(a.gate)[r];
-    }
-    float h[C][8];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        widen<HW>(a.h_type, h_raw[c], h[c]);
-        own_only<TINY>(at[c], cols, h[c]);
-    }
-    if constexpr (YW != 0) {
-        float y[C][8];
+    for (int c = 0; c < (WHOLE ? C : 1); ++c) fetch(c);
+    float h[C][8], y[POST || WHOLE ? C : 1][8];
+    if constexpr (POST) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             widen<YW>(a.y_type, y_raw[c], y[c]);
             own_only<TINY>(at[c], cols, y[c]);
         }
-        if constexpr (POST) {
-            if (a.post.kind >= 0) norm_row<LANES, C, TINY>(a, a.post, at, lds, y);
+        if (a.post.kind >= 0) norm_row<LANES, C, TINY>(a, a.post, at, lds, y);
+    }
+    auto open = [&](int c) {
+        widen<HW>(a.h_type, h_raw[c % SLOTS], h[c]);
+        own_only<TINY>(at[c], cols, h[c]);
+        if constexpr (YW != 0 && !POST) {
+            float(&v)[8] = y[WHOLE ? c : 0];
+            widen<YW>(a.y_type, y_raw[c % SLOTS], v);
+            own_only<TINY>(at[c], cols, v);
         }
-        float f = a.scale;
-        if (a.gate_kind == TC_GATE_ROW) {
-            const uint32_t bits = g_raw[0].a[0];
-            const float v = a.gate_type == kF32 ? __builtin_bit_cast(float, bits) : a.gate_type == kF16 ? h2f(bits) : __builtin_bit_cast(float, bits << 16);
-            f *= a.gate_sigmoid ? sigmoid(v) : v;
-        }
+    };
+    if constexpr (WHOLE)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; ++c) open(c);
+    float f = a.scale;
+    if (YW != 0 && a.gate_kind == TC_GATE_ROW) {
+        const float v = a.gate_type == kF32   ? __builtin_bit_cast(float, row_gate)
+                        : a.gate_type == kF16 ? h2f(row_gate)
+                                              : __builtin_bit_cast(float, row_gate << 16);
+        f *= a.gate_sigmoid ? sigmoid(v) : v;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if constexpr (!WHOLE) {
+            if (c + 1 < C) fetch(c + 1);
+            open(c);
+        }
+        if constexpr (YW != 0) {
+            float(&v)[8] = y[POST || WHOLE ? c : 0];
             if (gated) {
                 float g[8];
                 if (a.gate_type == kF32)
-                    widen<4>(kF32, g_raw[c], g);
+                    widen<4>(kF32, g_raw[c % SLOTS], g);
                 else
-                    widen<2>(a.gate_type, g_raw[c], g);
+                    widen<2>(a.gate_type, g_raw[c % SLOTS], g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[c][i] *= a.gate_sigmoid ? sigmoid(g[i]) : g[i];
+                for (int i = 0; i < 8; ++i) v[i] *= a.gate_sigmoid ? sigmoid(g[i]) : g[i];
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] = __builtin_fmaf(f, y[c][i], h[c][i]);
+            for (int i = 0; i < 8; ++i) h[c][i] = __builtin_fmaf(f, v[i], h[c][i]);
             if (a.h_out != nullptr) row_store<HW, TINY>(a.h_type, a.h_out, r * a.h_out_stride, at[c], cols, h[c]);
-            if constexpr (POST) own_only<TINY>(at[c], cols, h[c]);  // (`post` may have a bias)
+            own_only<TINY>(at[c], cols, h[c]);  // (`post` may have a bias, a gate infinities)
         }
+        if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // (or all loads move to the front again)
     }
     if (a.pre.kind < 0) return;
     norm_row<LANES, C, TINY>(a, a.pre, at, lds + 32, h);
