@@ -207,9 +207,12 @@ hipError_t launch_plan(const tc_plan &p, hipStream_t st) {
     const bool maps = p.sequence || p.position || p.slot;
     const bool here = maps && p.n_tokens <= kRowsHere;
     const uint32_t rows = here ? p.n_tokens : 0;
-    // (barriers of 4 waves cost less than those of 16, 64 sequences 4.6 us and 5.3; many rows and pages
-    // want the threads, 9000 rows 8.5 and 7.2)
-    if (p.n_seq <= 256 && (here ? rows <= 1024 : p.n_tokens <= 8192))
+    // (barriers of 4 waves cost less than those of 16, 64 sequences 4.6 us and 5.3, and one wave has none: 4.2;
+    // many rows and pages want the threads, 200 rows 6.3 with 64 and 4.7 with 256, 9000 rows 8.5 with
+    // 256 and 7.2 with 1024)
+    if (p.n_seq <= 64 && here && rows <= 64)
+        k_plan<64><<<1, 64, 0, st>>>(p, page, rows);
+    else if (p.n_seq <= 256 && (here ? rows <= 1024 : p.n_tokens <= 8192))
         k_plan<256><<<1, 256, 0, st>>>(p, page, rows);
     else
         k_plan<1024><<<1, 1024, 0, st>>>(p, page, rows);
