@@ -4,10 +4,15 @@
 // there in LDS (integer sums, so their order changes nothing), adds up the biases in their
 // order, and then takes the sequence's rows one after the other, each row's own token counted
 // on top: every logit is read and written once, with its count and bias out of LDS beside it.
-// Bound by HBM for many rows; for few by the history, which each chunk's workgroup reads.
+// Bound by HBM for many rows (219 of 152064 logits with masks: 59 us of kernel, 271 MB at 4.6
+// TB/s; VALU 0.31 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.7
+// us), and between these by the history, which every chunk's workgroup reads (256 rows of 32003
+// 18 us, 15 without it, 10 for the bytes).
 //
 // No list of tokens is sorted and no counts are kept in HBM: a table of counts of one sequence
-// would be as large as a row of its logits.
+// would be as large as a row of its logits. Larger chunks were slower (219 rows 73 us at 4096
+// tokens, 66 at 2048), stores past the caches too once their reader was counted (131 -> 136 us with
+// tc_spec_verify behind, 200 rows).
 #include "tc_kernels.hpp"
 #include "tc_step.hpp"
 
@@ -229,6 +234,10 @@ hipError_t launch(const LogitCall &c, uint32_t parts, hipStream_t st) {
 }
 template <int XT>
 hipError_t launch(const LogitCall &c, int num_cu, hipStream_t st) {
+    // Chunks of 2048 tokens where those of 1024 are more than 4 to a CU (8 sequences 6.8 -> 6.3 us, 48
+    // 80 -> 66; 4 sequences 5.3 and 5.5); a sequence's rows by several workgroups, each of which counts
+    // the history, up to 8 to a CU (6 rows of one sequence 9.3 -> 5.7 us; up to 16 to a CU 6
+    // rows of 8 sequences 14.5 -> 17.5).
     const uint64_t cu = num_cu, chunks = uint64_t((c.vocab + 1023) / 1024) * c.n_seq;
     const bool wide = chunks > 4 * cu;
     const uint64_t most = (c.n_tokens + c.n_seq - 1) / c.n_seq, fill = 8 * cu / (wide ? (chunks + 1) / 2 : chunks);

@@ -2,12 +2,17 @@
 //
 //   h' = h + scale * gate * post(y),   x = pre(h'),   norm(z) = (z - mean) / sqrt(mean(z^2) + eps) * w + b
 //
-// A workgroup has a row (a wave of it, where rows are short), held in registers from its load
-// to its stores: y and h are read once, h' and x written once, and the statistics of both
-// norms, of a layer norm's differences too, come from the registers in fp32: a sum over a
-// lane's values, over the wave, over the waves through LDS. So the kernel is bound by HBM for
-// many rows, and for few by the chain of one load, one sum over the row per statistic, and the
-// store; the weights' loads are issued in front of the sums.
+// A row is held in registers from its load to its stores, by a workgroup or, where it is short,
+// by 8 to 64 lanes: y and h are read once, h' and x written once, and the statistics of both norms,
+// of a layer norm's differences too, come from the registers in fp32: a sum over a lane's values,
+// over the wave, over the waves through LDS. So many rows are bound by HBM (8192 rows of 5120, bf16,
+// with both norms: 67 us, 336 MB at 5.0 TB/s, a large copy's rate; VALU 0.37 busy), and few by the
+// chain of one load, one sum over the row per statistic, the weights and the store (one row of
+// 3584 2.8 us, of which a launch is 2.4).
+//
+// Not kept: workgroups that go through many rows with the weights in registers and the next row on
+// its way (8192 rows 112 us: fewer rows of a CU at work), stores past the caches (67 -> 64, but
+// 2 more with the next kernel's reads).
 #include <algorithm>
 #include <cmath>
 
@@ -315,7 +320,10 @@ __global__ __launch_bounds__(MOST) void k_norm(NormCall a) {
     }
 }
 
-// Rows of a workgroup, or of its waves' parts.
+// Short rows by as many lanes as they have eights (200000 rows of 128 columns 96 us with a wave
+// each, 38 with 16 lanes). Others by a workgroup: one block a lane where there are few rows, whose sums
+// are short then; two from 512 rows on, of which a CU holds more (1000 rows of 5120 10.7 -> 9.5 us, 8192
+// 79 -> 76 when it was taken; 500 rows 6.4 and 6.7); as many as 1024 threads leave from 8192 columns on.
 template <int YW, int HW, bool POST>
 hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
     const uint32_t blocks = (a.cols + 511) / 512;  // of a wave's 512 columns

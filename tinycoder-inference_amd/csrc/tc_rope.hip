@@ -6,11 +6,17 @@
 // by whole turns (at 10^5 by 2^-7 radians). What is left of a turn, less the nearest
 // quarter, is at most an eighth, and sin and cos of it are their Taylor series in fp32.
 //
-// A lane has 8 consecutive dims of `U` heads of one token, whose angles it forms once; the
+// A lane has 8 consecutive dims of one or four heads of a token, whose angles it forms once; the
 // other halves of its pairs are in the same 8 dims (TC_ROPE_PAIRS) or are read a second time
 // from the row (TC_ROPE_HALF: out of L1, the row is loaded by the neighbouring lanes at the
-// same time). So each row goes from HBM to HBM once, and both kernels are bound by that for
-// prompts, and by the chain start -> len -> table -> store for single tokens.
+// same time). So each row goes from HBM to HBM once: prompts are bound by that (8190 rows of 36
+// heads of 128, bf16: 30 us, 151 MB at 5.0 TB/s; VALU 0.56 busy, half of it the angles and addresses
+// of a wave that does nothing twice), single tokens by the chain start -> len -> table -> store (3.5
+// us; 241 rows with norms and 8-bit values 6.2).
+//
+// Not kept: the same heads of several tokens in a wave, which makes the choice between q, k and v a
+// scalar's (38 us for 37, and 6.9 for 6.2: a wave's tokens are of several sequences), two, eight
+// or twelve heads a lane (36, 36, 37 for 34).
 #include "tc_kernels.hpp"
 #include "tc_kv_put.hpp"
 #include "tc_step.hpp"
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void k_rope(RopeCall a, RopeWalk w) {
         if (normed) load_norm<L>(a.rope, n, from, nw, no);
     }
     // (long calls have the turns on their way from here, 39 -> 35 us for 8190 rows; short ones'
-    // lookups would wait for them, 6.0 -> 6.7 for 208)
+    // lookups would wait for them, 6.0 -> 6.7 for 241)
     double turns[8];
     if constexpr (U > 1) load_turns<L>(a.rope, from, turns);
     int32_t pos;
@@ -305,6 +311,8 @@ template <int CT, int W, int L>
 hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
     uint32_t blocks;
     RopeWalk w = make_walk(c, units, 1, &blocks);
+    // (four heads a lane from where single ones are more than 4 workgroups per CU: 1024 rows 10.9 -> 8.7
+    // us, 8190 59 -> 39 when it was taken; from 512 on 64 rows of 48 heads 7.5 -> 9.6)
     if (blocks <= 1024) {
         k_rope<CT, W, L, 1><<<blocks, kThreads, 0, st>>>(c, w);
     } else {
