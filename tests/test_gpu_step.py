@@ -222,3 +222,35 @@ def test_calls_at_once(tc, dev):
     for outs in got:
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
+
+
+def test_calls_without_rows(tc, dev):
+    """Nothing to do is done anywhere."""
+    z = lambda *n: torch.zeros(n, device=dev)  # noqa: E731
+    i = lambda *n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
+    cache = tc_hip.KVCache.empty(torch.float16, 2, 2, 16, 64, device=dev)
+    rope = tc_hip.Rope(64)
+    for batch in (tc_hip.KVBatch(i(2), i(1), i(1, 2)), tc_hip.KVBatch(i(1), i(0), i(0, 2))):
+        assert tc.rope_kv_write(cache, batch, rope, z(0, 4, 64), z(0, 2, 64), z(0, 2, 64)).shape == (0, 4, 64)
+    q = z(3, 4, 64) + 5
+    tc.rope_kv_write(cache, tc_hip.KVBatch(i(1), i(0), i(0, 2)), rope, q, z(3, 2, 64) + 1, z(3, 2, 64) + 1, out=q)
+    assert (q == 5).all() and not cache.k.any() and not cache.v.any()
+    assert tc.logits_adjust(tc_hip.LogitRules(), z(0, 100), i(1)).shape == (0, 100)
+    l = z(2, 100) + 3
+    assert tc.logits_adjust(tc_hip.LogitRules(), l, i(1), out=l) is l and (l == 3).all()
+    h, x = tc.norm_add(z(0, 64), z(0, 64), pre=tc_hip.Norm())
+    assert h.shape == x.shape == (0, 64)
+
+
+def test_frequencies_are_there_when_made(tc, dev):
+    """A rope made on one stream serves another at once."""
+    x, pos = torch.ones(64, 1, 128, device=dev), torch.arange(64, dtype=torch.int32, device=dev)
+    want = tc.rope(tc_hip.Rope(128, 1e6, scaling="yarn", factor=4.0, original=4096), x, pos)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        rope = tc_hip.Rope(128, 1e6, scaling="yarn", factor=4.0, original=4096)
+        with torch.cuda.stream(side):
+            got = tc.rope(rope, x, pos)
+        side.synchronize()
+        assert torch.equal(got, want)

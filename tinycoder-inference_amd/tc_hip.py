@@ -117,6 +117,7 @@ def load_library(path=LIB_PATH):
         f = getattr(lib, name)
         f.restype = res
         f.argtypes = args
+    _elem_types()
     _LOADED[path] = lib
     return lib
 
@@ -327,6 +328,12 @@ class Norm:
         self.c = _CNorm(NORM_KINDS[kind], eps, *[None if t is None else t.data_ptr() for t in (weight, bias)], offset)
         self.ref = ctypes.addressof(self.c)
 
+    def of(self, cols, device):
+        """The C struct's address, for rows of `cols` values on a device."""
+        if self.cols is not None and (self.cols != cols or self.device != device):
+            raise TCError(TC_E_ARG, "a norm's weights are not the rows' or not on the current device")
+        return self.ref
+
 
 ROPE_LAYOUTS = {"half": 0, "pairs": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
@@ -418,6 +425,7 @@ class Library:
         self.lib = load_library(path)
         self.path = path
         import torch
+        self._torch = torch
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         # (torch.cuda's own look at whether it is initialised takes longer than the rest of it)
         quick = getattr(torch._C, "_cuda_getDevice", None)
@@ -704,29 +712,29 @@ class Library:
         return _u32(st[0], "row stride") if T > 1 else width
 
     def _norm_rows(self, h, y, h_out, x, pre, post, gate, sigmoid, scale, act_type, act):
-        shape, dev, types = h.shape, self._current_device(), _ELEM_TYPES or _elem_types()
+        shape, dev, types = h.shape, self._current_device(), _ELEM_TYPES
         if len(shape) != 2:
             raise TCError(TC_E_ARG, "h is [rows][cols]")
         T, D = shape
-        ph = py = po = px = hs = ys = os_ = xs = et_y = et_x = 0
-        et_h = types.get(h.dtype, -1)
-        ph, hs = h.data_ptr(), D if h.is_contiguous() else self._stride_of(h, T, D)
-        good = h.get_device() == dev
+        py = po = px = ys = os_ = xs = ty = tx = 0
+        th, good = h.dtype, h.get_device() == dev
+        hs = D if h.is_contiguous() else self._stride_of(h, T, D)
         if y is not None:
-            py, ys, et_y = y.data_ptr(), D if y.is_contiguous() else self._stride_of(y, T, D), types.get(y.dtype, -1)
+            py, ty, ys = y.data_ptr(), types.get(y.dtype, -1), D if y.is_contiguous() else self._stride_of(y, T, D)
             good = good and y.shape == shape and y.get_device() == dev
         if h_out is not None:
             po, os_ = h_out.data_ptr(), D if h_out.is_contiguous() else self._stride_of(h_out, T, D)
-            good = good and h_out.shape == shape and h_out.dtype == h.dtype and h_out.get_device() == dev
+            good = good and h_out.shape == shape and h_out.dtype == th and h_out.get_device() == dev
         if x is not None:
-            px, xs, et_x = x.data_ptr(), D if x.is_contiguous() else self._stride_of(x, T, D), types.get(x.dtype, -1)
+            px, tx, xs = x.data_ptr(), types.get(x.dtype, -1), D if x.is_contiguous() else self._stride_of(x, T, D)
             good = good and x.shape == shape and x.get_device() == dev
         if not good:
             raise TCError(TC_E_ARG, "rows are [rows][cols] on the current device, h_out of h's type")
-        for n in (pre, post):
-            if n is not None and n.cols is not None and (n.cols != D or n.device != dev):
-                raise TCError(TC_E_ARG, "a norm's weights are not the rows' or not on the current device")
-        kind = 0
+        ppre = ppost = pg = kind = tg = 0
+        if pre is not None:
+            ppre = pre.of(D, dev)
+        if post is not None:
+            ppost = post.of(D, dev)
         if gate is not None:
             if gate.shape == shape:
                 kind = 3
@@ -738,18 +746,19 @@ class Library:
                 raise TCError(TC_E_ARG, "a gate is [cols], [rows][1] or [rows][cols]")
             if not gate.is_contiguous() or gate.get_device() != dev:
                 raise TCError(TC_E_ARG, "a gate is contiguous, on the current device")
+            pg, tg = gate.data_ptr(), types.get(gate.dtype, -1)
         if act is not None and (not act.is_contiguous() or act.get_device() != dev or
                                 act.numel() * act.element_size() < self.lib.tc_act_bytes(act_type, T, D)):
             raise TCError(TC_E_ARG, "act is too small, not contiguous or not on the current device")
-        c = _PACK_NORM_ROWS(T, D, ph, py, po, px, et_h, et_y, et_x, hs, ys, os_, xs, 0 if post is None else post.ref,
-                            0 if pre is None else pre.ref, 0 if gate is None else gate.data_ptr(), kind,
-                            0 if gate is None else types.get(gate.dtype, -1), 1 if sigmoid else 0, scale,
-                            act_type, 0 if act is None else act.data_ptr())
-        self._check(self.lib.tc_norm_add(c, self._stream(dev)))
+        c = _PACK_NORM_ROWS(T, D, h.data_ptr(), py, po, px, types.get(th, -1), ty, tx, hs, ys, os_, xs, ppost, ppre, pg, kind, tg,
+                            1 if sigmoid else 0, scale, act_type, 0 if act is None else act.data_ptr())
+        rc = self.lib.tc_norm_add(c, self._stream(dev))
+        if rc:
+            self._check(rc)
 
     def norm(self, h, pre, out_dtype=None, out=None):
         """pre(h): the norm of rows [rows][cols] (which may be strided), of out_dtype (h's)."""
-        import torch
+        torch = self._torch
         if out is None:
             out = torch.empty_like(h, dtype=out_dtype, memory_format=torch.contiguous_format)
         self._norm_rows(h, None, None, out, pre, None, None, False, 1.0, 0, None)
@@ -761,7 +770,7 @@ class Library:
         out_dtype (h's) into out: (h_out, out); without `pre` out is None. gate [cols],
         [rows][1] or [rows][cols]. act: a buffer of
         tc_act_bytes for the activations quantized for weights of act_type, as act_quantize."""
-        import torch
+        torch = self._torch
         if h_out is None:
             h_out = torch.empty_like(h, memory_format=torch.contiguous_format)
         if out is None and pre is not None:
@@ -794,61 +803,72 @@ class Library:
         """Queries [n_tokens][heads][head_dim] rotated into out (new; contiguous), keys rotated
         and values as they are into their slots of the cache (tc_rope_kv_write). q_norm, k_norm:
         fp32 weights [head_dim] of an RMS norm of the heads before. q may be None."""
-        import torch
-        shape, kv, D, dev = k.shape, cache.kv_heads, cache.head_dim, self._current_device()
-        if len(shape) != 3 or shape[1] != kv or shape[2] != D or v.shape != shape or v.dtype != k.dtype:
+        shape, kv, D, dev, dtype = k.shape, cache.kv_heads, cache.head_dim, self._current_device(), k.dtype
+        if len(shape) != 3 or shape[1] != kv or shape[2] != D or v.shape != shape or v.dtype != dtype:
             raise TCError(TC_E_ARG, "k and v are not [n_tokens][kv_heads][head_dim] of the cache, of one type")
-        T, heads, pq, qs, po = shape[0], 0, None, 0, None
-        ks = kv * D if k.is_contiguous() else self._stride_of(k, T, kv * D)
-        vs = kv * D if v.is_contiguous() else self._stride_of(v, T, kv * D)
-        if not k.get_device() == v.get_device() == dev:
-            raise TCError(TC_E_ARG, "tensors are not on the current device")
+        T, width, heads, pq, qs, po = shape[0], kv * D, 0, None, 0, None
+        ks = width if k.is_contiguous() else self._stride_of(k, T, width)
+        vs = width if v.is_contiguous() else self._stride_of(v, T, width)
+        good = k.get_device() == v.get_device() == cache.device == batch.device == rope.device == dev
         if q is not None:
-            if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
             shape = q.shape
-            if len(shape) != 3 or shape[0] != T or shape[2] != D or q.dtype != k.dtype or out.shape != shape or \
-                    out.dtype != q.dtype or not out.is_contiguous() or not q.get_device() == out.get_device() == dev:
-                raise TCError(TC_E_ARG, "q is not [n_tokens][heads][head_dim] of k's type, or out not that, contiguous")
+            if len(shape) != 3 or shape[0] != T or shape[2] != D or q.dtype != dtype:
+                raise TCError(TC_E_ARG, "q is not [n_tokens][heads][head_dim] of k's type")
+            if out is None:
+                out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
+            elif out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.get_device() != dev:
+                raise TCError(TC_E_ARG, "out is not like q, contiguous, on the current device")
             heads = shape[1]
+            good = good and q.get_device() == dev
             pq, po, qs = q.data_ptr(), out.data_ptr(), heads * D if q.is_contiguous() else self._stride_of(q, T, heads * D)
         elif out is not None:
             raise TCError(TC_E_ARG, "out without q")
-        if not cache.device == batch.device == rope.device == dev:
-            raise TCError(TC_E_ARG, "cache, batch or rope are not on the current device")
-        for w in (q_norm, k_norm):
-            if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or w.stride(0) != 1 or w.get_device() != dev):
-                raise TCError(TC_E_ARG, "norms of heads are fp32 [head_dim] on the current device")
-        self._check(self.lib.tc_rope_kv_write(
-            cache.ref, batch.of(T), rope.ref, _elem_type(k.dtype), pq, qs, po, heads, k.data_ptr(), ks, v.data_ptr(), vs,
-            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps, self._stream(dev)))
+        if not good:
+            raise TCError(TC_E_ARG, "rows, cache, batch or rope are not on the current device")
+        pqn = pkn = None
+        if q_norm is not None:
+            pqn = self._head_norm(q_norm, D, dev)
+        if k_norm is not None:
+            pkn = self._head_norm(k_norm, D, dev)
+        rc = self.lib.tc_rope_kv_write(cache.ref, batch.of(T), rope.ref, _ELEM_TYPES.get(dtype, -1), pq, qs, po, heads, k.data_ptr(), ks,
+                                       v.data_ptr(), vs, pqn, pkn, eps, self._stream(dev))
+        if rc:
+            self._check(rc)
         return out
+
+    def _head_norm(self, w, D, dev):
+        if w.dtype != self._torch.float32 or w.dim() != 1 or w.numel() != D or not w.is_contiguous() or w.get_device() != dev:
+            raise TCError(TC_E_ARG, "norms of heads are fp32 [head_dim], contiguous, on the current device")
+        return w.data_ptr()
 
     def logits_adjust(self, rules, logits, start, tokens=None, out=None):
         """Rules on logits [n_tokens][vocab] (rows may be strided) of the sequences' rows start
         int32 [n_seq + 1]: fp32 [n_tokens][vocab] in out (which may be logits). tokens int32
         [n_tokens]: the step's tokens, counted behind the history up to each row's own."""
-        import torch
         shape, dev = logits.shape, self._current_device()
         if out is None:
-            out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
-        st, to = logits.stride(), out.stride()
-        if len(shape) != 2 or out.shape != shape or not logits.get_device() == out.get_device() == dev or \
-                (shape[0] != 0 and shape[1] > 1 and not st[1] == to[1] == 1):
-            raise TCError(TC_E_ARG, "logits are [n_tokens][vocab], a row's next to each other, on the current device")
+            out = self._torch.empty_like(logits, dtype=self._torch.float32, memory_format=self._torch.contiguous_format)
+        if len(shape) != 2 or out.shape != shape or not logits.get_device() == out.get_device() == dev:
+            raise TCError(TC_E_ARG, "logits and out are [n_tokens][vocab] on the current device")
         T, V = shape
         S = start.numel() - 1
-        for t in (start,) if tokens is None else (start, tokens):
-            if t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != dev:
-                raise TCError(TC_E_ARG, "start and tokens are contiguous int32 on the current device")
-        if out.dtype != torch.float32 or (tokens is not None and tokens.numel() != T) or S < 0 or \
-                (rules.device is not None and rules.device != dev) or (rules.n_seq is not None and rules.n_seq != S) or \
-                (rules.rows is not None and rules.rows < T) or (rules.words is not None and rules.words * 32 < V):
+        ls = V if logits.is_contiguous() else self._stride_of(logits, T, V)
+        os_ = V if out.is_contiguous() else self._stride_of(out, T, V)
+        i32, pt = self._torch.int32, None
+        good = start.dtype == i32 and start.is_contiguous() and start.get_device() == dev
+        if tokens is not None:
+            pt = tokens.data_ptr()
+            good = good and tokens.dtype == i32 and tokens.numel() == T and tokens.is_contiguous() and tokens.get_device() == dev
+        if not good:
+            raise TCError(TC_E_ARG, "start and tokens [n_tokens] are contiguous int32 on the current device")
+        if out.dtype != self._torch.float32 or S < 0 or (rules.device is not None and rules.device != dev) or \
+                (rules.n_seq is not None and rules.n_seq != S) or (rules.rows is not None and rules.rows < T) or \
+                (rules.words is not None and rules.words * 32 < V):
             raise TCError(TC_E_ARG, "out is not fp32, or sizes or devices do not agree")
-        self._check(self.lib.tc_logits_adjust(
-            rules.ref, _elem_type(logits.dtype), logits.data_ptr(), V if T <= 1 else _u32(st[0], "row stride"), V, S, T,
-            start.data_ptr(), None if tokens is None else tokens.data_ptr(), out.data_ptr(),
-            V if T <= 1 else _u32(to[0], "row stride"), self._stream(dev)))
+        rc = self.lib.tc_logits_adjust(rules.ref, _ELEM_TYPES.get(logits.dtype, -1), logits.data_ptr(), ls, V, S, T, start.data_ptr(), pt,
+                                       out.data_ptr(), os_, self._stream(dev))
+        if rc:
+            self._check(rc)
         return out
 
 
