@@ -162,7 +162,7 @@ int tc_rope_apply(const tc_rope *rope, int xtype, const void *x, uint32_t x_stri
 /* What lies between the q/k/v product and tc_attn, in one launch. For each row of the
  * batch, at its position (tc_kv_batch): the queries' heads are normalised (RMS over
  * head_dim, times q_norm[head_dim], fp32; NULL: not), rotated, and written to q_out
- * ([n_tokens][heads][head_dim] contiguous, of `xtype`; may be q where q is contiguous); the
+ * ([n_tokens][heads][head_dim] contiguous, of `xtype`; or q itself: in place, at q's stride); the
  * keys' heads likewise with k_norm, and written to their slots of the cache, as tc_kv_write
  * writes k; the values are written as tc_kv_write writes v. Between loading and the one
  * rounding at the end values are fp32 (a norm's squares too: heads with values past 10^18 get an infinite

@@ -189,6 +189,15 @@ def test_in_place_and_keys_alone(tc, dev):
     tc.rope_kv_write(b.cache, b.batch, rope, qc, k, v, out=qc)
     live = int(b.start[-1])
     assert torch.equal(qc[:live], out[:live]) and torch.equal(qc[live:], q[live:])
+    # in place among the rows of one product: keys, values and padding as they were
+    whole = x.clone()
+    part = whole[:, :6]
+    assert tc.rope_kv_write(b.cache, b.batch, rope, part, whole[:, 6:8], whole[:, 8:], out=part) is part
+    assert torch.equal(whole[:live, :6], out[:live]) and torch.equal(whole[live:], x[live:]) and torch.equal(whole[:, 6:], x[:, 6:])
+    assert all(torch.equal(t, held[n]) for n, t in b.dev.items())
+    for bad in (whole[:, 1:7], whole.view(-1)[:b.T * 6 * 64].view(b.T, 6, 64), out[:, :5], out.float()):
+        with pytest.raises(tc_hip.TCError):
+            tc.rope_kv_write(b.cache, b.batch, rope, part, whole[:, 6:8], whole[:, 8:], out=bad)
     for t in b.dev.values():
         t.zero_()
     assert tc.rope_kv_write(b.cache, b.batch, rope, None, k, v) is None

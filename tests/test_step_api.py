@@ -155,7 +155,7 @@ def test_rope_row_refusals(lib):
     assert apply(lib, n=0) == OK
     for kw, code in ((dict(xtype=24), UNSUPPORTED), (dict(q=None), ARG), (dict(qo=None), ARG), (dict(heads=0), ARG),
                      (dict(heads=0, q=None), ARG), (dict(heads=4097, qs=1 << 20), UNSUPPORTED), (dict(qs=255), ARG),
-                     (dict(qs=260), ARG), (dict(qs=258, qo=P + 16), UNSUPPORTED), (dict(q=P + 8), UNSUPPORTED),
+                     (dict(qs=258, qo=P + 16), UNSUPPORTED), (dict(q=P + 8), UNSUPPORTED),
                      (dict(qo=P + 8), UNSUPPORTED), (dict(k=None), ARG), (dict(ks=127), ARG), (dict(vs=130), UNSUPPORTED),
                      (dict(v=P + 4), UNSUPPORTED), (dict(qn=P + 2), UNSUPPORTED), (dict(kn=P + 2), UNSUPPORTED),
                      (dict(eps=NAN), ARG), (dict(eps=-1.0), ARG), (dict(c=cache(head_dim=32)), UNSUPPORTED),

@@ -221,7 +221,6 @@ int tc_rope_kv_write(const tc_kv_cache *cache, const tc_kv_batch *batch, const t
     if (heads != 0) {
         if ((rc = check_rows("q", q, q_stride, q_width, n, xtype))) return rc;
         if ((rc = check_rows("q_out", q_out, uint32_t(q_width), q_width, n, xtype))) return rc;
-        if (q == q_out && n > 1 && q_stride != q_width) return refuse(TC_E_ARG, "q_out is q with another stride");
     }
     if ((rc = check_rows("k", k, k_stride, width, n, xtype))) return rc;
     if ((rc = check_rows("v", v, v_stride, width, n, xtype))) return rc;
@@ -230,7 +229,7 @@ int tc_rope_kv_write(const tc_kv_cache *cache, const tc_kv_batch *batch, const t
     c.k = {k, k_stride, c.kv.kv_heads, k_norm};
     c.v = {v, v_stride, c.kv.kv_heads, nullptr};
     c.q_out = q_out;
-    c.q_out_stride = q_width;
+    c.q_out_stride = q_out == q ? q_stride : q_width;  // in place: where q's rows are
     c.eps = eps;
     c.xtype = xtype;
     return hip_rc(tc::launch_rope_kv(c, cache->type, static_cast<hipStream_t>(stream)), "rope and cache write");

@@ -800,7 +800,7 @@ class Library:
         return out
 
     def rope_kv_write(self, cache, batch, rope, q, k, v, q_norm=None, k_norm=None, eps=1e-6, out=None):
-        """Queries [n_tokens][heads][head_dim] rotated into out (new; contiguous), keys rotated
+        """Queries [n_tokens][heads][head_dim] rotated into out (new, contiguous, or q itself), keys rotated
         and values as they are into their slots of the cache (tc_rope_kv_write). q_norm, k_norm:
         fp32 weights [head_dim] of an RMS norm of the heads before. q may be None."""
         shape, kv, D, dev, dtype = k.shape, cache.kv_heads, cache.head_dim, self._current_device(), k.dtype
@@ -816,8 +816,9 @@ class Library:
                 raise TCError(TC_E_ARG, "q is not [n_tokens][heads][head_dim] of k's type")
             if out is None:
                 out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
-            elif out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.get_device() != dev:
-                raise TCError(TC_E_ARG, "out is not like q, contiguous, on the current device")
+            elif out is not q and (out.shape != shape or out.dtype != dtype or out.get_device() != dev or
+                                   not (out.stride() == q.stride() if out.data_ptr() == q.data_ptr() else out.is_contiguous())):
+                raise TCError(TC_E_ARG, "out is neither q nor like q, contiguous, on the current device")
             heads = shape[1]
             good = good and q.get_device() == dev
             pq, po, qs = q.data_ptr(), out.data_ptr(), heads * D if q.is_contiguous() else self._stride_of(q, T, heads * D)
