@@ -193,6 +193,16 @@ def test_quantized_activations_alone(tc, dev):
     assert torch.equal(act, other) and act.any()
 
 
+def test_norm_of_a_sum_that_is_not_kept(tc, dev):
+    """x without h_out."""
+    rng = np.random.default_rng(2)
+    for D in (64, 999, 5120):
+        h, y, x = rows(rng, 3, D, "BF16", dev), rows(rng, 3, D, "F32", dev), torch.empty(3, D, device=dev)
+        pre, _ = weights(rng, D, dev, "rms")
+        tc._norm_rows(h, y, None, x, pre, None, None, False, 0.5, 0, None)
+        assert torch.equal(x, tc.norm_add(h, y, pre=pre, scale=0.5, out_dtype=torch.float32)[1])
+
+
 def test_binding_refusals(tc, dev):
     h = torch.zeros(4, 4, device=dev)
     n = tc_hip.Norm(torch.ones(4, device=dev))

@@ -157,7 +157,8 @@ def test_kv_write(tc, dev, layout, heads, kv, dim, page, n_rot, xtype, ctype, no
 
 @pytest.mark.parametrize("ctype", CTYPES)
 @pytest.mark.parametrize("layout", ["half", "pairs"])
-@pytest.mark.parametrize("seqs", [RAGGED, [(1, 40)], [(700, 900), (1, 5), (350, 350)]])
+@pytest.mark.parametrize("seqs", [RAGGED, [(1, 40)], [(700, 900), (1, 5), (350, 350)], [(k % 4, 5 + k % 37) for k in range(300)]],
+                         ids=["ragged", "one", "long", "many"])
 def test_fused_is_the_parts(tc, dev, seqs, layout, ctype):
     """fp32 rows: rotating, then tc_kv_write, gives the same bits in the cache and the queries."""
     rng = np.random.default_rng(len(seqs))
@@ -205,6 +206,20 @@ def test_in_place_and_keys_alone(tc, dev):
         if b.slot(s, p):
             pg, sl = b.slot(s, p)
             assert torch.equal(b.dev["k"][pg, :, sl], held["k"][pg, :, sl])
+
+
+def test_many_heads(tc, dev):
+    """More heads than a model has: units of a token over many workgroups."""
+    rng = np.random.default_rng(8)
+    b, x, q, k, v = setup(rng, dev, "BF16", "I8", 1000, 20, 32, 16, seqs=[(2, 20), (1, 1)], pad=0)
+    rope = tc_hip.Rope(32, layout="pairs")
+    out = tc.rope_kv_write(b.cache, b.batch, rope, q, k, v)
+    want, err = rope_exact(f64(q), np.array([18, 19, 0]), turns_exact(32, 1e4)[0], 32, "pairs", 1.0)
+    near(out, want, err, "BF16")
+    got = tc.kv_read(b.cache, b.batch, 3, torch.float32)[0]
+    want, err = rope_exact(f64(k), np.array([18, 19, 0]), turns_exact(32, 1e4)[0], 32, "pairs", 1.0)
+    step = np.abs(want).max(-1, keepdims=True) / 127 / 2
+    assert (np.abs(f64(got) - want) <= step * 1.001 + 2 * err.max(-1, keepdims=True) + 3 * 2.0 ** -24 * np.abs(want)).all()
 
 
 def test_rows_without_slots(tc, dev):
