@@ -61,17 +61,38 @@ __device__ __forceinline__ uint32_t around(uint32_t at, uint32_t by, uint32_t ri
     return i >= ring ? i % ring : i;
 }
 
-// Of the first n entries of an ascending list the last that is at most v (list[0] is).
-__device__ __forceinline__ uint32_t find_last(const uint32_t *list, uint32_t n, uint32_t v) {
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (list[mid] <= v)
-            lo = mid;
-        else
-            hi = mid;
+// Half of the least power of two that n (at least 1) is not above.
+__device__ __forceinline__ uint32_t first_step(uint32_t n) { return n <= 1 ? 0 : 1u << (31 - __builtin_clz(n - 1)); }
+// Of an ascending list the last entry that is at most v (list[0] is), among as many as `first` is the
+// first step of, and those up to twice that.
+__device__ __forceinline__ uint32_t find_last(const uint32_t *list, uint32_t first, uint32_t v) {
+    uint32_t at = 0;
+    for (uint32_t step = first; step != 0; step /= 2) at += list[at + step] <= v ? step : 0;
+    return at;
+}
+// put(j, i, get(j, i)) for the pages j < n of a lot of sequences, i the sequence's place in it. Where
+// there are more pages than threads, a thread's next four side by side: each one's search and
+// fetch are a chain of their own.
+template <uint32_t THREADS, class Get, class Put>
+__device__ __forceinline__ void each_page(const uint32_t *before, uint32_t first, uint32_t n, Get get, Put put) {
+    uint32_t j0 = threadIdx.x;
+    for (; j0 + 3 * THREADS < n; j0 += 4 * THREADS) {
+        uint32_t i[4];
+        int32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) i[k] = 0;
+        for (uint32_t step = first; step != 0; step /= 2)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) i[k] += before[i[k] + step] <= j0 + k * THREADS ? step : 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = get(j0 + k * THREADS, i[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) put(j0 + k * THREADS, i[k], v[k]);
     }
-    return lo;
+    for (; j0 < n; j0 += THREADS) {
+        const uint32_t i = find_last(before, first, j0);
+        put(j0, i, get(j0, i));
+    }
 }
 
 // A row's sequence (-1: none), position (below 0: none, where a length was held to the largest)
@@ -102,6 +123,7 @@ __global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32
     __shared__ int32_t shift[THREADS];  // of a sequence's rows to their positions
     const uint32_t S = a.n_seq, R = a.ring_pages, W = a.table_pages, tid = threadIdx.x;
     const uint32_t at = bounded(a.free[0], R - 1), left0 = bounded(a.free[1], R);
+    const uint32_t first = first_step(min(S, uint32_t(THREADS)));  // of searches among a lot of sequences
     int turn = 0;
     // pages of ended sequences behind the free ones, and where there is one lot of sequences only, their rows
     uint32_t back_all = 0, row_all = 0;
@@ -121,10 +143,9 @@ __global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32
             before[tid] = back_of.before;
             __syncthreads();
             const uint32_t room = left0 + back_all < R ? R - left0 - back_all : 0;
-            for (uint32_t j = tid; j < min(back_of.all, room); j += THREADS) {
-                const uint32_t i = find_last(before, THREADS, j);
-                a.ring[around(at, left0 + back_all + j, R)] = a.table[size_t(s0 + i) * W + (j - before[i])];
-            }
+            each_page<THREADS>(
+                before, first, min(back_of.all, room), [&](uint32_t j, uint32_t i) { return a.table[size_t(s0 + i) * W + (j - before[i])]; },
+                [&](uint32_t j, uint32_t, int32_t page) { a.ring[around(at, left0 + back_all + j, R)] = page; });
             __threadfence_block();
             __syncthreads();
         }
@@ -159,10 +180,9 @@ __global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32
             before[tid] = want_of.before;
             had_of[tid] = had;
             __syncthreads();
-            for (uint32_t j = tid; j < want_of.all; j += THREADS) {
-                const uint32_t i = find_last(before, THREADS, j), k = want_all + j;
-                a.table[size_t(s0 + i) * W + had_of[i] + (j - before[i])] = k < left ? a.ring[around(at, k, R)] : -1;
-            }
+            each_page<THREADS>(
+                before, first, want_of.all, [&](uint32_t j, uint32_t) { return want_all + j < left ? a.ring[around(at, want_all + j, R)] : -1; },
+                [&](uint32_t j, uint32_t i, int32_t page) { a.table[size_t(s0 + i) * W + had_of[i] + (j - before[i])] = page; });
             __syncthreads();
         }
         want_all += want_of.all;
@@ -182,7 +202,7 @@ __global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32
         int seq = -1;
         int32_t pos = -1;
         if (t < row_all) {
-            seq = S > THREADS ? find_seq(a.start, S, t) : int(find_last(begins, S, t));
+            seq = S > THREADS ? find_seq(a.start, S, t) : int(find_last(begins, first, t));
             pos = S > THREADS ? position_of(a, t, seq) : shift[seq] + int32_t(t);
         }
         put_row_maps(a, page, t, seq, pos);
