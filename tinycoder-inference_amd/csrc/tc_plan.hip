@@ -4,8 +4,8 @@
 // pages wanted, which depend on the rows. One workgroup forms them, as many sequences at a time
 // as it has threads, and enters the pages, a thread a page whosever it is; with that done, a row's
 // sequence, position and slot are looked up as the other kernels do. Few rows are looked up by the
-// same workgroup, with the sequences' starts in LDS (1200 rows 5.4 us, 6.3 with a launch of their own;
-// from 4000 on that is the faster, one workgroup's stores reaching some 60 GB/s, 16 bytes a row).
+// same workgroup, with the sequences' starts in LDS (1200 rows 4.8 us, 5.7 with a launch of their own;
+// 4000 rows 6.0 and 5.8).
 // Bound by the chain lengths -> sums -> ring -> table -> slots, not by any traffic.
 //
 // Sums of rows saturate at n_tokens, and those of missing pages at 2^30, so that they stay in 32
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(THREADS) void k_plan(tc_plan a, DivMod page, uint32
 }
 
 // The rows' maps, a row a thread. Up to 1024 sequences' starts are held in LDS: one fetch and a
-// search there, where each step of a search in memory waits for the one before (plan_mixed 10.8 -> 10.0
-// us).
+// search there, where each step of a search in memory waits for the one before (301 sequences with 165000
+// rows, both launches, 9.9 us where that took 10.7).
 constexpr uint32_t kSeqsHere = 1024;
 __global__ __launch_bounds__(256) void k_plan_rows(tc_plan a, DivMod page) {
     __shared__ uint32_t begins[kSeqsHere];
@@ -245,12 +245,13 @@ hipError_t launch_plan(const tc_plan &p, hipStream_t st) {
     const bool maps = p.sequence || p.position || p.slot;
     const bool here = maps && p.n_tokens <= kRowsHere;
     const uint32_t rows = here ? p.n_tokens : 0;
-    // (barriers of 4 waves cost less than those of 16, 64 sequences 4.6 us and 5.3, and one wave has none: 4.2;
-    // many rows and pages want the threads, 200 rows 6.3 with 64 and 4.7 with 256, 9000 rows 8.5 with
-    // 256 and 7.2 with 1024)
+    // (barriers of 4 waves cost less than those of 16, 32 sequences of a row each 4.2 us and 4.8, and one wave
+    // has none: 3.9; many rows and pages want the threads, 256 rows 5.8 with 64, 4.3 with 256 and 4.8 with
+    // 1024, 800 rows 5.0 with 256 and 4.6 with 1024. Pages alone, of 4000 rows, 5.8 with 256 and 6.4 with
+    // 1024, of 12000 7.3 and 6.7)
     if (p.n_seq <= 64 && here && rows <= 64)
         k_plan<64><<<1, 64, 0, st>>>(p, page, rows);
-    else if (p.n_seq <= 256 && (here ? rows <= 1024 : p.n_tokens <= 8192))
+    else if (p.n_seq <= 256 && (here ? rows <= 512 : p.n_tokens <= 8192))
         k_plan<256><<<1, 256, 0, st>>>(p, page, rows);
     else
         k_plan<1024><<<1, 1024, 0, st>>>(p, page, rows);
