@@ -106,7 +106,7 @@ typedef struct tc_norm_rows {
                                        * bytes, 256-byte aligned), for tc_gemv_q8; NULL: none. cols % 256 = 0, up to 12288 */
 } tc_norm_rows;
 
-/* One launch. Everything between the inputs and the outputs' rounding is held in fp32: x is
+/* One launch for every 2^21 rows. Everything between the inputs and the outputs' rounding is held in fp32: x is
  * the norm of h + scale * gate * post(y) before that is rounded to h's type; act is formed
  * from the fp32 values that an F32 x has, and is tc_act_quantize's of them bit for bit.
  * cols up to 32768. Rows may have any stride that keeps them apart and any

@@ -203,6 +203,34 @@ def test_norm_of_a_sum_that_is_not_kept(tc, dev):
         assert torch.equal(x, tc.norm_add(h, y, pre=pre, scale=0.5, out_dtype=torch.float32)[1])
 
 
+@pytest.mark.parametrize("gate_of", ["row", "full", "channel"])
+def test_rows_of_several_launches(tc, dev, gate_of):
+    """More rows than a launch takes: the last ones are what they are by themselves."""
+    T, D, tail = (1 << 21) + 5, 17, 9
+    rng = np.random.default_rng(3)
+    g = torch.Generator(device=dev).manual_seed(3)
+    h, y = (torch.randn(T, D + 2, device=dev, generator=g).to(dt)[:, 1:D + 1] for dt in (torch.bfloat16, torch.float32))
+    pre, _ = weights(rng, D, dev, "layer")
+    gate = torch.randn(*{"row": (T, 1), "full": (T, D), "channel": (D,)}[gate_of], device=dev, generator=g)
+    h2, x = tc.norm_add(h, y, pre=pre, gate=gate, scale=0.7, out_dtype=torch.float32)
+    part = gate if gate_of == "channel" else gate[-tail:].contiguous()
+    for got, want in zip((h2, x), tc.norm_add(h[-tail:], y[-tail:], pre=pre, gate=part, scale=0.7, out_dtype=torch.float32)):
+        assert torch.equal(got[-tail:], want)
+    assert torch.equal(tc.norm(h, pre)[-tail:], tc.norm(h[-tail:], pre))
+
+
+@pytest.mark.parametrize("qtype", [Q8_0, Q4_K])
+def test_quantized_rows_of_several_launches(tc, dev, qtype):
+    T, D = (1 << 21) + 5, 256
+    pre, _ = weights(np.random.default_rng(4), D, dev, "rms")
+    h = torch.randn(T, D, device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    act, other = (torch.zeros(tc.lib.tc_act_bytes(qtype, T, D), dtype=torch.uint8, device=dev) for _ in range(2))
+    x = torch.empty_like(h)
+    tc._norm_rows(h, None, None, x, pre, None, None, False, 1.0, qtype, act)
+    tc._check(tc.lib.tc_act_quantize(qtype, tc_hip._ptr(x), T, D, tc_hip._ptr(other), tc._stream()))
+    assert torch.equal(act, other) and torch.equal(x[-3:], tc.norm(h[-3:], pre))
+
+
 def test_binding_refusals(tc, dev):
     h = torch.zeros(4, 4, device=dev)
     n = tc_hip.Norm(torch.ones(4, device=dev))

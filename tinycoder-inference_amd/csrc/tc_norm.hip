@@ -15,6 +15,7 @@
 // 2 more with the next kernel's reads).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tc_actquant.hpp"
 #include "tc_kernels.hpp"
@@ -367,6 +368,22 @@ hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
     return hipGetLastError();
 }
 
+hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
+    const bool wide = a.h_type == kF32;
+    if (a.y == nullptr) return wide ? launch<0, 4>(a, num_cu, st) : launch<0, 2>(a, num_cu, st);
+    if (a.y_type == kF32) return wide ? launch<4, 4>(a, num_cu, st) : launch<4, 2>(a, num_cu, st);
+    return wide ? launch<2, 4>(a, num_cu, st) : launch<2, 2>(a, num_cu, st);
+}
+
+// `rows` rows further on.
+template <class T>
+T *on(T *p, uint64_t rows, uint64_t bytes) {
+    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return p == nullptr ? p : reinterpret_cast<T *>(reinterpret_cast<Byte *>(p) + rows * bytes);
+}
+
+constexpr uint32_t kRowsMost = 1u << 21;  // of a launch: a grid has less than 2^32 threads
+
 }  // namespace
 
 hipError_t launch_norm(const NormCall &call, int num_cu, hipStream_t st) {
@@ -376,10 +393,22 @@ hipError_t launch_norm(const NormCall &call, int num_cu, hipStream_t st) {
     a.inv_cols = 1.0f / float(a.cols);
     a.down = std::ldexp(1.0f, -up);
     a.inv_cols_down = std::ldexp(a.inv_cols, up);
-    const bool wide = a.h_type == kF32;
-    if (a.y == nullptr) return wide ? launch<0, 4>(a, num_cu, st) : launch<0, 2>(a, num_cu, st);
-    if (a.y_type == kF32) return wide ? launch<4, 4>(a, num_cu, st) : launch<4, 2>(a, num_cu, st);
-    return wide ? launch<2, 4>(a, num_cu, st) : launch<2, 2>(a, num_cu, st);
+    for (uint32_t left = call.rows;;) {
+        a.rows = std::min(left, kRowsMost);
+        const hipError_t e = launch(a, num_cu, st);
+        if (e != hipSuccess || (left -= a.rows) == 0) return e;
+        const uint64_t h_bytes = elem_bytes(a.h_type), x_bytes = elem_bytes(a.x_type), block = a.act_q8_0 ? 32 : 256;
+        a.h = on(a.h, a.rows, a.h_stride * h_bytes);
+        a.y = on(a.y, a.rows, a.y_stride * elem_bytes(a.y_type));
+        a.h_out = on(a.h_out, a.rows, a.h_out_stride * h_bytes);
+        a.x = on(a.x, a.rows, a.x_stride * x_bytes);
+        if (a.gate_kind == TC_GATE_ROW || a.gate_kind == TC_GATE_FULL)
+            a.gate = on(a.gate, a.rows, (a.gate_kind == TC_GATE_ROW ? 1 : a.cols) * elem_bytes(a.gate_type));
+        a.qs = on(a.qs, a.rows, a.cols);
+        a.d = on(a.d, a.rows, a.cols / block * 4);
+        a.bsums = on(a.bsums, a.rows, a.cols / 16 * 2);
+        a.dg = on(a.dg, a.rows, a.cols / 256 * (a.act_q8_0 ? 32 : 16) * 2);
+    }
 }
 
 }  // namespace tc
