@@ -88,6 +88,15 @@ def test_long_history(tc, dev):
     same(tc, dev, r, l, start, tokens)
 
 
+# borders of the chunks of few sequences and of many
+@pytest.mark.parametrize("V", [2047, 2048, 2049, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("n_seq", [3, 600])
+def test_borders_of_chunks(tc, dev, V, n_seq):
+    rng = np.random.default_rng(V + n_seq)
+    rows, hist = ([int(n) for n in rng.integers(0, most, n_seq)] for most in (3, 20))
+    same(tc, dev, *make(rng, V, rows, hist, bias=5, masks=2, xtype="BF16"))
+
+
 def test_repeated_entries(tc, dev):
     """One token many times among the biases (added in their order: the sum depends on it), the history and the drafts."""
     V = 2000

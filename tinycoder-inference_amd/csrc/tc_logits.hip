@@ -5,13 +5,14 @@
 // order, and then takes the sequence's rows one after the other, each row's own token counted
 // on top: every logit is read and written once, with its count and bias out of LDS beside it.
 // Bound by HBM for many rows (219 of 152064 logits with masks: 59 us of kernel, 271 MB at 4.6
-// TB/s; VALU 0.31 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.7
+// TB/s; VALU 0.31 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.3
 // us), and between these by the history, which every chunk's workgroup reads (256 rows of 32003
 // 18 us, 15 without it, 10 for the bytes).
 //
 // No list of tokens is sorted and no counts are kept in HBM: a table of counts of one sequence
-// would be as large as a row of its logits. Larger chunks were slower (219 rows 73 us at 4096
-// tokens, 66 at 2048), stores past the caches too once their reader was counted (131 -> 136 us with
+// would be as large as a row of its logits. More tokens of a lane were slower (219 rows 72 us
+// with 16, 65 with 8), fewer lanes too (66 with 256 to a workgroup, which then counts more histories; one
+// row 4.7 for 4.3), stores past the caches too once their reader was counted (131 -> 136 us with
 // tc_spec_verify behind, 200 rows).
 #include "tc_kernels.hpp"
 #include "tc_step.hpp"
@@ -19,7 +20,7 @@
 namespace tc {
 namespace {
 
-constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
+constexpr uint32_t kThreads = 512, kWaves = kThreads / 64;
 constexpr uint32_t kSeen = 0x80000000u;  // in a count: the token is in the history
 constexpr float kInf = __builtin_inff();
 
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
     }
     for (; i < h1; i += kThreads) count(a.r.history[i], i);
     if (biased) {
-        // each wave has a quarter of the chunk, and adds the biases there one after the other
+        // each wave has a part of the chunk, and adds the biases there one after the other
         constexpr uint32_t part = chunk / kWaves;
         const uint32_t p0 = lo + wave * part;
         for (uint32_t i0 = b0;;) {
@@ -234,13 +235,13 @@ hipError_t launch(const LogitCall &c, uint32_t parts, hipStream_t st) {
 }
 template <int XT>
 hipError_t launch(const LogitCall &c, int num_cu, hipStream_t st) {
-    // Chunks of 2048 tokens where those of 1024 are more than 4 to a CU (8 sequences 6.8 -> 6.3 us, 48
-    // 80 -> 66; 4 sequences 5.3 and 5.5); a sequence's rows by several workgroups, each of which counts
-    // the history, up to 8 to a CU (6 rows of one sequence 9.3 -> 5.7 us; up to 16 to a CU 6
-    // rows of 8 sequences 14.5 -> 17.5).
-    const uint64_t cu = num_cu, chunks = uint64_t((c.vocab + 1023) / 1024) * c.n_seq;
-    const bool wide = chunks > 4 * cu;
-    const uint64_t most = (c.n_tokens + c.n_seq - 1) / c.n_seq, fill = 8 * cu / (wide ? (chunks + 1) / 2 : chunks);
+    // Chunks of 4096 tokens where those of 2048 are more than 2 to a CU (6 rows of each of 8 sequences of
+    // 152064: 13.7 us, 16.1 with 2048; 4 sequences of a row 5.1 and 4.95); a sequence's rows by several
+    // workgroups, each of which counts the history, up to 4 to a CU (6 rows of each of 4 sequences
+    // 10.3 us, 12.9 with up to 2, 11.8 with up to 8).
+    const uint64_t cu = num_cu, chunks = uint64_t((c.vocab + 2047) / 2048) * c.n_seq;
+    const bool wide = chunks > 2 * cu;
+    const uint64_t most = (c.n_tokens + c.n_seq - 1) / c.n_seq, fill = 4 * cu / (wide ? (chunks + 1) / 2 : chunks);
     const uint32_t parts = uint32_t(fill < 1 ? 1 : fill < most ? fill : most);
     return wide ? launch<XT, 2>(c, parts, st) : launch<XT, 1>(c, parts, st);
 }
