@@ -97,6 +97,14 @@ def test_borders_of_chunks(tc, dev, V, n_seq):
     same(tc, dev, *make(rng, V, rows, hist, bias=5, masks=2, xtype="BF16"))
 
 
+# histories shorter than a load, and around what a workgroup loads at once, at the array's end and before it
+@pytest.mark.parametrize("hist", [[0, 0], [1, 0], [0, 2], [1, 2], [3, 1], [2, 0], [2047, 1], [1, 2048], [2049, 0], [6143, 2], [3, 6144],
+                                  [1, 6145], [10240, 3]])
+def test_lengths_of_histories(tc, dev, hist):
+    rng = np.random.default_rng(sum(hist))
+    same(tc, dev, *make(rng, 300, [1, 2], hist))
+
+
 def test_repeated_entries(tc, dev):
     """One token many times among the biases (added in their order: the sum depends on it), the history and the drafts."""
     V = 2000

@@ -4,8 +4,8 @@
 // there in LDS (integer sums, so their order changes nothing), adds up the biases in their
 // order, and then takes the sequence's rows one after the other, each row's own token counted
 // on top: every logit is read and written once, with its count and bias out of LDS beside it.
-// Bound by HBM for many rows (219 of 152064 logits with masks: 59 us of kernel, 271 MB at 4.6
-// TB/s; VALU 0.31 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.3
+// Bound by HBM for many rows (219 of 152064 logits with masks: 58 us of kernel, 272 MB at 4.7
+// TB/s; VALU 0.30 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.1
 // us), and between these by the history, which every chunk's workgroup reads (256 rows of 32003
 // 18 us, 15 without it, 10 for the bytes).
 //
@@ -24,8 +24,9 @@ constexpr uint32_t kThreads = 512, kWaves = kThreads / 64;
 constexpr uint32_t kSeen = 0x80000000u;  // in a count: the token is in the history
 constexpr float kInf = __builtin_inff();
 
-// (aligned to their elements: rows of an odd vocabulary)
+// (aligned to their elements: rows of an odd vocabulary, histories from any token on)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 __device__ __forceinline__ float widened(int type, uint32_t w) {
@@ -132,8 +133,12 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
             if (mask && i < n) words[v] = mask[i >> 5];
         }
     };
-    // each lane's first token of the history and of the biases
-    const int32_t first = h0 + tid < h1 ? a.r.history[h0 + tid] : -1;
+    // each lane's first four tokens of the history and its first of the biases; at the end of all
+    // histories the last four, of which a lane counts its own (219 rows 64.7 -> 64.4 us, one row 4.3 ->
+    // 4.1 with 16 bytes a load instead of 4)
+    auto four = [&](uint32_t i) { return u32x4(*reinterpret_cast<const u32x4u *>(a.r.history + min(i, a.r.n_history - 4))); };
+    u32x4 first = {0, 0, 0, 0};
+    if (h0 != h1 && a.r.n_history >= 4) first = four(h0 + 4 * tid);
     uint32_t bias_token = b0 + lane < b1 ? uint32_t(a.r.bias_token[b0 + lane]) : ~0u;
     float bias_value = b0 + lane < b1 ? a.r.bias_value[b0 + lane] : 0.0f;
     load(row);
@@ -154,17 +159,27 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
                 atomicAdd(counts + t, 1u);
         }
     };
-    uint32_t i = h0 + tid;
-    count(first, i);
-    // (8 on their way at a time)
-    for (i += kThreads; i + 7 * kThreads < h1; i += 8 * kThreads) {
-        int32_t t[8];
+    auto count4 = [&](const u32x4 &t, uint32_t i) {
+        const uint32_t at = min(i, a.r.n_history - 4);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = a.r.history[i + j * kThreads];
+        for (int j = 0; j < 4; ++j)
+            if (at + j >= i && at + j < h1) count(int32_t(t[j]), at + j);
+    };
+    uint32_t i = h0 + 4 * tid;
+    if (a.r.n_history >= 4) {
+        if (h0 != h1) {
+            count4(first, i);
+            for (i += 4 * kThreads; i < h1; i += 8 * kThreads) {
+                u32x4 t[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) count(t[j], i + j * kThreads);
+                for (int j = 0; j < 2; ++j) t[j] = four(i + j * 4 * kThreads);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) count4(t[j], i + j * 4 * kThreads);
+            }
+        }
+    } else {
+        for (i = h0 + tid; i < h1; i += kThreads) count(a.r.history[i], i);
     }
-    for (; i < h1; i += kThreads) count(a.r.history[i], i);
     if (biased) {
         // each wave has a part of the chunk, and adds the biases there one after the other
         constexpr uint32_t part = chunk / kWaves;
