@@ -258,3 +258,76 @@ def test_extreme_rows(tc, dev):
     kv = tc.kv_read(b.cache, b.batch, b.T, torch.float32)[0]
     assert not torch.isfinite(kv[0, 0]).any() and not torch.isfinite(kv[2, 1]).any()
     assert torch.isfinite(kv[[1, 3, 4, 5]]).all() and torch.isfinite(kv[0, 1]).all()
+
+
+# a prompt and sequences around it: enough rows that a lane has four heads, five and three of which leave some lanes fewer
+PROMPTS = [(1900, 1900), (1, 70), (0, 5), (160, 333), (3, 3)]
+
+
+@pytest.mark.parametrize("norms", [False, True])
+@pytest.mark.parametrize("ctype", ["F16", "BF16", "E4M3", "I8"])
+@pytest.mark.parametrize("xtype", ["F16", "BF16", "F32"])
+@pytest.mark.parametrize("layout,dim,n_rot", [("half", 128, 128), ("half", 128, 90), ("pairs", 128, 64), ("half", 80, 48),
+                                              ("pairs", 256, 250)])
+def test_prompts(tc, dev, layout, dim, n_rot, xtype, ctype, norms):
+    """Prompts' rows: queries in place among the rows of one product, cached keys and values; the rest as it was."""
+    rng = np.random.default_rng(dim + n_rot)
+    heads, kv, page = 5, 3, 32
+    b, x, q, k, v = setup(rng, dev, xtype, ctype, heads, kv, dim, page, PROMPTS, pad=3)
+    # (four heads a lane from 1024 workgroups of 256 lanes with one head each)
+    lanes = 16 if dim <= 128 else 32
+    assert b.T * (heads + 2 * kv) * lanes > 1200 * 256
+    rope = tc_hip.Rope(n_rot, 1e6, layout=layout, factor_of_values=1.25)
+    turns, _ = turns_exact(n_rot, 1e6)
+    w = [1 + 0.3 * rng.standard_normal(dim).astype(np.float32) if norms else None for _ in range(2)]
+    dw = [None if a is None else tensor(a, dev) for a in w]
+    before = {n: t.clone() for n, t in b.dev.items()}
+    given = x.clone()
+    assert tc.rope_kv_write(b.cache, b.batch, rope, q, k, v, q_norm=dw[0], k_norm=dw[1], eps=1e-5, out=q) is q
+    T = int(b.start[-1])
+    assert torch.equal(x[:, heads:], given[:, heads:]) and torch.equal(x[T:], given[T:])
+    pos = np.array([p for _, _, p in b.rows()])
+    page_of, place = (np.array(a) for a in zip(*(b.slot(s, p) for _, s, p in b.rows())))
+    want, err = rope_exact(f64(given[:T, :heads]), pos, turns, n_rot, layout, 1.25, w[0], 1e-5)
+    near(x[:T, :heads], want, err, xtype)
+    val, off = rope_exact(f64(given[:T, heads:heads + kv]), pos, turns, n_rot, layout, 1.25, w[1], 1e-5)
+    for name, val, off in (("k", val, off), ("v", f64(given[:T, heads + kv:]), np.zeros_like(val))):
+        got, old = (t[name].float().cpu().numpy().astype(np.float64) for t in (b.dev, before))
+        have = got[page_of, :, place]
+        if scaled(ctype):
+            # the factor's and the quotient's roundings, then half a step of the 8-bit number
+            have = have * f64(b.dev[name + "_scale"])[page_of, :, place][..., None]
+            d = np.abs(val).max(-1, keepdims=True) / TOP[ctype]
+            step = d / 2 if ctype == "I8" else np.maximum(2.0 ** -4 * np.abs(val), 2.0 ** -10 * d)
+            half = step * 1.001 + 3 * 2.0 ** -24 * np.abs(val) + 2 * off.max(-1, keepdims=True)
+        else:
+            half = HALF[ctype] * (np.abs(val) + off) + LEAST[ctype]
+        bad = np.abs(have - val) > off + half
+        assert not bad.any(), (name, np.argwhere(bad)[:4], have[bad][:4], val[bad][:4])
+        touched = np.zeros(got.shape[:1] + got.shape[2:3], bool)
+        touched[page_of, place] = True
+        keep = ~touched[:, None, :].repeat(kv, 1)
+        assert np.array_equal(got[keep], old[keep])
+        if scaled(ctype):
+            assert np.array_equal(f64(b.dev[name + "_scale"])[keep], f64(before[name + "_scale"])[keep])
+
+
+@pytest.mark.parametrize("layout,n_rot", [("half", 128), ("half", 122), ("pairs", 128)])
+@pytest.mark.parametrize("xtype", ["F16", "BF16", "F32"])
+def test_apply_prompts(tc, dev, xtype, layout, n_rot):
+    """Rows at positions, four heads a lane, in place at a stride."""
+    rng = np.random.default_rng(n_rot)
+    T, heads = 2500, 9
+    pos = rng.integers(-3, 200000, T).astype(np.int32)
+    pos[::7] = -1
+    wide = torch.from_numpy(rng.standard_normal((T, heads + 1, 128)).astype(np.float32)).to(DT[xtype]).to(dev)
+    before = wide.clone()
+    rope = tc_hip.Rope(n_rot, 1e6, layout=layout)
+    tc.rope(rope, wide[:, :heads], tensor(pos, dev), out=wide[:, :heads])
+    assert torch.equal(wide[:, heads], before[:, heads])
+    given = f64(before[:, :heads])
+    want, err = rope_exact(given, pos, turns_exact(n_rot, 1e6)[0], n_rot, layout, 1.0)
+    # (at 2 10^5 the product with the fp64 frequency and that itself are off by 2^-53 of 2^15 turns)
+    err += np.abs(given).max() * 2 * np.maximum(pos, 0)[:, None, None] * 2.0 ** -52
+    want[pos < 0], err[pos < 0] = given[pos < 0], 0
+    near(wide[:, :heads], want, err, xtype)
