@@ -26,7 +26,8 @@ def weights(rng, D, dev, kind, offset=0.0, bias=None):
     return n, (w.astype(np.float64), None if b is None else b.astype(np.float64), float(np.float32(1e-5)), kind, offset)
 
 
-# every kernel variant: a wave per row, one and several waves, 2 and 4 blocks of a lane, at their borders; odd widths
+# few rows: 8, 16 and 64 lanes to a row, one and several waves, 2, 3 and 4 blocks of a lane, at their borders; odd widths (rows of
+# 129 to 256 columns, and prompts' many rows: test_rows_of_half_a_wave, test_rows_of_prompts)
 COLS = [1, 7, 8, 100, 512, 513, 520, 1024, 3584, 5119, 5120, 8192, 8200, 16384, 16392, 17407, 32768]
 
 
@@ -242,3 +243,39 @@ def test_binding_refusals(tc, dev):
                 lambda: tc.norm_add(h, h, pre=n, act_type=Q4_K, act=torch.zeros(8, dtype=torch.uint8, device=dev))):
         with pytest.raises(tc_hip.TCError):
             bad()
+
+
+@pytest.mark.parametrize("cols", [129, 200, 255, 256])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("h_type,y_type,x_type", [("F32", "F32", "F32"), ("BF16", "BF16", "BF16"), ("F32", "F16", "BF16")])
+def test_rows_of_half_a_wave(tc, dev, cols, kind, h_type, y_type, x_type):
+    """Widths that 32 lanes have, rows that the last workgroup has not all of."""
+    both_norms(tc, dev, 21, cols, kind, h_type, y_type, x_type)
+
+
+# more rows than two for each of the card's 256 CUs: two blocks of a lane, workgroups of up to 512
+@pytest.mark.parametrize("cols", [513, 1000, 1024, 5119, 5120, 8192])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("h_type,y_type,x_type", [("F32", "F32", "F32"), ("BF16", "BF16", "BF16"), ("F32", "F16", "BF16")])
+def test_rows_of_prompts(tc, dev, cols, kind, h_type, y_type, x_type):
+    both_norms(tc, dev, 530, cols, kind, h_type, y_type, x_type)
+
+
+def both_norms(tc, dev, T, cols, kind, h_type, y_type, x_type):
+    """Both norms, one of them and none, with a gate of each row."""
+    rng = np.random.default_rng(cols + T)
+    h, y = rows(rng, T, cols, h_type, dev, 3.0), rows(rng, T, cols, y_type, dev)
+    post, p = weights(rng, cols, dev, kind)
+    pre, r = weights(rng, cols, dev, kind, offset=1.0)
+    gate = torch.from_numpy(rng.standard_normal((T, 1)).astype(np.float32)).to(dev)
+    scale = float(np.float32(0.22))
+    for a, b in ((post, p), (None, None)):
+        want = norm_add_exact(f64(h), f64(y), r, b, f64(gate), True, scale)
+        h2, x = tc.norm_add(h, y, pre=pre, post=a, gate=gate, sigmoid=True, scale=0.22, out_dtype=DT[x_type])
+        near(h2, want[0], want[1], h_type, "h")
+        near(x, want[2], want[3], x_type, "x")
+        mine = h.clone()
+        h3, none = tc.norm_add(mine, y, post=a, gate=gate, sigmoid=True, scale=0.22, h_out=mine)
+        assert h3 is mine and none is None and torch.equal(h3, h2)
+    want = norm_add_exact(f64(h), None, r, None, None, False, 1.0)
+    near(tc.norm(h, pre, out_dtype=DT[x_type]), want[2], want[3], x_type, "norm")
