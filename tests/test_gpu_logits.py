@@ -193,3 +193,16 @@ def test_strides_and_in_place(tc, dev, xtype):
                 lambda: tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev), out=torch.zeros(5, 1001, device=dev).half())):
         with pytest.raises(tc_hip.TCError):
             bad()
+
+
+def test_rows_of_no_sequence(tc, dev):
+    """Rows in front of the first sequence, behind the last and between borders that go backwards stay as they are."""
+    rng = np.random.default_rng(13)
+    r, l, _, tokens = make(rng, 2100, [3, 3, 2], [9, 9, 9], bias=3, masks=2)
+    for start, own in (([1, 3, 3, 5], [1, 2, 3, 4]), ([5, 2, 4, 4], [2, 3]), ([2, 4, 3, 3], [2, 3]), ([6, 6, 1, 0], [])):
+        start = np.array(start, np.int32)
+        out = torch.full(l.shape, 7.0, device=dev)
+        tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev), tokens=tensor(tokens, dev), out=out)
+        rest = [t for t in range(8) if t not in own]
+        assert (out[rest] == 7.0).all(), start
+        close(out[own], logits_exact(f64(l), start, tokens, **r)[own])
