@@ -181,7 +181,9 @@ typedef struct tc_logit_rules {
     const float *repetition, *frequency, *presence;   /* [n_seq]; NULL: 1, 0, 0 */
     const int32_t *history;           /* [n_history] tokens, sequence s's from history_start[s] to history_start[s + 1] - 1; */
     const int32_t *history_start;     /* [n_seq + 1]; NULL: nothing has gone before the step's tokens */
-    const int32_t *prompt;            /* [n_seq] how many of them were asked, not answered; NULL: none */
+    const int32_t *prompt;            /* [n_seq] how many of them were asked, not answered; -n: the first n of them and of
+                                       * the step's tokens behind them (a sequence's prompt may be among its rows then);
+                                       * NULL: none */
     uint32_t n_history;
     const int32_t *bias_start;        /* [n_seq + 1]; NULL: no biases */
     const int32_t *bias_token;        /* [n_bias], sequence s's from bias_start[s] to bias_start[s + 1] - 1 */
@@ -199,7 +201,9 @@ typedef struct tc_logit_rules {
  *   + the biases for t, added up in their order
  *   -infinity,                                where the row's mask has a 0 for t, whatever l is
  * For row start[s]+i the tokens start[s] .. start[s]+i of `tokens` ([n_tokens], the step's tokens; NULL:
- * none are counted) have been answered after the history. Where a token's logit changes it is formed in
+ * none are counted) have come after the history: answered, but for those that prompt[s] below 0 goes on
+ * over. So a prompt of n tokens, given as -n from its first chunk to its sequence's last token, is never
+ * taken for answers, while any number above 0 (or NULL) wants rows without prompts in them. Where a token's logit changes it is formed in
  * fp64 and rounded once (the sum of its biases is fp32). Tokens outside [0, vocab) are passed over.
  * logits: [n_tokens] rows of xtype at x_stride elements, aligned to their type; out: fp32 rows at
  * out_stride; out may be logits, if these are F32 with the same stride, and does not overlap them

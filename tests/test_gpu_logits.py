@@ -195,6 +195,67 @@ def test_strides_and_in_place(tc, dev, xtype):
             bad()
 
 
+def row_by_row(l, start, tokens, r):
+    """logits_exact where prompt[s] below 0 counts -prompt[s] tokens of the history and of the step's behind it: every row by
+    itself, with its tokens at the end of its history and what of all that was asked worked out here."""
+    want = np.full(l.shape, np.nan)
+    for s in range(len(start) - 1):
+        had = r["history"][r["history_start"][s]:r["history_start"][s + 1]]
+        for t in range(start[s], start[s + 1]):
+            now = had if tokens is None else np.concatenate([had, tokens[start[s]:t + 1]])
+            p = int(r["prompt"][s])
+            one = dict(history=now, history_start=[0, len(now)], prompt=[-p if p < 0 else min(p, len(had))])
+            one.update({n: r[n][s:s + 1] for n in ("repetition", "frequency", "presence")})
+            if "bias_start" in r:
+                one.update(bias_start=r["bias_start"][s:s + 2], bias_token=r["bias_token"], bias_value=r["bias_value"])
+            if "mask" in r:
+                one.update(mask=r["mask"], mask_of=r["mask_of"][t:t + 1])
+            want[t] = logits_exact(l[t:t + 1], [0, 1], None, **one)[0]
+    return want
+
+
+# prompts from their first token on, chunks of prompts, prompts that end among the rows (drafts behind them), decoding
+# sequences, and rows that several workgroups share
+@pytest.mark.parametrize("xtype", ["F32", "BF16"])
+@pytest.mark.parametrize("V", [50, 2049, 9001])
+@pytest.mark.parametrize("rows,hist,asked", [
+    ([30], [0], [30]), ([30], [0], [100]), ([9, 1, 5, 4], [0, 40, 20, 7], [9, 12, 24, 11]), ([6, 6], [3000, 10], [3003, 4]),
+    ([1] * 300, [3] * 300, list(range(1, 301))), ([700], [20], [650]), ([2, 3], [5, 5], [2 ** 31, 2 ** 31 - 1])])
+def test_tokens_that_were_asked(tc, dev, rows, hist, asked, V, xtype):
+    """A prompt's own rows are asked, not answered: repetition alone counts them."""
+    rng = np.random.default_rng(V + len(rows))
+    r, l, start, tokens = make(rng, V, rows, hist, bias=3, masks=2, xtype=xtype)
+    r["prompt"][:] = [-a for a in asked]
+    x = tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev), tokens=tensor(tokens, dev))
+    close(x, row_by_row(f64(l), start, tokens, r))
+    # without the rows' tokens: of the history alone, as with the same number above 0
+    x = tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev))
+    r["prompt"][:] = [min(a, 2 ** 31 - 1) for a in asked]
+    assert torch.equal(x, tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev)))
+    # above 0: of the history alone, whatever else stands there
+    got = tc.logits_adjust(rules(r, dev), l.to(dev), tensor(start, dev), tokens=tensor(tokens, dev))
+    close(got, logits_exact(f64(l), start, tokens, **r))
+
+
+def test_a_prompts_first_answer(tc, dev):
+    """A prompt in chunks gets the logits that it gets as a history all at once, and no penalty on what it only asked."""
+    rng = np.random.default_rng(12)
+    V, n = 500, 37
+    text = rng.integers(0, V, n).astype(np.int32)
+    l = torch.from_numpy(rng.standard_normal((n, V)).astype(np.float32)).to(dev)
+    f = lambda v: np.full(1, v, np.float32)  # noqa: E731
+    base = dict(repetition=f(1.0), frequency=f(0.5), presence=f(0.7), prompt=np.array([-n], np.int32))
+    for done in (0, 20, 36):
+        r = dict(base, history=text[:done], history_start=np.array([0, done], np.int32))
+        x = tc.logits_adjust(rules(r, dev), l[done:], tensor(np.array([0, n - done], np.int32), dev), tokens=tensor(text[done:], dev))
+        assert torch.equal(x, l[done:])
+    r = dict(base, history=text, history_start=np.array([0, n], np.int32))
+    answer = np.array([text[3], text[3]], np.int32)
+    x = tc.logits_adjust(rules(r, dev), l[:2], tensor(np.array([0, 2], np.int32), dev), tokens=tensor(answer, dev))
+    close(x, logits_exact(f64(l[:2]), [0, 2], answer, **dict(r, prompt=[n])))
+    assert (x != l[:2]).sum() == 2
+
+
 def test_rows_of_no_sequence(tc, dev):
     """Rows in front of the first sequence, behind the last and between borders that go backwards stay as they are."""
     rng = np.random.default_rng(13)

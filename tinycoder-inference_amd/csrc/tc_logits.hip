@@ -3,7 +3,7 @@
 // A workgroup has a chunk of the vocabulary for one sequence. It counts the sequence's history
 // there in LDS (integer sums, so their order changes nothing), adds up the biases in their
 // order, and then takes the sequence's rows one after the other, each row's own token counted
-// on top: every logit is read and written once, with its count and bias out of LDS beside it.
+// on top (as seen alone while it is the prompt's): every logit is read and written once, with its count and bias out of LDS beside it.
 // Bound by HBM for many rows (219 of 152064 logits with masks: 58 us of kernel, 272 MB at 4.7
 // TB/s; VALU 0.30 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.1
 // us), and between these by the history, which every chunk's workgroup reads (256 rows of 32003
@@ -114,7 +114,10 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
     if (row >= end) return;
     const bool counted = rep != 1.0f || freq != 0.0f || pres != 0.0f, biased = b0 != b1;
     if (!counted) h1 = h0;
-    const uint32_t answers = h0 + min(asked < 0 ? 0u : uint32_t(asked), h1 - h0);
+    // tokens that were asked: of the history those before `answers`, and of the rows' own, where
+    // the number goes on over them (below 0), the first asked_rows
+    const uint32_t ask = asked < 0 ? 0u - uint32_t(asked) : uint32_t(asked), past = min(ask, h1 - h0);
+    const uint32_t answers = h0 + past, asked_rows = asked < 0 ? ask - past : 0;
     // the first row is on its way while the history is counted, each other one while the row
     // before it is worked on
     float l[V][4];
@@ -150,10 +153,10 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) *reinterpret_cast<u32x4 *>(lds + chunk + tid * 4 + v * step) = zero;
     __syncthreads();
-    auto count = [&](int32_t token, uint32_t i) {
+    auto count = [&](int32_t token, bool only_seen) {
         const uint32_t t = uint32_t(token) - lo;
         if (t < n) {
-            if (i < answers)
+            if (only_seen)
                 atomicOr(counts + t, kSeen);
             else
                 atomicAdd(counts + t, 1u);
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
         const uint32_t at = min(i, a.r.n_history - 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (at + j >= i && at + j < h1) count(int32_t(t[j]), at + j);
+            if (at + j >= i && at + j < h1) count(int32_t(t[j]), at + j < answers);
     };
     uint32_t i = h0 + 4 * tid;
     if (a.r.n_history >= 4) {
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
             }
         }
     } else {
-        for (i = h0 + tid; i < h1; i += kThreads) count(a.r.history[i], i);
+        for (i = h0 + tid; i < h1; i += kThreads) count(a.r.history[i], i < answers);
     }
     if (biased) {
         // each wave has a part of the chunk, and adds the biases there one after the other
@@ -203,10 +206,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitCall a) {
     const bool own_tokens = counted && a.tokens;
     for (uint32_t told = begin; row < end; row += gridDim.z) {
         if (own_tokens) {
-            for (told += tid; told <= row; told += kThreads) {
-                const uint32_t t = uint32_t(a.tokens[told]) - lo;
-                if (t < n) atomicAdd(counts + t, 1u);
-            }
+            for (told += tid; told <= row; told += kThreads) count(a.tokens[told], told - begin < asked_rows);
             told = row + 1;
             __syncthreads();
         }

@@ -379,7 +379,8 @@ class LogitRules:
     """What is done to a batch's logits (tc_logit_rules), every tensor contiguous, on one
     device, or None: repetition, frequency, presence fp32 [n_seq]; history int32 (the
     sequences' tokens one behind the other) with history_start int32 [n_seq + 1] and
-    prompt int32 [n_seq]; bias_token int32, bias_value fp32 with bias_start int32
+    prompt int32 [n_seq] (how many of them were asked; -n: n of them and of the step's tokens
+    behind them, for prompts among the rows); bias_token int32, bias_value fp32 with bias_start int32
     [n_seq + 1]; mask int32 [n_masks][words] (32 tokens a word) with mask_of int32
     [n_tokens]. Other numbers may be written into the tensors between calls."""
 
