@@ -279,3 +279,24 @@ def both_norms(tc, dev, T, cols, kind, h_type, y_type, x_type):
         assert h3 is mine and none is None and torch.equal(h3, h2)
     want = norm_add_exact(f64(h), None, r, None, None, False, 1.0)
     near(tc.norm(h, pre, out_dtype=DT[x_type]), want[2], want[3], x_type, "norm")
+
+
+def test_norm_add_without_a_block(tc, dev):
+    """No block's output: the residual stream is what it was, and no other memory is given for it."""
+    rng = np.random.default_rng(7)
+    h = rows(rng, 3, 512, "BF16", dev)
+    pre, _ = weights(rng, 512, dev, "rms")
+    act, other = (torch.zeros(tc.lib.tc_act_bytes(Q4_K, 3, 512), dtype=torch.uint8, device=dev) for _ in range(2))
+    got, x = tc.norm_add(h, None, pre=pre, act_type=Q4_K, act=act)
+    assert got is h and torch.equal(x, tc.norm(h, pre))
+    wide = tc.norm(h, pre, out_dtype=torch.float32)
+    tc._check(tc.lib.tc_act_quantize(Q4_K, tc_hip._ptr(wide), 3, 512, tc_hip._ptr(other), tc._stream()))
+    assert torch.equal(act, other)
+    assert tc.norm_add(h, None, pre=pre, h_out=h)[0] is h
+    got, none = tc.norm_add(h, None)
+    assert got is h and none is None
+    keep = torch.full_like(h, 7.0)
+    for bad in (dict(h_out=keep), dict(gate=torch.ones(3, 1, device=dev)), dict(post=pre)):
+        with pytest.raises(tc_hip.TCError):
+            tc.norm_add(h, None, pre=pre, **bad)
+    assert (keep == 7.0).all()

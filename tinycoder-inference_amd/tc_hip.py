@@ -768,11 +768,15 @@ class Library:
     def norm_add(self, h, y, pre=None, post=None, gate=None, sigmoid=False, scale=1.0, out_dtype=None, h_out=None, out=None,
                  act_type=0, act=None):
         """h + scale * gate * post(y) into h_out (h itself may be given), and pre of that, of
-        out_dtype (h's) into out: (h_out, out); without `pre` out is None. gate [cols],
+        out_dtype (h's) into out: (h_out, out); without `pre` out is None, without y the first is h. gate [cols],
         [rows][1] or [rows][cols]. act: a buffer of
         tc_act_bytes for the activations quantized for weights of act_type, as act_quantize."""
         torch = self._torch
-        if h_out is None:
+        if y is None:  # (the call writes no h_out then)
+            if h_out is not None and h_out is not h:
+                raise TCError(TC_E_ARG, "h_out without the block's output y")
+            h_out = h
+        elif h_out is None:
             h_out = torch.empty_like(h, memory_format=torch.contiguous_format)
         if out is None and pre is not None:
             out = torch.empty_like(h, dtype=out_dtype, memory_format=torch.contiguous_format)
