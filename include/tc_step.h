@@ -111,8 +111,8 @@ typedef struct tc_norm_rows {
  * from the fp32 values that an F32 x has, and is tc_act_quantize's of them bit for bit.
  * cols up to 32768. Rows may have any stride that keeps them apart and any
  * alignment that fits their elements. Outputs do not overlap inputs, apart from h_out = h with the same stride. An
- * infinity or NaN stays in its row; squares that pass fp32's range (values past 10^19) give
- * an infinite mean. */
+ * infinity or NaN stays in its row; squares that pass fp32's range (values past 1.8 10^19) give
+ * an infinite mean, and rows whose root mean square is below 10^-16 lose bits of it where eps is below 10^-30. */
 int tc_norm_add(const tc_norm_rows *rows, void *stream);
 
 /* ---- rotary positions ------------------------------------------------------------ */

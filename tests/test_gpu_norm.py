@@ -281,6 +281,26 @@ def both_norms(tc, dev, T, cols, kind, h_type, y_type, x_type):
     near(tc.norm(h, pre, out_dtype=DT[x_type]), want[2], want[3], x_type, "norm")
 
 
+def test_squares_near_the_range(tc, dev):
+    """A square that fp32 holds makes no infinite mean, whatever the width; without eps, rows down to 10^-16 keep their bits."""
+    rng = np.random.default_rng(6)
+    for cols in (5, 100, 200, 600, 3584, 5119, 12000, 24577, 32767, 32768):
+        sign = np.where(rng.random((3, cols)) < 0.5, -1.0, 1.0)
+        for kind in ("rms", "layer"):
+            for big in (1.8e19, 1e-16):
+                z = (big * sign).astype(np.float32)
+                if big > 1:
+                    z[1] = np.abs(z[1])  # (of a layer norm's: a constant row, zeros over eps)
+                h = tensor(z, dev)
+                eps = float(np.float32(1e-5)) if big > 1 else 0.0
+                if kind == "layer" and big > 1:  # (differences from the mean stay below the largest value)
+                    h = h * 0.5
+                want = norm_add_exact(f64(h), None, (None, None, eps, kind, 0.0), None, None, False, 1.0)
+                x = tc.norm(h, tc_hip.Norm(eps=eps, kind=kind))
+                use = [0, 2] if kind == "layer" else [0, 1, 2]
+                near(x[use], want[2][use], want[3][use], "F32", (cols, kind, big))
+
+
 def test_norm_add_without_a_block(tc, dev):
     """No block's output: the residual stream is what it was, and no other memory is given for it."""
     rng = np.random.default_rng(7)

@@ -170,8 +170,8 @@ __device__ __forceinline__ void norm_row(const NormCall &a, const NormArgs &n, c
             own_only<TINY>(at[c], cols, z[c]);
         }
     }
-    // (squares times a power of two near 1 / cols, so that their sum passes fp32's range no sooner
-    // than the largest square does)
+    // (squares times a power of two, 1 / cols or just below, so that their sum passes fp32's range no
+    // sooner than the largest square does)
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -389,7 +389,7 @@ constexpr uint32_t kRowsMost = 1u << 21;  // of a launch: a grid has less than 2
 hipError_t launch_norm(const NormCall &call, int num_cu, hipStream_t st) {
     NormCall a = call;
     int up = 0;
-    while ((2u << up) <= a.cols) ++up;
+    while ((1u << up) < a.cols) ++up;
     a.inv_cols = 1.0f / float(a.cols);
     a.down = std::ldexp(1.0f, -up);
     a.inv_cols_down = std::ldexp(a.inv_cols, up);

@@ -69,7 +69,7 @@ struct NormCall {
     int16_t *bsums;
     uint16_t *dg;
     int32_t act_q8_0;  // 32-wide blocks instead of 256-wide ones
-    // (set by the launcher) 1 / cols, a power of two near it, their quotient
+    // (set by the launcher) 1 / cols, the power of two at it or below, their quotient
     float inv_cols, down, inv_cols_down;
 };
 hipError_t launch_norm(const NormCall &c, int num_cu, hipStream_t st);
