@@ -155,7 +155,9 @@ int tc_rope_turns(const tc_rope_scaling *scaling, uint32_t n_rot, double theta, 
 /* Rotates rows of `xtype`, [heads][head_dim] each, row t at x + t * x_stride elements, at
  * position[t], into out ([n_tokens] rows at out_stride); out may be x with the same
  * stride. Rows with a position below 0 are not touched. head_dim: a multiple of 16, up to
- * 256; bases and strides of 16 bytes' multiples. */
+ * 256; bases and strides of 16 bytes' multiples. Up to 4096 heads and 2^24 rows; n_tokens * heads
+ * below 2^31 - 256, and n_tokens * ceil(heads / 4) * (head_dim / 8, up to a power of two) at
+ * most 2^32 - 256. */
 int tc_rope_apply(const tc_rope *rope, int xtype, const void *x, uint32_t x_stride, void *out, uint32_t out_stride,
                   const int32_t *position, uint32_t n_tokens, uint32_t heads, uint32_t head_dim, void *stream);
 
@@ -166,10 +168,11 @@ int tc_rope_apply(const tc_rope *rope, int xtype, const void *x, uint32_t x_stri
  * keys' heads likewise with k_norm, and written to their slots of the cache, as tc_kv_write
  * writes k; the values are written as tc_kv_write writes v. Between loading and the one
  * rounding at the end values are fp32 (a norm's squares too: heads with values past 10^18 get an infinite
- * mean). Rows are laid out as tc_kv_write's k and v, and q
+ * mean, and those whose root mean square is below 10^-18 lose bits of it where eps is below 10^-34). Rows are laid out as tc_kv_write's k and v, and q
  * as tc_attn's; parts of one fused product's rows are fine. q may be NULL (heads 0): keys and
  * values only. Rows past the last sequence are not touched; q_out is written also for rows
- * whose position has no slot. heads up to 4096. eps: finite, at least 0. */
+ * whose position has no slot. heads up to 4096; sizes as tc_rope_apply's, with keys' and values' heads
+ * counted too. eps: finite, at least 0. */
 int tc_rope_kv_write(const tc_kv_cache *cache, const tc_kv_batch *batch, const tc_rope *rope, int xtype, const void *q,
                      uint32_t q_stride, void *q_out, uint32_t heads, const void *k, uint32_t k_stride, const void *v,
                      uint32_t v_stride, const float *q_norm, const float *k_norm, float eps, void *stream);

@@ -331,3 +331,17 @@ def test_apply_prompts(tc, dev, xtype, layout, n_rot):
     err += np.abs(given).max() * 2 * np.maximum(pos, 0)[:, None, None] * 2.0 ** -52
     want[pos < 0], err[pos < 0] = given[pos < 0], 0
     near(wide[:, :heads], want, err, xtype)
+
+
+def test_head_norms_near_the_range(tc, dev):
+    """Squares of values around 10^18 and 10^-18, without eps."""
+    rng = np.random.default_rng(9)
+    for dim in (64, 256):
+        b, x, q, k, v = setup(rng, dev, "F32", "BF16", 3, 1, dim, 16, seqs=[(9, 9)], pad=0)
+        for size in (1e18, 1e-18):
+            sign = np.where(rng.random((9, 3, dim)) < 0.5, -1.0, 1.0)
+            q.copy_(tensor((size * sign).astype(np.float32), dev))
+            rope = tc_hip.Rope(dim, 1e4)
+            out = tc.rope_kv_write(b.cache, b.batch, rope, q, k, v, q_norm=torch.ones(dim, device=dev), eps=0.0)
+            want, err = rope_exact(f64(q), np.arange(9), turns_exact(dim, 1e4)[0], dim, "half", 1.0, np.ones(dim), 0.0)
+            near(out, want, err, "F32")

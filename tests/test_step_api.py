@@ -267,3 +267,27 @@ def test_rules_class_refusals():
         with pytest.raises(tc_hip.TCError):
             tc_hip.LogitRules(**bad)
     tc_hip.LogitRules()
+
+
+def test_rope_launch_limits(lib):
+    """More lanes than a grid has threads (below 2^32) are refused by name, before a launch. Four heads of a row are a
+    lane's; a head has head_dim / 8 lanes, rounded up to a power of two."""
+    row = 33 * 144
+    for kw, dim in ((dict(n=1 << 24, heads=33, xs=row, os=row, dim=144, xtype=30), 144),
+                    (dict(n=1 << 24, heads=32, xs=32 * 256, os=32 * 256, dim=256, xtype=30), 256),
+                    (dict(n=1 << 24, heads=64, xs=64 * 128, os=64 * 128, dim=128, xtype=30), 128)):
+        assert apply(lib, **kw) == UNSUPPORTED
+        assert "lanes" in lib.tc_last_error().decode(), kw
+    # one step below each of them is a matter of the device alone
+    for kw in (dict(n=1 << 24, heads=28, xs=28 * 144, os=28 * 144, dim=144, xtype=30),
+               dict(n=1 << 24, heads=60, xs=60 * 128, os=60 * 128, dim=128, xtype=30)):
+        if not torch.cuda.is_available():
+            assert apply(lib, **kw) == UNSUPPORTED
+            assert "gfx950" in lib.tc_last_error().decode(), kw
+    c = cache(head_dim=144, kv_heads=1)
+    kw = dict(c=c, xtype=30, ks=144, vs=144, eps=0.0)
+    assert rope_write(lib, b=batch(n_tokens=1 << 24), heads=31, qs=31 * 144, qo=P + 16, **kw) == UNSUPPORTED
+    assert "lanes" in lib.tc_last_error().decode()
+    if not torch.cuda.is_available():
+        assert rope_write(lib, b=batch(n_tokens=1 << 24), heads=26, qs=26 * 144, qo=P + 16, **kw) == UNSUPPORTED
+        assert "gfx950" in lib.tc_last_error().decode()

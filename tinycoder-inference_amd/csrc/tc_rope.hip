@@ -296,8 +296,8 @@ __global__ __launch_bounds__(64) void k_rope_turns(TurnsCall a) {
 
 RopeWalk make_walk(const RopeCall &c, uint32_t units, uint32_t per_lane, uint32_t *blocks) {
     RopeWalk w;
-    w.lanes = 2, w.lane_log = 1;
-    while (w.lanes * 8 < c.kv.dim) w.lanes *= 2, ++w.lane_log;
+    w.lane_log = rope_lane_log(c.kv.dim);
+    w.lanes = 1u << w.lane_log;
     w.units = units;
     const uint32_t groups = (units + per_lane - 1) / per_lane;
     w.groups = make_divmod(groups);
@@ -316,8 +316,8 @@ hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
     if (blocks <= 1024) {
         k_rope<CT, W, L, 1><<<blocks, kThreads, 0, st>>>(c, w);
     } else {
-        w = make_walk(c, units, 4, &blocks);
-        k_rope<CT, W, L, 4><<<blocks, kThreads, 0, st>>>(c, w);
+        w = make_walk(c, units, kRopeUnits, &blocks);
+        k_rope<CT, W, L, kRopeUnits><<<blocks, kThreads, 0, st>>>(c, w);
     }
     return hipGetLastError();
 }

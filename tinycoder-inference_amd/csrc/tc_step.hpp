@@ -36,6 +36,13 @@ struct RopeCall {
     float eps;
     int xtype;
 };
+constexpr uint32_t kRopeUnits = 4;  // heads of a lane in long calls
+// Lanes that have a head between them.
+inline uint32_t rope_lane_log(uint32_t dim) {
+    uint32_t log = 1;
+    while ((16u << (log - 1)) < dim) ++log;
+    return log;
+}
 hipError_t launch_rope_kv(const RopeCall &c, int ctype, hipStream_t st);
 hipError_t launch_rope_rows(const RopeCall &c, hipStream_t st);
 // Turns of pair i: theta^(-2i / n_rot) / 2 pi, changed as the kind says; first, ramp: where

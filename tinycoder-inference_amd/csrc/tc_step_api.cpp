@@ -26,6 +26,16 @@ int check_rope(const tc_rope *r, uint32_t head_dim, tc::RopeArgs *a) {
     return TC_OK;
 }
 
+// `units` heads of each of n rows: what the kernels count in 32 bits, and the threads of a grid, whose
+// workgroups are of 256.
+int check_rope_size(uint32_t n, uint64_t units, uint32_t head_dim) {
+    if (n * units >= (uint64_t(1) << 31) - 256) return refuse(TC_E_UNSUPPORTED, "2^31 heads of rows or more");
+    const uint64_t groups = (units + tc::kRopeUnits - 1) / tc::kRopeUnits;
+    if ((n * groups << tc::rope_lane_log(head_dim)) > (uint64_t(1) << 32) - 256)
+        return refuse(TC_E_UNSUPPORTED, "2^32 lanes or more (head_dim / 8, up to a power of two, for every 4 heads of a row)");
+    return TC_OK;
+}
+
 int check_norm(const tc_norm *n, tc::NormArgs *a) {
     *a = {nullptr, nullptr, 0.0f, 0.0f, -1};
     if (!n) return TC_OK;
@@ -181,8 +191,8 @@ int tc_rope_apply(const tc_rope *rope, int xtype, const void *x, uint32_t x_stri
     tc::RopeCall c{};
     int rc = check_rope(rope, head_dim, &c.rope);
     if (rc) return rc;
-    if (n_tokens > (1u << 24) || uint64_t(n_tokens) * heads >= (uint64_t(1) << 31) - 256)
-        return refuse(TC_E_UNSUPPORTED, "2^24 rows, or 2^31 heads of rows, or more");
+    if (n_tokens > (1u << 24)) return refuse(TC_E_UNSUPPORTED, "more than 2^24 rows");
+    if ((rc = check_rope_size(n_tokens, heads, head_dim))) return rc;
     if (n_tokens == 0) return TC_OK;
     const uint64_t width = uint64_t(heads) * head_dim;
     if ((rc = check_rows("x", x, x_stride, width, n_tokens, xtype))) return rc;
@@ -214,8 +224,7 @@ int tc_rope_kv_write(const tc_kv_cache *cache, const tc_kv_batch *batch, const t
     if (!aligned_to(q_norm, 4) || !aligned_to(k_norm, 4))
         return refuse(TC_E_UNSUPPORTED, "a norm's weights must be 4-byte aligned");
     const uint32_t n = c.kv.n_tokens;
-    const uint64_t units = uint64_t(heads) + 2 * c.kv.kv_heads;
-    if (uint64_t(n) * units >= (uint64_t(1) << 31) - 256) return refuse(TC_E_UNSUPPORTED, "2^31 heads of rows or more");
+    if ((rc = check_rope_size(n, uint64_t(heads) + 2 * c.kv.kv_heads, c.kv.dim))) return rc;
     if (n == 0 || c.kv.n_seq == 0) return TC_OK;
     const uint64_t width = uint64_t(c.kv.kv_heads) * c.kv.dim, q_width = uint64_t(heads) * c.kv.dim;
     if (heads != 0) {
