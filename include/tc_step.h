@@ -211,7 +211,7 @@ typedef struct tc_logit_rules {
  * logits: [n_tokens] rows of xtype at x_stride elements, aligned to their type; out: fp32 rows at
  * out_stride; out may be logits, if these are F32 with the same stride, and does not overlap them
  * otherwise. Rows past the last sequence are not touched. n_seq and n_tokens up to 65535,
- * vocab to 2^30, n_history and n_bias to 2^31 - 1. */
+ * vocab to 2^30, n_history to 2^31 - 2^16, n_bias to 2^31 - 1. */
 int tc_logits_adjust(const tc_logit_rules *rules, int xtype, const void *logits, uint32_t x_stride, uint32_t vocab,
                      uint32_t n_seq, uint32_t n_tokens, const int32_t *start, const int32_t *tokens, float *out,
                      uint32_t out_stride, void *stream);

@@ -291,3 +291,13 @@ def test_rope_launch_limits(lib):
     if not torch.cuda.is_available():
         assert rope_write(lib, b=batch(n_tokens=1 << 24), heads=26, qs=26 * 144, qo=P + 16, **kw) == UNSUPPORTED
         assert "gfx950" in lib.tc_last_error().decode()
+
+
+def test_history_limit(lib):
+    """A history's counts and the rows' own tokens behind them stay in 31 bits."""
+    most = (1 << 31) - (1 << 16)
+    assert logits(lib, n_history=most + 1) == UNSUPPORTED
+    assert "2^31" in lib.tc_last_error().decode()
+    if not torch.cuda.is_available():
+        assert logits(lib, n_history=most) == UNSUPPORTED
+        assert "gfx950" in lib.tc_last_error().decode()

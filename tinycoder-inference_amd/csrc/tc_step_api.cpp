@@ -251,7 +251,9 @@ int tc_logits_adjust(const tc_logit_rules *r, int xtype, const void *logits, uin
     if (!row_type(xtype)) return refuse(TC_E_UNSUPPORTED, "unsupported row type " + std::to_string(xtype));
     if (vocab == 0 || vocab > (1u << 30) || n_tokens > 65535 || n_seq > 65535)
         return refuse(TC_E_UNSUPPORTED, "an empty vocabulary, more than 2^30 tokens in it, 65535 rows or 65535 sequences");
-    if (r->n_history > 0x7FFFFFFFu || r->n_bias > 0x7FFFFFFFu) return refuse(TC_E_UNSUPPORTED, "2^31 listed tokens or more");
+    // (a token's count, of the history and 65535 rows, has 31 bits)
+    if (r->n_history > 0x7FFF0000u || r->n_bias > 0x7FFFFFFFu)
+        return refuse(TC_E_UNSUPPORTED, "more than 2^31 - 2^16 tokens of history, or 2^31 biases or more");
     if (r->history_start && r->n_history != 0 && !r->history) return refuse(TC_E_ARG, "a history without its tokens");
     if (r->bias_start && r->n_bias != 0 && (!r->bias_token || !r->bias_value)) return refuse(TC_E_ARG, "biases without tokens or values");
     if (r->mask && uint64_t(r->mask_words) * 32 < vocab) return refuse(TC_E_ARG, "mask_words is too small for the vocabulary");
