@@ -59,8 +59,8 @@ typedef struct tc_plan {
 
 /* Rows go to the sequences in their order: start[s] = min(n_tokens, sum of new_tokens[r]
  * over r < s), and len[s] = held[s] + the rows of s. A sequence that has ended gets no
- * rows, length 0 and no pages; its pages go behind the free ones, sequences in their order,
- * before any is given out (those that the ring has no room for are lost: a ring has room
+ * rows, length 0 and no pages; the first pages[s] entries of its table's row go behind the free ones,
+ * sequences in their order, before any is given out (those that the ring has no room for are lost: a ring has room
  * where ring_pages is the cache's number of pages and no page is in two tables). Then the
  * sequences in their order get, from the front of the free ones, what ceil(len[s] /
  * page_tokens) is more than pages[s]. Where none is left, the table's entry is -1, its

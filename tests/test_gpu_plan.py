@@ -172,3 +172,28 @@ def test_plan_steps_in_a_graph(tc, dev):
         torch.cuda.synchronize()
         check(p, want)
         st = dict(held=want["length"], pages=want["pages_out"], table=want["table"], ring=want["ring"], free=want["free_out"])
+
+
+def test_plan_pages_in_two_tables(tc, dev):
+    """Sequences with a common beginning: a sequence that ends gives back the first `pages` entries of its row. With its own
+    pages moved there and `pages` their number, the common ones stay with the other sequence, and no page comes twice."""
+    rng = np.random.default_rng(10)
+    page, common = 16, 3
+    st = state(rng, [70, 0, 40], ring=30, width=12)
+    pages, table = st["pages"], st["table"]
+    # the second sequence begins with the first one's first three pages, and has 20 tokens of its own behind them
+    own = st["ring"][:2].copy()
+    table[1, :common], table[1, common:common + 2] = table[0, :common], own
+    pages[1], st["held"][1] = common + 2, common * page + 20
+    st["free"][0], st["free"][1] = 2, st["free"][1] - 2
+    want = same(tc, dev, st, [1, 30, 1], page, 40)
+    st = dict(held=want["length"], pages=want["pages_out"], table=want["table"], ring=want["ring"], free=want["free_out"])
+    mine = int(st["pages"][1]) - common
+    assert mine == 4
+    st["table"][1, :mine] = st["table"][1, common:common + mine].copy()
+    st["pages"][1] = mine
+    want = same(tc, dev, st, [1, -1, 1], page, 2)
+    at, left = want["free_out"][:2]
+    free = [int(want["ring"][(at + i) % 30]) for i in range(left)]
+    used = [int(p) for s in (0, 2) for p in want["table"][s, :want["pages_out"][s]]]
+    assert sorted(free + used) == list(range(30)) and want["free_out"][2] == 0
