@@ -73,6 +73,7 @@ def test_left_out(tc, dev, leave, drafts):
         assert torch.equal(got.cpu(), l)
 
 
+# (chunks: 2048 tokens, or 4096 where those of 2048 are more than two to a CU)
 def test_many_sequences_and_chunk_sizes(tc, dev):
     """Chunks of 1024 to 8192 tokens of the vocabulary."""
     rng = np.random.default_rng(6)

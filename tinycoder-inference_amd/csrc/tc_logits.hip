@@ -4,7 +4,7 @@
 // there in LDS (integer sums, so their order changes nothing), adds up the biases in their
 // order, and then takes the sequence's rows one after the other, each row's own token counted
 // on top (as seen alone while it is the prompt's): every logit is read and written once, with its count and bias out of LDS beside it.
-// Bound by HBM for many rows (219 of 152064 logits with masks: 58 us of kernel, 272 MB at 4.7
+// Bound by HBM for many rows (219 of 152064 logits with masks: 57 to 58 us, 272 MB at 4.7
 // TB/s; VALU 0.30 busy); for few by the chain lists' borders -> history -> LDS -> stores (one row 4.1
 // us), and between these by the history, which every chunk's workgroup reads (256 rows of 32003
 // 18 us, 15 without it, 10 for the bytes).

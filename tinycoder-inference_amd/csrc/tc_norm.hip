@@ -323,8 +323,9 @@ __global__ __launch_bounds__(MOST) void k_norm(NormCall a) {
 
 // Short rows by as many lanes as they have eights (200000 rows of 128 columns 96 us with a wave
 // each, 38 with 16 lanes). Others by a workgroup: one block a lane where there are few rows, whose sums
-// are short then; two from 512 rows on, of which a CU holds more (1000 rows of 5120 10.7 -> 9.5 us, 8192
-// 79 -> 76 when it was taken; 500 rows 6.4 and 6.7); as many as 1024 threads leave from 8192 columns on.
+// are short then; two from 512 rows on, of which a CU holds more (16-bit rows of 5120, us with one and with two: 500 rows
+// 6.35 and 6.8, 520 7.6 and 7.2, 8192 65 and 61; with a norm behind the block 6.95 and 7.2, 8.8 and 7.8, 76 and 65);
+// as many as 1024 threads leave from 8192 columns on.
 template <int YW, int HW, bool POST>
 hipError_t launch(const NormCall &a, int num_cu, hipStream_t st) {
     const uint32_t blocks = (a.cols + 511) / 512;  // of a wave's 512 columns

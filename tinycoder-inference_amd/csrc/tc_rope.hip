@@ -12,7 +12,10 @@
 // same time). So each row goes from HBM to HBM once: prompts are bound by that (8190 rows of 36
 // heads of 128, bf16: 30 us, 151 MB at 5.0 TB/s; VALU 0.56 busy, half of it the angles and addresses
 // of a wave that does nothing twice), single tokens by the chain start -> len -> table -> store (3.5
-// us; 241 rows with norms and 8-bit values 6.2).
+// us; 241 rows with norms and 8-bit values 5.9 to 6.2).
+// That prompt is of pairs, half of each head. All of it rotated, pairs take 32 us, halves 35, since both lanes of
+// their pairs form the angles and load both values; with norms of heads 36 and 44; halves of n_rot / 2 = 61, whose
+// partners are loaded one by one, 48.
 //
 // Not kept: the same heads of several tokens in a wave, which makes the choice between q, k and v a
 // scalar's (38 us for 37, and 6.9 for 6.2: a wave's tokens are of several sequences), two, eight
@@ -311,8 +314,10 @@ template <int CT, int W, int L>
 hipError_t launch(const RopeCall &c, uint32_t units, hipStream_t st) {
     uint32_t blocks;
     RopeWalk w = make_walk(c, units, 1, &blocks);
-    // (four heads a lane from where single ones are more than 4 workgroups per CU: 1024 rows 10.9 -> 8.7
-    // us, 8190 59 -> 39 when it was taken; from 512 on 64 rows of 48 heads 7.5 -> 9.6)
+    // (four heads a lane from where single ones are more than 4 workgroups per CU. Rows and cache of 16
+    // bits, 28 + 2 x 4 heads of 128, us with one and with four: halves, 8190 rows 61 and 35, 1024 10.4 and 8.6,
+    // 512 6.4 and 6.5, 256 5.1 and 5.4; pairs 42.5 and 32.5, 7.9 and 7.1, 5.3 and 5.4, 4.2 and 4.8; halves with
+    // norms of heads 66 and 44, 11.2 and 9.7, 6.9 and 7.4, 5.3 and 6.1)
     if (blocks <= 1024) {
         k_rope<CT, W, L, 1><<<blocks, kThreads, 0, st>>>(c, w);
     } else {

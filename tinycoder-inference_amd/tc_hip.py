@@ -344,7 +344,8 @@ class Rope:
     frequencies on `device`. layout: "half" (dims i and i + n_rot / 2 are a pair) or
     "pairs" (2i and 2i + 1). scaling: "none", "linear", "ntk", "yarn" or "bands", with the
     numbers of tc_rope_scaling; divisors: fp32 [n_rot / 2]. factor_of_values: instead of the
-    scaling's own factor of the rotated values."""
+    scaling's own factor of the rotated values. The table is there when the object is, for any stream; one made
+    during a capture is filled when the graph runs."""
 
     def __init__(self, n_rot, theta=10000.0, layout="half", scaling="none", factor=1.0, original=0.0, low=0.0, high=0.0,
                  divisors=None, factor_of_values=None, device="cuda"):
