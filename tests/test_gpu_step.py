@@ -254,3 +254,81 @@ def test_frequencies_are_there_when_made(tc, dev):
             got = tc.rope(rope, x, pos)
         side.synchronize()
         assert torch.equal(got, want)
+
+
+def test_prompts_in_chunks_under_rules(tc, dev):
+    """Plan and rules of a captured step, replayed while prompts come in chunks beside sequences that answer: a prompt's tokens
+    are asked in whichever step they come, answers count from the first, and nothing of a step stays for the next."""
+    rng = np.random.default_rng(3)
+    S, T, room, vocab = 3, 16, 64, 300
+    z = lambda *n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
+    asked = np.array([25, 7, 1], np.int32)
+    text = [list(rng.integers(0, 40, n)) for n in asked]
+    new, tokens, history = z(S), z(T), z(S * room)
+    free = tensor(np.array([0, 30, 0], np.int32), dev)
+    plan = tc_hip.KVPlan(new, z(S), z(S), z(S, 8), torch.arange(30, dtype=torch.int32, device=dev), free, PAGE, T, in_place=True)
+    r = dict(repetition=np.array([1.3, 1.0, 0.7], np.float32), frequency=np.array([0.2, 0.5, -0.3], np.float32),
+             presence=np.array([0.4, 0.9, 0.1], np.float32))
+    rules = tc_hip.LogitRules(**{k: tensor(v, dev) for k, v in r.items()}, history=history, history_start=z(S + 1),
+                              prompt=tensor(-asked, dev))
+    starts = rules.held[4]
+    raw = tensor(rng.standard_normal((T, vocab)).astype(np.float32), dev)
+    out = torch.full((T, vocab), 7.0, device=dev)
+
+    def step():
+        tc.kv_plan(plan)
+        tc.logits_adjust(rules, raw, plan.start, tokens=tokens, out=out)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    done = [0, 0, 0]
+    for chunk in ([12, 3, 1], [8, 4, 2], [5, 2, 0], [1, 1, 1], [2, 3, 1]):
+        rows = []
+        for s, n in enumerate(chunk):
+            while len(text[s]) < done[s] + n:  # what it answers
+                text[s].append(int(rng.integers(0, 40)))
+            rows += text[s][done[s]:done[s] + n]
+        past = [text[s][:done[s]] for s in range(S)]
+        sums = np.concatenate([[0], np.cumsum([len(p) for p in past])]).astype(np.int32)
+        new.copy_(tensor(np.array(chunk, np.int32), dev))
+        tokens.copy_(tensor(np.array(rows + [5] * (T - len(rows)), np.int32), dev))
+        flat = np.full(S * room, 7, np.int32)
+        flat[:sums[-1]] = [t for p in past for t in p]
+        history.copy_(tensor(flat, dev))
+        starts.copy_(tensor(sums, dev))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        start = np.concatenate([[0], np.cumsum(chunk)])
+        assert plan.start.tolist() == list(start) and int(plan.free_out[2]) == 0
+        got = f64(out)
+        assert (got[start[-1]:] == 7.0).all()
+        for s in range(S):
+            one = {k: v[s:s + 1] for k, v in r.items()}
+            for t in range(start[s], start[s + 1]):
+                now = np.array(text[s][:done[s] + t - start[s] + 1])
+                e = logits_exact(f64(raw)[t:t + 1], [0, 1], None, history=now, history_start=[0, len(now)], prompt=asked[s:s + 1], **one)[0]
+                assert (np.abs(got[t] - e) <= U * np.abs(e) * 1.001 + 2.0 ** -40).all(), (chunk, s, t)
+            done[s] += chunk[s]
+
+
+def test_frequencies_made_in_a_graph(tc, dev):
+    """A rope made during a capture is filled by each replay, in front of the calls that use it."""
+    x, pos = torch.ones(64, 1, 128, device=dev), torch.arange(64, dtype=torch.int32, device=dev)
+    want = tc.rope(tc_hip.Rope(128, 1e6, scaling="linear", factor=4.0), x, pos)
+    out = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rope = tc_hip.Rope(128, 1e6, scaling="linear", factor=4.0)
+        tc.rope(rope, x, pos, out=out)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert torch.equal(tc.rope(rope, x, pos), want)
